@@ -9,7 +9,7 @@ the framework's calls; both work on the tensors that ``prepare`` makes.
 The cache: pages of P tokens (P a multiple of 32), all heads of a page together.
 
     k        float8_e4m3fn [pages, heads, P, D]
-    v        float8_e4m3fn [pages, heads, P / 32, D, 32]    32 tokens of one channel side by side
+    v        float8_e4m3fn [pages, heads, P / 16, D, 16]    16 tokens of one channel side by side
     k_scale  uint8 [pages, heads, P / 32]                   2^(s - 127), one for each block of
     v_scale  (the same)                                     32 tokens and head
     table    int32 [sequences, most pages]                  a sequence's pages in order
@@ -28,7 +28,7 @@ import torch
 own = False
 DEV = "cuda"
 DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
-BLOCK = 32
+BLOCK, SIDE = 32, 16
 F8 = torch.float8_e4m3fn
 MOST_SCORES = 64 * 4096 * 4096   # query rows x cached tokens of the largest listed prompt
 MOST_CACHED = 2 * 8 * 100003     # tokens x heads of the largest listed cache that is read
@@ -165,7 +165,8 @@ def _cache(case, g, extra=0):
     v, vs = _filled(g, pages, case["hkv"], page, case["D"])
     table = torch.randperm(pages, generator=g, device=DEV).int().reshape(B, per + extra)
     k = k.reshape(pages, case["hkv"], page, case["D"])
-    v = v.view(torch.uint8).transpose(-1, -2).contiguous().view(F8)
+    v = v.view(torch.uint8).view(pages, case["hkv"], page // SIDE, SIDE, -1)
+    v = v.transpose(-1, -2).contiguous().view(F8)
     return {"k": k, "v": v, "k_scale": ks, "v_scale": vs, "table": table}
 
 
@@ -270,7 +271,9 @@ def _put(s, name, codes, byte, at, page_of):
     """Writes blocks [n, heads, 32, D] of fp32 codes and their bytes at (page, block) pairs."""
     b = codes.to(F8).view(torch.uint8)
     if name == "v":
-        s["v"].view(torch.uint8)[page_of, :, at] = b.transpose(-1, -2)
+        pages, h, n, D, _ = s["v"].shape
+        s["v"].view(torch.uint8).view(pages, h, n // 2, 2, D, SIDE)[page_of, :, at] = \
+            b.view(*b.shape[:2], 2, SIDE, D).transpose(-1, -2)
     else:
         pages, h, page, D = s["k"].shape
         s["k"].view(torch.uint8).view(pages, h, page // BLOCK, BLOCK, D)[page_of, :, at] = b
@@ -292,8 +295,11 @@ def _plain_append(s):
     fresh = fresh[:, None, :, None]
     kept = (blk * BLOCK < start[seq])[:, None]
     for name, x in (("k", s["xk"]), ("v", s["xv"])):
-        was = s["v"][page_of, :, at].float().transpose(-1, -2) if name == "v" else \
-            s["k"].view(*s["k"].shape[:2], per, BLOCK, -1)[page_of, :, at].float()
+        if name == "v":
+            was = s["v"].view(*s["v"].shape[:2], per, 2, -1, SIDE)[page_of, :, at].float()
+            was = was.transpose(-1, -2).flatten(2, 3)
+        else:
+            was = s["k"].view(*s["k"].shape[:2], per, BLOCK, -1)[page_of, :, at].float()
         byte = s[name + "_scale"][page_of, :, at].int()
         x = x[row].float().transpose(1, 2)
         need = _byte(torch.where(fresh, x.abs(), 0.0).amax((-1, -2)))
@@ -459,7 +465,7 @@ def _written64(s, pool, name, pages, first, codes, e):
     if name == "k":
         pool["k"][page, :, at] = codes
     else:
-        pool["v"][page, :, at // BLOCK, :, at % BLOCK] = codes
+        pool["v"][page, :, at // SIDE, :, at % SIDE] = codes
     pool[name + "_scale"][page, :, at // BLOCK] = e.transpose(0, 1).repeat_interleave(
         BLOCK, 0)[:len(pos)].to(torch.uint8) + 127
 
