@@ -9,10 +9,14 @@ from .linear import (PackedWeight, QuantLinear, fp4_mfma_shared, fwht_block_for,
 from .brecq import adaround_levels, pack_quantized_linears, replace_forward  # noqa: F401
 from .jenks import (bias_mask, jenks2, linear_mask, module_bias, module_conv,  # noqa: F401
                     module_weights)
+from .kvcache import (Evicted, KVCache, cache_append, cache_attention,  # noqa: F401
+                      cache_evict)
+from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
 from . import _capi  # noqa: F401
 
 __all__ = ["PackedWeight", "QuantLinear", "fp4_mfma_shared", "fwht_block_for", "packed_k",
            "packed_linear",
            "quantize_module", "adaround_levels", "pack_quantized_linears", "replace_forward",
            "jenks2", "linear_mask", "bias_mask", "module_weights", "module_bias",
-           "module_conv"]
+           "module_conv", "KVCache", "cache_append", "cache_attention", "cache_evict", "Evicted",
+           "token_logprobs", "TokenLogprobs"]

@@ -44,12 +44,28 @@ EXPORTED = (
     "fb_gemm", "fb_gemm_workspace_bytes", "fb_grad_x", "fb_grad_x_workspace_bytes",
     "fb_to_device_gpu", "fb_cast_rows", "fb_add_bias", "fb_grad_bias", "fb_grad_bias_ws",
     "fb_grad_bias_workspace_bytes",
+    "fb_cache_append", "fb_cache_attention", "fb_cache_attention_workspace_bytes",
+    "fb_cache_evict", "fb_token_logprobs", "fb_token_logprobs_grad",
 )
 
 
 class FbShape(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in
                 ("N", "K", "B", "group", "fmt", "fwht_block", "x_dtype", "y_dtype")]
+
+
+class FbCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page", ctypes.c_int32)]
+
+
+class FbSeqs(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("seqs", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("tokens", ctypes.c_int32),
+                ("max_new", ctypes.c_int32), ("max_len", ctypes.c_int32)]
 
 
 _lib = None
@@ -67,6 +83,7 @@ def lib() -> ctypes.CDLL:
     L = ctypes.CDLL(str(LIB_PATH))
     vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
     sp = ctypes.POINTER(FbShape)
+    i64, cp, qp = ctypes.c_int64, ctypes.POINTER(FbCache), ctypes.POINTER(FbSeqs)
     sigs = {
         "fb_abi_version": (i32, []),
         "fb_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -114,6 +131,16 @@ def lib() -> ctypes.CDLL:
         "fb_jenks2_ssd_gpu": (ctypes.c_int, [vp, ctypes.c_int64, i32, vp, vp, sz, vp]),
         "fb_jenks2_ssd_filters_host": (ctypes.c_int, [vp, ctypes.c_int64, i32, i32, vp, i32]),
         "fb_jenks2_ssd_filters_gpu": (ctypes.c_int, [vp, ctypes.c_int64, i32, i32, vp, vp]),
+        "fb_cache_append": (ctypes.c_int, [cp, qp, vp, i64, i64, vp, i64, i64, i32, vp]),
+        "fb_cache_attention": (ctypes.c_int, [cp, qp, vp, i64, i64, i32, i32, ctypes.c_float, vp,
+                                              vp, vp, i64, i64, i32, vp, sz, vp]),
+        "fb_cache_attention_workspace_bytes": (sz, [cp, qp, i32]),
+        "fb_cache_evict": (ctypes.c_int, [cp, qp, vp, i64, i64, i32, i32, i32, vp, i64, i32, vp,
+                                          vp, vp, vp]),
+        "fb_token_logprobs": (ctypes.c_int, [vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp, vp,
+                                             vp]),
+        "fb_token_logprobs_grad": (ctypes.c_int, [vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp,
+                                                  vp, vp, vp, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

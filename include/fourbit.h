@@ -427,6 +427,125 @@ int fb_jenks2_ssd_filters_host(const void* sorted, int64_t nf, int32_t n, int32_
 int fb_jenks2_ssd_filters_gpu(const void* sorted, int64_t nf, int32_t n, int32_t dtype,
                               void* ssd, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * A key/value cache held in 8 bits, for attention between the packed linear layers.  The
+ * reference has no attention and no cache: no counterpart.
+ *
+ * Pages of `page` tokens (a multiple of 32), all heads of a page together:
+ *   k        uint8 [pages, heads, page, D]           E4M3 codes (no infinities, NaN = 0x7F)
+ *   v        uint8 [pages, heads, page / 16, D, 16]  16 tokens of one channel side by side
+ *   k_scale  uint8 [pages, heads, page / 32]         2^(s - 127) of a block of 32 tokens
+ *   v_scale  (the same)
+ * A block's exponent e is the least one from -100 up with amax <= 448 * 2^e over its finite
+ * values; a code is x * 2^-e rounded to nearest even, and a non-finite x is held as NaN.
+ * A sequence's tokens lie in the pages its row of `table` names, in order.
+ * ------------------------------------------------------------------------------- */
+typedef struct {
+  void* k;          /* device, 16-byte aligned, as k_scale, v and v_scale             */
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t pages;    /* 1 .. 2^31 - 1                                                   */
+  int32_t heads;    /* 1 .. 4096                                                       */
+  int32_t head_dim; /* D: a multiple of 16, 16 .. 256                                  */
+  int32_t page;     /* tokens of a page: a multiple of 32, 32 .. 2^24                  */
+} fb_cache_t;
+
+/* The sequences of a call.  All pointers are device pointers: nothing in them is read on the
+ * host, so a call can be captured in a HIP graph and replayed with other contents. */
+typedef struct {
+  const int32_t* table;  /* [seqs, max_pages], rows table_stride apart                     */
+  int64_t table_stride;
+  const int32_t* lens;   /* [seqs]; what it counts, each function says                     */
+  const int32_t* cu;     /* [seqs + 1]: sequence b's new tokens are rows cu[b] .. cu[b+1]-1;
+                            NULL: one token each (tokens == seqs)                          */
+  int32_t seqs;          /* 1 .. 65535                                                     */
+  int32_t max_pages;
+  int32_t tokens;        /* rows of x or q in all                                          */
+  int32_t max_new;       /* at least the most new tokens of one sequence                   */
+  int32_t max_len;       /* about the most tokens a sequence holds: how work is split goes
+                            by it, the result does not                                     */
+} fb_seqs_t;
+
+/* Writes new keys and values into the cache: sequence b's at lens[b], lens[b] + 1, ... (lens:
+ * the tokens held before the call).  A block that holds earlier tokens keeps the larger of its
+ * scale and the new tokens' own; where it grows, the earlier codes are rounded to the new scale.
+ * Slots behind the new tokens are left as they are.  Tokens beyond a sequence's last page or
+ * of pages outside the pool are not written.
+ *   k, v  [tokens, heads, D] of dtype FB_DT_F16, BF16 or F32; strides in elements, the last
+ *         dimension contiguous; element-aligned pointers */
+int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int64_t k_token,
+                    int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                    int32_t dtype, void* stream);
+
+/* Attention of q [tokens, q_heads, D] over the cache: q_heads is a multiple of the cache's
+ * heads, and query head j reads cache head j / (q_heads / heads).  lens: the tokens held, the
+ * new ones among them; row i of a sequence's n new rows sees the first lens - n + i + 1 tokens.
+ *   q      FB_DT_F16 or BF16; strides in elements, the last dimension contiguous
+ *   out    [tokens, q_heads, D] of q's dtype, contiguous, 16-byte aligned: softmax(scale * q.k) v
+ *   lse    fp32 [tokens, q_heads] or NULL: log of the sum of exp(scale * q.k)
+ *   weights fp32 [seqs, heads, >= max_len] or NULL: weights[b, h, t] grows by the attention
+ *          weight that token t got from all rows and query heads of this call (needs lse)
+ *   ws     256-byte aligned, fb_cache_attention_workspace_bytes (its contents are not kept)
+ * A row that sees no token gets 0, with an lse of -inf.  Products are exact and summed in fp32;
+ * attention weights enter the sum over v as fp16 (relative to the row's largest).  Page numbers
+ * outside the pool and lengths beyond the table give undefined numbers, but nothing outside the
+ * buffers is read. */
+int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, int64_t q_token,
+                       int64_t q_head, int32_t q_heads, int32_t dtype, float scale, void* out,
+                       float* lse, float* weights, int64_t w_seq, int64_t w_head,
+                       int32_t w_tokens, void* ws, size_t ws_bytes, void* stream);
+/* Workspace of that call (0 where it needs none, and for invalid arguments). */
+size_t fb_cache_attention_workspace_bytes(const fb_cache_t* c, const fb_seqs_t* s,
+                                          int32_t q_heads);
+
+/* Cuts every sequence (and head for itself) to `keep` tokens: its last `recent` ones and, of the
+ * others, those of largest weight (ties: the earlier token; NaN counts as less than any number).
+ * Sequences of at most `keep` tokens keep all.  The kept tokens' keys and values go, in their
+ * order and as a first append would write them, to the pages of new_table (none of them a page
+ * that is read); the block the last one lies in is filled with zeros.
+ *   s           table and lens (the tokens held); tokens, max_new and cu are not read
+ *   weights     fp32, strides as for fb_cache_attention, w_tokens >= every length
+ *   new_table   int32 [seqs, >= ceil(keep / page)]
+ *   kept        int32 [seqs, heads, keep]: the kept tokens' places, ascending, then -1
+ *   new_weights fp32 [seqs, heads, keep] (their weights, then 0) or NULL
+ *   new_lens    int32 [seqs]: min(lens, keep) */
+int fb_cache_evict(const fb_cache_t* c, const fb_seqs_t* s, const float* weights, int64_t w_seq,
+                   int64_t w_head, int32_t w_tokens, int32_t keep, int32_t recent,
+                   const int32_t* new_table, int64_t new_stride, int32_t new_pages,
+                   int32_t* kept, float* new_weights, int32_t* new_lens, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Log probabilities of given tokens, with the entropy of the distribution and its `top` most
+ * likely tokens.  No counterpart in the reference.
+ *   logits   [rows, vocab] of dtype FB_DT_F16, BF16 or F32, rows `stride` elements apart
+ *   token    int64 [rows]; one outside [0, vocab) is no token: its logprob is 0
+ *   logprob  fp32 [rows]: logit[token] - lse, lse = log sum exp(logit)
+ *   entropy  fp32 [rows]: -sum p log p (p = 0: nothing)
+ *   top_logprobs fp32 [rows, top], top_ids int64 [rows, top]: descending, ties: lowest id first;
+ *            0 <= top <= FB_LOGPROBS_TOP_MAX, top <= vocab
+ *   stats    fp32 [rows, 2]: (largest logit, log sum exp(logit - largest)), what the gradient
+ *            needs; NULL: not wanted
+ * A row of -inf alone has logprobs of -inf and no entropy; NaN or +inf makes its row NaN (NaN
+ * counts as the largest among the alternatives).
+ * ------------------------------------------------------------------------------- */
+#define FB_LOGPROBS_TOP_MAX 64
+int fb_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int64_t rows,
+                      int32_t vocab, const int64_t* token, int32_t top, float* logprob,
+                      float* entropy, float* top_logprobs, int64_t* top_ids, float* stats,
+                      void* stream);
+
+/* The gradient: grad[r, i] = g_logprob [i = token] + sum_j g_top[j] [i = top_ids[j]]
+ *   - (g_logprob + sum_j g_top[j]) p_i - g_entropy p_i (log p_i + entropy).
+ *   grad      [rows, vocab] of the logits' dtype, contiguous
+ *   g_*       fp32 or NULL (taken as 0); g_top and top_ids [rows, top]
+ *   stats, entropy  as fb_token_logprobs wrote them */
+int fb_token_logprobs_grad(const void* logits, int32_t dtype, int64_t stride, int64_t rows,
+                           int32_t vocab, const int64_t* token, int32_t top,
+                           const int64_t* top_ids, const float* stats, const float* entropy,
+                           const float* g_logprob, const float* g_entropy, const float* g_top,
+                           void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,477 @@
+"""The 8-bit key/value cache on the GPU (append, attention, eviction) against its restatement in
+fp64, from one token to several hundred, at the edges of blocks, pages, tiles and splits.
+
+Codes, scales and choices are exact.  The bound of an attention output, with u = 2^-24:
+ - a score is an fp32 sum of D exact products, scaled by a few roundings: off by at most
+   d = (D + 8) u * (its sum of magnitudes) + 8 u * |score|;
+ - a weight is off by exp(2 d) - 1 (numerator and sum), 4 u * score for the exponential's
+   argument in base 2, and 2^-11 for its fp16 copy, or 2^-25 of the largest value's unit where that
+   is subnormal;
+ - the fp32 sum over n tokens adds n u, and the result is rounded once to its 16 bits."""
+import numpy as np
+import pytest
+import torch
+
+from if_i_could_turn_back_time_amd import KVCache, cache_append, cache_attention, cache_evict
+from oracle import cache_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+
+
+def _pool(pages, heads, D, page, fill=0x7F):
+    """A pool whose unwritten places hold NaN codes and the largest scale."""
+    c = KVCache.new(pages, heads, D, page, DEV)
+    c.k.view(torch.uint8).fill_(fill)
+    c.v.view(torch.uint8).fill_(fill)
+    c.k_scale.fill_(255)
+    c.v_scale.fill_(255)
+    return c
+
+
+class Case:
+    """Sequences of the given lengths in a pool (pages in random order, some unused), written by
+    appends in `parts` uneven parts; the same in the oracle."""
+
+    def __init__(self, lens, heads, D, page, dt=torch.bfloat16, parts=2, seed=0, gain=1.0):
+        self.g = torch.Generator().manual_seed(seed)
+        self.heads, self.D, self.dt = heads, D, dt
+        self.lens = list(lens)
+        B = len(lens)
+        per = max(1, -(-max(lens) // page)) + 1
+        self.cache = _pool(B * per + 3, heads, D, page)
+        self.table = torch.randperm(B * per + 3, generator=self.g)[:B * per].int().view(B, per)
+        self.table = self.table.to(DEV)
+        self.k = [[O.Tokens(D) for _ in range(heads)] for _ in range(B)]
+        self.v = [[O.Tokens(D) for _ in range(heads)] for _ in range(B)]
+        cuts = [[round(n * i / parts) for i in range(parts + 1)] for n in lens]
+        for i in range(parts):
+            self.append([c[i] for c in cuts], [c[i + 1] - c[i] for c in cuts], gain * 3.0 ** i)
+
+    def append(self, start, count, gain=1.0, spoil=None):
+        T = sum(count)
+        x = torch.randn(T, 2, self.heads, self.D, generator=self.g) * gain
+        x[:, 0, :, ::5] *= 4
+        if spoil:
+            spoil(x)
+        x = x.to(self.dt)
+        cu = torch.tensor([0] + list(np.cumsum(count)), dtype=torch.int32, device=DEV)
+        xd = x.to(DEV)
+        cache_append(self.cache, xd[:, 0], xd[:, 1], self.table,
+                     torch.tensor(start, dtype=torch.int32, device=DEV), cu,
+                     max_new=max(count))
+        x, at = x.double().numpy(), 0
+        for b, (s, n) in enumerate(zip(start, count)):
+            for h in range(self.heads):
+                if n:
+                    self.k[b][h].append(x[at:at + n, 0, h], s)
+                    self.v[b][h].append(x[at:at + n, 1, h], s)
+            at += n
+
+    def check_codes(self):
+        for b, n in enumerate(self.lens):
+            if not n:
+                continue
+            k, v = self.cache.read(self.table[b], n)
+            for h in range(self.heads):
+                for got, want in ((k[h], self.k[b][h]), (v[h], self.v[b][h])):
+                    np.testing.assert_array_equal(got.double().cpu().numpy(), want.values())
+
+    def attend(self, new, group, scale=None, weights=None, dt=None, q_view=False, **kw):
+        dt = dt or self.dt
+        T, Hq = sum(new), self.heads * group
+        q = torch.randn(T, Hq, self.D, generator=self.g).to(dt)
+        qd = q.to(DEV)
+        if q_view:  # odd strides, an element off alignment
+            buf = torch.zeros(T * (Hq * self.D + 13) + 1, dtype=dt, device=DEV)
+            qd = buf[1:].view(T, Hq * self.D + 13)[:, 1:1 + Hq * self.D].view(T, Hq, self.D)
+            qd.copy_(q)
+        cu = torch.tensor([0] + list(np.cumsum(new)), dtype=torch.int32, device=DEV)
+        lens = torch.tensor(self.lens, dtype=torch.int32, device=DEV)
+        before = None if weights is None else weights.clone()
+        out, lse = cache_attention(qd, self.cache, self.table, lens, cu, scale=scale,
+                                   weights=weights, return_lse=True, **kw)
+        assert out.shape == q.shape and out.dtype == dt and out.is_contiguous()
+        self.check(q, new, group, scale, out, lse, weights, before)
+        return out, lse
+
+    def check(self, q, new, group, scale, out, lse, weights, before):
+        scale = self.D ** -0.5 if scale is None else scale
+        q, out, lse = (x.double().cpu().numpy() for x in (q, out, lse))
+        ulp = 2.0 ** -11 if self.dt == torch.float16 else 2.0 ** -8
+        least = 2.0 ** -25 if self.dt == torch.float16 else 2.0 ** -134
+        at = 0
+        for b, n in enumerate(new):
+            for h in range(self.heads):
+                k, v = self.k[b][h].values(), self.v[b][h].values()
+                t = len(k)
+                vmax = np.nanmax(np.abs(v)) if t and not np.isnan(v).all() else 0.0
+                wsum, werr = np.zeros(t), np.zeros(t)
+                for j in range(h * group, (h + 1) * group):
+                    o, l, p, mags, pv = O.attention(q[at:at + n, j], k, v, scale)
+                    got, gl = out[at:at + n, j], lse[at:at + n, j]
+                    d = ((self.D + 8) * U + 16 * U) * mags
+                    fin = np.isfinite(l)
+                    np.testing.assert_array_equal(gl[~fin], l[~fin])
+                    assert (np.abs(gl[fin] - l[fin]) <= d[fin] + 8 * U * (1 + np.abs(l[fin]))).all()
+                    rel = np.expm1(2 * d) + 8 * U * mags + 2.0 ** -11 + t * U
+                    bound = rel[:, None] * pv + t * 2.0 ** -24 * vmax
+                    bound = bound + ulp * (np.abs(o) + bound) + least
+                    nan = np.isnan(o)
+                    np.testing.assert_array_equal(np.isnan(got), nan)
+                    bad = ~(np.abs(got - o) <= bound) & ~nan
+                    assert not bad.any(), (b, h, j, np.abs(got - o)[bad].max())
+                    assert (got[~fin & ~np.isnan(l)] == 0).all()  # rows that see nothing
+                    wsum += p.sum(0)
+                    werr += (np.expm1(2 * d) + 24 * U * (1 + mags)) @ p
+                if weights is not None:
+                    gw = (weights[b, h].double() - before[b, h].double()).cpu().numpy()
+                    assert (gw[t:] == 0).all()
+                    total = np.abs(before[b, h, :t].double().cpu().numpy()) + wsum
+                    err = np.abs(gw[:t] - wsum)
+                    assert (err <= werr + len(new) * group * U * wsum + 2 * U * total).all()
+            at += n
+
+
+# ------------------------------------------------------------------ append
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens,heads,D,page,parts", [
+    ([1], 1, 16, 32, 1), ([31, 32, 33], 2, 64, 32, 3), ([5, 0, 100], 3, 80, 96, 2),
+    ([700, 257], 2, 128, 64, 5), ([64, 129], 1, 256, 128, 4), ([40], 5, 48, 64, 40)])
+def test_append_codes_are_exact(dt, lens, heads, D, page, parts):
+    c = Case(lens, heads, D, page, dt, parts)
+    c.check_codes()
+
+
+def test_append_leaves_other_places():
+    """Slots behind the new tokens and every page of nobody keep their bytes."""
+    c = Case([45, 64], 2, 64, 64, parts=3)
+    k = c.cache.k.view(torch.uint8)
+    used = c.table.long()
+    idle = torch.ones(k.shape[0], dtype=torch.bool, device=DEV)
+    idle[used[0, 0]] = idle[used[1, 0]] = False
+    assert bool((k[idle] == 0x7F).all()) and bool((c.cache.v.view(torch.uint8)[idle] == 0x7F).all())
+    assert bool((c.cache.k_scale[idle] == 255).all())
+    assert bool((k[used[0, 0], :, 45:] == 0x7F).all())
+    v = c.cache.v.view(torch.uint8)[used[0, 0]].transpose(-1, -2).reshape(2, 64, 64)
+    assert bool((v[:, 45:] == 0x7F).all())
+
+
+def test_append_again_from_an_earlier_place():
+    """Tokens that were written for nothing (a rejected guess) are overwritten, and a block that
+    starts over forgets its scale."""
+    c = Case([70], 2, 64, 64, parts=1, gain=100.0)
+    c.append([64], [9], 0.01)
+    c.lens = [73]
+    c.check_codes()
+    c.append([40], [5], 1000.0)
+    c.lens = [45]
+    c.check_codes()
+
+
+def test_append_special_values():
+    """Non-finite values are NaN and move no scale; tiny and huge blocks keep theirs."""
+    def spoil(x):
+        x[3, 0, 0, 2], x[5, 1, 1, 7] = float("nan"), float("inf")
+        x[40:72] *= 1e-30
+        x[72:104] *= 1e30
+        x[104:] = 0
+    c = Case([0], 2, 32, 64, torch.float32, parts=1)
+    c.table = torch.arange(3, dtype=torch.int32, device=DEV).view(1, 3)
+    c.append([0], [140], 1.0, spoil)
+    c.lens = [140]
+    c.check_codes()
+
+
+def test_append_strided_unaligned_and_beyond_the_pages():
+    g = torch.Generator().manual_seed(5)
+    c, ref = _pool(4, 2, 64, 32), _pool(4, 2, 64, 32)
+    x = torch.randn(40, 2 * 64 * 3 + 1, generator=g).half().to(DEV)
+    k, v = x[:, 1:129].view(40, 2, 64), x[:, 130:258].view(40, 2, 64)
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=DEV)
+    start = torch.tensor([30], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 40], dtype=torch.int32, device=DEV)
+    cache_append(c, k, v, table, start, cu)  # places 64.. have no page
+    cu[1] = 34
+    cache_append(ref, k[:34].contiguous(), v[:34].contiguous(), table, start, cu)
+    for a, b in zip(c, ref):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    table[0, 1] = 77  # not in the pool
+    cache_append(c, k[:34], v[:34], table, start, cu)
+    table[0, 1] = -1
+    cache_append(c, k[:34], v[:34], table, start, cu)
+    for a, b in zip(c, ref):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,heads,group,D,page", [
+    ([1], 1, 1, 64, 32), ([33, 0, 128], 2, 4, 128, 64), ([127, 129, 511, 640], 2, 8, 128, 64),
+    ([2100], 1, 16, 128, 256), ([95, 300], 3, 5, 80, 96), ([700], 2, 2, 256, 32),
+    ([260, 31], 4, 1, 192, 64), ([77], 2, 3, 16, 32), ([513], 1, 16, 48, 64)])
+def test_one_token(dt, lens, heads, group, D, page):
+    print("one token", dt, lens, heads, group, D, page, flush=True)
+    c = Case(lens, heads, D, page, dt)
+    c.attend([1] * len(lens), group)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,new,heads,group,D,page", [
+    ([5], [5], 1, 1, 64, 32), ([40, 7, 300], [3, 0, 4], 2, 4, 128, 64),
+    ([130, 64], [130, 33], 2, 2, 128, 64), ([300, 17], [129, 17], 1, 8, 64, 32),
+    ([700, 350], [33, 200], 2, 5, 80, 96), ([150], [150], 1, 3, 256, 64),
+    ([1100], [64], 1, 1, 192, 128), ([3], [7], 2, 2, 64, 32), ([260], [100], 1, 20, 48, 64)])
+def test_several_tokens(dt, lens, new, heads, group, D, page):
+    """Prompts, parts behind a cache, guesses; with more rows than tokens the first see none."""
+    print("several", dt, lens, new, heads, group, D, page, flush=True)
+    c = Case(lens, heads, D, page, dt)
+    c.attend(new, group)
+
+
+@pytest.mark.parametrize("new", [[1, 1], [3, 1], [50, 21]])
+def test_bounds_change_speed_only(new):
+    c = Case([900, 333], 2, 128, 64)
+    c.g.manual_seed(1)
+    ref, _ = c.attend(new, 4)
+    for kw in ({"max_len": 1}, {"max_len": 100}, {"max_new": 1}, {"max_new": 5, "max_len": 400},
+               {"max_new": 10 ** 6, "max_len": 10 ** 9}):
+        c.g.manual_seed(1)
+        c.attend(new, 4, **kw)
+
+
+@pytest.mark.parametrize("new,group", [([1, 1], 2), ([40, 3], 2), ([1, 1], 8)])
+def test_scale_and_odd_strides(new, group):
+    c = Case([200, 65], 2, 64, 32, torch.float16)
+    c.attend(new, group, scale=0.37, q_view=True)
+
+
+@pytest.mark.parametrize("new,group", [([1, 1, 1], 8), ([5, 0, 2], 2), ([150, 100, 1], 4),
+                                       ([1, 1, 1], 20)])
+def test_weights(new, group):
+    c = Case([600, 101, 33], 2, 128, 64)
+    w = torch.rand(3, 3, 700, generator=torch.Generator().manual_seed(1)).to(DEV)[:, :2]
+    c.attend(new, group, weights=w, max_len=600)
+
+
+@pytest.mark.parametrize("new", [[1], [4], [70]])
+def test_nan_reaches_only_who_sees_it(new):
+    """NaN in a value or key, in a place that some rows see and some do not; the places behind the
+    end hold NaN throughout."""
+    def spoil(x):
+        x[-2, 1, 0, 3] = float("nan")   # a value
+        x[-1, 0, 1, 5] = float("inf")   # a key: its score, so the whole row
+        x[1, 1, 1, 0] = float("nan")
+    c = Case([0], 2, 64, 32, parts=1)
+    c.table = torch.arange(4, dtype=torch.int32, device=DEV).view(1, 4)
+    c.append([0], [75], 1.0, spoil)
+    c.lens = [75]
+    c.attend(new, 2)
+
+
+def test_scales_far_apart():
+    """Blocks whose values differ by 2^60 and more: the large ones decide, nothing overflows."""
+    for gains in ((1e-20, 1.0, 1e15), (1e15, 1.0, 1e-20)):
+        c = Case([0], 1, 64, 32, torch.float32, parts=1)
+        c.table = torch.arange(4, dtype=torch.int32, device=DEV).view(1, 4)
+        for i, gain in enumerate(gains):
+            def spoil(x, gain=gain):
+                x[:, 0] = x[:, 0].clamp(-3, 3)
+                x[:, 1] *= gain
+            c.append([32 * i], [32], 1.0, spoil)
+        c.lens = [96]
+        c.dt = torch.bfloat16
+        c.attend([1], 4, dt=torch.bfloat16)
+        c.attend([40], 4, dt=torch.bfloat16)
+
+
+def test_large_scores():
+    """Scores far beyond the exponential's range on both sides."""
+    c = Case([300], 1, 64, 32, torch.bfloat16, gain=30.0)
+    c.attend([1], 4, scale=1.0)
+    c.attend([60], 4, scale=1.0)
+
+
+def test_empty_calls():
+    c = Case([10, 20], 2, 64, 32)
+    q = torch.empty(0, 4, 64, dtype=torch.bfloat16, device=DEV)
+    cu = torch.zeros(3, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([10, 20], dtype=torch.int32, device=DEV)
+    out, lse = cache_attention(q, c.cache, c.table, lens, cu, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    x = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=DEV)
+    cache_append(c.cache, x, x, c.table, lens, cu)
+    c.check_codes()
+
+
+def test_places_past_32_bits():
+    """A pool of more than 2^32 bytes: pages at its end are found."""
+    page, heads, D = 1024, 8, 128
+    pages = (1 << 32) // (page * heads * D) + 3
+    cache = KVCache.new(pages, heads, D, page, DEV)
+    c = Case([90], heads, D, 32)
+    k, v = c.cache.read(c.table[0], 90)
+    table = torch.tensor([[pages - 1]], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 90], dtype=torch.int32, device=DEV)
+    cache_append(cache, k.transpose(0, 1).contiguous(), v.transpose(0, 1).contiguous(), table,
+                 torch.zeros(1, dtype=torch.int32, device=DEV), cu)
+    c.cache, c.table = cache, table
+    c.check_codes()
+    c.attend([1], 2)
+    c.attend([50], 2)
+
+
+def test_other_stream_and_graph():
+    """On a stream of its own, and captured: replays follow the contents of tables, lengths and
+    inputs."""
+    c = Case([300, 129], 2, 128, 64)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    lens = torch.tensor(c.lens, dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    kv = torch.randn(2, 2, 2, 128, dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros(2, 2, 400, device=DEV)
+
+    def step():
+        cache_append(c.cache, kv[:, 0], kv[:, 1], c.table, lens - 1, cu, max_new=1)
+        return cache_attention(q, c.cache, c.table, lens, cu, max_new=1, max_len=400, weights=w)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(first, step())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(4):
+        q.normal_()
+        kv.normal_()
+        lens += min(i, 1)  # the next place
+        w.zero_()
+        want = step()
+        sums = w.clone()
+        w.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want) and torch.equal(w, sums)
+
+
+# ------------------------------------------------------------------ eviction
+@pytest.mark.parametrize("lens,heads,D,page,keep,recent", [
+    ([100], 1, 64, 32, 33, 5), ([300, 20, 0, 64], 2, 128, 64, 64, 16), ([1500], 3, 80, 96, 700, 0),
+    ([2500, 1200], 2, 64, 64, 40, 40), ([130], 2, 256, 32, 129, 1), ([65], 1, 16, 32, 1, 0)])
+def test_evict(lens, heads, D, page, keep, recent):
+    print("evict", lens, heads, D, page, keep, recent, flush=True)
+    c = Case(lens, heads, D, page)
+    B = len(lens)
+    most = max(lens)
+    w = torch.rand(B, heads, most + 9, generator=c.g)
+    w = torch.round(w * 50) / 50 - 0.2  # many equal ones, negative ones, both zeros
+    w[:, :, 3::17] = float("nan")
+    w[:, :, 5::29] = float("inf")
+    w[:, :, 6::31] = -0.0
+    need = -(-keep // page)
+    pool = _pool(c.cache.k.shape[0] + B * need, heads, D, page)
+    for a, b in zip(pool, c.cache):
+        a.view(torch.uint8)[:b.shape[0]] = b.view(torch.uint8)
+    c.cache = pool
+    new_table = (torch.randperm(B * need, generator=c.g) + pool.k.shape[0] - B * need).int()
+    new_table = new_table.view(B, need).to(DEV)
+    r = cache_evict(pool, c.table, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                    w.to(DEV), keep, recent, new_table, max_len=most)
+    c.check_codes()  # what was read is as it was
+    assert r.lens.tolist() == [min(n, keep) for n in lens]
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert bool((r.kept[b] == -1).all()) and bool((r.weights[b] == 0).all())
+            continue
+        m = min(n, keep)
+        k, v = pool.read(new_table[b], (m + 31) // 32 * 32)
+        for h in range(heads):
+            ids = O.evict(w[b, h, :n].numpy(), keep, recent)
+            assert r.kept[b, h].tolist() == list(ids) + [-1] * (keep - m)
+            got = r.weights[b, h].cpu().numpy()
+            np.testing.assert_array_equal(got[:m], w[b, h].numpy()[ids])
+            assert (got[m:] == 0).all()
+            for got, old in ((k[h], c.k[b][h]), (v[h], c.v[b][h])):
+                want = O.Tokens(D)
+                want.append(old.values()[ids])
+                got = got.double().cpu().numpy()
+                np.testing.assert_array_equal(got[:m], want.values())
+                assert (got[m:] == 0).all()
+
+
+def test_evict_then_append_and_attend():
+    c = Case([200], 2, 64, 32)
+    pool = _pool(40, 2, 64, 32)
+    for a, b in zip(pool, c.cache):
+        a.view(torch.uint8)[:b.shape[0]] = b.view(torch.uint8)
+    c.cache = pool
+    w = torch.rand(1, 2, 200, generator=c.g).to(DEV)
+    new_table = torch.arange(30, 35, dtype=torch.int32, device=DEV).view(1, 5)
+    r = cache_evict(pool, c.table, torch.tensor([200], dtype=torch.int32, device=DEV), w, 90, 20,
+                    new_table)
+    for h in range(2):
+        ids = r.kept[0, h].cpu().numpy()
+        for side in (c.k, c.v):
+            cut = O.Tokens(64)
+            cut.append(side[0][h].values()[ids])
+            side[0][h] = cut
+    c.table = new_table
+    c.append([90], [7], 5.0)
+    c.lens = [97]
+    c.check_codes()
+    c.attend([7], 4)
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    c = Case([40, 10], 2, 64, 32)
+    q = torch.randn(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    kv = torch.randn(2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    lens = torch.tensor([40, 10], dtype=torch.int32, device=DEV)
+    w = torch.zeros(2, 2, 64, device=DEV)
+    ok = dict(q=q, cache=c.cache, table=c.table, lens=lens)
+
+    def attend(**kw):
+        extra = {k: kw.pop(k) for k in list(kw) if k not in ok}
+        a = {**ok, **kw}
+        return cache_attention(a["q"], a["cache"], a["table"], a["lens"], **extra)
+
+    attend()
+    for kw in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q[0]),
+               dict(q=q.cpu()), dict(q=q[..., ::2].expand(2, 4, 32)), dict(lens=lens.long()),
+               dict(lens=lens[:1]), dict(table=c.table.long()), dict(table=c.table[0]),
+               dict(table=c.table.cpu()), dict(cu_seqlens=lens), dict(q=q[:1]),
+               dict(max_new=-1, cu_seqlens=torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)),
+               dict(max_len=-2), dict(weights=w.half()), dict(weights=w[:, :1]),
+               dict(weights=w[..., :10], max_len=40), dict(weights=w.expand(2, 2, 64).cpu()),
+               dict(weights=w[:1].expand(2, 2, 64)),
+               dict(cache=c.cache._replace(k=c.cache.k.view(torch.uint8))),
+               dict(cache=c.cache._replace(v=c.cache.v[:, :, :1])),
+               dict(cache=c.cache._replace(k_scale=c.cache.k_scale[:1])),
+               dict(cache=c.cache._replace(k=c.cache.k[:, :1]))):
+        with pytest.raises((ValueError, RuntimeError)):
+            attend(**kw)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        attend(q=q.clone().requires_grad_(True))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        cache_append(c.cache, kv.clone().requires_grad_(True), kv, c.table, lens)
+    for k, v in ((kv[:, :1], kv), (kv, kv.half()), (kv.double(), kv.double()), (kv[:1], kv[:1]),
+                 (kv.cpu(), kv.cpu()), (kv.transpose(1, 2), kv)):
+        with pytest.raises((ValueError, RuntimeError)):
+            cache_append(c.cache, k, v, c.table, lens)
+    new = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    for keep, recent, nt, ww in ((0, 0, new, w), (8, 9, new, w), (33, 2, new, w), (8, -1, new, w),
+                                 (8, 2, new.long(), w), (8, 2, new[:1], w), (8, 2, new, w[..., :4])):
+        with pytest.raises((ValueError, RuntimeError)):
+            cache_evict(c.cache, c.table, lens, ww, keep, recent, nt, max_len=40)
+    with pytest.raises(ValueError):
+        KVCache.new(4, 2, 64, 48, DEV)
+    with pytest.raises(ValueError):
+        KVCache.new(4, 2, 72, 64, DEV)
+    torch.cuda.synchronize()
