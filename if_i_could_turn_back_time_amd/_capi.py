@@ -134,7 +134,7 @@ def lib() -> ctypes.CDLL:
         "fb_cache_append": (ctypes.c_int, [cp, qp, vp, i64, i64, vp, i64, i64, i32, vp]),
         "fb_cache_attention": (ctypes.c_int, [cp, qp, vp, i64, i64, i32, i32, ctypes.c_float, vp,
                                               vp, vp, i64, i64, i32, vp, sz, vp]),
-        "fb_cache_attention_workspace_bytes": (sz, [cp, qp, i32]),
+        "fb_cache_attention_workspace_bytes": (sz, [cp, qp, i32, i32]),
         "fb_cache_evict": (ctypes.c_int, [cp, qp, vp, i64, i64, i32, i32, i32, vp, i64, i32, vp,
                                           vp, vp, vp]),
         "fb_token_logprobs": (ctypes.c_int, [vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp, vp,

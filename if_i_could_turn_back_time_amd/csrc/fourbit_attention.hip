@@ -13,6 +13,7 @@
 #include "fourbit_cache.h"
 
 #include <algorithm>
+#include <type_traits>
 
 // Host helper of fourbit_gemv.hip.  Not part of the library's ABI.
 namespace fb_gpu {
@@ -37,7 +38,10 @@ struct Attn {
   float* lse;         // or null
   int splits, split_tokens;
   float* part;        // [splits][T * Hq][D]
-  float2* part_ml;    // [splits][T * Hq]: largest score (base 2), sum
+  float2* part_ml;    // [splits][T * Hq]: what the sums are relative to (base 2), sum
+  int per_shift;      // log2 of a page's blocks, -1: no power of two
+  float* scores;      // or null: [B][H][score_rows][score_tokens], base 2
+  int score_rows, score_tokens;
 };
 
 __device__ inline float exp2f_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -125,31 +129,49 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 
 // ---------------------------------------------------------------------------------
 // Few rows (at most 16 a cached head and sequence: decoding).  Bound by reading the cache once,
-// so nothing is staged: each wave takes 128 tokens at a time and reads keys and values straight
-// into operands of 16x16x32 products.  Workgroup = (split of the tokens, head, sequence), its 4
-// waves take chunks in turn and join their sums through LDS.
-//  - K operand row r of product j: token 32 (r / 4) + 4 j + r % 4, channels 64 p + 16 q + 8 u.. of
-//    lane group q: then a lane's scores are the tokens of block q, 4 j + i.
-//  - V operand: channel 16 d + r, tokens 8 s.. of block q, which lie side by side.
+// so nothing is staged: each wave takes 64 tokens at a time and reads keys and values straight
+// into operands of 16x16x32 products.  The next keys are asked for when the scores are there, the
+// next values when the sums are: a wave always has one of the two on its way.  Workgroup =
+// (split of the tokens, head, sequence); its waves take chunks in turn and join their sums through
+// LDS.
+//  - K operand row r of product j: token 16 (r / 4) + 4 j + r % 4, channels 64 p + 16 q + 8 u.. of
+//    lane group q: then a lane's scores are the tokens of side q, 4 j + i.
+//  - V operand: channel 16 d + r, tokens 8 s.. of side q, which lie side by side.
+//  - the sums are kept relative to a row's largest score of some earlier time, and are brought up
+//    to date only when a score passes it by more than 2^kSlack, which is rare after the first.
 // ---------------------------------------------------------------------------------
-constexpr int kChunk = 128;
+constexpr int kChunk = 64;
+constexpr float kSlack = 8.f;  // weights up to 2^8 in fp16
 
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void attn_few_kernel(Attn a) {
+template <int DP>
+constexpr int few_waves() {
+  return DP > 128 ? 4 : 8;  // registers of one wave a SIMD, or of two
+}
+
+template <int DT, int DP, bool EX>
+__global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) {
   using H = Half<DT>;
-  constexpr int NP = DP / 64, ND = DP / 16;
-  constexpr int PASS = DP < 128 ? DP : 128;  // channels joined at a time
-  __shared__ float join[4][16][PASS + 4];
-  __shared__ float wave_m[4][16], wave_l[4][16];
-  __shared__ int wave_e[4];
+  using F = Half<FB_DT_F16>;
+  constexpr int NP = DP / 64, ND = DP / 16, NW = few_waves<DP>();
+  constexpr int PASS = 64;  // channels joined at a time
+  __shared__ float join[NW][16][PASS + 4];
+  __shared__ float wave_m[NW][16], wave_l[NW][16];
+  __shared__ int wave_e[NW];
   const Cache& c = a.c;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int D = EX ? DP : c.D;  // known: the loads' addresses differ by constants
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q4 = lane >> 4;
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   int row0, n;
   c.rows(b, row0, n);
   const int len = min(max(c.lens[b], 0), c.capacity());
   const int rows = n * a.group;
+  const unsigned per = (unsigned)c.P / kBlock;
+  const int32_t* const table = c.table + b * c.table_stride;
+  // within a block: where the lane's keys and values begin
+  const int k_from = (16 * ((r >> 2) & 1) + (r & 3)) * D + q4 * 16;
+  const int v_from = ((q4 & 1) * D + r) * 16;
   for (int tile = 0; tile < rows; tile += 16) {
     const int row = tile + r, i = row / a.group;
     const bool there = row < rows;
@@ -162,49 +184,77 @@ __global__ __launch_bounds__(256) void attn_few_kernel(Attn a) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int d = 64 * p + 16 * q4 + 8 * u;
-        qf[p][u] = load_q<DT>(a, there && d < c.D,
+        qf[p][u] = load_q<DT>(a, there && d < D,
                               (int64_t)(row0 + i) * a.q_token + head * a.q_head + d);
       }
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
-    float m = -__builtin_inff(), l = 0.f;
-    int E = kMinExp;  // the accumulators' unit is 2^E
+    float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
+    int E = kMinExp;                       // and their unit's exponent
 
-    const int first = split * (a.split_tokens / kChunk);
-    const int last = split + 1 == a.splits ? (len + kChunk - 1) / kChunk
-                                           : min((len + kChunk - 1) / kChunk,
-                                                 first + a.split_tokens / kChunk);
-    for (int ch = first + wave; ch < last; ch += 4) {
-      // keys: lane's rows are 4 j + r % 4 of block r / 4; values: block q4
-      int at_k, at_v;
-      const int pk = max(c.page_of(b, ch * 4 + (r >> 2), at_k), 0);
-      const int pv = max(c.page_of(b, ch * 4 + q4, at_v), 0);
-      const int64_t bk = c.block_index(pk, h, at_k), bv = c.block_index(pv, h, at_v);
-      const uint8_t* const kp = c.k + bk * kBlock * c.D + (r & 3) * c.D + q4 * 16;
-      const uint8_t* const vp = c.v + bv * kBlock * c.D + r * 16;
-      u32x4 kf[8][NP], vf[ND][2];
+    const int all = (len + kChunk - 1) / kChunk;
+    const int first = min(all, split * (a.split_tokens / kChunk));
+    const int last =
+        split + 1 == a.splits ? all : min(all, first + a.split_tokens / kChunk);
+    // the two blocks of a chunk: entries of the table (read a chunk ahead) and places in the pages
+    int id[2], at[2];
+    const auto look = [&](int ch) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int y = 0; y < 2; ++y) {
+        const unsigned blk = (unsigned)ch * 2 + y;
+        const unsigned pg = a.per_shift >= 0 ? blk >> a.per_shift : blk / per;
+        at[y] = (int)(blk - pg * per);
+        id[y] = pg < (unsigned)c.max_pages ? table[pg] : 0;
+      }
+    };
+    u32x4 kf[4][NP], vf[ND];
+    int sk, sv;
+    int64_t blk_k, blk_v;  // the lane's blocks in the pool
+    const auto place = [&] {
+      int64_t idx[2];
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
-          kf[j][p] = 64 * p + 16 * q4 < c.D
-                         ? *reinterpret_cast<const u32x4*>(kp + 4 * j * c.D + 64 * p)
-                         : u32x4{0, 0, 0, 0};
+      for (int y = 0; y < 2; ++y) {
+        const int pg = (unsigned)id[y] < (unsigned)c.pages ? id[y] : 0;
+        idx[y] = c.block_index(pg, h, at[y]);
+      }
+      blk_k = r >> 3 ? idx[1] : idx[0];
+      blk_v = q4 >> 1 ? idx[1] : idx[0];
+    };
+    const auto load_k = [&] {
+      const uint8_t* const p0 = c.k + blk_k * kBlock * D + k_from;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          // pieces past D meet zeros of q: any others of the row
+          const int off = 64 * p + 16 * q4 < D ? 64 * p : -16 * q4;
+          kf[j][p] = *reinterpret_cast<const u32x4*>(p0 + 4 * j * D + off);
+        }
+      sk = c.ks[blk_v];
+    };
+    const auto load_v = [&] {
+      const uint8_t* const p0 = c.v + blk_v * kBlock * D + v_from;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
+        vf[d] = 16 * d < D ? *reinterpret_cast<const u32x4*>(p0 + d * 256) : u32x4{0, 0, 0, 0};
+      sv = c.vs[blk_v];
+    };
+    int ch = first + wave;
+    if (ch < last) {
+      look(ch);
+      place();
+      load_k();
+      load_v();
+      if (ch + NW < last) look(ch + NW);
+    }
+    for (; ch < last; ch += NW) {
+      const bool masked = ch * kChunk + kChunk > least;  // the same for the wave
+      // tokens of the lane's side that its row sees, and that are held
+      const int seen = sees - ch * kChunk - q4 * 16, held = len - ch * kChunk - q4 * 16;
+      f32x4 s[4];
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-          vf[d][p] = 16 * d < c.D
-                         ? *reinterpret_cast<const u32x4*>(vp + p * c.D * kSide + d * 256)
-                         : u32x4{0, 0, 0, 0};
-      const float ks = a.scale2 * exp2i(min(max((int)c.ks[bv] - 127, -126), 127));
-      const bool held = ch * kChunk + q4 * kBlock < len;
-      const int ev = held ? min(max((int)c.vs[bv] - 127, -126), 126) : kMinExp;
-
-      f32x4 s[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         s[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
@@ -212,97 +262,107 @@ __global__ __launch_bounds__(256) void attn_few_kernel(Attn a) {
           s[j] = H::mfma16(H::decode(kf[j][p][2], kf[j][p][3]), qf[p][1], s[j]);
         }
       }
-      const int t0 = ch * kChunk + q4 * kBlock;  // the lane's tokens: t0 + 4 j + i
+      const float ks = a.scale2 * exp2i(min(max(sk - 127, -126), 127));
+      const bool more = ch + NW < last;
+      if (more) {
+        place();
+        load_k();
+        if (ch + 2 * NW < last) look(ch + 2 * NW);
+      }
+      if (masked) {
+        asm volatile("");  // a branch, not selects in every chunk
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] *= ks;
-      f32x4 bad[ND];
-      bool any_bad = false;
-      if (ch * kChunk + kChunk > least) {
-        unsigned nan = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (t0 + 4 * j + k >= sees) s[j][k] = -__builtin_inff();
-        // what lies behind the end may be anything: no NaN from there
+            if (4 * j + k >= seen) s[j][k] = -__builtin_inff();
+      }
+      if (a.scores && there && row < a.score_rows && ch * kChunk < a.score_tokens) {
+        float* const to = a.scores +
+                          (((int64_t)b * c.H + h) * a.score_rows + row) * a.score_tokens +
+                          ch * kChunk + q4 * 16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(to + 4 * j) = s[j] * ks;
+      }
+      float big = s[0][0];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) big = fmaxf(big, s[j][k]);
+      big *= ks;  // positive
+      big = fmaxf(big, __shfl_xor(big, 16));
+      big = fmaxf(big, __shfl_xor(big, 32));
+      // of the lane's block, where it is held
+      const bool block_held = !masked || ch * kChunk + (q4 >> 1) * kBlock < len;
+      const int ev = block_held ? min(max(sv - 127, -126), 126) : kMinExp;
+      const int e = max(E, max(ev, __shfl_xor(ev, 32)));
+      if (__any(e > E || big > m + kSlack)) {
+        const float up = fmaxf(m, big);
+        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
+        const float unit = alpha * exp2i(max(E - e, -126));
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= unit;
+        m = up;
+        E = e;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
+      // the value block's scale joins in the exponent and leaves the sum again
+      const int fold = max(ev - E, -64);
+      const float shift = (float)fold - base;
+      float sum = 0.f;
+      h16x8 pf[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float p = exp2f_(__builtin_fmaf(s[j][k], ks, shift));
+          sum += p;
+          pf[j / 2][4 * (j & 1) + k] = (_Float16)p;
+        }
+      l = __builtin_fmaf(sum, exp2i(-fold), l);
+      if (masked) {
+        asm volatile("");
+        unsigned nan = 0;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              vf[d][p][w] &= keep_bytes(t0 + 16 * p + 4 * w, len);
-              nan |= nan_bytes(vf[d][p][w]);
-            }
-        any_bad = __any(nan != 0);
-        if (any_bad) {
+          for (int w = 0; w < 4; ++w) {
+            vf[d][w] &= keep_bytes(4 * w, held);  // what lies behind the end may be anything
+            nan |= nan_bytes(vf[d][w]);
+          }
+        if (__any(nan != 0)) {
           // a NaN value reaches the rows that see its token, and no others: 0 * NaN must not
           // come up, so those channels are marked apart
+          h16x8 see[2];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) see[k / 8][k & 7] = k < seen ? (_Float16)1 : (_Float16)0;
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            bad[d] = f32x4{0, 0, 0, 0};
+            f32x4 bad{0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              h16x8 see;
+            for (int x = 0; x < 2; ++x)
+              bad = F::mfma16(F::decode(nan_ones(vf[d][2 * x]), nan_ones(vf[d][2 * x + 1])),
+                              see[x], bad);
 #pragma unroll
-              for (int k = 0; k < 8; ++k) see[k] = t0 + 8 * x + k < sees ? (_Float16)1 : (_Float16)0;
-              bad[d] = Half<FB_DT_F16>::mfma16(
-                  Half<FB_DT_F16>::decode(nan_ones(vf[d][x / 2][2 * (x & 1)]),
-                                          nan_ones(vf[d][x / 2][2 * (x & 1) + 1])),
-                  see, bad[d]);
-            }
+            for (int k = 0; k < 4; ++k)
+              if (bad[k] > 0.f) o[d][k] = __builtin_nanf("");
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) vf[d][p][w] &= ~nan_bytes(vf[d][p][w]);
+            for (int w = 0; w < 4; ++w) vf[d][w] &= ~nan_bytes(vf[d][w]);
           }
         }
       }
-      float mx = m;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, s[j][k]);
-      mx = fmaxf(mx, __shfl_xor(mx, 16));
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      int e = max(ev, __shfl_xor(ev, 16));
-      e = max(e, __shfl_xor(e, 32));
-      e = max(e, E);
-      const float base = mx == -__builtin_inff() ? 0.f : mx;
-      const float alpha = exp2f_(m - base);
-      const float fold = exp2i(max(ev - e, -64));
-      const float unit = alpha * exp2i(max(E - e, -126));
-      m = mx;
-      E = e;
-      float sum = 0.f;
-      h16x8 pf[4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float p = exp2f_(s[j][k] - base);
-          sum += p;
-          pf[j / 2][4 * (j & 1) + k] = (_Float16)(p * fold);
-        }
-      l = l * alpha + sum;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        o[d] *= unit;
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          o[d] = Half<FB_DT_F16>::mfma16(
-              Half<FB_DT_F16>::decode(vf[d][x / 2][2 * (x & 1)], vf[d][x / 2][2 * (x & 1) + 1]),
-              pf[x], o[d]);
-        if (any_bad)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (bad[d][k] > 0.f) o[d][k] = __builtin_nanf("");
+        o[d] = F::mfma16(F::decode(vf[d][0], vf[d][1]), pf[0], o[d]);
+        o[d] = F::mfma16(F::decode(vf[d][2], vf[d][3]), pf[1], o[d]);
       }
+      if (more) load_v();
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
-    // the four waves' sums, in wave order
+    // the waves' sums, in wave order
     __syncthreads();
     if (q4 == 0) {
       wave_m[wave][r] = m;
@@ -310,20 +370,26 @@ __global__ __launch_bounds__(256) void attn_few_kernel(Attn a) {
     }
     if (lane == 0) wave_e[wave] = E;
     __syncthreads();
-    const int eM = max(max(wave_e[0], wave_e[1]), max(wave_e[2], wave_e[3]));
+    int eM = wave_e[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) eM = max(eM, wave_e[w]);
     const auto largest = [&](int rr) {
-      return fmaxf(fmaxf(wave_m[0][rr], wave_m[1][rr]), fmaxf(wave_m[2][rr], wave_m[3][rr]));
+      float x = wave_m[0][rr];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) x = fmaxf(x, wave_m[w][rr]);
+      return x;
     };
     const auto share = [&](int w, int rr, float M) {
       return M == -__builtin_inff() ? 0.f : exp2f_(wave_m[w][rr] - M);
     };
     const float mine = share(wave, r, largest(r)) * exp2i(max(E - eM, -126));
     // of the row that this thread writes
-    const int wr = threadIdx.x >> 4, wi = (tile + wr) / a.group;
+    constexpr int TR = 4 * NW, E8 = PASS / TR;  // threads of a row, channels of a thread
+    const int wr = threadIdx.x / TR, wi = (tile + wr) / a.group;
     const float M = largest(wr);
     float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) L += wave_l[w][wr] * share(w, wr, M);
+    for (int w = 0; w < NW; ++w) L += wave_l[w][wr] * share(w, wr, M);
     const bool writes = tile + wr < rows;
     const int64_t orow = (int64_t)(row0 + wi) * a.Hq + h * a.group + (tile + wr - wi * a.group);
     const float out_scale =
@@ -336,25 +402,29 @@ __global__ __launch_bounds__(256) void attn_few_kernel(Attn a) {
         *reinterpret_cast<f32x4*>(&join[wave][r][16 * d + 4 * q4]) =
             o[pass * (PASS / 16) + d] * mine;
       __syncthreads();
-      constexpr int E8 = PASS / 16;  // channels of a thread
+      const int dd = (threadIdx.x % TR) * E8, d = pass * PASS + dd;
+      float v[E8];
 #pragma unroll
-      for (int x = 0; x < E8; x += 4) {
-        const int dd = (threadIdx.x & 15) * E8 + x, d = pass * PASS + dd;
-        f32x4 v = *reinterpret_cast<const f32x4*>(&join[0][wr][dd]);
+      for (int x = 0; x < E8; ++x) {
+        v[x] = join[0][wr][dd + x];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(&join[w][wr][dd]);
-        v *= out_scale;
-        if (!writes || d >= c.D) continue;
-        if (a.splits > 1) {
-          *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * c.T * a.Hq + orow) * c.D + d) = v;
-        } else {
-          const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
-                        (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
-          *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + orow * c.D + d) = w;
-        }
+        for (int w = 1; w < NW; ++w) v[x] += join[w][wr][dd + x];
+        v[x] *= out_scale;
+      }
+      if (!writes || d >= D) continue;
+      if (a.splits > 1) {
+        float* const to = a.part + ((int64_t)split * c.T * a.Hq + orow) * D + d;
+#pragma unroll
+        for (int x = 0; x < E8; ++x) to[x] = v[x];
+      } else {
+        unsigned* const to = reinterpret_cast<unsigned*>(static_cast<unsigned short*>(a.out) +
+                                                         orow * D + d);
+#pragma unroll
+        for (int x = 0; x < E8; x += 2)
+          to[x / 2] = (unsigned)H::round(v[x]) | (unsigned)H::round(v[x + 1]) << 16;
       }
     }
-    if (writes && (threadIdx.x & 15) == 0) {
+    if (writes && threadIdx.x % TR == 0) {
       if (a.splits > 1)
         a.part_ml[(int64_t)split * c.T * a.Hq + orow] = float2{M, L};
       else if (a.lse)
@@ -365,23 +435,65 @@ __global__ __launch_bounds__(256) void attn_few_kernel(Attn a) {
 
 // ---------------------------------------------------------------------------------
 // Many rows (prompts).  Workgroup = (128 rows, head, sequence, split): wave w holds rows 32 w.. as
-// the columns of 32x32x16 products; 64 tokens at a time go through LDS as codes and are decoded by
-// each wave.
-//  - K operand row 8 a + 4 x + y: token 16 x + 4 a + y of the block, in this order in LDS.
+// the columns of 32x32x16 products.  64 tokens at a time go to LDS as codes, straight from memory
+// (no registers between), the next ones while these are worked on; each wave decodes its operands.
+//  - K operand row 8 a + 4 x + y: token 16 x + 4 a + y of the block, in this order in LDS, the
+//    16-byte pieces of a row exchanged by row number so that 8 rows' equal pieces lie in
+//    different banks.
 //  - a lane's scores are then tokens 16 (lane / 32) + i of the block, i < 16; V operand: channel
 //    32 d + lane % 32, tokens 16 (lane / 32) + 8 s..: one 16-byte side of the cache.
+//  - the sums are brought up to date as above.
 // ---------------------------------------------------------------------------------
 constexpr int kRows = 128, kTile = 64;
 
-template <int DT, int DP>
-__global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
+// Walks over the blocks of a sequence, two at a time; the table is read one step ahead.
+struct Walk {
+  int page, at, per;  // the first block: entry of the table, place in the page
+  int id[2];          // the two blocks' pages as the table has them
+  __device__ Walk(const Cache& c, int b, int block) : per(c.P / kBlock) {
+    page = block / per;
+    at = block - page * per;
+    read(c, b);
+  }
+  __device__ void read(const Cache& c, int b) {
+    const int32_t* const row = c.table + b * c.table_stride;
+    const int p = at + 1 >= per ? page + 1 : page;
+    id[0] = page < c.max_pages ? row[page] : 0;
+    id[1] = p < c.max_pages ? row[p] : 0;
+  }
+  __device__ void next(const Cache& c, int b) {
+    at += 2;
+    while (at >= per) {
+      at -= per;
+      ++page;
+    }
+    read(c, b);
+  }
+  // Index of the first (y = 0) or second block in the pool; any block where there is none.
+  __device__ int64_t index(const Cache& c, int h, int y) const {
+    const int a = at + y >= per ? at + y - per : at + y;
+    const int p =
+        __builtin_amdgcn_readfirstlane((unsigned)id[y] < (unsigned)c.pages ? id[y] : 0);
+    return c.block_index(p, h, a);
+  }
+};
+
+__device__ inline void load_to_lds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+template <int DT, int DP, bool EX>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a) {
   using H = Half<DT>;
-  constexpr int NP = DP / 32, ND = DP / 32, KROW = DP + 16;
-  constexpr int LK = kTile * DP / 16 / 256;  // 16-byte pieces a thread loads of each
-  __shared__ __align__(16) uint8_t lk[kTile * KROW], lv[kTile * DP];
-  __shared__ int lscale[2][2];
+  using F = Half<FB_DT_F16>;
+  constexpr int NP = DP / 32, ND = DP / 32, NPC = DP / 16;
+  constexpr int NI = NPC / 4;  // loads of a wave: 16 rows of K, one side of V
+  __shared__ __align__(16) uint8_t lk[2][kTile * DP], lv[2][kTile * DP];
   const Cache& c = a.c;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int D = EX ? DP : c.D;  // known: the loads' addresses differ by constants
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, x2 = lane >> 5;
   const int h = blockIdx.y, b = blockIdx.z / a.splits, split = blockIdx.z - b * a.splits;
   int row0, n;
@@ -389,6 +501,21 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
   const int len = min(max(c.lens[b], 0), c.capacity());
   const int rows = n * a.group;
   const int tiles = (rows + kRows - 1) / kRows;
+  const auto exchange = [](int row, int pc) {
+    return pc ^ (NPC == 4 ? (row >> 1) & 3 : row & 7);
+  };
+  // what a lane loads of a block: K rows 16 (wave % 2).., V side wave % 2.  Pieces past D are
+  // others of the same row: they meet zeros of q, or channels that are not written.
+  int k_from[NI], v_from[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int piece = i * 64 + lane;
+    const int rho = (wave & 1) * 16 + piece / NPC;
+    const int tok = ((rho & 4) << 2) | ((rho >> 1) & 12) | (rho & 3);
+    const int pc = exchange(rho, piece % NPC);
+    k_from[i] = tok * D + (pc * 16 < D ? pc : pc % (D / 16)) * 16;
+    v_from[i] = ((wave & 1) * D + min(piece, D - 1)) * 16;
+  }
   for (int ti = blockIdx.x; ti < tiles; ti += gridDim.x) {
     const int tile = (tiles - 1 - ti) * kRows;  // the longest first
     const int row = tile + wave * 32 + r, i = row / a.group;
@@ -399,8 +526,7 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
     const int i_lo = (tile + wave * 32) / a.group;
     const int least = min(max(len - n + i_lo + 1, 0), len);
     const int i_hi = (min(tile + wave * 32 + 32, rows) - 1) / a.group;
-    const int wave_most =
-        tile + wave * 32 < rows ? min(max(len - n + i_hi + 1, 0), len) : 0;
+    const int wave_most = tile + wave * 32 < rows ? min(max(len - n + i_hi + 1, 0), len) : 0;
     const int j_hi = (min(tile + kRows, rows) - 1) / a.group;
     const int most = min(max(len - n + j_hi + 1, 0), len);
     typename H::x8 qf[NP][2];
@@ -409,7 +535,7 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int d = 32 * p + 16 * x2 + 8 * u;
-        qf[p][u] = load_q<DT>(a, there && d < c.D,
+        qf[p][u] = load_q<DT>(a, there && d < D,
                               (int64_t)(row0 + i) * a.q_token + head * a.q_head + d);
       }
     f32x16 o[ND];
@@ -417,148 +543,154 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[d][k] = 0.f;
-    float m = -__builtin_inff(), l = 0.f;
-    int E = kMinExp;
+    float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
+    int E = kMinExp;                       // and their unit's exponent
 
     const int first = split * (a.split_tokens / kTile);
     const int all = (most + kTile - 1) / kTile;
     const int last = split + 1 == a.splits ? all : min(all, first + a.split_tokens / kTile);
-    u32x4 gk[LK], gv[LK];
-    int gs = 0;
-    const auto fetch = [&](int t) {
+    Walk walk(c, b, first * 2);
+    int scale_k[2], scale_v[2];  // of the tile that is on its way
+    const auto fetch = [&](int buf) {
+      const int64_t b0 = walk.index(c, h, 0), b1 = walk.index(c, h, 1);
+      const int64_t mine = (wave >> 1 ? b1 : b0) * kBlock * D;
 #pragma unroll
-      for (int x = 0; x < LK; ++x) {
-        gk[x] = gv[x] = u32x4{0, 0, 0, 0};
-        const int e = tid + 256 * x;
-        {
-          const int tok = e / (DP / 16), pc = e % (DP / 16);
-          int at;
-          const int page = max(c.page_of(b, t * 2 + tok / kBlock, at), 0);
-          if (t * kTile + tok < len && pc * 16 < c.D)
-            gk[x] = *reinterpret_cast<const u32x4*>(
-                c.k + (c.block_index(page, h, at) * kBlock + tok % kBlock) * c.D + pc * 16);
-        }
-        {
-          const int sub = e / DP, d = e % DP;
-          int at;
-          const int page = max(c.page_of(b, t * 2 + sub / 2, at), 0);
-          const int tok = t * kTile + sub * kSide;
-          if (tok < len && d < c.D) {
-            gv[x] = *reinterpret_cast<const u32x4*>(
-                c.v + c.block_index(page, h, at) * kBlock * c.D +
-                ((int64_t)(sub & 1) * c.D + d) * kSide);
-            if (tok + kSide > len)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) gv[x][w] &= keep_bytes(tok + 4 * w, len);
-          }
-        }
+      for (int k = 0; k < NI; ++k) {
+        load_to_lds(c.k + mine + k_from[k], lk[buf] + (wave * NI + k) * 1024);
+        load_to_lds(c.v + mine + v_from[k], lv[buf] + (wave * NI + k) * 1024);
       }
-      if (tid < 4) {
-        int at;
-        const int page = max(c.page_of(b, t * 2 + (tid & 1), at), 0);
-        const int64_t bi = c.block_index(page, h, at);
-        gs = (int)(tid < 2 ? c.ks : c.vs)[bi] - 127;
-      }
+      scale_k[0] = c.ks[b0];
+      scale_k[1] = c.ks[b1];
+      scale_v[0] = c.vs[b0];
+      scale_v[1] = c.vs[b1];
+      walk.next(c, b);
     };
-    if (first < last) fetch(first);
+    __syncthreads();  // the buffers of the row tile before are free
+    if (first < last) fetch(first & 1);
     for (int t = first; t < last; ++t) {
-      __syncthreads();
+      const int buf = t & 1;
+      __syncthreads();  // this tile has arrived; everyone is done with the other buffer
+      float ks[2];
+      int ev[2];
 #pragma unroll
-      for (int x = 0; x < LK; ++x) {
-        const int e = tid + 256 * x;
-        const int tok = e / (DP / 16), pc = e % (DP / 16);
-        const int w = tok % kBlock;
-        const int rho = ((w & 12) << 1) | ((w & 16) >> 2) | (w & 3);
-        *reinterpret_cast<u32x4*>(lk + ((tok & kBlock) + rho) * KROW + pc * 16) = gk[x];
-        *reinterpret_cast<u32x4*>(lv + e * 16) = gv[x];
+      for (int y = 0; y < 2; ++y) {
+        const int ek = __builtin_amdgcn_readfirstlane(scale_k[y]) - 127;
+        ks[y] = a.scale2 * exp2i(max(ek, -126));
+        ev[y] = t * kTile + y * kBlock < len
+                    ? max(__builtin_amdgcn_readfirstlane(scale_v[y]) - 127, -126)
+                    : kMinExp;
+        ev[y] = min(ev[y], 126);
       }
-      if (tid < 4) lscale[tid >> 1][tid & 1] = gs;
-      __syncthreads();
-      if (t + 1 < last) fetch(t + 1);
+      if (t + 1 < last) fetch(buf ^ 1);
       if (t * kTile >= wave_most) continue;  // the same for the wave; the barriers are above
+      const bool masked = t * kTile + kTile > least;  // the same for the wave
+      // tokens of the lane's part of the tile that its row sees, and that are held
+      const int seen = sees - t * kTile - x2 * 16, held = len - t * kTile - x2 * 16;
       f32x16 s[2];
-      float mx = m;
-      const bool masked = t * kTile + kTile > least;
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) s[y][k] = 0.f;
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-          const u32x4 w =
-              *reinterpret_cast<const u32x4*>(lk + (y * 32 + r) * KROW + p * 32 + x2 * 16);
+          const u32x4 w = *reinterpret_cast<const u32x4*>(
+              lk[buf] + ((y * 32 + r) * NPC + exchange(r, 2 * p + x2)) * 16);
           s[y] = H::mfma32(H::decode(w[0], w[1]), qf[p][0], s[y]);
           s[y] = H::mfma32(H::decode(w[2], w[3]), qf[p][1], s[y]);
         }
-        const float ks = a.scale2 * exp2i(min(max(lscale[0][y], -126), 127));
-        const int t0 = t * kTile + y * kBlock + x2 * 16;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          s[y][k] *= ks;
-          if (masked && t0 + k >= sees) s[y][k] = -__builtin_inff();
-          mx = fmaxf(mx, s[y][k]);
-        }
       }
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const int ev0 = min(max(lscale[1][0], -126), 126);
-      const int ev1 = t * kTile + kBlock < len ? min(max(lscale[1][1], -126), 126) : kMinExp;
-      const int e = max(E, max(ev0, ev1));
-      const float base = mx == -__builtin_inff() ? 0.f : mx;
-      const float alpha = exp2f_(m - base);
-      const float unit = alpha * exp2i(max(E - e, -126));
-      m = mx;
-      E = e;
-      float sum = 0.f;
+      if (masked) {
+        asm volatile("");  // a branch, not selects in every tile
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (y * kBlock + k >= seen) s[y][k] = -__builtin_inff();
+      }
+      float mx[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        mx[y] = s[y][0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) mx[y] = fmaxf(mx[y], s[y][k]);
+      }
+      float big = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);  // the scales are positive
+      big = fmaxf(big, __shfl_xor(big, 32));
+      const int e = max(E, max(ev[0], ev[1]));
+      if (e > E || __any(big > m + kSlack)) {
+        const float up = fmaxf(m, big);
+        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
+        const float unit = alpha * exp2i(max(E - e, -126));
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= unit;
+        m = up;
+        E = e;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
       h16x8 pf[2][2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const float fold = exp2i(max((y ? ev1 : ev0) - e, -64));
+        // the value block's scale joins in the exponent and leaves the sum again
+        const int fold = max(ev[y] - E, -64);
+        const float shift = (float)fold - base;
+        float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float p = exp2f_(s[y][k] - base);
+          const float p = exp2f_(__builtin_fmaf(s[y][k], ks[y], shift));
           sum += p;
-          pf[y][k / 8][k & 7] = (_Float16)(p * fold);
+          pf[y][k / 8][k & 7] = (_Float16)p;
         }
+        l = __builtin_fmaf(sum, exp2i(-fold), l);
       }
-      l = l * alpha + sum;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        o[d] *= unit;
-        f32x16 bad;
-        bool any_bad = false;
+        u32x4 w[2];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          u32x4 w = *reinterpret_cast<const u32x4*>(lv + ((2 * y + x2) * DP + 32 * d + r) * 16);
-          if (masked) {
-            const unsigned nan = nan_bytes(w[0]) | nan_bytes(w[1]) | nan_bytes(w[2]) |
-                                 nan_bytes(w[3]);
-            if (__any(nan != 0)) {
-              // a NaN value reaches the rows that see its token, and no others
-              if (!any_bad)
+        for (int y = 0; y < 2; ++y)
+          w[y] = *reinterpret_cast<const u32x4*>(lv[buf] + ((2 * y + x2) * DP + 32 * d + r) * 16);
+        if (masked) {
+          asm volatile("");
+          unsigned nan = 0;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) bad[k] = 0.f;
-              any_bad = true;
-              const int t0 = t * kTile + y * kBlock + x2 * 16;
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              // what lies behind the end may be anything
+              w[y][u] &= keep_bytes(y * kBlock + 4 * u, held);
+              nan |= nan_bytes(w[y][u]);
+            }
+          if (__any(nan != 0)) {
+            // a NaN value reaches the rows that see its token, and no others: 0 * NaN must not
+            // come up, so those channels are marked apart
+            f32x16 bad;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) bad[k] = 0.f;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 h16x8 see;
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                  see[k] = t0 + 8 * u + k < sees ? (_Float16)1 : (_Float16)0;
-                bad = Half<FB_DT_F16>::mfma32(
-                    Half<FB_DT_F16>::decode(nan_ones(w[2 * u]), nan_ones(w[2 * u + 1])), see, bad);
+                  see[k] = y * kBlock + 8 * u + k < seen ? (_Float16)1 : (_Float16)0;
+                bad = F::mfma32(F::decode(nan_ones(w[y][2 * u]), nan_ones(w[y][2 * u + 1])), see,
+                                bad);
               }
 #pragma unroll
-              for (int u = 0; u < 4; ++u) w[u] &= ~nan_bytes(w[u]);
-            }
-          }
-          o[d] = Half<FB_DT_F16>::mfma32(Half<FB_DT_F16>::decode(w[0], w[1]), pf[y][0], o[d]);
-          o[d] = Half<FB_DT_F16>::mfma32(Half<FB_DT_F16>::decode(w[2], w[3]), pf[y][1], o[d]);
-        }
-        if (any_bad)
+            for (int k = 0; k < 16; ++k)
+              if (bad[k] > 0.f) o[d][k] = __builtin_nanf("");
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (bad[k] > 0.f) o[d][k] = __builtin_nanf("");
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) w[y][u] &= ~nan_bytes(w[y][u]);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          o[d] = F::mfma32(F::decode(w[y][0], w[y][1]), pf[y][0], o[d]);
+          o[d] = F::mfma32(F::decode(w[y][2], w[y][3]), pf[y][1], o[d]);
+        }
       }
     }
     l += __shfl_xor(l, 32);
@@ -571,14 +703,14 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
 #pragma unroll
         for (int k = 0; k < 16; k += 4) {
           const int ch = 32 * d + 2 * k + 4 * x2;
-          if (ch >= c.D) continue;
+          if (ch >= D) continue;
           const f32x4 v = f32x4{o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]} * unit;
           if (a.splits > 1) {
-            *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * c.T * a.Hq + orow) * c.D + ch) = v;
+            *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * c.T * a.Hq + orow) * D + ch) = v;
           } else {
             const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
                           (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
-            *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + orow * c.D + ch) = w;
+            *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + orow * D + ch) = w;
           }
         }
       if (x2 == 0) {
@@ -591,32 +723,48 @@ __global__ __launch_bounds__(256, 2) void attn_many_kernel(Attn a) {
   }
 }
 
-// The splits' sums of a row, in order.  One wave a row.
+// The splits' sums of the rows, in a fixed order.  D / 4 threads go over every `ways`-th split of a
+// row, and the first of these groups adds up what the others found.
 template <int DT>
-__global__ __launch_bounds__(256) void attn_join_kernel(Attn a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int ways) {
+  using H = Half<DT>;
+  __shared__ f32x4 part_v[256];
+  __shared__ float part_l[64];
+  const int width = a.c.D / 4, groups = 256 / width / ways * ways;
+  const int g = threadIdx.x / width, d = (threadIdx.x - g * width) * 4, way = g % ways;
   const int64_t rows = (int64_t)a.c.T * a.Hq;
-  if (row >= rows) return;
+  const int64_t row = (int64_t)blockIdx.x * (groups / ways) + g / ways;
+  const bool works = g < groups && row < rows;
   float M = -__builtin_inff(), L = 0.f;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[s * rows + row].x);
-  const int d = lane * 4;
   f32x4 v{0, 0, 0, 0};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[s * rows + row];
-    if (ml.y == 0.f) continue;
-    const float f = exp2f_(ml.x - M);
-    L += ml.y * f;
-    if (d < a.c.D) v += *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * a.c.D + d) * f;
+  if (works) {
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[s * rows + row].x);
+#pragma unroll 4
+    for (int s = way; s < a.splits; s += ways) {
+      const float2 ml = a.part_ml[s * rows + row];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * a.c.D + d);
+      const float f = ml.y == 0.f ? 0.f : exp2f_(ml.x - M);
+      L += ml.y * f;
+      v += x * f;
+    }
   }
+  if (ways > 1) {
+    part_v[threadIdx.x] = v;
+    if (d == 0 && g < 64) part_l[g] = L;
+    __syncthreads();
+    if (works && way == 0)
+      for (int w = 1; w < ways; ++w) {
+        v += part_v[threadIdx.x + w * width];
+        L += part_l[g + w];
+      }
+  }
+  if (!works || way) return;
   v *= L == 0.f ? 0.f : 1.f / L;
-  if (d < a.c.D) {
-    using H = Half<DT>;
-    const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
-                  (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
-    *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + row * a.c.D + d) = w;
-  }
-  if (lane == 0 && a.lse)
+  const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
+                (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
+  *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + row * a.c.D + d) = w;
+  if (d == 0 && a.lse)
     a.lse[row] = L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * kLn2;
 }
 
@@ -625,20 +773,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Attn a) {
 // tokens, head, sequence), each wave holds 32 tokens' keys as operands and walks over the rows
 // that see them, so that every sum belongs to one wave and is added in row order.
 // ---------------------------------------------------------------------------------
+struct Weights {
+  float* to;
+  int64_t seq, head;
+  int tokens;
+};
+
 template <int DT, int DP>
-__global__ __launch_bounds__(256) void attn_weights_kernel(Attn a, float* weights, int64_t w_seq,
-                                                           int64_t w_head, int w_tokens) {
+__device__ void add_weights(const Attn& a, const Weights& w, int b, int h, int row0, int n,
+                            int len) {
   using H = Half<DT>;
   constexpr int NP = DP / 32;
   const Cache& c = a.c;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, x2 = lane >> 5;
-  const int h = blockIdx.y, b = blockIdx.z;
-  int row0, n;
-  c.rows(b, row0, n);
-  const int len = min(max(c.lens[b], 0), c.capacity());
   const int rows = n * a.group;
-  const int end = min(len, w_tokens);
+  const int end = min(len, w.tokens);
   for (int blk = blockIdx.x * 4 + wave; blk * kBlock < end; blk += gridDim.x * 4) {
     int at;
     const int page = max(c.page_of(b, blk, at), 0);
@@ -685,22 +835,50 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(Attn a, float* weight
 #pragma unroll
       for (int o = 16; o; o >>= 1) v += __shfl_xor(v, o);
       const int t = blk * kBlock + 8 * (k / 4) + 4 * x2 + k % 4;
-      if (r == k && t < end) weights[b * w_seq + h * w_head + t] += v;
+      if (r == k && t < end) w.to[b * w.seq + h * w.head + t] += v;
     }
   }
+}
+
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void attn_weights_kernel(Attn a, Weights w) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  int row0, n;
+  a.c.rows(b, row0, n);
+  const int len = min(max(a.c.lens[b], 0), a.c.capacity());
+  if (a.scores && n * a.group <= a.score_rows) {
+    // few rows: their scores were written down
+    const int end = min(len, w.tokens), rows = n * a.group;
+    const float* const s0 =
+        a.scores + ((int64_t)b * a.c.H + h) * a.score_rows * a.score_tokens;
+    float* const to = w.to + b * w.seq + h * w.head;
+    for (int t = blockIdx.x * 256 + threadIdx.x; t < end; t += gridDim.x * 256) {
+      float sum = 0.f;
+      for (int row = 0; row < rows; ++row) {
+        const int i = row / a.group;
+        const float lse = a.lse[(int64_t)(row0 + i) * a.Hq + h * a.group + (row - i * a.group)];
+        const float s = s0[(int64_t)row * a.score_tokens + t];
+        if (t < len - n + i + 1) sum += exp2f_(s - lse * kLog2e);
+      }
+      to[t] += sum;
+    }
+    return;
+  }
+  add_weights<DT, DP>(a, w, b, h, row0, n, len);
 }
 
 // ------------------------------------------------------------------ host side
 struct Plan {
   bool few;
-  int splits, split_tokens;
-  size_t part, total;
+  int splits, split_tokens, ways;  // ways: of attn_join_kernel
+  int score_rows, score_tokens;
+  size_t part, ml, total;
 };
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // How a call is split.  It goes by host numbers alone, so that a captured call fits any lengths.
-Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads) {
+Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   Plan p{};
   const int group = q_heads / c->heads;
   const int64_t rows = (int64_t)std::max(1, std::min(s->max_new, s->tokens)) * group;
@@ -709,16 +887,25 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads) {
   const int64_t len = std::max<int64_t>(1, std::min<int64_t>(s->max_len, capacity));
   const int64_t tiles = p.few ? 1 : (rows + kRows - 1) / kRows;
   const int64_t units = tiles * c->heads * s->seqs;
-  const int step = p.few ? 4 * kChunk : 4 * kTile;
+  const int step = p.few ? 1024 : 4 * kTile;
   const int64_t most = (len + step - 1) / step;
-  const int64_t want = std::max<int64_t>(1, 4 * (int64_t)fb_gpu::cu_count() / units);
+  const int64_t want =
+      std::max<int64_t>(1, (p.few ? 4 : 2) * (int64_t)fb_gpu::cu_count() / units);
   const int64_t per = (most + std::min(want, most) - 1) / std::min(want, most);
   p.split_tokens = (int)(per * step);
   p.splits = (int)((most + per - 1) / per);
   const size_t n = (size_t)s->tokens * q_heads;
   if (p.splits > 1) {
     p.part = align256((size_t)p.splits * n * c->head_dim * 4);
-    p.total = p.part + align256((size_t)p.splits * n * 8);
+    p.ml = align256((size_t)p.splits * n * 8);
+    // about 4 splits a thread
+    for (p.ways = 1; p.ways * 4 < p.splits && p.ways * 2 * (c->head_dim / 4) <= 256;) p.ways *= 2;
+  }
+  p.total = p.part + p.ml;
+  if (p.few && w_tokens > 0) {
+    p.score_rows = (int)rows;
+    p.score_tokens = (w_tokens + kChunk - 1) / kChunk * kChunk;
+    p.total += align256((size_t)s->seqs * c->heads * p.score_rows * p.score_tokens * 4);
   }
   return p;
 }
@@ -732,30 +919,32 @@ int check_attention(const fb_cache_t* c, const fb_seqs_t* s, int32_t q_heads, Ca
   return FB_OK;
 }
 
-template <int DT, int DP>
-int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, float* weights, int64_t w_seq,
-           int64_t w_head, int w_tokens, hipStream_t hs) {
+template <int DT, int DP, bool EX>
+int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, const Weights& w, hipStream_t hs) {
   const int64_t rows = (int64_t)std::min(s->max_new, s->tokens) * a.group;
   if (p.few) {
-    hipLaunchKernelGGL((attn_few_kernel<DT, DP>), dim3(p.splits, a.c.H, a.c.B), dim3(256), 0, hs, a);
+    hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, a.c.B),
+                       dim3(64 * few_waves<DP>()), 0, hs, a);
   } else {
     if ((int64_t)p.splits * a.c.B > 65535) return FB_ERR_SHAPE;
-    hipLaunchKernelGGL((attn_many_kernel<DT, DP>),
+    hipLaunchKernelGGL((attn_many_kernel<DT, DP, EX>),
                        dim3((unsigned)((rows + kRows - 1) / kRows), a.c.H, a.c.B * p.splits),
                        dim3(256), 0, hs, a);
   }
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   if (p.splits > 1) {
     const int64_t n = (int64_t)a.c.T * a.Hq;
-    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, hs, a);
+    const int64_t rows = 256 / (a.c.D / 4) / p.ways;  // of a workgroup
+    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)((n + rows - 1) / rows)), dim3(256), 0,
+                       hs, a, p.ways);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
-  if (weights) {
-    const int64_t cap = std::min<int64_t>((int64_t)a.c.max_pages * a.c.P, w_tokens);
+  if (w.to) {
+    const int64_t cap = std::min<int64_t>((int64_t)a.c.max_pages * a.c.P, w.tokens);
     const int64_t len = std::max<int64_t>(1, std::min<int64_t>(cap, s->max_len));
-    const int64_t nx = std::min<int64_t>((len + 127) / 128, 1 << 20);
+    const int64_t nx = (len + (a.scores ? 255 : 127)) / (a.scores ? 256 : 128);
     hipLaunchKernelGGL((attn_weights_kernel<DT, DP>), dim3((unsigned)nx, a.c.H, a.c.B), dim3(256), 0,
-                       hs, a, weights, w_seq, w_head, w_tokens);
+                       hs, a, w);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
   return FB_OK;
@@ -766,10 +955,10 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, float* weights, int
 extern "C" {
 
 size_t fb_cache_attention_workspace_bytes(const fb_cache_t* c, const fb_seqs_t* s,
-                                          int32_t q_heads) {
+                                          int32_t q_heads, int32_t w_tokens) {
   Cache k;
   if (check_attention(c, s, q_heads, k) != FB_OK) return 0;
-  return plan(c, s, q_heads).total;
+  return plan(c, s, q_heads, w_tokens).total;
 }
 
 int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, int64_t q_token,
@@ -780,6 +969,7 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   const int st = check_attention(c, s, q_heads, a.c);
   if (st != FB_OK) return st;
   if (dtype != FB_DT_F16 && dtype != FB_DT_BF16) return FB_ERR_DTYPE;
+  if (!(scale > 0.f) || !(scale < 1e30f)) return FB_ERR_VALUE;
   if (s->tokens == 0 || s->max_new == 0) return FB_OK;
   if (!q || !out || (weights && !lse)) return FB_ERR_NULL;
   if (weights && w_tokens < 1) return FB_ERR_SHAPE;
@@ -787,7 +977,7 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
       (reinterpret_cast<uintptr_t>(lse) & 3u) || (reinterpret_cast<uintptr_t>(weights) & 3u) ||
       (reinterpret_cast<uintptr_t>(ws) & 255u))
     return FB_ERR_ALIGN;
-  const Plan p = plan(c, s, q_heads);
+  const Plan p = plan(c, s, q_heads, weights ? w_tokens : 0);
   if (p.total && !ws) return FB_ERR_NULL;
   if (p.total > ws_bytes) return FB_ERR_WORKSPACE;
   a.q = q;
@@ -804,18 +994,32 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   a.split_tokens = p.split_tokens;
   a.part = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.part);
-  const int dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  const int per = c->page / kBlock;
+  a.per_shift = per & (per - 1) ? -1 : __builtin_ctz(per);
+  if (p.score_rows) {
+    a.scores = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part + p.ml);
+    a.score_rows = p.score_rows;
+    a.score_tokens = p.score_tokens;
+  }
+  const Weights w{weights, w_seq, w_head, w_tokens};
   hipStream_t hs = static_cast<hipStream_t>(stream);
-  const auto go = [&](auto kernel) {
-    return kernel(a, p, s, weights, w_seq, w_head, w_tokens, hs);
+  const auto go = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    switch (c->head_dim) {
+      case 64:
+        return launch<DT, 64, true>(a, p, s, w, hs);
+      case 128:
+        return launch<DT, 128, true>(a, p, s, w, hs);
+      case 256:
+        return launch<DT, 256, true>(a, p, s, w, hs);
+      default:
+        return c->head_dim < 64    ? launch<DT, 64, false>(a, p, s, w, hs)
+               : c->head_dim < 128 ? launch<DT, 128, false>(a, p, s, w, hs)
+                                   : launch<DT, 256, false>(a, p, s, w, hs);
+    }
   };
-  if (dtype == FB_DT_F16)
-    return dp == 64    ? go(launch<FB_DT_F16, 64>)
-           : dp == 128 ? go(launch<FB_DT_F16, 128>)
-                       : go(launch<FB_DT_F16, 256>);
-  return dp == 64    ? go(launch<FB_DT_BF16, 64>)
-         : dp == 128 ? go(launch<FB_DT_BF16, 128>)
-                     : go(launch<FB_DT_BF16, 256>);
+  return dtype == FB_DT_F16 ? go(std::integral_constant<int, FB_DT_F16>{})
+                            : go(std::integral_constant<int, FB_DT_BF16>{});
 }
 
 }  // extern "C"

@@ -379,6 +379,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
        "the query heads must be a multiple of the cache's heads");
   want(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
        "q must be float16 or bfloat16");
+  want(!scale || (*scale > 0 && *scale < 1e30), "scale must be positive");
   const fb_seqs_t s = seqs_of(table, lens, cu, q.size(0), max_new, max_len, c.page, ck);
   float* wp = nullptr;
   if (weights) {
@@ -397,7 +398,8 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse;
   if (want_lse || wp) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
-  const size_t need = fb_cache_attention_workspace_bytes(&c, &s, (int32_t)q.size(1));
+  const size_t need = fb_cache_attention_workspace_bytes(
+      &c, &s, (int32_t)q.size(1), wp ? (int32_t)weights->size(2) : 0);
   const at::Tensor ws = need ? scratch(need, q) : at::Tensor();
   check(fb_cache_attention(
       &c, &s, q.data_ptr(), q.stride(0), q.stride(1), (int32_t)q.size(1),

@@ -481,6 +481,7 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
 /* Attention of q [tokens, q_heads, D] over the cache: q_heads is a multiple of the cache's
  * heads, and query head j reads cache head j / (q_heads / heads).  lens: the tokens held, the
  * new ones among them; row i of a sequence's n new rows sees the first lens - n + i + 1 tokens.
+ * scale is positive (FB_ERR_VALUE).
  *   q      FB_DT_F16 or BF16; strides in elements, the last dimension contiguous
  *   out    [tokens, q_heads, D] of q's dtype, contiguous, 16-byte aligned: softmax(scale * q.k) v
  *   lse    fp32 [tokens, q_heads] or NULL: log of the sum of exp(scale * q.k)
@@ -495,9 +496,10 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
                        int64_t q_head, int32_t q_heads, int32_t dtype, float scale, void* out,
                        float* lse, float* weights, int64_t w_seq, int64_t w_head,
                        int32_t w_tokens, void* ws, size_t ws_bytes, void* stream);
-/* Workspace of that call (0 where it needs none, and for invalid arguments). */
+/* Workspace of that call (0 where it needs none, and for invalid arguments); w_tokens: 0 without
+ * weights. */
 size_t fb_cache_attention_workspace_bytes(const fb_cache_t* c, const fb_seqs_t* s,
-                                          int32_t q_heads);
+                                          int32_t q_heads, int32_t w_tokens);
 
 /* Cuts every sequence (and head for itself) to `keep` tokens: its last `recent` ones and, of the
  * others, those of largest weight (ties: the earlier token; NaN counts as less than any number).

@@ -44,7 +44,7 @@ def test_cache_and_sequences(i):
     assert L.fb_cache_attention(r(c), r(s), P, 256, 64, 4, 0, 1.0, P, P, None, 0, 0, 0, P, 0,
                                 None) == rc
     assert L.fb_cache_evict(r(c), r(s), P, 200, 100, 100, 8, 2, P, 1, 1, P, P, P, None) == rc
-    assert L.fb_cache_attention_workspace_bytes(r(c), r(s), 4) == 0
+    assert L.fb_cache_attention_workspace_bytes(r(c), r(s), 4, 0) == 0
 
 
 def test_append():
@@ -75,7 +75,7 @@ def test_attention():
     assert rc(w=P + 1, wt=9) == ALIGN and rc(ws=P + 16) == ALIGN
     assert rc(s=_seqs(cu=P, tokens=0), q=None) == 0
     long = _seqs(max_pages=10000, table_stride=10000, max_len=500000)
-    need = L.fb_cache_attention_workspace_bytes(r(c), r(long), 4)
+    need = L.fb_cache_attention_workspace_bytes(r(c), r(long), 4, 0)
     assert need > 0
     assert rc(s=long, ws=None) == NULL and rc(s=long, nb=need - 1) == WORKSPACE
 
