@@ -141,7 +141,9 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //    to date only when a score passes it by more than 2^kSlack, which is rare after the first.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
-constexpr float kSlack = 8.f;  // weights up to 2^8 in fp16
+constexpr float kSlack = 8.f;
+// Weights enter the products as fp16 times 2^kLift, up to 2^15 in all: small ones keep their bits.
+constexpr int kLift = 7;
 
 template <int DP>
 constexpr int few_waves() {
@@ -309,7 +311,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
       const float base = m == -__builtin_inff() ? 0.f : m;
       // the value block's scale joins in the exponent and leaves the sum again
       const int fold = max(ev - E, -64);
-      const float shift = (float)fold - base;
+      const float shift = (float)(fold + kLift) - base;
       float sum = 0.f;
       h16x8 pf[2];
 #pragma unroll
@@ -320,7 +322,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
           sum += p;
           pf[j / 2][4 * (j & 1) + k] = (_Float16)p;
         }
-      l = __builtin_fmaf(sum, exp2i(-fold), l);
+      l = __builtin_fmaf(sum, exp2i(-fold - kLift), l);
       if (masked) {
         asm volatile("");
         unsigned nan = 0;
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
     const bool writes = tile + wr < rows;
     const int64_t orow = (int64_t)(row0 + wi) * a.Hq + h * a.group + (tile + wr - wi * a.group);
     const float out_scale =
-        exp2i(min(max(eM, -126), 127)) * (a.splits == 1 ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
+        exp2i(min(max(eM - kLift, -126), 127)) * (a.splits == 1 ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
 #pragma unroll
     for (int pass = 0; pass < DP / PASS; ++pass) {
       if (pass) __syncthreads();
@@ -443,6 +445,8 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
 //  - a lane's scores are then tokens 16 (lane / 32) + i of the block, i < 16; V operand: channel
 //    32 d + lane % 32, tokens 16 (lane / 32) + 8 s..: one 16-byte side of the cache.
 //  - the sums are brought up to date as above.
+// Heads and sequences vary fastest over the workgroups, then the tiles, the longest first: the
+// last ones to start are short, and where the heads are a multiple of 8 one XCD's L2 holds few.
 // ---------------------------------------------------------------------------------
 constexpr int kRows = 128, kTile = 64;
 
@@ -495,7 +499,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, x2 = lane >> 5;
-  const int h = blockIdx.y, b = blockIdx.z / a.splits, split = blockIdx.z - b * a.splits;
+  const int h = blockIdx.x % c.H, bs = blockIdx.x / c.H;
+  const int b = bs / a.splits, split = bs - b * a.splits;
   int row0, n;
   c.rows(b, row0, n);
   const int len = min(max(c.lens[b], 0), c.capacity());
@@ -516,7 +521,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
     k_from[i] = tok * D + (pc * 16 < D ? pc : pc % (D / 16)) * 16;
     v_from[i] = ((wave & 1) * D + min(piece, D - 1)) * 16;
   }
-  for (int ti = blockIdx.x; ti < tiles; ti += gridDim.x) {
+  for (int ti = blockIdx.y; ti < tiles; ti += gridDim.y) {
     const int tile = (tiles - 1 - ti) * kRows;  // the longest first
     const int row = tile + wave * 32 + r, i = row / a.group;
     const bool there = row < rows;
@@ -575,7 +580,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int ek = __builtin_amdgcn_readfirstlane(scale_k[y]) - 127;
-        ks[y] = a.scale2 * exp2i(max(ek, -126));
+        ks[y] = a.scale2 * exp2i(min(max(ek, -126), 127));
         ev[y] = t * kTile + y * kBlock < len
                     ? max(__builtin_amdgcn_readfirstlane(scale_v[y]) - 127, -126)
                     : kMinExp;
@@ -633,7 +638,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
       for (int y = 0; y < 2; ++y) {
         // the value block's scale joins in the exponent and leaves the sum again
         const int fold = max(ev[y] - E, -64);
-        const float shift = (float)fold - base;
+        const float shift = (float)(fold + kLift) - base;
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -641,7 +646,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           sum += p;
           pf[y][k / 8][k & 7] = (_Float16)p;
         }
-        l = __builtin_fmaf(sum, exp2i(-fold), l);
+        l = __builtin_fmaf(sum, exp2i(-fold - kLift), l);
       }
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
@@ -696,7 +701,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
     l += __shfl_xor(l, 32);
     if (there) {
       const int64_t orow = (int64_t)(row0 + i) * a.Hq + head;
-      const float unit = exp2i(min(max(E, -126), 127)) *
+      const float unit = exp2i(min(max(E - kLift, -126), 127)) *
                          (a.splits == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
@@ -926,10 +931,11 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, const Weights& w, h
     hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, a.c.B),
                        dim3(64 * few_waves<DP>()), 0, hs, a);
   } else {
-    if ((int64_t)p.splits * a.c.B > 65535) return FB_ERR_SHAPE;
-    hipLaunchKernelGGL((attn_many_kernel<DT, DP, EX>),
-                       dim3((unsigned)((rows + kRows - 1) / kRows), a.c.H, a.c.B * p.splits),
-                       dim3(256), 0, hs, a);
+    const int64_t nx = (int64_t)a.c.H * a.c.B * p.splits;
+    if (nx > INT32_MAX) return FB_ERR_SHAPE;
+    const int64_t ny = std::min<int64_t>((rows + kRows - 1) / kRows, 65535);
+    hipLaunchKernelGGL((attn_many_kernel<DT, DP, EX>), dim3((unsigned)nx, (unsigned)ny), dim3(256),
+                       0, hs, a);
   }
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   if (p.splits > 1) {
