@@ -137,13 +137,15 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //  - K operand row r of product j: token 16 (r / 4) + 4 j + r % 4, channels 64 p + 16 q + 8 u.. of
 //    lane group q: then a lane's scores are the tokens of side q, 4 j + i.
 //  - V operand: channel 16 d + r, tokens 8 s.. of side q, which lie side by side.
-//  - the sums are kept relative to a row's largest score of some earlier time, and are brought up
-//    to date only when a score passes it by more than 2^kSlack, which is rare after the first.
+//  - the sums are kept relative to a row's largest score of some earlier time.  It is looked for
+//    again only where the weights relative to it become too large, which their sum tells: rare
+//    after the first tile, and no maximum is taken in the others.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
-constexpr float kSlack = 8.f;
-// Weights enter the products as fp16 times 2^kLift, up to 2^15 in all: small ones keep their bits.
+// Weights enter the products as fp16 times 2^kLift, so that small ones keep their bits.
 constexpr int kLift = 7;
+// A tile's sum of them that asks for the row's largest score anew: none is above fp16's range.
+constexpr float kMost = 32768.f;
 
 template <int DP>
 constexpr int few_waves() {
@@ -194,6 +196,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
     int E = kMinExp;                       // and their unit's exponent
+    unsigned dead[(ND + 7) / 8] = {};      // bit 4 (d % 8) + k of d / 8: o[d][k] saw a NaN value
 
     const int all = (len + kChunk - 1) / kChunk;
     const int first = min(all, split * (a.split_tokens / kChunk));
@@ -286,42 +289,52 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
 #pragma unroll
         for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(to + 4 * j) = s[j] * ks;
       }
-      float big = s[0][0];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) big = fmaxf(big, s[j][k]);
-      big *= ks;  // positive
-      big = fmaxf(big, __shfl_xor(big, 16));
-      big = fmaxf(big, __shfl_xor(big, 32));
       // of the lane's block, where it is held
       const bool block_held = !masked || ch * kChunk + (q4 >> 1) * kBlock < len;
       const int ev = block_held ? min(max(sv - 127, -126), 126) : kMinExp;
-      const int e = max(E, max(ev, __shfl_xor(ev, 32)));
-      if (__any(e > E || big > m + kSlack)) {
-        const float up = fmaxf(m, big);
-        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
-        const float unit = alpha * exp2i(max(E - e, -126));
-        l *= alpha;
+      const int e = max(ev, __shfl_xor(ev, 32));
+      if (__any(e > E)) {  // the same for the wave
+        asm volatile("");
+        const float unit = exp2i(max(E - e, -126));
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= unit;
-        m = up;
         E = e;
       }
-      const float base = m == -__builtin_inff() ? 0.f : m;
       // the value block's scale joins in the exponent and leaves the sum again
       const int fold = max(ev - E, -64);
-      const float shift = (float)(fold + kLift) - base;
-      float sum = 0.f;
+      float sum;
       h16x8 pf[2];
+      const auto weigh = [&]() __attribute__((always_inline)) {
+        const float shift = (float)(fold + kLift) - (m == -__builtin_inff() ? 0.f : m);
+        sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float p = exp2f_(__builtin_fmaf(s[j][k], ks, shift));
-          sum += p;
-          pf[j / 2][4 * (j & 1) + k] = (_Float16)p;
-        }
+          for (int k = 0; k < 4; ++k) {
+            const float p = exp2f_(__builtin_fmaf(s[j][k], ks, shift));
+            sum += p;
+            pf[j / 2][4 * (j & 1) + k] = (_Float16)p;
+          }
+      };
+      weigh();
+      if (__any(m == -__builtin_inff() || sum > kMost)) {
+        asm volatile("");
+        float big = s[0][0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) big = fmaxf(big, s[j][k]);
+        big *= ks;  // positive
+        big = fmaxf(big, __shfl_xor(big, 16));
+        big = fmaxf(big, __shfl_xor(big, 32));
+        const float up = fmaxf(m, big);
+        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= alpha;
+        m = up;
+        weigh();
+      }
       l = __builtin_fmaf(sum, exp2i(-fold - kLift), l);
       if (masked) {
         asm volatile("");
@@ -348,7 +361,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
                               see[x], bad);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (bad[k] > 0.f) o[d][k] = __builtin_nanf("");
+              if (bad[k] > 0.f) dead[d / 8] |= 1u << (4 * (d & 7) + k);
 #pragma unroll
             for (int w = 0; w < 4; ++w) vf[d][w] &= ~nan_bytes(vf[d][w]);
           }
@@ -363,6 +376,11 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (dead[d / 8] >> (4 * (d & 7) + k) & 1) o[d][k] = __builtin_nanf("");
 
     // the waves' sums, in wave order
     __syncthreads();
@@ -437,11 +455,13 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
 
 // ---------------------------------------------------------------------------------
 // Many rows (prompts).  Workgroup = (128 rows, head, sequence, split): wave w holds rows 32 w.. as
-// the columns of 32x32x16 products.  64 tokens at a time go to LDS as codes, straight from memory
-// (no registers between), the next ones while these are worked on; each wave decodes its operands.
+// the columns of 32x32x16 products.  128 tokens at a time go to LDS as codes, straight from memory
+// (no registers between), the next ones while these are worked on, 64 at a time; each wave decodes
+// its operands.
 //  - K operand row 8 a + 4 x + y: token 16 x + 4 a + y of the block, in this order in LDS, the
-//    16-byte pieces of a row exchanged by row number so that 8 rows' equal pieces lie in
-//    different banks.
+//    16-byte pieces of a row exchanged by row number: a 16-byte LDS read serves lanes 0-3, 12-15,
+//    20-27 together (and 4-11, 16-19, 28-31), and these rows' equal pieces then lie in different
+//    banks.
 //  - a lane's scores are then tokens 16 (lane / 32) + i of the block, i < 16; V operand: channel
 //    32 d + lane % 32, tokens 16 (lane / 32) + 8 s..: one 16-byte side of the cache.
 //  - the sums are brought up to date as above.
@@ -450,37 +470,11 @@ __global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) 
 // ---------------------------------------------------------------------------------
 constexpr int kRows = 128, kTile = 64;
 
-// Walks over the blocks of a sequence, two at a time; the table is read one step ahead.
-struct Walk {
-  int page, at, per;  // the first block: entry of the table, place in the page
-  int id[2];          // the two blocks' pages as the table has them
-  __device__ Walk(const Cache& c, int b, int block) : per(c.P / kBlock) {
-    page = block / per;
-    at = block - page * per;
-    read(c, b);
-  }
-  __device__ void read(const Cache& c, int b) {
-    const int32_t* const row = c.table + b * c.table_stride;
-    const int p = at + 1 >= per ? page + 1 : page;
-    id[0] = page < c.max_pages ? row[page] : 0;
-    id[1] = p < c.max_pages ? row[p] : 0;
-  }
-  __device__ void next(const Cache& c, int b) {
-    at += 2;
-    while (at >= per) {
-      at -= per;
-      ++page;
-    }
-    read(c, b);
-  }
-  // Index of the first (y = 0) or second block in the pool; any block where there is none.
-  __device__ int64_t index(const Cache& c, int h, int y) const {
-    const int a = at + y >= per ? at + y - per : at + y;
-    const int p =
-        __builtin_amdgcn_readfirstlane((unsigned)id[y] < (unsigned)c.pages ? id[y] : 0);
-    return c.block_index(p, h, a);
-  }
-};
+// Tokens that are staged at once: a barrier for each, so two tiles where LDS has room for it.
+template <int DP>
+constexpr int stage_tokens() {
+  return DP > 128 ? kTile : 2 * kTile;
+}
 
 __device__ inline void load_to_lds(const uint8_t* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
@@ -492,8 +486,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   using H = Half<DT>;
   using F = Half<FB_DT_F16>;
   constexpr int NP = DP / 32, ND = DP / 32, NPC = DP / 16;
-  constexpr int NI = NPC / 4;  // loads of a wave: 16 rows of K, one side of V
-  __shared__ __align__(16) uint8_t lk[2][kTile * DP], lv[2][kTile * DP];
+  constexpr int ST = stage_tokens<DP>(), SB = ST / kBlock;
+  constexpr int RW = ST / 4;            // rows of K that a wave loads, and as much of V
+  constexpr int NI = RW * NPC / 64;     // 16-byte loads of a lane for each
+  // Arrays of their own: the compiler waits for a load to LDS before it reads where that may go.
+  __shared__ __align__(16) uint8_t lk0[ST * DP], lv0[ST * DP], lk1[ST * DP], lv1[ST * DP];
   const Cache& c = a.c;
   const int D = EX ? DP : c.D;  // known: the loads' addresses differ by constants
   const int tid = threadIdx.x, lane = tid & 63;
@@ -507,20 +504,33 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   const int rows = n * a.group;
   const int tiles = (rows + kRows - 1) / kRows;
   const auto exchange = [](int row, int pc) {
-    return pc ^ (NPC == 4 ? (row >> 1) & 3 : row & 7);
+    return pc ^ (NPC == 4 ? (row >> 2) & 3 : NPC == 8 ? (row >> 1) & 7 : row & 15);
   };
-  // what a lane loads of a block: K rows 16 (wave % 2).., V side wave % 2.  Pieces past D are
-  // others of the same row: they meet zeros of q, or channels that are not written.
-  int k_from[NI], v_from[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
+  // What a lane loads of the wave's block.  Pieces past D are others of the same row: they meet
+  // zeros of q, or channels that are not written.
+  const int wave_block = wave * RW / kBlock, wave_row = wave * RW % kBlock;
+  const auto k_from = [&](int i) {
     const int piece = i * 64 + lane;
-    const int rho = (wave & 1) * 16 + piece / NPC;
+    const int rho = wave_row + piece / NPC;
     const int tok = ((rho & 4) << 2) | ((rho >> 1) & 12) | (rho & 3);
     const int pc = exchange(rho, piece % NPC);
-    k_from[i] = tok * D + (pc * 16 < D ? pc : pc % (D / 16)) * 16;
-    v_from[i] = ((wave & 1) * D + min(piece, D - 1)) * 16;
-  }
+    return tok * D + (pc * 16 < D ? pc : pc % (D / 16)) * 16;
+  };
+  const auto v_from = [&](int i) {
+    const int piece = i * 64 + lane, side = wave_row / kSide + piece / DP;
+    return (side * D + min(piece % DP, D - 1)) * 16;
+  };
+  const int k0 = k_from(0), v0 = v_from(0);
+  // the i-th: where D is known it differs from the first by constants
+  const auto k_at = [&](int i) {
+    if constexpr (!EX) return k_from(i);
+    if constexpr (NPC == 4) return k0 + 8 * i * DP;
+    if constexpr (NPC == 8) return (k0 ^ (i & 1) * 64) + 4 * i * DP;
+    return (k0 ^ i * 64) + (16 * (i & 1) + 4 * (i >> 1)) * DP;
+  };
+  const auto v_at = [&](int i) { return EX ? v0 + i * 1024 : v_from(i); };
+  const unsigned per = (unsigned)c.P / kBlock;
+  const int32_t* const table = c.table + b * c.table_stride;
   for (int ti = blockIdx.y; ti < tiles; ti += gridDim.y) {
     const int tile = (tiles - 1 - ti) * kRows;  // the longest first
     const int row = tile + wave * 32 + r, i = row / a.group;
@@ -530,6 +540,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
     // least and most that the wave's and the workgroup's rows see
     const int i_lo = (tile + wave * 32) / a.group;
     const int least = min(max(len - n + i_lo + 1, 0), len);
+    const int least_wg = min(max(len - n + tile / a.group + 1, 0), len);
     const int i_hi = (min(tile + wave * 32 + 32, rows) - 1) / a.group;
     const int wave_most = tile + wave * 32 < rows ? min(max(len - n + i_hi + 1, 0), len) : 0;
     const int j_hi = (min(tile + kRows, rows) - 1) / a.group;
@@ -550,60 +561,147 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
       for (int k = 0; k < 16; ++k) o[d][k] = 0.f;
     float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
     int E = kMinExp;                       // and their unit's exponent
+    unsigned dead[(ND + 1) / 2] = {};      // bit 16 (d % 2) + k of d / 2: o[d][k] saw a NaN value
 
-    const int first = split * (a.split_tokens / kTile);
-    const int all = (most + kTile - 1) / kTile;
-    const int last = split + 1 == a.splits ? all : min(all, first + a.split_tokens / kTile);
-    Walk walk(c, b, first * 2);
-    int scale_k[2], scale_v[2];  // of the tile that is on its way
-    const auto fetch = [&](int buf) {
-      const int64_t b0 = walk.index(c, h, 0), b1 = walk.index(c, h, 1);
-      const int64_t mine = (wave >> 1 ? b1 : b0) * kBlock * D;
+    const int first = split * (a.split_tokens / ST);
+    const int all = (most + ST - 1) / ST;
+    const int last = split + 1 == a.splits ? all : min(all, first + a.split_tokens / ST);
+    // lane j has block j % SB of the next stage: its page as the table has it (read a stage ahead)
+    // and place in the page
+    int id, at;
+    const auto look = [&](int t) {
+      const unsigned blk = (unsigned)t * SB + lane % SB;
+      const unsigned pg = a.per_shift >= 0 ? blk >> a.per_shift : blk / per;
+      at = (int)(blk - pg * per);
+      id = pg < (unsigned)c.max_pages ? table[pg] : 0;
+    };
+    int scale_k, scale_v;  // lane j: of block j % SB of the stage that is on its way
+    const auto fetch = [&](uint8_t* to_k, uint8_t* to_v, int t) __attribute__((always_inline)) {
+      const int64_t bi = c.block_index((unsigned)id < (unsigned)c.pages ? id : 0, h, at);
+      const int64_t mine =
+          ((int64_t)__builtin_amdgcn_readlane((int)(bi >> 32), wave_block) << 32 |
+           (unsigned)__builtin_amdgcn_readlane((int)bi, wave_block)) * kBlock * D;
 #pragma unroll
       for (int k = 0; k < NI; ++k) {
-        load_to_lds(c.k + mine + k_from[k], lk[buf] + (wave * NI + k) * 1024);
-        load_to_lds(c.v + mine + v_from[k], lv[buf] + (wave * NI + k) * 1024);
+        load_to_lds(c.k + mine + k_at(k), to_k + (wave * NI + k) * 1024);
+        load_to_lds(c.v + mine + v_at(k), to_v + (wave * NI + k) * 1024);
       }
-      scale_k[0] = c.ks[b0];
-      scale_k[1] = c.ks[b1];
-      scale_v[0] = c.vs[b0];
-      scale_v[1] = c.vs[b1];
-      walk.next(c, b);
+      scale_k = c.ks[bi];
+      scale_v = c.vs[bi];
+      if (t + 1 < last) look(t + 1);
     };
     __syncthreads();  // the buffers of the row tile before are free
-    if (first < last) fetch(first & 1);
-    for (int t = first; t < last; ++t) {
-      const int buf = t & 1;
-      __syncthreads();  // this tile has arrived; everyone is done with the other buffer
+    if (first < last) {
+      look(first);
+      fetch(lk0, lv0, first);
+    }
+    const auto run = [&](int st, const uint8_t* in_k, uint8_t* in_v, uint8_t* to_k,
+                         uint8_t* to_v) __attribute__((always_inline)) {
+      __syncthreads();  // this stage has arrived; everyone is done with the other buffers
+      const int stage_k = scale_k, stage_v = scale_v;
+      if (st + 1 < last) fetch(to_k, to_v, st + 1);
+#pragma unroll 1
+      for (int part = 0; part < ST / kTile; ++part) {
+      const int t = st * (ST / kTile) + part;
+      const uint8_t* const tk = in_k + part * kTile * DP;
+      uint8_t* const tv = in_v + part * kTile * DP;
+      const auto values = [&](int i) {  // block i % 2, channels 32 (i / 2)..
+        return *reinterpret_cast<const u32x4*>(tv + ((2 * (i & 1) + x2) * DP + 32 * (i / 2) + r) * 16);
+      };
+      if (t * kTile + kTile > least_wg) {
+        asm volatile("");
+        // Some row does not see some token here.  A NaN value reaches the rows that see its token,
+        // and no others, and what lies behind the end may be anything; but 0 * NaN must not come
+        // up.  So NaNs are noted for the rows that see them, and taken out of the tile.  Every
+        // wave looks at the same tile and comes to the same decision.
+        const int seen = sees - t * kTile - x2 * 16, held = len - t * kTile - x2 * 16;
+        unsigned nan = 0;
+#pragma unroll 1
+        for (int i = 0; i < 2 * ND; ++i) {
+          const u32x4 w = values(i);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) nan |= nan_bytes(w[u]);
+        }
+        if (__any(nan != 0)) {
+          h16x8 see[2][2];
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            see[k / 16][k / 8 & 1][k & 7] =
+                (k / 16) * kBlock + k % 16 < seen ? (_Float16)1 : (_Float16)0;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            f32x16 bad;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) bad[k] = 0.f;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              u32x4 w = values(2 * d + y);
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                w[u] = nan_ones(w[u] & keep_bytes(y * kBlock + 4 * u, held));
+              bad = F::mfma32(F::decode(w[0], w[1]), see[y][0], bad);
+              bad = F::mfma32(F::decode(w[2], w[3]), see[y][1], bad);
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (bad[k] > 0.f) dead[d / 2] |= 1u << (16 * (d & 1) + k);
+          }
+          __syncthreads();
+          for (int i = tid; i < kTile * DP / 16; i += 256) {
+            u32x4 w = *reinterpret_cast<const u32x4*>(tv + i * 16);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] &= ~nan_bytes(w[u]);
+            *reinterpret_cast<u32x4*>(tv + i * 16) = w;
+          }
+          __syncthreads();
+        }
+      }
+      if (t * kTile >= wave_most) continue;  // the same for the wave
       float ks[2];
       int ev[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int ek = __builtin_amdgcn_readfirstlane(scale_k[y]) - 127;
+        const int ek = __builtin_amdgcn_readlane(stage_k, 2 * part + y) - 127;
         ks[y] = a.scale2 * exp2i(min(max(ek, -126), 127));
         ev[y] = t * kTile + y * kBlock < len
-                    ? max(__builtin_amdgcn_readfirstlane(scale_v[y]) - 127, -126)
+                    ? max(__builtin_amdgcn_readlane(stage_v, 2 * part + y) - 127, -126)
                     : kMinExp;
         ev[y] = min(ev[y], 126);
       }
-      if (t + 1 < last) fetch(buf ^ 1);
-      if (t * kTile >= wave_most) continue;  // the same for the wave; the barriers are above
       const bool masked = t * kTile + kTile > least;  // the same for the wave
-      // tokens of the lane's part of the tile that its row sees, and that are held
-      const int seen = sees - t * kTile - x2 * 16, held = len - t * kTile - x2 * 16;
+      const int seen = sees - t * kTile - x2 * 16;    // tokens of the lane's part
+      // Keys: piece i is 16 channels of block i % 2.  A piece is read two ahead of its products, and
+      // decoded between the products of the one before: left to itself the compiler reads,
+      // waits, decodes and multiplies in turn, and a wave waits for LDS at every piece.
       f32x16 s[2];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int k = 0; k < 16; ++k) s[y][k] = 0.f;
+      {
+        const auto read = [&](int i) {
+          return *reinterpret_cast<const u32x4*>(
+              tk + (((i & 1) * 32 + r) * NPC + exchange(r, (i & ~1) + x2)) * 16);
+        };
+        u32x4 w[2] = {read(0), read(1)};
+        typename H::x8 lo = H::decode(w[0][0], w[0][1]), hi = H::decode(w[0][2], w[0][3]);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(
-              lk[buf] + ((y * 32 + r) * NPC + exchange(r, 2 * p + x2)) * 16);
-          s[y] = H::mfma32(H::decode(w[0], w[1]), qf[p][0], s[y]);
-          s[y] = H::mfma32(H::decode(w[2], w[3]), qf[p][1], s[y]);
+        for (int i = 0; i < 2 * NP; ++i) {
+          typename H::x8 next_lo = lo, next_hi = hi;
+          if (i + 2 < 2 * NP) w[i & 1] = read(i + 2);
+          const u32x4 n = w[(i + 1) & 1];
+          __builtin_amdgcn_sched_barrier(0);
+          s[i & 1] = H::mfma32(lo, qf[i / 2][0], s[i & 1]);
+          if (i + 1 < 2 * NP) next_lo = H::decode(n[0], n[1]);
+          __builtin_amdgcn_sched_barrier(0);
+          s[i & 1] = H::mfma32(hi, qf[i / 2][1], s[i & 1]);
+          if (i + 1 < 2 * NP) next_hi = H::decode(n[2], n[3]);
+          __builtin_amdgcn_sched_barrier(0);
+          lo = next_lo;
+          hi = next_hi;
         }
       }
+      u32x4 vw[2] = {values(0), values(1)};  // on their way during the weights
       if (masked) {
         asm volatile("");  // a branch, not selects in every tile
 #pragma unroll
@@ -612,93 +710,85 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           for (int k = 0; k < 16; ++k)
             if (y * kBlock + k >= seen) s[y][k] = -__builtin_inff();
       }
-      float mx[2];
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        mx[y] = s[y][0];
-#pragma unroll
-        for (int k = 1; k < 16; ++k) mx[y] = fmaxf(mx[y], s[y][k]);
-      }
-      float big = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);  // the scales are positive
-      big = fmaxf(big, __shfl_xor(big, 32));
-      const int e = max(E, max(ev[0], ev[1]));
-      if (e > E || __any(big > m + kSlack)) {
-        const float up = fmaxf(m, big);
-        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
-        const float unit = alpha * exp2i(max(E - e, -126));
-        l *= alpha;
+      const int e = max(ev[0], ev[1]);
+      if (e > E) {  // the same for the wave
+        asm volatile("");
+        const float unit = exp2i(max(E - e, -126));
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= unit;
-        m = up;
         E = e;
       }
-      const float base = m == -__builtin_inff() ? 0.f : m;
+      // the value block's scale joins in the exponent and leaves the sum again
+      const int fold[2] = {max(ev[0] - E, -64), max(ev[1] - E, -64)};
+      float sum[2];
       h16x8 pf[2][2];
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        // the value block's scale joins in the exponent and leaves the sum again
-        const int fold = max(ev[y] - E, -64);
-        const float shift = (float)(fold + kLift) - base;
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float p = exp2f_(__builtin_fmaf(s[y][k], ks[y], shift));
-          sum += p;
-          pf[y][k / 8][k & 7] = (_Float16)p;
-        }
-        l = __builtin_fmaf(sum, exp2i(-fold - kLift), l);
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        u32x4 w[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          w[y] = *reinterpret_cast<const u32x4*>(lv[buf] + ((2 * y + x2) * DP + 32 * d + r) * 16);
-        if (masked) {
-          asm volatile("");
-          unsigned nan = 0;
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              // what lies behind the end may be anything
-              w[y][u] &= keep_bytes(y * kBlock + 4 * u, held);
-              nan |= nan_bytes(w[y][u]);
-            }
-          if (__any(nan != 0)) {
-            // a NaN value reaches the rows that see its token, and no others: 0 * NaN must not
-            // come up, so those channels are marked apart
-            f32x16 bad;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) bad[k] = 0.f;
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                h16x8 see;
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  see[k] = y * kBlock + 8 * u + k < seen ? (_Float16)1 : (_Float16)0;
-                bad = F::mfma32(F::decode(nan_ones(w[y][2 * u]), nan_ones(w[y][2 * u + 1])), see,
-                                bad);
-              }
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-              if (bad[k] > 0.f) o[d][k] = __builtin_nanf("");
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-              for (int u = 0; u < 4; ++u) w[y][u] &= ~nan_bytes(w[y][u]);
-          }
-        }
+      const auto weigh = [&]() __attribute__((always_inline)) {
+        const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          o[d] = F::mfma32(F::decode(w[y][0], w[y][1]), pf[y][0], o[d]);
-          o[d] = F::mfma32(F::decode(w[y][2], w[y][3]), pf[y][1], o[d]);
+          const float shift = (float)(fold[y] + kLift) - base;
+          sum[y] = 0.f;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float p = exp2f_(__builtin_fmaf(s[y][k], ks[y], shift));
+            sum[y] += p;
+            pf[y][k / 8][k & 7] = (_Float16)p;
+          }
+        }
+      };
+      weigh();
+      if (__any(m == -__builtin_inff() || fmaxf(sum[0], sum[1]) > kMost)) {
+        asm volatile("");
+        float mx[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          mx[y] = s[y][0];
+#pragma unroll
+          for (int k = 1; k < 16; ++k) mx[y] = fmaxf(mx[y], s[y][k]);
+        }
+        float big = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);  // the scales are positive
+        big = fmaxf(big, __shfl_xor(big, 32));
+        const float up = fmaxf(m, big);
+        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= alpha;
+        m = up;
+        weigh();
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) l = __builtin_fmaf(sum[y], exp2i(-fold[y] - kLift), l);
+      {
+        h16x8 lo = F::decode(vw[0][0], vw[0][1]), hi = F::decode(vw[0][2], vw[0][3]);
+#pragma unroll
+        for (int i = 0; i < 2 * ND; ++i) {
+          h16x8 next_lo = lo, next_hi = hi;
+          if (i + 2 < 2 * ND) vw[i & 1] = values(i + 2);
+          const u32x4 n = vw[(i + 1) & 1];
+          __builtin_amdgcn_sched_barrier(0);
+          o[i / 2] = F::mfma32(lo, pf[i & 1][0], o[i / 2]);
+          if (i + 1 < 2 * ND) next_lo = F::decode(n[0], n[1]);
+          __builtin_amdgcn_sched_barrier(0);
+          o[i / 2] = F::mfma32(hi, pf[i & 1][1], o[i / 2]);
+          if (i + 1 < 2 * ND) next_hi = F::decode(n[2], n[3]);
+          __builtin_amdgcn_sched_barrier(0);
+          lo = next_lo;
+          hi = next_hi;
         }
       }
+      }
+    };
+    for (int st = first; st < last; st += 2) {
+      run(st, lk0, lv0, lk1, lv1);
+      if (st + 1 < last) run(st + 1, lk1, lv1, lk0, lv0);
     }
     l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      if (dead[d / 2])
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (dead[d / 2] >> (16 * (d & 1) + k) & 1) o[d][k] = __builtin_nanf("");
     if (there) {
       const int64_t orow = (int64_t)(row0 + i) * a.Hq + head;
       const float unit = exp2i(min(max(E - kLift, -126), 127)) *
@@ -892,7 +982,7 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t len = std::max<int64_t>(1, std::min<int64_t>(s->max_len, capacity));
   const int64_t tiles = p.few ? 1 : (rows + kRows - 1) / kRows;
   const int64_t units = tiles * c->heads * s->seqs;
-  const int step = p.few ? 1024 : 4 * kTile;
+  const int step = p.few ? 1024 : 4 * kTile;  // a whole number of stages
   const int64_t most = (len + step - 1) / step;
   const int64_t want =
       std::max<int64_t>(1, (p.few ? 4 : 2) * (int64_t)fb_gpu::cu_count() / units);
