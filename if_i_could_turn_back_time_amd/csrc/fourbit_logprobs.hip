@@ -1,13 +1,18 @@
 // Log probabilities of given tokens, entropy and the likeliest alternatives of rows of logits, and
 // their gradient.
 //
-// With m the largest logit, Z = sum exp(x - m) and W = sum exp(x - m) (x - m) come from one walk
-// over the row with a running maximum:  log p_i = x_i - m - log Z,  entropy = log Z - W / Z.
+// In base 2: with y = x log2(e) - R for a whole number R near the row's largest, z = sum 2^y and
+// w = sum 2^y y come from one walk over the row:  log p_i = ln 2 (y_i - log2 z), entropy =
+// ln 2 (log2 z - w / z).  Each thread has its own R, raised when a value passes it by 2^kSlack; a
+// whole R is subtracted without rounding (one fma) and threads are joined by exact powers of two.
 // The alternatives: lane l's largest value over all waves is one of 64 different values of the
-// row, so the top-th largest of these 64 bounds the row's top-th largest from below.  A second
-// walk collects what is not below the bound (about as many as are wanted, plus ties), and the
-// collected ones are ranked by (value, lowest id).  Where more qualify than the list holds (many
-// equal values), a radix select over all 32 key bits and a walk in id order take its place.
+// row, so the top-th largest of these 64 bounds the row's top-th largest from below.  Only threads
+// whose own largest reaches the bound hold candidates (about as many as are wanted), and only
+// their shares of the row, 1 KiB or so each, are read again, a wave a share; the collected
+// ones are ranked by (value, lowest id).  Where more qualify than the list holds (many equal
+// values), those above the bound are taken and the equal ones in the order of their ids; where
+// even those above it are too many, a radix select over all 32 key bits takes their place.
+// One walk bounds it: 7 to 8 VALU instructions a value, fewer cycles than its bytes take.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -53,48 +58,90 @@ __device__ inline float value_of(unsigned key) {
   return __builtin_bit_cast(float, key >> 31 ? key & 0x7FFFFFFFu : ~key);
 }
 
+// A row's 16-byte vectors, from its first aligned element on: vector v belongs to thread
+// v % kThreads; what is left at both ends (fewer than 2 V values) goes one by one to the first
+// threads.
 template <int DT>
-__device__ inline void load_vec(const void* row, int i, float* v) {
+struct Row {
   using T = typename Type<DT>::T;
-  const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const T*>(row) + i);
-  if constexpr (DT == FB_DT_F32) {
+  static constexpr int V = Type<DT>::V;
+  const T* p;
+  int n, head, vecs;
+  __device__ Row(const void* row, int vocab) : p(static_cast<const T*>(row)), n(vocab) {
+    head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(T));
+    vecs = (n - head) / V;
+  }
+  __device__ int first(int v) const { return head + v * V; }  // id of vector v's first value
+  __device__ int rest() const { return n - vecs * V; }
+  __device__ int rest_id(int i) const { return i < head ? i : vecs * V + i; }
+  __device__ u32x4 raw(int v) const { return *reinterpret_cast<const u32x4*>(p + first(v)); }
+  __device__ static void unpack(u32x4 w, float (&x)[V]) {
+    if constexpr (DT == FB_DT_F32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned u = w[j];  // a bit cast of a vector's element takes the first one
-      v[j] = __builtin_bit_cast(float, u);
-    }
-  } else {
+      for (int j = 0; j < 4; ++j) {
+        const unsigned u = w[j];  // a bit cast of a vector's element takes the first one
+        x[j] = __builtin_bit_cast(float, u);
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const unsigned short u = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
-      v[j] = DT == FB_DT_F16 ? (float)__builtin_bit_cast(_Float16, u)
-                             : __builtin_bit_cast(float, (unsigned)u << 16);
+      for (int j = 0; j < 8; ++j) {
+        const unsigned u = w[j / 2];
+        if constexpr (DT == FB_DT_F16)
+          x[j] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u >> (16 * (j & 1))));
+        else
+          x[j] = __builtin_bit_cast(float, j & 1 ? u & 0xFFFF0000u : u << 16);
+      }
     }
   }
+  // Calls f(id, value) for the thread's whole share.
+  template <typename F>
+  __device__ void walk(F&& f) const {
+    for (int v = threadIdx.x; v < vecs; v += kThreads) {
+      float x[V];
+      unpack(raw(v), x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f(first(v) + j, x[j]);
+    }
+    if ((int)threadIdx.x < rest()) f(rest_id(threadIdx.x), (float)p[rest_id(threadIdx.x)]);
+  }
+};
+
+// Largest of three, NaN passed over.  (fmaxf would first copy every value that comes from bits, for
+// signalling NaNs; here such a NaN may only cost a maximum of values that a NaN outranks anyway.)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
-// Calls f(id, value) for the thread's share of a row; 16 bytes at a time where the row allows it.
-// The first `head` elements (up to the first aligned one) and the tail go one by one.
-template <int DT, typename F>
-__device__ inline void walk(const void* row, int n, F&& f) {
-  using T = typename Type<DT>::T;
-  constexpr int V = Type<DT>::V;
-  const int tid = threadIdx.x;
-  const int head =
-      min(n, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(T));
-  const int body = (n - head) / V * V;
-  float v[V];
-  for (int i = tid * V; i < body; i += kThreads * V) {
-    load_vec<DT>(static_cast<const T*>(row) + head, i, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f(head + i + j, v[j]);
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 24.f;     // a thread's sums stay below 2^24 * its values
+constexpr float kLow = -200.f;     // 2^y is 0 from here on, and y itself may be -inf
+constexpr float kHuge = 1.2676506e30f;  // 2^100: logits beyond it would overflow in base 2
+
+// Sums of 2^y and 2^y y relative to R.
+struct Sums {
+  float R, z, w;
+  __device__ void add(float y) {
+    const float e = __builtin_amdgcn_exp2f(y);
+    z += e;
+    w = __builtin_fmaf(e, fmaxf(y, kLow), w);
   }
-  const int rest = n - body;  // head and tail, fewer than 2 V
-  if (tid < rest) {
-    const int i = tid < head ? tid : body + tid;
-    f(i, (float)static_cast<const T*>(row)[i]);
+  __device__ void rebase(float to) {  // to >= R
+    const float d = R - to, f = __builtin_amdgcn_exp2f(d);
+    w = f * __builtin_fmaf(fmaxf(d, -kHuge), z, w);
+    z *= f;
+    R = to;
   }
-}
+  __device__ void join(Sums o) {
+    const float to = fmaxf(R, o.R);
+    rebase(to);
+    o.rebase(to);
+    z += o.z;
+    w += o.w;
+  }
+};
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(
@@ -102,67 +149,108 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
     int top, float* __restrict__ logprob, float* __restrict__ entropy,
     float* __restrict__ top_logprobs, int64_t* __restrict__ top_ids, float* __restrict__ stats) {
   using T = typename Type<DT>::T;
+  constexpr int V = Type<DT>::V;
   __shared__ float red[kWaves][3];
   __shared__ float lane_max[kWaves][64];
   __shared__ unsigned bound;
-  __shared__ int count;
+  __shared__ int count, shares;
   __shared__ unsigned list_key[kList];
   __shared__ int list_id[kList];
+  __shared__ int share[kThreads];
   __shared__ unsigned hist[256], chosen[2];
-  __shared__ int wave_count[2][kWaves];
+  __shared__ int wave_count[kWaves];
   const int64_t r = blockIdx.x;
-  const T* const row = static_cast<const T*>(logits) + r * stride;
+  const Row<DT> row(static_cast<const T*>(logits) + r * stride, vocab);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float inf = __builtin_inff();
 
-  float m = -inf, z = 0.f, w = 0.f;
-  const auto merge = [&](float om, float oz, float ow) {
-    const float big = fmaxf(m, om);
-    const float base = big == -inf ? 0.f : big;
-    const float a = __expf(m - base), b = __expf(om - base);
-    // (m - base) z: 0 where nothing is there yet
-    w = a * (w + (z == 0.f ? 0.f : (m - base) * z)) + b * (ow + (oz == 0.f ? 0.f : (om - base) * oz));
-    z = a * z + b * oz;
-    m = big;
+  const int64_t t = token[r];  // early: read while the row is on its way
+  const bool given = t >= 0 && t < vocab;
+  const float at_token = given ? (float)row.p[t] : 0.f;
+  float m = -inf;  // the thread's largest value
+  Sums s{-kHuge, 0.f, 0.f};
+  const auto raise = [&](float x) {  // to a whole number near x
+    const float to = fminf(__builtin_rintf(x * kLog2e), 3e38f);
+    if (to > s.R + kSlack) s.rebase(to);
   };
-  walk<DT>(row, vocab, [&](int, float x) {
-    if (x > m) {
-      const float a = m == -inf ? 0.f : __expf(m - x);
-      w = a * (w + (z == 0.f ? 0.f : (m - x) * z));
-      z *= a;
-      m = x;
+  constexpr int U = 8;  // vectors on their way at once
+  for (int v0 = tid; v0 < row.vecs; v0 += U * kThreads) {
+    u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + u * kThreads < row.vecs) raw[u] = row.raw(v0 + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v0 + u * kThreads >= row.vecs) break;
+      float x[V];
+      row.unpack(raw[u], x);
+      float big = max3(x[0], x[1], x[2]);
+#pragma unroll
+      for (int j = 3; j + 1 < V; j += 2) big = max3(big, x[j], x[j + 1]);
+      big = max3(big, x[V - 1], x[V - 1]);
+      m = fmaxf(m, big);
+      raise(big);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s.add(__builtin_fmaf(x[j], kLog2e, -s.R));
     }
-    const float d = x - (m == -inf ? 0.f : m);
-    const float e = __expf(d);
-    z += e;
-    w += d == -inf ? 0.f : e * d;
-  });
+  }
+  if (tid < row.rest()) {
+    const float x = (float)row.p[row.rest_id(tid)];
+    m = fmaxf(m, x);
+    raise(x);
+    s.add(__builtin_fmaf(x, kLog2e, -s.R));
+  }
+  const float mine = m;
   lane_max[wave][lane] = m;
-  for (int o = 32; o; o >>= 1) {
-    const float om = __shfl_xor(m, o), oz = __shfl_xor(z, o), ow = __shfl_xor(w, o);
-    merge(om, oz, ow);
-  }
+  for (int o = 32; o; o >>= 1) s.join(Sums{__shfl_xor(s.R, o), __shfl_xor(s.z, o), __shfl_xor(s.w, o)});
   if (lane == 0) {
-    red[wave][0] = m;
-    red[wave][1] = z;
-    red[wave][2] = w;
+    red[wave][0] = s.R;
+    red[wave][1] = s.z;
+    red[wave][2] = s.w;
   }
-  if (tid == 0) count = 0;
+  if (tid == 0) count = shares = 0;
   __syncthreads();
-  m = red[0][0];
-  z = red[0][1];
-  w = red[0][2];
-  for (int i = 1; i < kWaves; ++i) merge(red[i][0], red[i][1], red[i][2]);
-  const float base = m == -inf ? 0.f : m;
-  const float logz = logf(z);
+  s = Sums{red[0][0], red[0][1], red[0][2]};
+  for (int i = 1; i < kWaves; ++i) s.join(Sums{red[i][0], red[i][1], red[i][2]});
+  // Logits beyond 2^100, or nothing but -inf: relative to the largest itself, then scaled.
+  float shift = 0.f;  // y = (x - shift) log2(e) - R
+  if (!(s.z > 0.f) || __builtin_fabsf(s.R) >= kHuge) {
+    m = -inf;
+    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, lane_max[i][lane]);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (__builtin_fabsf(m) < inf && s.z == s.z) {
+      shift = m;
+      s = Sums{0.f, 0.f, 0.f};
+      row.walk([&](int, float x) { s.add((x - shift) * kLog2e); });
+      for (int o = 32; o; o >>= 1) {
+        s.z += __shfl_xor(s.z, o);
+        s.w += __shfl_xor(s.w, o);
+      }
+      __syncthreads();
+      if (lane == 0) {
+        red[wave][1] = s.z;
+        red[wave][2] = s.w;
+      }
+      __syncthreads();
+      s.z = s.w = 0.f;
+      for (int i = 0; i < kWaves; ++i) {
+        s.z += red[i][1];
+        s.w += red[i][2];
+      }
+    }
+  }
+  if (s.z == inf) s.z = __builtin_nanf("");  // of a logit of +inf
+  const float log2z = __builtin_log2f(s.z);
+  const auto logp = [&](float x) {
+    return s.z == 0.f ? -inf : kLn2 * (__builtin_fmaf(x - shift, kLog2e, -s.R) - log2z);
+  };
   if (tid == 0) {
-    const int64_t t = token ? token[r] : -1;
-    if (logprob)
-      logprob[r] = t >= 0 && t < vocab ? (z == 0.f ? -inf : ((float)row[t] - base) - logz) : 0.f;
-    if (entropy) entropy[r] = z == 0.f ? 0.f : logz - w / z;
+    logprob[r] = given ? logp(at_token) : 0.f;
+    entropy[r] = s.z == 0.f ? 0.f : kLn2 * (log2z - s.w / s.z);
     if (stats) {
-      stats[2 * r] = base;
-      stats[2 * r + 1] = z == 0.f ? 0.f : logz;  // p = exp(-inf) = 0 then
+      stats[3 * r] = shift;
+      stats[3 * r + 1] = s.z == 0.f ? 0.f : s.R;  // p = 2^-inf = 0 then
+      stats[3 * r + 2] = s.z == 0.f ? 0.f : log2z;
     }
   }
   if (!top) return;
@@ -180,84 +268,106 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   }
   __syncthreads();
   const unsigned least = bound;
-  walk<DT>(row, vocab, [&](int id, float x) {
+  // NaN counts as the largest, but no maximum shows it: then every share is looked at
+  const bool all = s.z != s.z;
+  if (all || key_of(mine) >= least) share[atomicAdd(&shares, 1)] = tid;
+  __syncthreads();
+  const auto take = [&](int id, float x, unsigned from) {
     const unsigned k = key_of(x);
-    if (k >= least) {
+    if (k >= from) {
       const int at = atomicAdd(&count, 1);
       if (at < kList) {
         list_key[at] = k;
         list_id[at] = id;
       }
     }
-  });
-  __syncthreads();
-  int found = count;
-  if (found > kList) {
-    unsigned prefix = 0, mask = 0;
-    int left = top, above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
-      __syncthreads();
-      walk<DT>(row, vocab, [&](int, float x) {
-        const unsigned k = key_of(x);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-      });
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255;
-        unsigned sum = 0;
-        while (d > 0 && sum + hist[d] < (unsigned)left) sum += hist[d--];
-        chosen[0] = d;
-        chosen[1] = sum;
+  };
+  // The shares with candidates, a wave each: what is at least `from`.
+  const auto collect = [&](unsigned from) {
+    for (int i = wave; i < shares; i += kWaves) {
+      const int owner = share[i];
+#pragma unroll 2
+      for (int v = owner + lane * kThreads; v < row.vecs; v += 64 * kThreads) {
+        float x[V];
+        row.unpack(row.raw(v), x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) take(row.first(v) + j, x[j], from);
       }
-      __syncthreads();
-      prefix |= chosen[0] << shift;
-      mask |= 255u << shift;
-      left -= (int)chosen[1];
-      above += (int)chosen[1];
-      __syncthreads();
+      if (lane == 0 && owner < row.rest())
+        take(row.rest_id(owner), (float)row.p[row.rest_id(owner)], from);
     }
+    __syncthreads();
+  };
+  collect(least);
+  int found = count;
+  if (found > kList) {  // many equal values, or large ones side by side
+    __syncthreads();
     if (tid == 0) count = 0;
     __syncthreads();
-    walk<DT>(row, vocab, [&](int id, float x) {  // fewer than top
-      const unsigned k = key_of(x);
-      if (k > prefix) {
-        const int at = atomicAdd(&count, 1);
-        list_key[at] = k;
-        list_id[at] = id;
+    unsigned last = least;  // the key of which not all may be taken
+    collect(last + 1);      // last is no NaN's: a bound of NaN has fewer than the list holds
+    int above = count;
+    __syncthreads();
+    if (above >= top) {
+      unsigned prefix = 0, mask = 0;
+      int left = top;
+      for (int b = 24; b >= 0; b -= 8) {
+        for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+        __syncthreads();
+        row.walk([&](int, float x) {
+          const unsigned k = key_of(x);
+          if ((k & mask) == prefix) atomicAdd(&hist[(k >> b) & 255u], 1u);
+        });
+        __syncthreads();
+        if (tid == 0) {
+          int d = 255;
+          unsigned sum = 0;
+          while (d > 0 && sum + hist[d] < (unsigned)left) sum += hist[d--];
+          chosen[0] = d;
+          chosen[1] = sum;
+          count = 0;
+        }
+        __syncthreads();
+        prefix |= chosen[0] << b;
+        mask |= 255u << b;
+        left -= (int)chosen[1];
+        __syncthreads();
       }
-    });
-    int have = above;  // then the first `left` equal ones in id order
+      last = prefix;
+      if (last != 0xFFFFFFFFu) collect(last + 1);  // fewer than top
+      above = top - left;
+    }
+    int have = above;  // then equal ones in the order of their ids
     for (int i0 = 0; i0 < vocab && have < top; i0 += kThreads) {
       const int id = i0 + tid;
-      const bool equal = id < vocab && key_of((float)row[id]) == prefix;
+      const bool equal = id < vocab && key_of((float)row.p[id]) == last;
       const unsigned long long eq = __ballot(equal);
-      if (lane == 0) wave_count[0][wave] = __popcll(eq);
+      if (lane == 0) wave_count[wave] = __popcll(eq);
       __syncthreads();
-      int at = have + __popcll(eq & ((1ull << lane) - 1)), all = 0;
+      int at = have + __popcll(eq & ((1ull << lane) - 1)), sum = 0;
       for (int i = 0; i < kWaves; ++i) {
-        if (i < wave) at += wave_count[0][i];
-        all += wave_count[0][i];
+        if (i < wave) at += wave_count[i];
+        sum += wave_count[i];
       }
       if (equal && at < top) {
-        list_key[at] = prefix;
+        list_key[at] = last;
         list_id[at] = id;
       }
-      have += all;
+      have += sum;
       __syncthreads();
     }
     __syncthreads();
-    found = top;
+    found = min(have, top);
   }
   for (int i = tid; i < found; i += kThreads) {
     const unsigned k = list_key[i];
     const int id = list_id[i];
     int better = 0;
-    for (int j = 0; j < found; ++j) better += list_key[j] > k || (list_key[j] == k && list_id[j] < id);
+    for (int j = 0; j < found; ++j)
+      better += list_key[j] > k || (list_key[j] == k && list_id[j] < id);
     if (better < top) {
       top_ids[r * top + better] = id;
-      top_logprobs[r * top + better] =
-          z == 0.f ? -inf : ((float)row[id] - base) - logz;
+      top_logprobs[r * top + better] = logp(value_of(k));
     }
   }
 }
@@ -279,17 +389,19 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
     const T* const row = static_cast<const T*>(logits) + r * stride;
     T* const out = static_cast<T*>(grad) + r * vocab;
-    const float base = stats[2 * r], logz = stats[2 * r + 1];
+    const float shift = stats[3 * r], R = stats[3 * r + 1], log2z = stats[3 * r + 2];
     const int64_t t = token ? token[r] : -1;
     const float g = g_logprob && t >= 0 && t < vocab ? g_logprob[r] : 0.f;
-    const float ge = g_entropy ? g_entropy[r] : 0.f, H = g_entropy ? entropy[r] : 0.f;
-    float all = g;
+    const float ge = g_entropy ? g_entropy[r] : 0.f;
+    float all = g + (g_entropy ? ge * entropy[r] : 0.f);
     if (g_top)
       for (int j = 0; j < top; ++j) all += g_top[r * top + j];
+    all = -__builtin_fmaf(0.f, log2z, all);  // NaN throughout where the row has one
+    const float slope = -ge * kLn2;
     const auto one = [&](int i, float x) {
-      const float lp = (x - base) - logz;
-      const float p = __expf(lp);
-      float v = p == 0.f ? 0.f : -p * (all + ge * (lp + H));
+      const float y = __builtin_fmaf(x - shift, kLog2e, -R) - log2z;
+      const float p = __builtin_amdgcn_exp2f(y);
+      float v = p * __builtin_fmaf(slope, fmaxf(y, kLow), all);
       if (i == t) v += g;
       return v;
     };
@@ -305,7 +417,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(
     if (vec) {
       for (int i = i0 + tid * V; i + V <= i1; i += 256 * V) {
         float v[V];
-        load_vec<DT>(row, i, v);
+        Row<DT>::unpack(*reinterpret_cast<const u32x4*>(row + i), v);
         T o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = (T)with_top(i + j, one(i + j, v[j]));

@@ -456,7 +456,7 @@ std::vector<at::Tensor> logprobs_forward(const at::Tensor& x, const at::Tensor& 
   const auto f = x.options().dtype(at::kFloat);
   at::Tensor lp = at::empty({M}, f), ent = at::empty({M}, f), tl = at::empty({M, top}, f);
   at::Tensor ti = at::empty({M, top}, x.options().dtype(at::kLong));
-  at::Tensor st = stats ? at::empty({M, 2}, f) : at::Tensor();
+  at::Tensor st = stats ? at::empty({M, 3}, f) : at::Tensor();
   check(fb_token_logprobs(x.data_ptr(), dtype_code(x.scalar_type()), x.stride(0), M, (int32_t)V,
                           static_cast<const int64_t*>(token.data_ptr()), (int32_t)top,
                           static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()),

@@ -526,8 +526,8 @@ int fb_cache_evict(const fb_cache_t* c, const fb_seqs_t* s, const float* weights
  *   entropy  fp32 [rows]: -sum p log p (p = 0: nothing)
  *   top_logprobs fp32 [rows, top], top_ids int64 [rows, top]: descending, ties: lowest id first;
  *            0 <= top <= FB_LOGPROBS_TOP_MAX, top <= vocab
- *   stats    fp32 [rows, 2]: (largest logit, log sum exp(logit - largest)), what the gradient
- *            needs; NULL: not wanted
+ *   stats    fp32 [rows, 3]: (a, R, b) with log p = ln 2 ((logit - a) log2(e) - R - b), what the
+ *            gradient needs; NULL: not wanted
  * A row of -inf alone has logprobs of -inf and no entropy; NaN or +inf makes its row NaN (NaN
  * counts as the largest among the alternatives).
  * ------------------------------------------------------------------------------- */
