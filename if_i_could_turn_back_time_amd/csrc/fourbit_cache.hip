@@ -134,10 +134,14 @@ __global__ __launch_bounds__(256) void cache_append_kernel(Cache c, NewTokens x)
 }
 
 // ---------------------------------------------------------------------------------
-// Eviction, first half: which tokens of a head stay.  Workgroup = (head, sequence).  A radix
-// select over the order-preserving 32-bit keys of the weights, 8 bits a pass, finds the key of
-// the last token that stays; a second walk in token order writes down what lies above it, as
-// many of its equals as are left, earliest first, and the recent ones.
+// Eviction, first half: which tokens of a head stay.  Workgroup = (head, sequence).  The key of the
+// last token that stays is searched for two bits at a time over the order-preserving 32-bit keys of
+// the weights, which stay in registers (KEYS of them a thread; longer sequences are read again for
+// each step): comparisons are counted by ballot, so equal weights cost no more than others (a
+// histogram's atomics do), and the search ends as soon as a bound parts the right number.  Then
+// every 64 tokens are counted once, the counts summed in token order, and what lies above the
+// key, as many of its equals as are left, earliest first, and the recent ones written down.  Bound
+// by its barriers (16 steps), a few microseconds.
 // ---------------------------------------------------------------------------------
 __device__ inline unsigned weight_key(float w) {
   unsigned b = __builtin_bit_cast(unsigned, w);
@@ -146,92 +150,142 @@ __device__ inline unsigned weight_key(float w) {
   return (b >> 31) ? ~b : (b | 0x80000000u);
 }
 
-constexpr int kSelect = 1024;
+constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
 
+template <int KEYS>
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(
     Cache c, const float* __restrict__ weights, int64_t w_seq, int64_t w_head, int w_tokens,
     int keep, int recent, int32_t* __restrict__ kept, float* __restrict__ new_weights,
     int32_t* __restrict__ new_lens) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned chosen[2];  // digit, how many above it
-  __shared__ int wave_count[2][kSelect / 64];
+  constexpr int kChunk = KEYS * kSelect;  // tokens held at once
+  __shared__ int counted[17][3];  // keys above the bounds of each step, all waves' together
+  __shared__ int chunk_sums[2];
+  __shared__ int2 before[KEYS * kSelectWaves];  // larger and equal keys before 64 tokens
   const int tid = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
   const int lane = tid & 63, wave = tid >> 6;
   const int n = min(min(max(c.lens[b], 0), c.capacity()), w_tokens);
   const float* const w = weights + b * w_seq + h * w_head;
   const int64_t out = ((int64_t)b * c.H + h) * keep;
   if (h == 0 && tid == 0) new_lens[b] = min(n, keep);
-  const int m = max(n - recent, 0);          // the tokens that compete
-  int need = keep - min(recent, n);          // for so many places
+  const int m = max(n - recent, 0);       // the tokens that compete
+  const int need = keep - min(recent, n); // for so many places
   const bool all = n <= keep;
-  unsigned last = 0;  // key of the last one that stays
-  int above = 0;      // how many have a larger one
+  unsigned key[KEYS];
+  float weight[KEYS];
+  const auto load = [&](int t0) {  // all of them asked for before the first is used
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) weight[j] = w[min(t0 + j * kSelect + tid, max(n - 1, 0))];
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j)
+      key[j] = t0 + j * kSelect + tid < m ? weight_key(weight[j]) : 0u;
+  };
+  const int chunks = (n + kChunk - 1) / kChunk;
+  load(0);
+  for (int i = tid; i < 17 * 3; i += kSelect) counted[i / 3][i % 3] = 0;
+  __syncthreads();
+  // the largest `last` with at least `need` keys >= last (0: all of them; a key of 0 is a NaN's)
+  unsigned last = 0;
+  int reached = m;  // keys >= last
   if (!all && need > 0) {
-    unsigned prefix = 0, mask = 0;
-    int left = need;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelect) hist[i] = 0;
-      __syncthreads();
-      for (int t = tid; t < m; t += kSelect) {
-        const unsigned key = weight_key(w[t]);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+    for (int shift = 30; shift >= 0 && reached != need; shift -= 2) {
+      int found[3] = {0, 0, 0};
+      for (int ch = 0; ch < chunks; ++ch) {
+        if (chunks > 1) load(ch * kChunk);
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j)
+#pragma unroll
+          for (int d = 0; d < 3; ++d)
+            found[d] += __popcll(__ballot(key[j] >= (last | (unsigned)(d + 1) << shift)));
       }
+      int(&total)[3] = counted[shift >> 1];
+      if (lane < 3) atomicAdd(&total[lane], lane == 0 ? found[0] : lane == 1 ? found[1] : found[2]);
       __syncthreads();
-      if (tid == 0) {
-        int d = 255;
-        unsigned sum = 0;
-        while (d > 0 && sum + hist[d] < (unsigned)left) sum += hist[d--];
-        chosen[0] = d;
-        chosen[1] = sum;
+      int digit = 0;
+#pragma unroll
+      for (int d = 0; d < 3; ++d) {
+        const int sum = __builtin_amdgcn_readfirstlane(total[d]);
+        if (sum >= need) {
+          digit = d + 1;
+          reached = sum;
+        }
       }
-      __syncthreads();
-      prefix |= chosen[0] << shift;
-      mask |= 255u << shift;
-      left -= (int)chosen[1];
-      above += (int)chosen[1];
-      __syncthreads();
+      last |= (unsigned)digit << shift;
     }
-    last = prefix;
   }
-  // tokens in order: larger keys, the first need - above equal ones, and the recent ones
-  int written = 0, equal_seen = 0;
-  const int equal_most = need - above;
-  for (int t0 = 0; t0 < n; t0 += kSelect) {
-    const int t = t0 + tid;
-    bool more = false, equal = false;
-    if (t < n) {
-      if (all || t >= m) {
-        more = true;
-      } else if (need > 0) {
-        const unsigned key = weight_key(w[t]);
-        more = key > last;
-        equal = key == last;
+  // Where `reached` is the number needed, every key >= last stays; else last is a key that
+  // several have, and of these the earliest stay.
+  const bool exact = reached == need;
+  const auto state = [&](int t, unsigned k, bool& more, bool& equal) {
+    more = t < n && (all || t >= m || (need > 0 && (exact ? k >= last : k > last)));
+    equal = t < m && !all && need > 0 && !exact && k == last;
+  };
+  int more_before = 0, equal_before = 0;  // in earlier chunks
+  int equal_most = 0;
+  if (!all && need > 0 && !exact) {
+    int above = 0;
+    for (int ch = 0; ch < chunks; ++ch) {
+      if (chunks > 1) load(ch * kChunk);
+#pragma unroll
+      for (int j = 0; j < KEYS; ++j) above += __popcll(__ballot(key[j] > last));
+    }
+    if (lane == 0) atomicAdd(&counted[16][0], above);
+    __syncthreads();
+    above = counted[16][0];
+    equal_most = need - above;
+  }
+  int written = 0;
+  for (int t0 = 0; t0 < n; t0 += kChunk) {
+    if (chunks > 1) load(t0);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      bool more, equal;
+      state(t0 + j * kSelect + tid, key[j], more, equal);
+      const int cm = __popcll(__ballot(more)), ce = __popcll(__ballot(equal));
+      if (lane == 0) before[j * kSelectWaves + wave] = int2{cm, ce};
+    }
+    __syncthreads();
+    if (wave == 0) {  // exclusive sums, 64 entries at a time
+      int cm = more_before, ce = equal_before;
+      for (int i0 = 0; i0 < KEYS * kSelectWaves; i0 += 64) {
+        const int2 v = before[i0 + lane];
+        int sm = v.x, se = v.y;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int pm = __shfl_up(sm, o), pe = __shfl_up(se, o);
+          if (lane >= o) {
+            sm += pm;
+            se += pe;
+          }
+        }
+        before[i0 + lane] = int2{cm + sm - v.x, ce + se - v.y};
+        cm += __shfl(sm, 63);
+        ce += __shfl(se, 63);
+      }
+      if (lane == 0) {
+        chunk_sums[0] = cm;
+        chunk_sums[1] = ce;
       }
     }
-    const unsigned long long eq = __ballot(equal);
-    if (lane == 0) wave_count[0][wave] = __popcll(eq);
     __syncthreads();
-    int rank = equal_seen + __popcll(eq & ((1ull << lane) - 1)), eq_all = 0;
-    for (int i = 0; i < kSelect / 64; ++i) {
-      if (i < wave) rank += wave_count[0][i];
-      eq_all += wave_count[0][i];
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      const int t = t0 + j * kSelect + tid;
+      bool more, equal;
+      state(t, key[j], more, equal);
+      const unsigned long long below = (1ull << lane) - 1;
+      const unsigned long long bm = __ballot(more), be = __ballot(equal);
+      const int2 base = before[j * kSelectWaves + wave];
+      const int rank = base.y + __popcll(be & below);
+      const int place = base.x + __popcll(bm & below) + min(rank, equal_most);
+      if ((more || (equal && rank < equal_most)) && place < keep) {
+        kept[out + place] = t;
+        if (new_weights) new_weights[out + place] = weight[j];
+      }
     }
-    const bool stays = more || (equal && rank < equal_most);
-    const unsigned long long st = __ballot(stays);
-    if (lane == 0) wave_count[1][wave] = __popcll(st);
-    __syncthreads();
-    int place = written + __popcll(st & ((1ull << lane) - 1)), st_all = 0;
-    for (int i = 0; i < kSelect / 64; ++i) {
-      if (i < wave) place += wave_count[1][i];
-      st_all += wave_count[1][i];
-    }
-    if (stays && place < keep) {
-      kept[out + place] = t;
-      if (new_weights) new_weights[out + place] = w[t];
-    }
-    written += st_all;
-    equal_seen += eq_all;
-    __syncthreads();
+    more_before = chunk_sums[0];
+    equal_before = chunk_sums[1];
+    written = more_before + min(equal_before, equal_most);
   }
   for (int i = written + tid; i < keep; i += kSelect) {
     kept[out + i] = -1;
@@ -240,80 +294,171 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(
 }
 
 // ---------------------------------------------------------------------------------
-// Second half: the kept tokens to their new pages.  Workgroup = (one new block, keys or values)
-// x head x sequence, as an append of 32 tokens that are decoded from the cache.
+// Second half: the kept tokens to their new pages.  Workgroup = (one new block, head, sequence),
+// as an append of 32 tokens that are decoded from the cache.  Keys: 8 channels of a token a thread,
+// as in the append.  Values: a thread has one channel of 16 new tokens, a side of the new block,
+// which it writes in one piece; of each of its tokens it reads the 16 bytes of the channel's side
+// (the others of which are its neighbours' for the other tokens there: a cache that turns values
+// for the matrix cores is read whole where a quarter of it is kept).  What bounds it is the chain
+// id, page, codes: keys, values and scales are asked for together.
 // ---------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void evict_move_kernel(Cache c, Cache to, int keep,
-                                                         const int32_t* __restrict__ kept) {
-  __shared__ float red[4];
-  __shared__ __align__(16) uint8_t side[kBlock * kMaxDim];
-  const int tid = threadIdx.x, which = blockIdx.x & 1, blk = blockIdx.x >> 1;
+// WIDE: D is a multiple of 64, so a wave's rows of values are of one side and its tokens uniform.
+// BIG: D is above 128.
+template <bool WIDE, bool BIG>
+__global__ __launch_bounds__(256, BIG ? 4 : WIDE ? 6 : 5) void evict_move_kernel(
+    Cache c, Cache to, int keep, const int32_t* __restrict__ kept) {
+  constexpr int KC = BIG ? 4 : 2, VC = BIG ? 2 : 1;  // pieces of keys, rows of values a thread
+  __shared__ float red[2][4];
+  __shared__ int64_t from_block[kBlock];  // of a token in the pool; -1: none
+  __shared__ int from_slot[kBlock];
+  __shared__ float from_scale[2][kBlock];
+  const int tid = threadIdx.x, blk = blockIdx.x;
   const int h = blockIdx.y, b = blockIdx.z;
   const int32_t* const ids = kept + ((int64_t)b * c.H + h) * keep;
-  if (ids[blk * kBlock] < 0) return;
+  const int place = blk * kBlock + tid;
+  const int from = tid < kBlock && place < keep ? ids[place] : -1;
   int at;
   const int page = to.page_of(b, blk, at);
-  if (page < 0) return;
+  int64_t src = -1;
+  if (tid < kBlock) {
+    int src_at, src_page = -1;
+    if (from >= 0) src_page = c.page_of(b, from / kBlock, src_at);
+    if (src_page >= 0) src = c.block_index(src_page, h, src_at);
+    from_block[tid] = src;
+    from_slot[tid] = from & (kBlock - 1);
+  }
+  // nothing to write: no token of the block is kept, or it has no page
+  if (__syncthreads_or(from >= 0) == 0 || page < 0) return;
+  int scale[2] = {0, 0};
+  if (src >= 0) {
+    scale[0] = c.ks[src];
+    scale[1] = c.vs[src];
+  }
   const int pieces = c.D / 8, total = kBlock * pieces;
-  float val[4][8];
-  float amax = 0.f;
+  u32x2 key[KC];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < KC; ++i) {
     const int e = tid + 256 * i, t = e / pieces, d = (e - t * pieces) * 8;
+    key[i] = u32x2{0, 0};
+    if (e < total && from_block[t] >= 0)
+      key[i] = *reinterpret_cast<const u32x2*>(c.k + from_block[t] * kBlock * c.D +
+                                               from_slot[t] * c.D + d);
+  }
+  // values: rows (side, channel) of the new block, 2 D of them
+  u32x4 value[VC];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) val[i][j] = 0.f;
-    const int place = blk * kBlock + t;
-    const int from = e < total && place < keep ? ids[place] : -1;
-    int src_at, src = -1;
-    if (from >= 0) src = c.page_of(b, from / kBlock, src_at);
-    if (src >= 0) {
-      const int64_t bi = c.block_index(src, h, src_at);
-      const int slot = from % kBlock;
-      u32x2 code;
-      if (which) {
-        const uint8_t* p = c.v + bi * kBlock * c.D + (slot / kSide) * c.D * kSide + d * kSide +
-                           slot % kSide;
-        unsigned u[2] = {0, 0};
+  for (int i = 0; i < VC; ++i) {
+    const int e = tid + 256 * i;
+    const int side = WIDE ? __builtin_amdgcn_readfirstlane(e / c.D) : e / c.D;
+    const int d = e - side * c.D;
+    value[i] = u32x4{0, 0, 0, 0};
+    if (e >= 2 * c.D) continue;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j / 4] |= (unsigned)p[j * kSide] << (8 * (j & 3));
-        code = u32x2{u[0], u[1]};
-      } else {
-        code = *reinterpret_cast<const u32x2*>(c.k + bi * kBlock * c.D + slot * c.D + d);
+    for (int half = 0; half < 2; ++half) {
+      u32x4 row[8];
+      int slot[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int k = side * kSide + half * 8 + t;
+        int64_t block = from_block[k];
+        slot[t] = from_slot[k];
+        if (WIDE) {
+          block = (int64_t)__builtin_amdgcn_readfirstlane((int)(block >> 32)) << 32 |
+                  (unsigned)__builtin_amdgcn_readfirstlane((int)block);
+          slot[t] = __builtin_amdgcn_readfirstlane(slot[t]);
+        }
+        row[t] = u32x4{0, 0, 0, 0};
+        if (block >= 0)
+          row[t] = *reinterpret_cast<const u32x4*>(
+              c.v + block * kBlock * c.D + (slot[t] / kSide) * c.D * kSide + d * kSide);
       }
-      const float f = exp2i(min(max((int)(which ? c.vs : c.ks)[bi] - 127, -126), 127));
-      decode8(code, val[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        val[i][j] *= f;
-        amax = fmaxf(amax, finite_abs(val[i][j]));
+      for (int t = 0; t < 8; ++t) {
+        const unsigned word = slot[t] & 8 ? (slot[t] & 4 ? row[t][3] : row[t][2])
+                                          : (slot[t] & 4 ? row[t][1] : row[t][0]);
+        value[i][half * 2 + t / 4] |= (word >> (8 * (slot[t] & 3)) & 0xFFu) << (8 * (t & 3));
       }
+      __builtin_amdgcn_sched_barrier(0);  // the registers of one half at a time
     }
   }
-  amax = block_max(amax, red);
-  const int e2 = block_exp(amax);
-  const float inv = exp2i(min(max(-e2, -126), 127));
+  if (tid < kBlock) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      from_scale[x][tid] = src >= 0 ? exp2i(min(max(scale[x] - 127, -126), 127)) : 0.f;
+  }
+  __syncthreads();
+  const auto key_values = [&](int i, float (&v)[8]) {
+    const int t = min((tid + 256 * i) / pieces, kBlock - 1);
+    decode8(key[i], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= from_scale[0][t];
+  };
+  const auto value_values = [&](int i, int half, float (&v)[8]) {
+    const int t0 = min((tid + 256 * i) / c.D, 1) * kSide + half * 8;
+    decode8(u32x2{value[i][2 * half], value[i][2 * half + 1]}, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= from_scale[1][t0 + j];
+  };
+  float amax[2] = {0.f, 0.f}, val[8];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    key_values(i, val);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax[0] = fmaxf(amax[0], finite_abs(val[j]));
+  }
+#pragma unroll
+  for (int i = 0; i < VC; ++i)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      value_values(i, half, val);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax[1] = fmaxf(amax[1], finite_abs(val[j]));
+    }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    amax[0] = fmaxf(amax[0], __shfl_xor(amax[0], o));
+    amax[1] = fmaxf(amax[1], __shfl_xor(amax[1], o));
+  }
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = amax[0];
+    red[1][tid >> 6] = amax[1];
+  }
+  __syncthreads();
+  int e2[2];
+  float inv[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    e2[x] = block_exp(fmaxf(fmaxf(red[x][0], red[x][1]), fmaxf(red[x][2], red[x][3])));
+    inv[x] = exp2i(min(max(-e2[x], -126), 127));
+  }
   const int64_t bi = to.block_index(page, h, at);
-  uint8_t* const codes = (which ? to.v : to.k) + bi * kBlock * c.D;
-  if (tid == 0) (which ? to.vs : to.ks)[bi] = (uint8_t)(e2 + 127);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = tid + 256 * i, t = e / pieces, d = (e - t * pieces) * 8;
-    if (e >= total) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) val[i][j] *= inv;
-    const u32x2 code = encode8(val[i]);
-    if (!which) {
-      *reinterpret_cast<u32x2*>(codes + t * c.D + d) = code;
-      continue;
-    }
-    uint8_t* const s = side + (t / kSide) * c.D * kSide + d * kSide + t % kSide;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[j * kSide] = (uint8_t)(code[j / 4] >> (8 * (j & 3)));
+  if (tid == 0) {
+    to.ks[bi] = (uint8_t)(e2[0] + 127);
+    to.vs[bi] = (uint8_t)(e2[1] + 127);
   }
-  if (which) {
-    __syncthreads();
-    for (int e = tid; e < 2 * c.D; e += 256)
-      *reinterpret_cast<u32x4*>(codes + e * 16) = *reinterpret_cast<const u32x4*>(side + e * 16);
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    const int e = tid + 256 * i;
+    if (e >= total) continue;
+    key_values(i, val);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) val[j] *= inv[0];
+    *reinterpret_cast<u32x2*>(to.k + bi * kBlock * c.D + e * 8) = encode8(val);
+  }
+#pragma unroll
+  for (int i = 0; i < VC; ++i) {
+    const int e = tid + 256 * i;
+    if (e >= 2 * c.D) continue;
+    u32x2 w[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      value_values(i, half, val);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) val[j] *= inv[1];
+      w[half] = encode8(val);
+    }
+    *reinterpret_cast<u32x4*>(to.v + bi * kBlock * c.D + e * kSide) =
+        u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
   }
 }
 
@@ -372,14 +517,27 @@ int fb_cache_evict(const fb_cache_t* c, const fb_seqs_t* s, const float* weights
   to.table = new_table;
   to.table_stride = new_stride;
   to.max_pages = new_pages;
-  const int64_t nx = ((int64_t)keep + kBlock - 1) / kBlock * 2;
+  const int64_t nx = ((int64_t)keep + kBlock - 1) / kBlock;
   if (nx > INT32_MAX) return FB_ERR_SHAPE;
   hipStream_t hs = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(c->heads, s->seqs), dim3(kSelect), 0, hs, kc,
-                     weights, w_seq, w_head, w_tokens, keep, recent, kept, new_weights, new_lens);
+  const auto select = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(c->heads, s->seqs), dim3(kSelect), 0, hs, kc, weights, w_seq,
+                       w_head, w_tokens, keep, recent, kept, new_weights, new_lens);
+  };
+  // as many keys a thread as the longest sequence asks for, up to 32
+  const int longest = std::min(s->max_len, w_tokens);
+  if (longest <= 4 * kSelect)
+    select(evict_select_kernel<4>);
+  else if (longest <= 8 * kSelect)
+    select(evict_select_kernel<8>);
+  else
+    select(evict_select_kernel<32>);
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
-  hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)nx, c->heads, s->seqs), dim3(256), 0, hs,
-                     kc, to, keep, kept);
+  const bool big = c->head_dim > 128;
+  hipLaunchKernelGGL(c->head_dim % 64
+                         ? (big ? evict_move_kernel<false, true> : evict_move_kernel<false, false>)
+                         : (big ? evict_move_kernel<true, true> : evict_move_kernel<true, false>),
+                     dim3((unsigned)nx, c->heads, s->seqs), dim3(256), 0, hs, kc, to, keep, kept);
   return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
 }
 
