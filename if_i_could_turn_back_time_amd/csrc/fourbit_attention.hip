@@ -149,11 +149,11 @@ constexpr float kMost = 32768.f;
 
 template <int DP>
 constexpr int few_waves() {
-  return DP > 128 ? 4 : 8;  // registers of one wave a SIMD, or of two
+  return 4;
 }
 
 template <int DT, int DP, bool EX>
-__global__ __launch_bounds__(64 * few_waves<DP>()) void attn_few_kernel(Attn a) {
+__global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_few_kernel(Attn a) {
   using H = Half<DT>;
   using F = Half<FB_DT_F16>;
   constexpr int NP = DP / 64, ND = DP / 16, NW = few_waves<DP>();
@@ -982,10 +982,10 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t len = std::max<int64_t>(1, std::min<int64_t>(s->max_len, capacity));
   const int64_t tiles = p.few ? 1 : (rows + kRows - 1) / kRows;
   const int64_t units = tiles * c->heads * s->seqs;
-  const int step = p.few ? 1024 : 4 * kTile;  // a whole number of stages
+  const int step = p.few ? 512 : 4 * kTile;  // a whole number of stages
   const int64_t most = (len + step - 1) / step;
   const int64_t want =
-      std::max<int64_t>(1, (p.few ? 4 : 2) * (int64_t)fb_gpu::cu_count() / units);
+      std::max<int64_t>(1, (p.few ? 2 : 2) * (int64_t)fb_gpu::cu_count() / units);
   const int64_t per = (most + std::min(want, most) - 1) / std::min(want, most);
   p.split_tokens = (int)(per * step);
   p.splits = (int)((most + per - 1) / per);
