@@ -37,6 +37,7 @@ struct Attn {
   void* out;
   float* lse;         // or null
   int splits, split_tokens;
+  bool dealt;         // see find_part
   float* part;        // [splits][T * Hq][D]
   float2* part_ml;    // [splits][T * Hq]: what the sums are relative to (base 2), sum
   int per_shift;      // log2 of a page's blocks, -1: no power of two
@@ -142,10 +143,61 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //    after the first tile, and no maximum is taken in the others.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
+constexpr int kGrain = 8;  // chunks: two a wave
 // Weights enter the products as fp16 times 2^kLift, so that small ones keep their bits.
 constexpr int kLift = 7;
 // A tile's sum of them that asks for the row's largest score anew: none is above fp16's range.
 constexpr float kMost = 32768.f;
+
+// Which sequence and part of it a workgroup has.  Up to 64 sequences are dealt out by their lengths:
+// of `a.splits` parts a sequence gets its share of all tokens, at least one, and its parts are of
+// one size, so that none of the parts that run side by side is much longer than the others.  More
+// sequences have a.splits parts each.
+struct Part {
+  int b, first, last, parts, slot;  // chunks [first, last); place of its sums
+};
+
+__device__ inline int held(const Cache& c, int b) { return min(max(c.lens[b], 0), c.capacity()); }
+
+// `grain`: the least chunks of a part.  Every lane of a wave calls it; slot < 0: nothing to do.
+__device__ inline Part find_part(const Attn& a, int x, int z, int chunk, int grain) {
+  const Cache& c = a.c;
+  Part p;
+  if (!a.dealt) {
+    p.b = z;
+    p.slot = x;
+    p.parts = a.splits;
+    const int all = (held(c, z) + chunk - 1) / chunk;
+    p.first = min(all, x * (a.split_tokens / chunk));
+    p.last = x + 1 == a.splits ? all : min(all, p.first + a.split_tokens / chunk);
+    return p;
+  }
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < c.B ? (held(c, lane) + chunk - 1) / chunk : 0;
+  // in chunks, as floats: exact enough to share by, the same in every wave
+  float sum = (float)mine;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  int n = lane < c.B ? max(1, (int)((float)mine * (float)(a.splits - c.B) / fmaxf(sum, 1.f) + 0.5f))
+                     : 0;
+  n = min(n, max(1, (mine + grain - 1) / grain));
+  int end = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int before = __shfl_up(end, o);
+    if (lane >= o) end += before;
+  }
+  const unsigned long long past = __ballot(lane < c.B && end <= x);
+  const int b = __popcll(past);
+  p.b = min(b, c.B - 1);
+  p.parts = __shfl(n, p.b);
+  const int i = x - (__shfl(end, p.b) - p.parts), chunks = __shfl(mine, p.b);
+  p.slot = b < c.B ? i : -1;
+  const int size = (chunks + p.parts - 1) / p.parts;
+  p.first = min(chunks, i * size);
+  p.last = min(chunks, p.first + size);
+  return p;
+}
 
 template <int DP>
 constexpr int few_waves() {
@@ -166,7 +218,11 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q4 = lane >> 4;
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int h = blockIdx.y;
+  const Part part = find_part(a, blockIdx.x, blockIdx.z, kChunk, kGrain);
+  const int b = __builtin_amdgcn_readfirstlane(part.b);
+  const int split = __builtin_amdgcn_readfirstlane(part.slot);
+  if (split < 0) return;
   int row0, n;
   c.rows(b, row0, n);
   const int len = min(max(c.lens[b], 0), c.capacity());
@@ -198,10 +254,8 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     int E = kMinExp;                       // and their unit's exponent
     unsigned dead[(ND + 7) / 8] = {};      // bit 4 (d % 8) + k of d / 8: o[d][k] saw a NaN value
 
-    const int all = (len + kChunk - 1) / kChunk;
-    const int first = min(all, split * (a.split_tokens / kChunk));
-    const int last =
-        split + 1 == a.splits ? all : min(all, first + a.split_tokens / kChunk);
+    const int first = __builtin_amdgcn_readfirstlane(part.first);
+    const int last = __builtin_amdgcn_readfirstlane(part.last);
     // the two blocks of a chunk: entries of the table (read a chunk ahead) and places in the pages
     int id[2], at[2];
     const auto look = [&](int ch) {
@@ -411,9 +465,10 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
 #pragma unroll
     for (int w = 0; w < NW; ++w) L += wave_l[w][wr] * share(w, wr, M);
     const bool writes = tile + wr < rows;
+    const bool alone = part.parts == 1;  // no other part of the sequence: the result itself
     const int64_t orow = (int64_t)(row0 + wi) * a.Hq + h * a.group + (tile + wr - wi * a.group);
     const float out_scale =
-        exp2i(min(max(eM - kLift, -126), 127)) * (a.splits == 1 ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
+        exp2i(min(max(eM - kLift, -126), 127)) * (alone ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
 #pragma unroll
     for (int pass = 0; pass < DP / PASS; ++pass) {
       if (pass) __syncthreads();
@@ -432,7 +487,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
         v[x] *= out_scale;
       }
       if (!writes || d >= D) continue;
-      if (a.splits > 1) {
+      if (!alone) {
         float* const to = a.part + ((int64_t)split * c.T * a.Hq + orow) * D + d;
 #pragma unroll
         for (int x = 0; x < E8; ++x) to[x] = v[x];
@@ -445,9 +500,8 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
       }
     }
     if (writes && threadIdx.x % TR == 0) {
-      if (a.splits > 1)
-        a.part_ml[(int64_t)split * c.T * a.Hq + orow] = float2{M, L};
-      else if (a.lse)
+      if (!alone || a.scores) a.part_ml[(int64_t)split * c.T * a.Hq + orow] = float2{M, L};
+      if (alone && a.lse)
         a.lse[orow] = L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * kLn2;
     }
   }
@@ -818,49 +872,74 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   }
 }
 
-// The splits' sums of the rows, in a fixed order.  D / 4 threads go over every `ways`-th split of a
-// row, and the first of these groups adds up what the others found.
+// How many parts sequence b has, as find_part deals them.
+__device__ inline int parts_of(const Attn& a, int b, int chunk, int grain) {
+  if (!a.dealt) return a.splits;
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 63;
+  const int mine = lane < c.B ? (held(c, lane) + chunk - 1) / chunk : 0;
+  float sum = (float)mine;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  int n = max(1, (int)((float)mine * (float)(a.splits - c.B) / fmaxf(sum, 1.f) + 0.5f));
+  n = min(n, max(1, (mine + grain - 1) / grain));
+  return __shfl(n, b);
+}
+
+// The parts' sums of a sequence's rows, in a fixed order.  D / 4 threads go over every `ways`-th part
+// of a row, and the first of these groups adds up what the others found.  Workgroup: (some rows of
+// the cached head's, head, sequence).
 template <int DT>
-__global__ __launch_bounds__(256) void attn_join_kernel(Attn a, int ways) {
+__device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b) {
   using H = Half<DT>;
   __shared__ f32x4 part_v[256];
   __shared__ float part_l[64];
-  const int width = a.c.D / 4, groups = 256 / width / ways * ways;
+  const Cache& c = a.c;
+  int row0, n;
+  c.rows(b, row0, n);
+  const int rows = n * a.group;
+  const int parts = parts_of(a, b, kChunk, kGrain);
+  if (a.dealt && parts == 1) return;  // written already
+  const int64_t all = (int64_t)c.T * a.Hq;
+  const int width = c.D / 4, groups = 256 / width / ways * ways, per = groups / ways;
   const int g = threadIdx.x / width, d = (threadIdx.x - g * width) * 4, way = g % ways;
-  const int64_t rows = (int64_t)a.c.T * a.Hq;
-  const int64_t row = (int64_t)blockIdx.x * (groups / ways) + g / ways;
-  const bool works = g < groups && row < rows;
-  float M = -__builtin_inff(), L = 0.f;
-  f32x4 v{0, 0, 0, 0};
-  if (works) {
+  for (int r0 = x * per; r0 < rows; r0 += xs * per) {
+    const int r = r0 + g / ways, i = r / a.group;
+    const bool works = g < groups && r < rows;
+    const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (r - i * a.group);
+    float M = -__builtin_inff(), L = 0.f;
+    f32x4 v{0, 0, 0, 0};
+    if (works) {
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[s * rows + row].x);
+      for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[s * all + row].x);
 #pragma unroll 4
-    for (int s = way; s < a.splits; s += ways) {
-      const float2 ml = a.part_ml[s * rows + row];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (s * rows + row) * a.c.D + d);
-      const float f = ml.y == 0.f ? 0.f : exp2f_(ml.x - M);
-      L += ml.y * f;
-      v += x * f;
-    }
-  }
-  if (ways > 1) {
-    part_v[threadIdx.x] = v;
-    if (d == 0 && g < 64) part_l[g] = L;
-    __syncthreads();
-    if (works && way == 0)
-      for (int w = 1; w < ways; ++w) {
-        v += part_v[threadIdx.x + w * width];
-        L += part_l[g + w];
+      for (int s = way; s < parts; s += ways) {
+        const float2 ml = a.part_ml[s * all + row];
+        const f32x4 w = *reinterpret_cast<const f32x4*>(a.part + (s * all + row) * c.D + d);
+        const float f = ml.y == 0.f ? 0.f : exp2f_(ml.x - M);
+        L += ml.y * f;
+        v += w * f;
       }
+    }
+    if (ways > 1) {
+      __syncthreads();
+      part_v[threadIdx.x] = v;
+      if (d == 0 && g < 64) part_l[g] = L;
+      __syncthreads();
+      if (works && way == 0)
+        for (int w = 1; w < ways; ++w) {
+          v += part_v[threadIdx.x + w * width];
+          L += part_l[g + w];
+        }
+    }
+    if (!works || way) continue;
+    v *= L == 0.f ? 0.f : 1.f / L;
+    const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
+                  (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
+    *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + row * c.D + d) = w;
+    if (d == 0 && a.lse)
+      a.lse[row] = L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * kLn2;
   }
-  if (!works || way) return;
-  v *= L == 0.f ? 0.f : 1.f / L;
-  const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
-                (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
-  *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + row * a.c.D + d) = w;
-  if (d == 0 && a.lse)
-    a.lse[row] = L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------------
@@ -940,32 +1019,65 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(Attn a, Weights w) {
   const int h = blockIdx.y, b = blockIdx.z;
   int row0, n;
   a.c.rows(b, row0, n);
-  const int len = min(max(a.c.lens[b], 0), a.c.capacity());
-  if (a.scores && n * a.group <= a.score_rows) {
-    // few rows: their scores were written down
-    const int end = min(len, w.tokens), rows = n * a.group;
-    const float* const s0 =
-        a.scores + ((int64_t)b * a.c.H + h) * a.score_rows * a.score_tokens;
-    float* const to = w.to + b * w.seq + h * w.head;
-    for (int t = blockIdx.x * 256 + threadIdx.x; t < end; t += gridDim.x * 256) {
-      float sum = 0.f;
-      for (int row = 0; row < rows; ++row) {
-        const int i = row / a.group;
-        const float lse = a.lse[(int64_t)(row0 + i) * a.Hq + h * a.group + (row - i * a.group)];
-        const float s = s0[(int64_t)row * a.score_tokens + t];
-        if (t < len - n + i + 1) sum += exp2f_(s - lse * kLog2e);
-      }
-      to[t] += sum;
+  add_weights<DT, DP>(a, w, b, h, row0, n, held(a.c, b));
+}
+
+// Weights of few rows, from the scores that were written down: 4 tokens a thread.  Every row's sum
+// comes from its parts here too, so that this need not wait for their being joined.
+template <int DT, int DP>
+__device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, int h, int b) {
+  __shared__ float lse2[16];
+  const Cache& c = a.c;
+  int row0, n;
+  c.rows(b, row0, n);
+  const int rows = min(n * a.group, a.score_rows), len = held(c, b);
+  const int parts = parts_of(a, b, kChunk, kGrain);
+  const int64_t all = (int64_t)c.T * a.Hq;
+  if ((int)threadIdx.x < rows) {
+    const int i = threadIdx.x / a.group;
+    const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (threadIdx.x - i * a.group);
+    float M = -__builtin_inff(), L = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[s * all + row].x);
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) {
+      const float2 ml = a.part_ml[s * all + row];
+      L += ml.y == 0.f ? 0.f : ml.y * exp2f_(ml.x - M);
     }
-    return;
+    lse2[threadIdx.x] = L == 0.f ? 0.f : M + __builtin_log2f(L);  // 0: sees nothing
   }
-  add_weights<DT, DP>(a, w, b, h, row0, n, len);
+  __syncthreads();
+  const int end = min(len, w.tokens);
+  const float* const s0 = a.scores + ((int64_t)b * c.H + h) * a.score_rows * a.score_tokens;
+  float* const to = w.to + b * w.seq + h * w.head;
+  for (int t = (x * 256 + threadIdx.x) * 4; t < end; t += xs * 1024) {
+    f32x4 sum{0, 0, 0, 0};
+#pragma unroll 4
+    for (int row = 0; row < rows; ++row) {
+      const f32x4 s = *reinterpret_cast<const f32x4*>(s0 + (int64_t)row * a.score_tokens + t);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] += exp2f_(s[k] - lse2[row]);  // unseen: 2^-inf
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (t + k < end) to[t + k] += sum[k];
+  }
+}
+
+// What is left after the parts: blocks x < joins join them, the others add the weights.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void attn_finish_kernel(Attn a, Weights w, int joins, int ways) {
+  const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  if (x < joins)
+    join_parts<DT>(a, ways, x, joins, h, b);
+  else
+    add_few_weights<DT, DP>(a, w, x - joins, gridDim.x - joins, h, b);
 }
 
 // ------------------------------------------------------------------ host side
 struct Plan {
-  bool few;
-  int splits, split_tokens, ways;  // ways: of attn_join_kernel
+  bool few, dealt;
+  int splits, split_tokens, ways;  // ways: of join_parts
   int score_rows, score_tokens;
   size_t part, ml, total;
 };
@@ -982,20 +1094,29 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t len = std::max<int64_t>(1, std::min<int64_t>(s->max_len, capacity));
   const int64_t tiles = p.few ? 1 : (rows + kRows - 1) / kRows;
   const int64_t units = tiles * c->heads * s->seqs;
-  const int step = p.few ? 512 : 4 * kTile;  // a whole number of stages
+  const int step = p.few ? kGrain * kChunk : 4 * kTile;  // a whole number of stages
   const int64_t most = (len + step - 1) / step;
-  const int64_t want =
-      std::max<int64_t>(1, (p.few ? 2 : 2) * (int64_t)fb_gpu::cu_count() / units);
+  // two workgroups a CU run side by side
+  const int64_t slots = 2 * (int64_t)fb_gpu::cu_count();
+  const int64_t want = std::max<int64_t>(1, slots / units);
   const int64_t per = (most + std::min(want, most) - 1) / std::min(want, most);
   p.split_tokens = (int)(per * step);
   p.splits = (int)((most + per - 1) / per);
-  const size_t n = (size_t)s->tokens * q_heads;
-  if (p.splits > 1) {
-    p.part = align256((size_t)p.splits * n * c->head_dim * 4);
-    p.ml = align256((size_t)p.splits * n * 8);
-    // about 4 splits a thread
-    for (p.ways = 1; p.ways * 4 < p.splits && p.ways * 2 * (c->head_dim / 4) <= 256;) p.ways *= 2;
+  int parts = p.splits;  // of one sequence, at most
+  if (p.few && s->seqs > 1 && s->seqs <= 64 && p.splits > 1) {
+    p.dealt = true;
+    p.splits = s->seqs + (int)std::min<int64_t>(std::max<int64_t>(slots / c->heads, s->seqs),
+                                                most * s->seqs);
+    parts = (int)std::min<int64_t>(p.splits - s->seqs, (capacity + step - 1) / step) + 1;
   }
+  const size_t n = (size_t)s->tokens * q_heads;
+  p.ways = 1;
+  if (parts > 1) {
+    p.part = align256((size_t)parts * n * c->head_dim * 4);
+    // about 4 parts a thread
+    while (p.ways * 4 < parts && p.ways * 2 * (c->head_dim / 4) <= 256) p.ways *= 2;
+  }
+  if (parts > 1 || (p.few && w_tokens > 0)) p.ml = align256((size_t)parts * n * 8);
   p.total = p.part + p.ml;
   if (p.few && w_tokens > 0) {
     p.score_rows = (int)rows;
@@ -1018,7 +1139,7 @@ template <int DT, int DP, bool EX>
 int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, const Weights& w, hipStream_t hs) {
   const int64_t rows = (int64_t)std::min(s->max_new, s->tokens) * a.group;
   if (p.few) {
-    hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, a.c.B),
+    hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, p.dealt ? 1 : a.c.B),
                        dim3(64 * few_waves<DP>()), 0, hs, a);
   } else {
     const int64_t nx = (int64_t)a.c.H * a.c.B * p.splits;
@@ -1028,19 +1149,20 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, const Weights& w, h
                        0, hs, a);
   }
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
-  if (p.splits > 1) {
-    const int64_t n = (int64_t)a.c.T * a.Hq;
-    const int64_t rows = 256 / (a.c.D / 4) / p.ways;  // of a workgroup
-    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)((n + rows - 1) / rows)), dim3(256), 0,
-                       hs, a, p.ways);
+  const int64_t cap = std::min<int64_t>((int64_t)a.c.max_pages * a.c.P, w.tokens);
+  const int64_t len = std::max<int64_t>(1, std::min<int64_t>(cap, s->max_len));
+  const int64_t per = 256 / (a.c.D / 4) / p.ways;  // rows of a joining workgroup
+  const int joins = p.part ? (int)std::min<int64_t>((rows + per - 1) / per, 1 << 20) : 0;
+  const int adds = a.scores ? (int)((len + 1023) / 1024) : 0;
+  if (joins + adds) {
+    hipLaunchKernelGGL((attn_finish_kernel<DT, DP>), dim3(joins + adds, a.c.H, a.c.B), dim3(256), 0,
+                       hs, a, w, joins, p.ways);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
-  if (w.to) {
-    const int64_t cap = std::min<int64_t>((int64_t)a.c.max_pages * a.c.P, w.tokens);
-    const int64_t len = std::max<int64_t>(1, std::min<int64_t>(cap, s->max_len));
-    const int64_t nx = (len + (a.scores ? 255 : 127)) / (a.scores ? 256 : 128);
-    hipLaunchKernelGGL((attn_weights_kernel<DT, DP>), dim3((unsigned)nx, a.c.H, a.c.B), dim3(256), 0,
-                       hs, a, w);
+  if (w.to && !a.scores) {
+    hipLaunchKernelGGL((attn_weights_kernel<DT, DP>),
+                       dim3((unsigned)std::min<int64_t>((len + 127) / 128, 1 << 20), a.c.H, a.c.B),
+                       dim3(256), 0, hs, a, w);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
   return FB_OK;
@@ -1088,6 +1210,7 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   a.lse = lse;
   a.splits = p.splits;
   a.split_tokens = p.split_tokens;
+  a.dealt = p.dealt;
   a.part = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.part);
   const int per = c->page / kBlock;

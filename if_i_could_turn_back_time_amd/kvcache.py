@@ -107,7 +107,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: 
     sequence's n new rows sees the first ``lens - n + i + 1`` tokens.  A row that sees none gets
     0 (and an lse of -inf).  A value of a token that a row does not see never reaches it, NaN or
     not.  ``cu_seqlens`` and ``max_new`` as for :func:`cache_append` (``max_new`` too small
-    changes speed only); ``max_len``: about the longest length, by which the work is split.
+    changes speed only, except that ``weights`` may miss the rows beyond it); ``max_len``: about
+    the longest length, by which the work is split.
 
     ``weights`` (fp32 [sequences, heads, at least max_len]): grows in place by the attention
     weight that each held token got in this call, summed over rows and query heads; what
