@@ -43,6 +43,13 @@ struct Attn {
   int per_shift;      // log2 of a page's blocks, -1: no power of two
   float* scores;      // or null: [B][H][score_rows][score_tokens], base 2
   int score_rows, score_tokens;
+  unsigned div_mul, div_shift;
+
+  // row / group, of rows below 2^31: (mulhi(row, m) + row) >> s with s = ceil(log2 group) and
+  // m = floor(2^32 (2^s - group) / group) + 1
+  __device__ int token_of(int row) const {
+    return (int)((__umulhi((unsigned)row, div_mul) + (unsigned)row) >> div_shift);
+  }
 };
 
 __device__ inline float exp2f_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -233,11 +240,11 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
   const int k_from = (16 * ((r >> 2) & 1) + (r & 3)) * D + q4 * 16;
   const int v_from = ((q4 & 1) * D + r) * 16;
   for (int tile = 0; tile < rows; tile += 16) {
-    const int row = tile + r, i = row / a.group;
+    const int row = tile + r, i = a.token_of(row);
     const bool there = row < rows;
     const int head = h * a.group + (row - i * a.group);
     const int sees = there ? min(max(len - n + i + 1, 0), len) : 0;
-    const int least = min(max(len - n + tile / a.group + 1, 0), len);  // of the tile's rows
+    const int least = min(max(len - n + a.token_of(tile) + 1, 0), len);  // of the tile's rows
     typename H::x8 qf[NP][2];
 #pragma unroll
     for (int p = 0; p < NP; ++p)
@@ -459,7 +466,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     const float mine = share(wave, r, largest(r)) * exp2i(max(E - eM, -126));
     // of the row that this thread writes
     constexpr int TR = 4 * NW, E8 = PASS / TR;  // threads of a row, channels of a thread
-    const int wr = threadIdx.x / TR, wi = (tile + wr) / a.group;
+    const int wr = threadIdx.x / TR, wi = a.token_of(tile + wr);
     const float M = largest(wr);
     float L = 0.f;
 #pragma unroll
@@ -587,17 +594,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   const int32_t* const table = c.table + b * c.table_stride;
   for (int ti = blockIdx.y; ti < tiles; ti += gridDim.y) {
     const int tile = (tiles - 1 - ti) * kRows;  // the longest first
-    const int row = tile + wave * 32 + r, i = row / a.group;
+    const int row = tile + wave * 32 + r, i = a.token_of(row);
     const bool there = row < rows;
     const int head = h * a.group + (row - i * a.group);
     const int sees = there ? min(max(len - n + i + 1, 0), len) : 0;
     // least and most that the wave's and the workgroup's rows see
-    const int i_lo = (tile + wave * 32) / a.group;
+    const int i_lo = a.token_of(tile + wave * 32);
     const int least = min(max(len - n + i_lo + 1, 0), len);
-    const int least_wg = min(max(len - n + tile / a.group + 1, 0), len);
-    const int i_hi = (min(tile + wave * 32 + 32, rows) - 1) / a.group;
+    const int least_wg = min(max(len - n + a.token_of(tile) + 1, 0), len);
+    const int i_hi = a.token_of(min(tile + wave * 32 + 32, rows) - 1);
     const int wave_most = tile + wave * 32 < rows ? min(max(len - n + i_hi + 1, 0), len) : 0;
-    const int j_hi = (min(tile + kRows, rows) - 1) / a.group;
+    const int j_hi = a.token_of(min(tile + kRows, rows) - 1);
     const int most = min(max(len - n + j_hi + 1, 0), len);
     typename H::x8 qf[NP][2];
 #pragma unroll
@@ -904,7 +911,7 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
   const int width = c.D / 4, groups = 256 / width / ways * ways, per = groups / ways;
   const int g = threadIdx.x / width, d = (threadIdx.x - g * width) * 4, way = g % ways;
   for (int r0 = x * per; r0 < rows; r0 += xs * per) {
-    const int r = r0 + g / ways, i = r / a.group;
+    const int r = r0 + g / ways, i = a.token_of(r);
     const bool works = g < groups && r < rows;
     const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (r - i * a.group);
     float M = -__builtin_inff(), L = 0.f;
@@ -943,83 +950,186 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
 }
 
 // ---------------------------------------------------------------------------------
-// Accumulated weights: weights[t] += sum over the rows of exp(score - lse).  Workgroup = (128
-// tokens, head, sequence), each wave holds 32 tokens' keys as operands and walks over the rows
-// that see them, so that every sum belongs to one wave and is added in row order.
+// Accumulated weights of many rows: weights[t] += sum over the rows of exp(score - lse).  Workgroup =
+// (head and sequence, 256 tokens, a run of the rows).  Each wave holds 64 tokens' keys (32 of the
+// widest), decoded, as operands; the rows go to LDS, 128 at a time and straight from memory, and an operand that is read
+// there meets both blocks of keys (with one block the LDS reads took as long as the products).  A
+// lane's sums are of 16 tokens a block over the rows of its column, so nothing crosses lanes before
+// the end.  Runs of rows leave their sums apart, which
+// a last small kernel adds in order: no atomics.  Half the products of the attention itself.
 // ---------------------------------------------------------------------------------
 struct Weights {
   float* to;
   int64_t seq, head;
   int tokens;
+  float* part;   // or null: [runs][B][H][part_tokens]
+  int part_tokens, runs, run_rows;
 };
 
-template <int DT, int DP>
-__device__ void add_weights(const Attn& a, const Weights& w, int b, int h, int row0, int n,
-                            int len) {
-  using H = Half<DT>;
-  constexpr int NP = DP / 32;
-  const Cache& c = a.c;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 31, x2 = lane >> 5;
-  const int rows = n * a.group;
-  const int end = min(len, w.tokens);
-  for (int blk = blockIdx.x * 4 + wave; blk * kBlock < end; blk += gridDim.x * 4) {
-    int at;
-    const int page = max(c.page_of(b, blk, at), 0);
-    const int64_t bi = c.block_index(page, h, at);
-    u32x4 kf[NP];
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-      kf[p] = 32 * p + 16 * x2 < c.D ? *reinterpret_cast<const u32x4*>(
-                                           c.k + (bi * kBlock + r) * c.D + 32 * p + 16 * x2)
-                                     : u32x4{0, 0, 0, 0};
-    const float ks = a.scale2 * exp2i(min(max((int)c.ks[bi] - 127, -126), 127));
-    f32x16 sum;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) sum[k] = 0.f;
-    // the first row that sees the block's first token
-    const int from = max(blk * kBlock - (len - n), 0) * a.group / 32 * 32;
-    for (int tile = from; tile < rows; tile += 32) {
-      const int row = tile + r, i = row / a.group;
-      const bool there = row < rows;
-      const int head = h * a.group + (row - i * a.group);
-      const int sees = there ? min(max(len - n + i + 1, 0), len) : 0;
-      const float lse = there ? a.lse[(int64_t)(row0 + i) * a.Hq + head] * kLog2e : 0.f;
-      f32x16 s;
-#pragma unroll
-      for (int k = 0; k < 16; ++k) s[k] = 0.f;
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int d = 32 * p + 16 * x2 + 8 * u;
-          const auto qf = load_q<DT>(a, there && d < c.D,
-                                     (int64_t)(row0 + i) * a.q_token + head * a.q_head + d);
-          s = H::mfma32(H::decode(kf[p][2 * u], kf[p][2 * u + 1]), qf, s);
-        }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const int t = blk * kBlock + 8 * (k / 4) + 4 * x2 + k % 4;
-        if (t < sees) sum[k] += exp2f_(s[k] * ks - lse);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      float v = sum[k];
-#pragma unroll
-      for (int o = 16; o; o >>= 1) v += __shfl_xor(v, o);
-      const int t = blk * kBlock + 8 * (k / 4) + 4 * x2 + k % 4;
-      if (r == k && t < end) w.to[b * w.seq + h * w.head + t] += v;
-    }
-  }
+template <int DP>
+constexpr int weight_rows() {  // that are staged at once
+  return DP > 128 ? 32 : 128;
+}
+
+template <int DP>
+constexpr int weight_blocks() {  // of a wave
+  return DP > 128 ? 1 : 2;
 }
 
 template <int DT, int DP>
-__global__ __launch_bounds__(256) void attn_weights_kernel(Attn a, Weights w) {
-  const int h = blockIdx.y, b = blockIdx.z;
+__global__ __launch_bounds__(256, 2) void attn_weights_kernel(Attn a, Weights w) {
+  using H = Half<DT>;
+  constexpr int NP = DP / 32, NQ = DP / 8;   // 16-byte pieces of a row of q
+  constexpr int ROWS = weight_rows<DP>();
+  constexpr int NL = ROWS * NQ / 256;        // of which a thread loads so many
+  // arrays of their own, as in attn_many_kernel
+  __shared__ __align__(16) uint8_t lq0[ROWS * DP * 2], lq1[ROWS * DP * 2];
+  __shared__ float lse2[2][ROWS];
+  constexpr int KB = weight_blocks<DP>(), TOKENS = 4 * KB * kBlock;
+  const Cache& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, x2 = lane >> 5;
+  const int h = blockIdx.x % c.H, b = blockIdx.x / c.H, run = blockIdx.z;
   int row0, n;
-  a.c.rows(b, row0, n);
-  add_weights<DT, DP>(a, w, b, h, row0, n, held(a.c, b));
+  c.rows(b, row0, n);
+  const int len = held(c, b), rows = n * a.group;
+  const int end = min(len, w.tokens);
+  // where piece pc of a row lies: the lanes that one LDS read serves (0-3, 12-15, 20-27) read
+  // equal pieces of their rows from different banks
+  const auto exchange = [](int row, int pc) {
+    return pc ^ (NQ == 8 ? (row >> 1) & 7 : row & 15);
+  };
+  for (int tile = blockIdx.y * TOKENS; tile < end; tile += gridDim.y * TOKENS) {
+    const int t0 = tile + wave * KB * kBlock;  // the wave's tokens
+    typename H::x8 kf[KB][NP][2];
+    float ks[KB], sum[KB][16];
+#pragma unroll
+    for (int z = 0; z < KB; ++z) {
+      int at;
+      const int page = max(c.page_of(b, t0 / kBlock + z, at), 0);
+      const int64_t bi = c.block_index(page, h, at);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        // zeros past D: q's pieces there are others of the same row
+        const int ch = 32 * p + 16 * x2;
+        u32x4 k{0, 0, 0, 0};
+        if (ch < c.D) k = *reinterpret_cast<const u32x4*>(c.k + (bi * kBlock + r) * c.D + ch);
+        kf[z][p][0] = H::decode(k[0], k[1]);
+        kf[z][p][1] = H::decode(k[2], k[3]);
+      }
+      ks[z] = a.scale2 * exp2i(min(max((int)c.ks[bi] - 127, -126), 127));
+#pragma unroll
+      for (int k = 0; k < 16; ++k) sum[z][k] = 0.f;
+    }
+    // the rows that see the tile's first token, of the run
+    const int seeing = max(tile - (len - n), 0) * a.group;
+    const int from = max(run * w.run_rows, seeing / ROWS * ROWS);
+    const int to = run + 1 == w.runs ? rows : min(rows, (run + 1) * w.run_rows);
+    float next_lse = 0.f;
+    const auto fetch = [&](uint8_t* buf, int first) __attribute__((always_inline)) {
+#pragma unroll
+      for (int x = 0; x < NL; ++x) {
+        // a wave's 64 pieces lie side by side in LDS
+        const int e = (wave * NL + x) * 64 + lane, at = e / NQ;
+        const int row = min(first + at, to - 1), i = a.token_of(row);
+        const int pc = exchange(at, e % NQ);
+        load_to_lds(static_cast<const uint8_t*>(a.q) +
+                        2 * ((int64_t)(row0 + i) * a.q_token +
+                             (h * a.group + (row - i * a.group)) * a.q_head +
+                             (pc * 8 < c.D ? pc : pc % (c.D / 8)) * 8),
+                    buf + (wave * NL + x) * 1024);
+      }
+      if (tid < ROWS) {
+        const int row = min(first + tid, to - 1), i = a.token_of(row);
+        next_lse = a.lse[(int64_t)(row0 + i) * a.Hq + h * a.group + (row - i * a.group)];
+      }
+    };
+    const auto stage = [&](int first, const uint8_t* buf, uint8_t* other, int parity)
+        __attribute__((always_inline)) {
+      // a row that sees nothing gives no weight
+      if (tid < ROWS)
+        lse2[parity][tid] =
+            next_lse == -__builtin_inff() ? __builtin_inff() : next_lse * kLog2e;
+      __syncthreads();  // these rows are there; everyone is done with the other buffer
+      if (first + ROWS < to) fetch(other, first + ROWS);
+#pragma unroll 1
+      for (int y = 0; y < ROWS / 32; ++y) {
+        f32x16 s[KB];
+#pragma unroll
+        for (int z = 0; z < KB; ++z)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) s[z][k] = 0.f;
+        const int row = y * 32 + r;
+        const auto read = [&](int i) {
+          return *reinterpret_cast<const typename H::x8*>(
+              buf + row * DP * 2 + exchange(row, 4 * (i / 2) + 2 * x2 + (i & 1)) * 16);
+        };
+        typename H::x8 q[3] = {read(0), read(1), read(2)};  // read three ahead
+#pragma unroll
+        for (int i = 0; i < 2 * NP; ++i) {
+          const auto now = q[i % 3];
+          if (i + 3 < 2 * NP) q[i % 3] = read(i + 3);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int z = 0; z < KB; ++z) s[z] = H::mfma32(kf[z][i / 2][i & 1], now, s[z]);
+        }
+        const float l = lse2[parity][row];
+        // the tile's least row against the wave's last token, its last against the run's end
+        const bool masked = a.token_of(first + y * 32) + len - n + 1 < t0 + KB * kBlock ||
+                            first + y * 32 + 32 > to;
+        if (masked) {
+          asm volatile("");  // a branch, not selects in every tile
+          const int seen = first + row < to
+                               ? len - n + a.token_of(first + row) + 1 - t0 - 4 * x2
+                               : INT32_MIN;
+#pragma unroll
+          for (int z = 0; z < KB; ++z)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (z * kBlock + 8 * (k / 4) + k % 4 >= seen) s[z][k] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int z = 0; z < KB; ++z)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            sum[z][k] += exp2f_(__builtin_fmaf(s[z][k], ks[z], -l));
+      }
+    };
+    __syncthreads();  // the buffers of the tile before are free
+    if (from < to) fetch(lq0, from);
+    for (int first = from; first < to; first += 2 * ROWS) {
+      stage(first, lq0, lq1, 0);
+      if (first + ROWS < to) stage(first + ROWS, lq1, lq0, 1);
+    }
+#pragma unroll
+    for (int z = 0; z < KB; ++z)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        float v = sum[z][k];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor(v, o);
+        const int t = t0 + z * kBlock + 8 * (k / 4) + 4 * x2 + k % 4;
+        if (r == k && t < end) {
+          if (w.part)
+            w.part[((int64_t)(run * c.B + b) * c.H + h) * w.part_tokens + t] = v;
+          else
+            w.to[b * w.seq + h * w.head + t] += v;
+        }
+      }
+  }
+}
+
+// Adds the runs' sums, in order.
+__global__ __launch_bounds__(256) void attn_weights_join_kernel(Cache c, Weights w) {
+  const int h = blockIdx.y, b = blockIdx.z, end = min(held(c, b), w.tokens);
+  for (int t = blockIdx.x * 256 + threadIdx.x; t < end; t += gridDim.x * 256) {
+    float v = 0.f;
+#pragma unroll 4
+    for (int run = 0; run < w.runs; ++run)
+      v += w.part[((int64_t)(run * c.B + b) * c.H + h) * w.part_tokens + t];
+    w.to[b * w.seq + h * w.head + t] += v;
+  }
 }
 
 // Weights of few rows, from the scores that were written down: 4 tokens a thread.  Every row's sum
@@ -1034,7 +1144,7 @@ __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, 
   const int parts = parts_of(a, b, kChunk, kGrain);
   const int64_t all = (int64_t)c.T * a.Hq;
   if ((int)threadIdx.x < rows) {
-    const int i = threadIdx.x / a.group;
+    const int i = a.token_of(threadIdx.x);
     const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (threadIdx.x - i * a.group);
     float M = -__builtin_inff(), L = 0.f;
 #pragma unroll 8
@@ -1079,6 +1189,7 @@ struct Plan {
   bool few, dealt;
   int splits, split_tokens, ways;  // ways: of join_parts
   int score_rows, score_tokens;
+  int runs, run_rows;              // of attn_weights_kernel
   size_t part, ml, total;
 };
 
@@ -1122,6 +1233,17 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
     p.score_rows = (int)rows;
     p.score_tokens = (w_tokens + kChunk - 1) / kChunk * kChunk;
     p.total += align256((size_t)s->seqs * c->heads * p.score_rows * p.score_tokens * 4);
+  } else if (w_tokens > 0) {
+    // runs of rows until there are 6 workgroups for each place (a causal prompt leaves half of
+    // them empty), of 512 rows or more
+    const int tokens = c->head_dim > 128 ? 4 * kBlock : 8 * kBlock;  // of a workgroup
+    const int64_t wgs = (len + tokens - 1) / tokens * c->heads * s->seqs;
+    const int64_t runs = std::min((6 * slots + wgs - 1) / wgs, (rows + 511) / 512);
+    p.run_rows = (int)((rows + runs - 1) / runs + 127) / 128 * 128;  // whole stages
+    p.runs = (int)((rows + p.run_rows - 1) / p.run_rows);
+    p.score_tokens = w_tokens;
+    if (p.runs > 1)
+      p.total += align256((size_t)p.runs * s->seqs * c->heads * p.score_tokens * 4);
   }
   return p;
 }
@@ -1136,7 +1258,7 @@ int check_attention(const fb_cache_t* c, const fb_seqs_t* s, int32_t q_heads, Ca
 }
 
 template <int DT, int DP, bool EX>
-int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, const Weights& w, hipStream_t hs) {
+int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, Weights w, hipStream_t hs) {
   const int64_t rows = (int64_t)std::min(s->max_new, s->tokens) * a.group;
   if (p.few) {
     hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, p.dealt ? 1 : a.c.B),
@@ -1160,10 +1282,16 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, const Weights& w, h
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
   if (w.to && !a.scores) {
-    hipLaunchKernelGGL((attn_weights_kernel<DT, DP>),
-                       dim3((unsigned)std::min<int64_t>((len + 127) / 128, 1 << 20), a.c.H, a.c.B),
-                       dim3(256), 0, hs, a, w);
+    const int tokens = 4 * weight_blocks<DP>() * kBlock;
+    const unsigned ny = (unsigned)std::min<int64_t>((len + tokens - 1) / tokens, 65535);
+    hipLaunchKernelGGL((attn_weights_kernel<DT, DP>), dim3(a.c.H * a.c.B, ny, p.runs), dim3(256), 0,
+                       hs, a, w);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+    if (w.part) {
+      hipLaunchKernelGGL(attn_weights_join_kernel, dim3((unsigned)((len + 255) / 256), a.c.H, a.c.B),
+                         dim3(256), 0, hs, a.c, w);
+      if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+    }
   }
   return FB_OK;
 }
@@ -1196,6 +1324,10 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
       (reinterpret_cast<uintptr_t>(ws) & 255u))
     return FB_ERR_ALIGN;
   const Plan p = plan(c, s, q_heads, weights ? w_tokens : 0);
+  // the rows of q go to LDS 16 bytes at a time there
+  if (weights && !p.few &&
+      ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(q_token * 2) | (uintptr_t)(q_head * 2)) & 15u))
+    return FB_ERR_ALIGN;
   if (p.total && !ws) return FB_ERR_NULL;
   if (p.total > ws_bytes) return FB_ERR_WORKSPACE;
   a.q = q;
@@ -1205,6 +1337,8 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
               15u);
   a.Hq = q_heads;
   a.group = q_heads / c->heads;
+  while ((1u << a.div_shift) < (unsigned)a.group) ++a.div_shift;
+  a.div_mul = (unsigned)((((uint64_t)1 << 32) * (((uint64_t)1 << a.div_shift) - a.group)) / a.group) + 1;
   a.scale2 = scale * kLog2e;
   a.out = out;
   a.lse = lse;
@@ -1215,12 +1349,16 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.part);
   const int per = c->page / kBlock;
   a.per_shift = per & (per - 1) ? -1 : __builtin_ctz(per);
+  float* const rest = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part + p.ml);
+  Weights w{weights, w_seq, w_head, w_tokens, nullptr, 0, p.runs, p.run_rows};
   if (p.score_rows) {
-    a.scores = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part + p.ml);
+    a.scores = rest;
     a.score_rows = p.score_rows;
     a.score_tokens = p.score_tokens;
+  } else if (p.runs > 1) {
+    w.part = rest;
+    w.part_tokens = p.score_tokens;
   }
-  const Weights w{weights, w_seq, w_head, w_tokens};
   hipStream_t hs = static_cast<hipStream_t>(stream);
   const auto go = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

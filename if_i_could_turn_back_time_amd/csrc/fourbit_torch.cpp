@@ -364,23 +364,24 @@ void cache_append(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& 
 }
 
 std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
-    const at::Tensor& q, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& cks,
+    const at::Tensor& given, const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& cks,
     const at::Tensor& cvs, const at::Tensor& table, const at::Tensor& lens,
     const std::optional<at::Tensor>& cu, std::optional<int64_t> max_new,
     std::optional<int64_t> max_len, std::optional<double> scale,
     const std::optional<at::Tensor>& weights, bool want_lse) {
   const fb_cache_t c = cache_of(ck, cv, cks, cvs);
-  want_plain(q, ck, "q must be a tensor on the cache's GPU");
-  no_grad_through({q}, "attention over the cache has no gradient: call it under torch.no_grad() "
+  want_plain(given, ck, "q must be a tensor on the cache's GPU");
+  no_grad_through({given}, "attention over the cache has no gradient: call it under torch.no_grad() "
                        "or with a detached q");
-  want(q.dim() == 3 && q.size(2) == c.head_dim && (q.stride(2) == 1 || c.head_dim == 1),
+  want(given.dim() == 3 && given.size(2) == c.head_dim &&
+           (given.stride(2) == 1 || c.head_dim == 1),
        "q must be [tokens, query heads, D] with the cache's D, D contiguous");
-  want(q.size(1) >= c.heads && q.size(1) % c.heads == 0 && q.size(1) <= INT32_MAX,
+  want(given.size(1) >= c.heads && given.size(1) % c.heads == 0 && given.size(1) <= INT32_MAX,
        "the query heads must be a multiple of the cache's heads");
-  want(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+  want(given.scalar_type() == at::kHalf || given.scalar_type() == at::kBFloat16,
        "q must be float16 or bfloat16");
   want(!scale || (*scale > 0 && *scale < 1e30), "scale must be positive");
-  const fb_seqs_t s = seqs_of(table, lens, cu, q.size(0), max_new, max_len, c.page, ck);
+  const fb_seqs_t s = seqs_of(table, lens, cu, given.size(0), max_new, max_len, c.page, ck);
   float* wp = nullptr;
   if (weights) {
     want_plain(*weights, ck, "weights must be a tensor on the cache's GPU");
@@ -395,6 +396,12 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
     wp = static_cast<float*>(weights->data_ptr());
   }
   c10::DeviceGuard guard(ck.device());
+  // many rows' weights want q 16-byte aligned; a tensor of its own is
+  const at::Tensor q = wp && ((reinterpret_cast<uintptr_t>(given.data_ptr()) |
+                               (uintptr_t)(given.stride(0) * 2) | (uintptr_t)(given.stride(1) * 2)) &
+                              15u)
+                           ? given.clone(at::MemoryFormat::Contiguous)
+                           : given;
   at::Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   at::Tensor lse;
   if (want_lse || wp) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));

@@ -487,7 +487,8 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
  *   lse    fp32 [tokens, q_heads] or NULL: log of the sum of exp(scale * q.k)
  *   weights fp32 [seqs, heads, >= max_len] or NULL: weights[b, h, t] grows by the attention
  *          weight that token t got from all rows and query heads of this call (needs lse; rows
- *          beyond max_new may be missed here, and only here)
+ *          beyond max_new may be missed here, and only here).  With more than 16 rows a cached
+ *          head and sequence q must then be 16-byte aligned, its strides too
  *   ws     256-byte aligned, fb_cache_attention_workspace_bytes (its contents are not kept)
  * A row that sees no token gets 0, with an lse of -inf.  Products are exact and summed in fp32;
  * attention weights enter the sum over v as fp16 (relative to the row's largest).  Page numbers

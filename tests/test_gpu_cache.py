@@ -475,3 +475,11 @@ def test_refusals():
     with pytest.raises(ValueError):
         KVCache.new(4, 2, 72, 64, DEV)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("D,group,page", [(64, 3, 32), (80, 2, 96), (128, 20, 64), (256, 1, 32)])
+def test_weights_of_many_rows(D, group, page):
+    """Several runs of rows, rows that fill no tile, widths that fill no operand, q off alignment."""
+    c = Case([700, 330], 2, D, page, torch.float16)
+    w = torch.zeros(2, 2, 701, device=DEV)
+    c.attend([650, 100] if group < 10 else [90, 40], group, weights=w, q_view=True, max_len=700)
