@@ -96,15 +96,24 @@ __device__ inline float finite_abs(float v) {
   return a < __builtin_inff() ? a : 0.f;
 }
 
-// Eight values, scaled into range already, as E4M3 codes: round to nearest even; what is not
-// finite becomes NaN.
-__device__ inline u32x2 encode8(const float (&v)[8]) {
+// Eight finite values, scaled into range already, as E4M3 codes: round to nearest even.
+__device__ inline u32x2 encode8_finite(const float (&v)[8]) {
   u32x2 r;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     int x = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * w], v[4 * w + 1], 0, false);
     x = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * w + 2], v[4 * w + 3], x, true);
-    unsigned u = (unsigned)x;
+    r[w] = (unsigned)x;
+  }
+  return r;
+}
+
+// The same of any values: what is not finite becomes NaN.
+__device__ inline u32x2 encode8(const float (&v)[8]) {
+  u32x2 r = encode8_finite(v);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    unsigned u = r[w];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (!(__builtin_fabsf(v[4 * w + j]) < __builtin_inff()))
@@ -123,37 +132,6 @@ __device__ inline void decode8(u32x2 c, float (&v)[8]) {
     v[4 * w + 1] = lo[1];
     v[4 * w + 2] = hi[0];
     v[4 * w + 3] = hi[1];
-  }
-}
-
-// Eight values of a tensor of dtype DT; `vec`: 16-byte aligned (32 for FB_DT_F32 as two).
-template <int DT>
-__device__ inline void load8(const void* base, int64_t at, bool vec, float (&v)[8]) {
-  if constexpr (DT == FB_DT_F32) {
-    const float* p = static_cast<const float*>(base) + at;
-    if (vec) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = p[j];
-    }
-  } else {
-    const unsigned short* p = static_cast<const unsigned short*>(base) + at;
-    unsigned short u[8];
-    if (vec) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = (unsigned short)(a[j / 2] >> (16 * (j & 1)));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = p[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = DT == FB_DT_F16 ? (float)__builtin_bit_cast(_Float16, u[j])
-                             : __builtin_bit_cast(float, (unsigned)u[j] << 16);
   }
 }
 

@@ -7,15 +7,80 @@ namespace {
 
 using namespace fbc;
 
-// Largest of the workgroup's 256 values; `lds` holds 4 floats.  Every thread calls it.
-__device__ inline float block_max(float v, float* lds) {
+// Largest of the workgroup's values; `lds` holds 4.  Every thread calls it, once for each `lds`.
+__device__ inline unsigned block_max(unsigned v, unsigned* lds) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  for (int o = 32; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+  for (int w = 0; w < (int)blockDim.x / 64; ++w) v = max(v, lds[w]);
   return v;
 }
+
+// Eight values of a tensor of dtype DT, as they lie.
+template <int DT>
+struct Eight {
+  static constexpr int kWords = DT == FB_DT_F32 ? 8 : 4;
+  unsigned w[kWords];
+
+  __device__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  __device__ void load(const void* base, int64_t at, bool vec) {
+    const char* const p = static_cast<const char*>(base) + at * (DT == FB_DT_F32 ? 4 : 2);
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const u32x4 x = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * i + j] = x[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (DT == FB_DT_F32) {
+          w[i] = reinterpret_cast<const unsigned*>(p)[i];
+        } else {
+          const unsigned short* const u = reinterpret_cast<const unsigned short*>(p) + 2 * i;
+          w[i] = (unsigned)u[0] | (unsigned)u[1] << 16;
+        }
+      }
+    }
+  }
+  __device__ float value(int j) const {
+    if constexpr (DT == FB_DT_F32) {
+      return __builtin_bit_cast(float, w[j]);
+    } else {
+      const unsigned short u = (unsigned short)(w[j / 2] >> (16 * (j & 1)));
+      return DT == FB_DT_F16 ? (float)__builtin_bit_cast(_Float16, u)
+                             : __builtin_bit_cast(float, (unsigned)u << 16);
+    }
+  }
+  // Largest magnitude among these and `m`, as bits: of a type's values they are in order.
+  __device__ unsigned max_bits(unsigned m) const {
+    if constexpr (DT == FB_DT_F32) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+      return m;
+    } else {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 x = {(unsigned short)m, 0};
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const unsigned bits = w[i] & 0x7FFF7FFFu;
+        x = __builtin_elementwise_max(x, __builtin_bit_cast(u16x2, bits));
+      }
+      return max((unsigned)x[0], (unsigned)x[1]);
+    }
+  }
+  static constexpr unsigned kInf = DT == FB_DT_F32 ? 0x7F800000u : DT == FB_DT_F16 ? 0x7C00u : 0x7F80u;
+  static __device__ float magnitude(unsigned bits) {
+    if constexpr (DT == FB_DT_F32) return __builtin_bit_cast(float, bits);
+    if constexpr (DT == FB_DT_F16) return (float)__builtin_bit_cast(_Float16, (unsigned short)bits);
+    return __builtin_bit_cast(float, bits << 16);
+  }
+};
 
 struct NewTokens {
   const void *k, *v;
@@ -25,15 +90,16 @@ struct NewTokens {
 
 // ---------------------------------------------------------------------------------
 // Append.  Workgroup = (sequence, head, keys or values) x (one block of 32 tokens that gets new
-// ones): the block's scale needs all of its new values, 32 D at most, which stay in registers
-// (8 channels of one token per thread and step) between the maximum and the codes.  A value
-// block is turned to its 16-token sides through LDS when it is full; single tokens are written
-// byte by byte.  Earlier codes are read only where the scale grows.
+// ones), D threads rounded up to whole waves: the block's scale needs all of its new values, 32 D
+// at most, which stay in registers as they came (4 tokens of 8 channels a thread) between the
+// maximum, taken over their bits, and the codes.  Four tokens of a value's channel become one
+// word; a full block's words go through LDS to whole 16-token sides.  Earlier codes are read only
+// where the scale grows, and only a block that holds something not finite looks for it.
 // ---------------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(256) void cache_append_kernel(Cache c, NewTokens x) {
-  __shared__ float red[4];
-  __shared__ __align__(16) uint8_t side[kBlock * kMaxDim];
+  __shared__ unsigned red[2][4];
+  __shared__ u32x4 side[2 * kMaxDim];
   const int tid = threadIdx.x;
   const int which = blockIdx.x & 1;
   const unsigned bh = blockIdx.x >> 1;
@@ -51,64 +117,99 @@ __global__ __launch_bounds__(256) void cache_append_kernel(Cache c, NewTokens x)
   const int page = c.page_of(b, blk, at);
   if (page < 0) return;
 
+  const int pieces = c.D / 8;
+  const int lo = max(start - pos0, 0), hi = min(end - pos0, kBlock);  // the new ones' slots
+  const int quad = tid / pieces, piece = tid - quad * pieces;  // quad >= 8: nothing to do
+  const int t0 = 4 * quad, d = 8 * piece;
+  Eight<DT> raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    raw[i].clear();
+    if (t0 + i >= lo && t0 + i < hi) {
+      const int64_t row = row0 + (pos0 + t0 + i - start);
+      if (which)
+        raw[i].load(x.v, row * x.v_token + h * x.v_head + d, x.v_vec);
+      else
+        raw[i].load(x.k, row * x.k_token + h * x.k_head + d, x.k_vec);
+    }
+  }
   const int64_t bi = c.block_index(page, h, at);
   uint8_t* const scale = (which ? c.vs : c.ks) + bi;
   uint8_t* const codes = (which ? c.v : c.k) + bi * kBlock * c.D;
-  const int pieces = c.D / 8, total = kBlock * pieces;
-  const int lo = max(start - pos0, 0), hi = min(end - pos0, kBlock);  // the new ones' slots
-  float val[4][8];
-  float amax = 0.f;
+  const int before = lo > 0 ? (int)*scale - 127 : kMinExp;  // read before the barrier below
+  unsigned bits = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = tid + 256 * i, t = e / pieces, d = (e - t * pieces) * 8;
+  for (int i = 0; i < 4; ++i) bits = raw[i].max_bits(bits);
+  bits = block_max(bits, red[0]);
+  const bool finite = bits < Eight<DT>::kInf;
+  float amax = Eight<DT>::magnitude(bits);
+  if (!finite) {
+    amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) val[i][j] = 0.f;
-    if (e < total && t >= lo && t < hi) {
-      const int64_t row = row0 + (pos0 + t - start);
-      if (which)
-        load8<DT>(x.v, row * x.v_token + h * x.v_head + d, x.v_vec, val[i]);
-      else
-        load8<DT>(x.k, row * x.k_token + h * x.k_head + d, x.k_vec, val[i]);
-    }
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(val[i][j]));
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(raw[i].value(j)));
+    amax = __builtin_bit_cast(float, block_max(__builtin_bit_cast(unsigned, amax), red[1]));
   }
-  amax = block_max(amax, red);
-  const int before = (int)*scale - 127;
-  int e2 = block_exp(amax);
-  if (lo > 0) e2 = max(e2, before);  // earlier tokens keep what they have, or round to more
-  __syncthreads();  // every thread has read the scale
+  // earlier tokens keep what they have, or round to more
+  const int e2 = max(block_exp(amax), before);
   if (tid == 0) *scale = (uint8_t)(e2 + 127);
   const float inv = exp2i(min(max(-e2, -126), 127));
 
   u32x2 code[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    float val[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) val[i][j] *= inv;
-    code[i] = encode8(val[i]);
+    for (int j = 0; j < 8; ++j) val[j] = raw[i].value(j) * inv;
+    code[i] = finite ? encode8_finite(val) : encode8(val);
   }
-  const bool full = lo == 0 && hi == kBlock;
+  if (which) {
+    // word j: this quad's four tokens of channel d + j
+    unsigned word[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int e = tid + 256 * i, t = e / pieces, d = (e - t * pieces) * 8;
-    if (e >= total || t < lo || t >= hi) continue;
-    if (!which) {
-      *reinterpret_cast<u32x2*>(codes + t * c.D + d) = code[i];
-      continue;
+    for (int j = 0; j < 8; ++j) {
+      const unsigned pick = 0x0C0C0000u | (unsigned)(4 + (j & 3)) << 8 | (unsigned)(j & 3);
+      const unsigned ab = __builtin_amdgcn_perm(code[1][j / 4], code[0][j / 4], pick);
+      const unsigned cd = __builtin_amdgcn_perm(code[3][j / 4], code[2][j / 4], pick);
+      word[j] = ab | cd << 16;
     }
-    uint8_t* const to = (full ? side : codes) + (t / kSide) * c.D * kSide + d * kSide + t % kSide;
+    if (lo == 0 && hi == kBlock) {
+      // 16 bytes a channel, their order turned by the piece so that a wave's words meet no bank
+      // twice
+      const int turn = (piece >> 1) & 7;
+      if (quad < 8) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) to[j * kSide] = (uint8_t)(code[i][j / 4] >> (8 * (j & 3)));
-  }
-  if (which && full) {
-    __syncthreads();
-    for (int e = tid; e < 2 * c.D; e += 256)
-      *reinterpret_cast<u32x4*>(codes + e * 16) = *reinterpret_cast<const u32x4*>(side + e * 16);
+        for (int j = 0; j < 8; ++j)
+          reinterpret_cast<unsigned*>(side + (quad >> 2) * c.D + (d + (j ^ turn)))[quad & 3] = word[j];
+      }
+      __syncthreads();
+      for (int e = tid; e < 2 * c.D; e += blockDim.x) {
+        const int ch = e < c.D ? e : e - c.D;
+        reinterpret_cast<u32x4*>(codes)[e] = side[e - ch + (ch ^ ((ch >> 4) & 7))];
+      }
+    } else if (t0 + 3 >= lo && t0 < hi) {
+      uint8_t* const to = codes + (quad >> 2) * c.D * kSide + d * kSide + (t0 & 15);
+      if (t0 >= lo && t0 + 4 <= hi) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<unsigned*>(to + j * kSide) = word[j];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t0 + i >= lo && t0 + i < hi)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[j * kSide + i] = (uint8_t)(word[j] >> (8 * i));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t0 + i >= lo && t0 + i < hi)
+        *reinterpret_cast<u32x2*>(codes + (t0 + i) * c.D + d) = code[i];
   }
   if (lo > 0 && e2 > before) {  // the same for the whole workgroup
     const float f = exp2i(max(before - e2, -126));
-    for (int e = tid; e < lo * pieces; e += 256) {
+    for (int e = tid; e < lo * pieces; e += blockDim.x) {
       const int t = e / pieces, d = (e - t * pieces) * 8;
       u32x2 old;
       uint8_t* const from = which ? codes + (t / kSide) * c.D * kSide + d * kSide + t % kSide
@@ -488,14 +589,14 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
   if (ny > 65535 || nx > INT32_MAX) return FB_ERR_SHAPE;
   const NewTokens x{k,      v,      k_token, k_head, v_token,
                     v_head, vec16(k, k_token, k_head, bytes), vec16(v, v_token, v_head, bytes)};
-  const dim3 grid((unsigned)nx, (unsigned)ny);
+  const dim3 grid((unsigned)nx, (unsigned)ny), threads((unsigned)(c->head_dim + 63) / 64 * 64);
   hipStream_t hs = static_cast<hipStream_t>(stream);
   if (dtype == FB_DT_F16)
-    hipLaunchKernelGGL(cache_append_kernel<FB_DT_F16>, grid, dim3(256), 0, hs, kc, x);
+    hipLaunchKernelGGL(cache_append_kernel<FB_DT_F16>, grid, threads, 0, hs, kc, x);
   else if (dtype == FB_DT_BF16)
-    hipLaunchKernelGGL(cache_append_kernel<FB_DT_BF16>, grid, dim3(256), 0, hs, kc, x);
+    hipLaunchKernelGGL(cache_append_kernel<FB_DT_BF16>, grid, threads, 0, hs, kc, x);
   else
-    hipLaunchKernelGGL(cache_append_kernel<FB_DT_F32>, grid, dim3(256), 0, hs, kc, x);
+    hipLaunchKernelGGL(cache_append_kernel<FB_DT_F32>, grid, threads, 0, hs, kc, x);
   return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
 }
 
