@@ -2,6 +2,7 @@
 #include "fourbit_cache.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace {
 
@@ -236,22 +237,43 @@ __global__ __launch_bounds__(256) void cache_append_kernel(Cache c, NewTokens x)
 
 // ---------------------------------------------------------------------------------
 // Eviction, first half: which tokens of a head stay.  Workgroup = (head, sequence).  The key of the
-// last token that stays is searched for two bits at a time over the order-preserving 32-bit keys of
-// the weights, which stay in registers (KEYS of them a thread; longer sequences are read again for
-// each step): comparisons are counted by ballot, so equal weights cost no more than others (a
-// histogram's atomics do), and the search ends as soon as a bound parts the right number.  Then
-// every 64 tokens are counted once, the counts summed in token order, and what lies above the
-// key, as many of its equals as are left, earliest first, and the recent ones written down.  Bound
-// by its barriers (16 steps), a few microseconds.
+// last token that stays is searched for eight bits at a time over the order-preserving 32-bit keys
+// of the weights, which stay in registers (KEYS of them a thread; longer sequences are read again
+// for each step): a histogram of the keys that share the bits found so far, in eight copies so
+// that equal keys do not wait for each other, which every wave sums from the top by itself.  The
+// search ends as soon as a bound parts the right number.  A wave's tokens lie together, so one
+// exchange of the waves' counts gives every token its place: what lies above the key, as many of
+// its equals as are left, earliest first, and the recent ones, in their order.
 // ---------------------------------------------------------------------------------
+// Order-preserving keys of weights: numbers have them from 0x7FFFFF (-inf) to 0xFF800000 (inf).
+constexpr unsigned kNone = 0, kNan = 1, kNever = 2, kRecent = ~0u;
+
 __device__ inline unsigned weight_key(float w) {
   unsigned b = __builtin_bit_cast(unsigned, w);
-  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0;  // NaN: below every number
+  if ((b & 0x7FFFFFFFu) > 0x7F800000u) return kNan;  // below every number
   if (b == 0x80000000u) b = 0;
   return (b >> 31) ? ~b : (b | 0x80000000u);
 }
 
 constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
+constexpr int kCopies = 8;  // of a histogram of 256 bins: a lane adds to copy lane % kCopies
+constexpr int kCopy = 256 + 64 / kCopies;  // their bins are of different banks
+
+// Sum of v over this lane and those before it.
+__device__ inline int sum_to_lane(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+  return v;
+}
+
+// Bits of a ballot of lanes before this one.
+__device__ inline int before_lane(unsigned long long bits) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(bits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)bits, 0));
+}
 
 template <int KEYS>
 __global__ __launch_bounds__(kSelect) void evict_select_kernel(
@@ -259,136 +281,110 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(
     int keep, int recent, int32_t* __restrict__ kept, float* __restrict__ new_weights,
     int32_t* __restrict__ new_lens) {
   constexpr int kChunk = KEYS * kSelect;  // tokens held at once
-  __shared__ int counted[17][3];  // keys above the bounds of each step, all waves' together
-  __shared__ int chunk_sums[2];
-  __shared__ int2 before[KEYS * kSelectWaves];  // larger and equal keys before 64 tokens
+  __shared__ __align__(16) int bins[4][kCopies * kCopy];
+  __shared__ int2 totals[2][kSelectWaves];  // larger and equal keys of each wave
   const int tid = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
   const int lane = tid & 63, wave = tid >> 6;
   const int n = min(min(max(c.lens[b], 0), c.capacity()), w_tokens);
   const float* const w = weights + b * w_seq + h * w_head;
   const int64_t out = ((int64_t)b * c.H + h) * keep;
   if (h == 0 && tid == 0) new_lens[b] = min(n, keep);
-  const int m = max(n - recent, 0);       // the tokens that compete
-  const int need = keep - min(recent, n); // for so many places
   const bool all = n <= keep;
   unsigned key[KEYS];
   float weight[KEYS];
-  const auto load = [&](int t0) {  // all of them asked for before the first is used
+  // a wave's tokens lie together; all of them are asked for before the first is used
+  const int own = wave * 64 * KEYS + lane;
+  const auto load = [&](int t0) {
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j) weight[j] = w[min(t0 + j * kSelect + tid, max(n - 1, 0))];
+    for (int j = 0; j < KEYS; ++j) weight[j] = w[min(t0 + own + 64 * j, max(n - 1, 0))];
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j)
-      key[j] = t0 + j * kSelect + tid < m ? weight_key(weight[j]) : 0u;
+    for (int j = 0; j < KEYS; ++j) {
+      const int t = t0 + own + 64 * j;
+      key[j] = t >= n ? kNone : t >= n - recent ? kRecent : weight_key(weight[j]);
+    }
   };
   const int chunks = (n + kChunk - 1) / kChunk;
   load(0);
-  for (int i = tid; i < 17 * 3; i += kSelect) counted[i / 3][i % 3] = 0;
+  for (int i = tid; i < kCopies * kCopy; i += kSelect)
+    reinterpret_cast<u32x4*>(bins)[i] = u32x4{0, 0, 0, 0};
   __syncthreads();
-  // the largest `last` with at least `need` keys >= last (0: all of them; a key of 0 is a NaN's)
+  // the largest `last` with at least `keep` keys >= last, 8 bits at a time
   unsigned last = 0;
-  int reached = m;  // keys >= last
-  if (!all && need > 0) {
-    for (int shift = 30; shift >= 0 && reached != need; shift -= 2) {
-      int found[3] = {0, 0, 0};
+  int above = 0;          // keys whose bits so far are above last's
+  int reached = INT_MAX;  // and those with last's among them
+  if (!all) {
+    for (int pass = 0; pass < 4 && reached != keep; ++pass) {
+      const int shift = 24 - 8 * pass;
+      int* const bin = bins[pass];
       for (int ch = 0; ch < chunks; ++ch) {
         if (chunks > 1) load(ch * kChunk);
+        if (ch * kChunk + wave * 64 * KEYS >= n) break;
 #pragma unroll
         for (int j = 0; j < KEYS; ++j)
-#pragma unroll
-          for (int d = 0; d < 3; ++d)
-            found[d] += __popcll(__ballot(key[j] >= (last | (unsigned)(d + 1) << shift)));
+          if (pass == 0 || ((key[j] ^ last) >> shift) < 256u)
+            atomicAdd(bin + (key[j] >> shift & 255) + (lane & (kCopies - 1)) * kCopy, 1);
       }
-      int(&total)[3] = counted[shift >> 1];
-      if (lane < 3) atomicAdd(&total[lane], lane == 0 ? found[0] : lane == 1 ? found[1] : found[2]);
       __syncthreads();
-      int digit = 0;
+      // every wave for itself: lane l has the four bins from 255 - 4 l down
+      u32x4 count = {0, 0, 0, 0};
 #pragma unroll
-      for (int d = 0; d < 3; ++d) {
-        const int sum = __builtin_amdgcn_readfirstlane(total[d]);
-        if (sum >= need) {
-          digit = d + 1;
-          reached = sum;
+      for (int i = 0; i < kCopies; ++i)
+        count += *reinterpret_cast<const u32x4*>(bin + i * kCopy + 252 - 4 * lane);
+      const int four = (int)(count[0] + count[1] + count[2] + count[3]);
+      const int upto = sum_to_lane(four);
+      const int left = keep - above;  // at least 1, and at most all that are counted
+      const int l = __builtin_ctzll(__ballot(upto >= left) | 1ull << 63);
+      int run = upto - four, digit = 255 - 4 * lane, size = (int)count[3];
+#pragma unroll
+      for (int i = 1; i < 4; ++i)
+        if (run + size < left) {
+          run += size;
+          size = (int)count[3 - i];
+          digit = 255 - 4 * lane - i;
         }
-      }
-      last |= (unsigned)digit << shift;
+      above += __builtin_amdgcn_readlane(run, l);
+      reached = above + __builtin_amdgcn_readlane(size, l);
+      last |= (unsigned)__builtin_amdgcn_readlane(digit, l) << shift;
     }
   }
   // Where `reached` is the number needed, every key >= last stays; else last is a key that
   // several have, and of these the earliest stay.
-  const bool exact = reached == need;
-  const auto state = [&](int t, unsigned k, bool& more, bool& equal) {
-    more = t < n && (all || t >= m || (need > 0 && (exact ? k >= last : k > last)));
-    equal = t < m && !all && need > 0 && !exact && k == last;
-  };
-  int more_before = 0, equal_before = 0;  // in earlier chunks
-  int equal_most = 0;
-  if (!all && need > 0 && !exact) {
-    int above = 0;
-    for (int ch = 0; ch < chunks; ++ch) {
-      if (chunks > 1) load(ch * kChunk);
-#pragma unroll
-      for (int j = 0; j < KEYS; ++j) above += __popcll(__ballot(key[j] > last));
-    }
-    if (lane == 0) atomicAdd(&counted[16][0], above);
-    __syncthreads();
-    above = counted[16][0];
-    equal_most = need - above;
-  }
-  int written = 0;
-  for (int t0 = 0; t0 < n; t0 += kChunk) {
-    if (chunks > 1) load(t0);
-    __syncthreads();
+  const bool exact = all || reached == keep;
+  const unsigned least = exact ? max(last, kNan) : last + 1, same = exact ? kNever : last;
+  const int equal_most = exact ? 0 : keep - above;
+  int more_before = 0, equal_before = 0;  // of earlier chunks
+  for (int ch = 0; ch < chunks; ++ch) {
+    if (chunks > 1) load(ch * kChunk);
+    unsigned long long more[KEYS], equal[KEYS];
+    int cm = 0, ce = 0;
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
-      bool more, equal;
-      state(t0 + j * kSelect + tid, key[j], more, equal);
-      const int cm = __popcll(__ballot(more)), ce = __popcll(__ballot(equal));
-      if (lane == 0) before[j * kSelectWaves + wave] = int2{cm, ce};
+      more[j] = __ballot(key[j] >= least);
+      equal[j] = __ballot(key[j] == same);
+      cm += __popcll(more[j]);
+      ce += __popcll(equal[j]);
     }
-    __syncthreads();
-    if (wave == 0) {  // exclusive sums, 64 entries at a time
-      int cm = more_before, ce = equal_before;
-      for (int i0 = 0; i0 < KEYS * kSelectWaves; i0 += 64) {
-        const int2 v = before[i0 + lane];
-        int sm = v.x, se = v.y;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int pm = __shfl_up(sm, o), pe = __shfl_up(se, o);
-          if (lane >= o) {
-            sm += pm;
-            se += pe;
-          }
-        }
-        before[i0 + lane] = int2{cm + sm - v.x, ce + se - v.y};
-        cm += __shfl(sm, 63);
-        ce += __shfl(se, 63);
-      }
-      if (lane == 0) {
-        chunk_sums[0] = cm;
-        chunk_sums[1] = ce;
-      }
-    }
-    __syncthreads();
+    if (lane == 0) totals[ch & 1][wave] = int2{cm, ce};
+    __syncthreads();  // (the next chunk's totals go elsewhere)
+    const int2 v = lane < kSelectWaves ? totals[ch & 1][lane] : int2{0, 0};
+    const int sm = sum_to_lane(v.x), se = sum_to_lane(v.y);
+    cm = more_before + __builtin_amdgcn_readlane(sm, wave) - cm;
+    ce = equal_before + __builtin_amdgcn_readlane(se, wave) - ce;
+    more_before += __builtin_amdgcn_readlane(sm, 63);
+    equal_before += __builtin_amdgcn_readlane(se, 63);
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
-      const int t = t0 + j * kSelect + tid;
-      bool more, equal;
-      state(t, key[j], more, equal);
-      const unsigned long long below = (1ull << lane) - 1;
-      const unsigned long long bm = __ballot(more), be = __ballot(equal);
-      const int2 base = before[j * kSelectWaves + wave];
-      const int rank = base.y + __popcll(be & below);
-      const int place = base.x + __popcll(bm & below) + min(rank, equal_most);
-      if ((more || (equal && rank < equal_most)) && place < keep) {
-        kept[out + place] = t;
+      const int rank = ce + before_lane(equal[j]);
+      const int place = cm + before_lane(more[j]) + min(rank, equal_most);
+      if ((key[j] >= least || (key[j] == same && rank < equal_most)) && place < keep) {
+        kept[out + place] = ch * kChunk + own + 64 * j;
         if (new_weights) new_weights[out + place] = weight[j];
       }
+      cm += __popcll(more[j]);
+      ce += __popcll(equal[j]);
     }
-    more_before = chunk_sums[0];
-    equal_before = chunk_sums[1];
-    written = more_before + min(equal_before, equal_most);
   }
-  for (int i = written + tid; i < keep; i += kSelect) {
+  for (int i = more_before + min(equal_before, equal_most) + tid; i < keep; i += kSelect) {
     kept[out + i] = -1;
     if (new_weights) new_weights[out + i] = 0.f;
   }
@@ -397,19 +393,18 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(
 // ---------------------------------------------------------------------------------
 // Second half: the kept tokens to their new pages.  Workgroup = (one new block, head, sequence),
 // as an append of 32 tokens that are decoded from the cache.  Keys: 8 channels of a token a thread,
-// as in the append.  Values: a thread has one channel of 16 new tokens, a side of the new block,
-// which it writes in one piece; of each of its tokens it reads the 16 bytes of the channel's side
-// (the others of which are its neighbours' for the other tokens there: a cache that turns values
-// for the matrix cores is read whole where a quarter of it is kept).  What bounds it is the chain
-// id, page, codes: keys, values and scales are asked for together.
+// as they lie.  Values: a thread has one channel of 16 new tokens, a side of the new block, which it
+// writes in one piece; it reads their bytes one by one, 16 bytes from its neighbours' (a cache that
+// turns values for the matrix cores is read whole where a quarter of it is kept).  What bounds it is
+// the chain id, page, codes: all codes of a thread are asked for together.
 // ---------------------------------------------------------------------------------
 // WIDE: D is a multiple of 64, so a wave's rows of values are of one side and its tokens uniform.
 // BIG: D is above 128.
 template <bool WIDE, bool BIG>
-__global__ __launch_bounds__(256, BIG ? 4 : WIDE ? 6 : 5) void evict_move_kernel(
-    Cache c, Cache to, int keep, const int32_t* __restrict__ kept) {
+__global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, Cache to, int keep,
+                                                            const int32_t* __restrict__ kept) {
   constexpr int KC = BIG ? 4 : 2, VC = BIG ? 2 : 1;  // pieces of keys, rows of values a thread
-  __shared__ float red[2][4];
+  __shared__ unsigned red[2][2][4];
   __shared__ int64_t from_block[kBlock];  // of a token in the pool; -1: none
   __shared__ int from_slot[kBlock];
   __shared__ float from_scale[2][kBlock];
@@ -449,38 +444,27 @@ __global__ __launch_bounds__(256, BIG ? 4 : WIDE ? 6 : 5) void evict_move_kernel
   u32x4 value[VC];
 #pragma unroll
   for (int i = 0; i < VC; ++i) {
-    const int e = tid + 256 * i;
+    const int e = min(tid + 256 * i, 2 * c.D - 1);
     const int side = WIDE ? __builtin_amdgcn_readfirstlane(e / c.D) : e / c.D;
-    const int d = e - side * c.D;
-    value[i] = u32x4{0, 0, 0, 0};
-    if (e >= 2 * c.D) continue;
+    const unsigned d = (e - side * c.D) * kSide;
+    unsigned byte[kSide];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      u32x4 row[8];
-      int slot[8];
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const int k = side * kSide + half * 8 + t;
-        int64_t block = from_block[k];
-        slot[t] = from_slot[k];
-        if (WIDE) {
-          block = (int64_t)__builtin_amdgcn_readfirstlane((int)(block >> 32)) << 32 |
-                  (unsigned)__builtin_amdgcn_readfirstlane((int)block);
-          slot[t] = __builtin_amdgcn_readfirstlane(slot[t]);
-        }
-        row[t] = u32x4{0, 0, 0, 0};
-        if (block >= 0)
-          row[t] = *reinterpret_cast<const u32x4*>(
-              c.v + block * kBlock * c.D + (slot[t] / kSide) * c.D * kSide + d * kSide);
+    for (int t = 0; t < kSide; ++t) {
+      int64_t block = from_block[side * kSide + t];
+      int slot = from_slot[side * kSide + t];
+      if (WIDE) {
+        block = (int64_t)__builtin_amdgcn_readfirstlane((int)(block >> 32)) << 32 |
+                (unsigned)__builtin_amdgcn_readfirstlane((int)block);
+        slot = __builtin_amdgcn_readfirstlane(slot);
       }
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const unsigned word = slot[t] & 8 ? (slot[t] & 4 ? row[t][3] : row[t][2])
-                                          : (slot[t] & 4 ? row[t][1] : row[t][0]);
-        value[i][half * 2 + t / 4] |= (word >> (8 * (slot[t] & 3)) & 0xFFu) << (8 * (t & 3));
-      }
-      __builtin_amdgcn_sched_barrier(0);  // the registers of one half at a time
+      // where there is none, any byte: its scale is 0
+      const uint8_t* const row = c.v + max(block, (int64_t)0) * kBlock * c.D +
+                                 (slot / kSide * c.D * kSide + slot % kSide);
+      byte[t] = row[d];
     }
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      value[i][w] = byte[4 * w] | byte[4 * w + 1] << 8 | byte[4 * w + 2] << 16 | byte[4 * w + 3] << 24;
   }
   if (tid < kBlock) {
 #pragma unroll
@@ -488,48 +472,67 @@ __global__ __launch_bounds__(256, BIG ? 4 : WIDE ? 6 : 5) void evict_move_kernel
       from_scale[x][tid] = src >= 0 ? exp2i(min(max(scale[x] - 127, -126), 127)) : 0.f;
   }
   __syncthreads();
-  const auto key_values = [&](int i, float (&v)[8]) {
-    const int t = min((tid + 256 * i) / pieces, kBlock - 1);
-    decode8(key[i], v);
+  float kv[KC][8], vv[2 * VC][8];
+  unsigned bits[2] = {0, 0};
+  const auto largest = [](const float(&v)[8], unsigned m) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= from_scale[0][t];
+    for (int j = 0; j < 8; ++j) m = max(m, __builtin_bit_cast(unsigned, v[j]) & 0x7FFFFFFFu);
+    return m;
   };
-  const auto value_values = [&](int i, int half, float (&v)[8]) {
-    const int t0 = min((tid + 256 * i) / c.D, 1) * kSide + half * 8;
-    decode8(u32x2{value[i][2 * half], value[i][2 * half + 1]}, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= from_scale[1][t0 + j];
-  };
-  float amax[2] = {0.f, 0.f}, val[8];
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
-    key_values(i, val);
+    const float f = from_scale[0][min((tid + 256 * i) / pieces, kBlock - 1)];
+    decode8(key[i], kv[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax[0] = fmaxf(amax[0], finite_abs(val[j]));
+    for (int j = 0; j < 8; ++j) kv[i][j] *= f;
+    bits[0] = largest(kv[i], bits[0]);
   }
 #pragma unroll
-  for (int i = 0; i < VC; ++i)
+  for (int i = 0; i < 2 * VC; ++i) {
+    const int t0 = min((tid + 256 * (i / 2)) / c.D, 1) * kSide + (i & 1) * 8;
+    decode8(u32x2{value[i / 2][2 * (i & 1)], value[i / 2][2 * (i & 1) + 1]}, vv[i]);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      value_values(i, half, val);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax[1] = fmaxf(amax[1], finite_abs(val[j]));
+    for (int j = 0; j < 8; ++j) {
+      const float f = from_scale[1][t0 + j];
+      vv[i][j] = f > 0.f ? vv[i][j] * f : 0.f;
     }
+    bits[1] = largest(vv[i], bits[1]);
+  }
+  const auto block_max2 = [&](unsigned(&lds)[2][4]) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    amax[0] = fmaxf(amax[0], __shfl_xor(amax[0], o));
-    amax[1] = fmaxf(amax[1], __shfl_xor(amax[1], o));
+    for (int o = 32; o; o >>= 1) {
+      bits[0] = max(bits[0], (unsigned)__shfl_xor((int)bits[0], o));
+      bits[1] = max(bits[1], (unsigned)__shfl_xor((int)bits[1], o));
+    }
+    if ((tid & 63) == 0) {
+      lds[0][tid >> 6] = bits[0];
+      lds[1][tid >> 6] = bits[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      bits[x] = max(max(lds[x][0], lds[x][1]), max(lds[x][2], lds[x][3]));
+  };
+  block_max2(red[0]);
+  const bool finite = max(bits[0], bits[1]) < 0x7F800000u;
+  if (!finite) {
+    bits[0] = bits[1] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+        bits[0] = max(bits[0], __builtin_bit_cast(unsigned, finite_abs(kv[i][j])));
+#pragma unroll
+      for (int i = 0; i < 2 * VC; ++i)
+        bits[1] = max(bits[1], __builtin_bit_cast(unsigned, finite_abs(vv[i][j])));
+    }
+    block_max2(red[1]);
   }
-  if ((tid & 63) == 0) {
-    red[0][tid >> 6] = amax[0];
-    red[1][tid >> 6] = amax[1];
-  }
-  __syncthreads();
   int e2[2];
   float inv[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    e2[x] = block_exp(fmaxf(fmaxf(red[x][0], red[x][1]), fmaxf(red[x][2], red[x][3])));
+    e2[x] = block_exp(__builtin_bit_cast(float, bits[x]));
     inv[x] = exp2i(min(max(-e2[x], -126), 127));
   }
   const int64_t bi = to.block_index(page, h, at);
@@ -537,29 +540,24 @@ __global__ __launch_bounds__(256, BIG ? 4 : WIDE ? 6 : 5) void evict_move_kernel
     to.ks[bi] = (uint8_t)(e2[0] + 127);
     to.vs[bi] = (uint8_t)(e2[1] + 127);
   }
+  const auto code = [&](float(&v)[8], float by) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= by;
+    return finite ? encode8_finite(v) : encode8(v);
+  };
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
     const int e = tid + 256 * i;
-    if (e >= total) continue;
-    key_values(i, val);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) val[j] *= inv[0];
-    *reinterpret_cast<u32x2*>(to.k + bi * kBlock * c.D + e * 8) = encode8(val);
+    if (e < total)
+      *reinterpret_cast<u32x2*>(to.k + bi * kBlock * c.D + e * 8) = code(kv[i], inv[0]);
   }
 #pragma unroll
   for (int i = 0; i < VC; ++i) {
     const int e = tid + 256 * i;
     if (e >= 2 * c.D) continue;
-    u32x2 w[2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      value_values(i, half, val);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) val[j] *= inv[1];
-      w[half] = encode8(val);
-    }
+    const u32x2 w0 = code(vv[2 * i], inv[1]), w1 = code(vv[2 * i + 1], inv[1]);
     *reinterpret_cast<u32x4*>(to.v + bi * kBlock * c.D + e * kSide) =
-        u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+        u32x4{w0[0], w0[1], w1[0], w1[1]};
   }
 }
 
@@ -627,12 +625,14 @@ int fb_cache_evict(const fb_cache_t* c, const fb_seqs_t* s, const float* weights
   };
   // as many keys a thread as the longest sequence asks for, up to 32
   const int longest = std::min(s->max_len, w_tokens);
-  if (longest <= 4 * kSelect)
-    select(evict_select_kernel<4>);
-  else if (longest <= 8 * kSelect)
-    select(evict_select_kernel<8>);
+  if (longest <= 4096)
+    select(evict_select_kernel<4096 / kSelect>);
+  else if (longest <= 8192)
+    select(evict_select_kernel<8192 / kSelect>);
+  else if (longest <= 16384)
+    select(evict_select_kernel<16384 / kSelect>);
   else
-    select(evict_select_kernel<32>);
+    select(evict_select_kernel<32768 / kSelect>);
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   const bool big = c->head_dim > 128;
   hipLaunchKernelGGL(c->head_dim % 64
