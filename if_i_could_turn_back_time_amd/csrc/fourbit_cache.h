@@ -110,6 +110,7 @@ __device__ inline u32x2 encode8_finite(const float (&v)[8]) {
 
 // The same of any values: what is not finite becomes NaN.
 __device__ inline u32x2 encode8(const float (&v)[8]) {
+  asm volatile("");  // seldom wanted: not to be worked out beside the other and chosen from
   u32x2 r = encode8_finite(v);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {

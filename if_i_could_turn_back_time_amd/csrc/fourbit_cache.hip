@@ -398,16 +398,29 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(
 // turns values for the matrix cores is read whole where a quarter of it is kept).  What bounds it is
 // the chain id, page, codes: all codes of a thread are asked for together.
 // ---------------------------------------------------------------------------------
+// The codes of a word that are NaN: their top bits.
+__device__ inline unsigned nan_codes(unsigned w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// Largest magnitude of eight numbers; NaN is passed over.
+__device__ inline float largest(const float (&v)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2)
+    m = fmaxf(fmaxf(m, __builtin_fabsf(v[j])), __builtin_fabsf(v[j + 1]));
+  return m;
+}
+
 // WIDE: D is a multiple of 64, so a wave's rows of values are of one side and its tokens uniform.
 // BIG: D is above 128.
 template <bool WIDE, bool BIG>
 __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, Cache to, int keep,
                                                             const int32_t* __restrict__ kept) {
   constexpr int KC = BIG ? 4 : 2, VC = BIG ? 2 : 1;  // pieces of keys, rows of values a thread
-  __shared__ unsigned red[2][2][4];
-  __shared__ int64_t from_block[kBlock];  // of a token in the pool; -1: none
-  __shared__ int from_slot[kBlock];
-  __shared__ float from_scale[2][kBlock];
+  __shared__ float red[2][4];
+  __shared__ int any_nan;
+  __shared__ bool some, whole;
+  __shared__ int64_t from_key[kBlock], from_value[kBlock];  // a token's first code; key -1: none
+  __shared__ __align__(16) float from_scale[2][kBlock];
   const int tid = threadIdx.x, blk = blockIdx.x;
   const int h = blockIdx.y, b = blockIdx.z;
   const int32_t* const ids = kept + ((int64_t)b * c.H + h) * keep;
@@ -420,11 +433,22 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
     int src_at, src_page = -1;
     if (from >= 0) src_page = c.page_of(b, from / kBlock, src_at);
     if (src_page >= 0) src = c.block_index(src_page, h, src_at);
-    from_block[tid] = src;
-    from_slot[tid] = from & (kBlock - 1);
+    const int slot = from & (kBlock - 1);
+    const int64_t first = max(src, (int64_t)0) * kBlock * c.D;  // where there is none: any
+    from_key[tid] = src >= 0 ? first + slot * c.D : -1;
+    from_value[tid] = first + slot / kSide * c.D * kSide + slot % kSide;
   }
+  if (tid < 64) {
+    const unsigned long long held = __ballot(from >= 0), found = __ballot(src >= 0);
+    if (tid == 0) {
+      some = held != 0;
+      whole = found == 0xFFFFFFFFull;
+      any_nan = 0;
+    }
+  }
+  __syncthreads();
   // nothing to write: no token of the block is kept, or it has no page
-  if (__syncthreads_or(from >= 0) == 0 || page < 0) return;
+  if (!some || page < 0) return;
   int scale[2] = {0, 0};
   if (src >= 0) {
     scale[0] = c.ks[src];
@@ -436,9 +460,8 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
   for (int i = 0; i < KC; ++i) {
     const int e = tid + 256 * i, t = e / pieces, d = (e - t * pieces) * 8;
     key[i] = u32x2{0, 0};
-    if (e < total && from_block[t] >= 0)
-      key[i] = *reinterpret_cast<const u32x2*>(c.k + from_block[t] * kBlock * c.D +
-                                               from_slot[t] * c.D + d);
+    if (e < total && from_key[t] >= 0)
+      key[i] = *reinterpret_cast<const u32x2*>(c.k + from_key[t] + d);
   }
   // values: rows (side, channel) of the new block, 2 D of them
   u32x4 value[VC];
@@ -450,17 +473,16 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
     unsigned byte[kSide];
 #pragma unroll
     for (int t = 0; t < kSide; ++t) {
-      int64_t block = from_block[side * kSide + t];
-      int slot = from_slot[side * kSide + t];
-      if (WIDE) {
-        block = (int64_t)__builtin_amdgcn_readfirstlane((int)(block >> 32)) << 32 |
-                (unsigned)__builtin_amdgcn_readfirstlane((int)block);
-        slot = __builtin_amdgcn_readfirstlane(slot);
-      }
-      // where there is none, any byte: its scale is 0
-      const uint8_t* const row = c.v + max(block, (int64_t)0) * kBlock * c.D +
-                                 (slot / kSide * c.D * kSide + slot % kSide);
-      byte[t] = row[d];
+      int64_t row = from_value[side * kSide + t];
+      if (WIDE)
+        row = (int64_t)__builtin_amdgcn_readfirstlane((int)(row >> 32)) << 32 |
+              (unsigned)__builtin_amdgcn_readfirstlane((int)row);
+      byte[t] = (c.v + row)[d];
+    }
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < kSide; ++t)
+        if (from_key[side * kSide + t] < 0) byte[t] = 0;
     }
 #pragma unroll
     for (int w = 0; w < 4; ++w)
@@ -472,67 +494,44 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
       from_scale[x][tid] = src >= 0 ? exp2i(min(max(scale[x] - 127, -126), 127)) : 0.f;
   }
   __syncthreads();
-  float kv[KC][8], vv[2 * VC][8];
-  unsigned bits[2] = {0, 0};
-  const auto largest = [](const float(&v)[8], unsigned m) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __builtin_bit_cast(unsigned, v[j]) & 0x7FFFFFFFu);
-    return m;
-  };
+  // Magnitudes by the tokens' scales; a NaN is seen in the codes.
+  float amax[2] = {0.f, 0.f};
+  unsigned nan = 0;
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
-    const float f = from_scale[0][min((tid + 256 * i) / pieces, kBlock - 1)];
-    decode8(key[i], kv[i]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) kv[i][j] *= f;
-    bits[0] = largest(kv[i], bits[0]);
+    float v[8];
+    decode8(key[i], v);
+    nan |= nan_codes(key[i][0]) | nan_codes(key[i][1]);
+    amax[0] = fmaxf(amax[0], largest(v) * from_scale[0][min((tid + 256 * i) / pieces, kBlock - 1)]);
   }
 #pragma unroll
   for (int i = 0; i < 2 * VC; ++i) {
     const int t0 = min((tid + 256 * (i / 2)) / c.D, 1) * kSide + (i & 1) * 8;
-    decode8(u32x2{value[i / 2][2 * (i & 1)], value[i / 2][2 * (i & 1) + 1]}, vv[i]);
+    const u32x2 codes = {value[i / 2][2 * (i & 1)], value[i / 2][2 * (i & 1) + 1]};
+    float v[8];
+    decode8(codes, v);
+    nan |= nan_codes(codes[0]) | nan_codes(codes[1]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float f = from_scale[1][t0 + j];
-      vv[i][j] = f > 0.f ? vv[i][j] * f : 0.f;
-    }
-    bits[1] = largest(vv[i], bits[1]);
+    for (int j = 0; j < 8; ++j) v[j] *= from_scale[1][t0 + j];
+    amax[1] = fmaxf(amax[1], largest(v));
   }
-  const auto block_max2 = [&](unsigned(&lds)[2][4]) {
+  if (__ballot(nan != 0) && (tid & 63) == 0) any_nan = 1;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) {
-      bits[0] = max(bits[0], (unsigned)__shfl_xor((int)bits[0], o));
-      bits[1] = max(bits[1], (unsigned)__shfl_xor((int)bits[1], o));
-    }
-    if ((tid & 63) == 0) {
-      lds[0][tid >> 6] = bits[0];
-      lds[1][tid >> 6] = bits[1];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      bits[x] = max(max(lds[x][0], lds[x][1]), max(lds[x][2], lds[x][3]));
-  };
-  block_max2(red[0]);
-  const bool finite = max(bits[0], bits[1]) < 0x7F800000u;
-  if (!finite) {
-    bits[0] = bits[1] = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-      for (int i = 0; i < KC; ++i)
-        bits[0] = max(bits[0], __builtin_bit_cast(unsigned, finite_abs(kv[i][j])));
-#pragma unroll
-      for (int i = 0; i < 2 * VC; ++i)
-        bits[1] = max(bits[1], __builtin_bit_cast(unsigned, finite_abs(vv[i][j])));
-    }
-    block_max2(red[1]);
+  for (int o = 32; o; o >>= 1) {
+    amax[0] = fmaxf(amax[0], __shfl_xor(amax[0], o));
+    amax[1] = fmaxf(amax[1], __shfl_xor(amax[1], o));
   }
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = amax[0];
+    red[1][tid >> 6] = amax[1];
+  }
+  __syncthreads();
+  const bool finite = __builtin_amdgcn_readfirstlane(any_nan) == 0;
   int e2[2];
   float inv[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    e2[x] = block_exp(__builtin_bit_cast(float, bits[x]));
+    e2[x] = block_exp(fmaxf(fmaxf(red[x][0], red[x][1]), fmaxf(red[x][2], red[x][3])));
     inv[x] = exp2i(min(max(-e2[x], -126), 127));
   }
   const int64_t bi = to.block_index(page, h, at);
@@ -540,24 +539,33 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
     to.ks[bi] = (uint8_t)(e2[0] + 127);
     to.vs[bi] = (uint8_t)(e2[1] + 127);
   }
-  const auto code = [&](float(&v)[8], float by) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= by;
-    return finite ? encode8_finite(v) : encode8(v);
-  };
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
     const int e = tid + 256 * i;
-    if (e < total)
-      *reinterpret_cast<u32x2*>(to.k + bi * kBlock * c.D + e * 8) = code(kv[i], inv[0]);
+    if (e >= total) continue;
+    const float f = from_scale[0][e / pieces] * inv[0];
+    float v[8];
+    decode8(key[i], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+    *reinterpret_cast<u32x2*>(to.k + bi * kBlock * c.D + e * 8) = finite ? encode8_finite(v) : encode8(v);
   }
 #pragma unroll
   for (int i = 0; i < VC; ++i) {
     const int e = tid + 256 * i;
     if (e >= 2 * c.D) continue;
-    const u32x2 w0 = code(vv[2 * i], inv[1]), w1 = code(vv[2 * i + 1], inv[1]);
+    const float* const f = from_scale[1] + e / c.D * kSide;
+    u32x2 w[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float v[8];
+      decode8(u32x2{value[i][2 * half], value[i][2 * half + 1]}, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= f[half * 8 + j] * inv[1];
+      w[half] = finite ? encode8_finite(v) : encode8(v);
+    }
     *reinterpret_cast<u32x4*>(to.v + bi * kBlock * c.D + e * kSide) =
-        u32x4{w0[0], w0[1], w1[0], w1[1]};
+        u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
   }
 }
 
