@@ -38,6 +38,7 @@ struct Attn {
   float* lse;         // or null
   int splits, split_tokens;
   bool dealt;         // see find_part
+  int grain;          // chunks that a part has at least
   float* part;        // [splits][T * Hq][D]
   float2* part_ml;    // [splits][T * Hq]: what the sums are relative to (base 2), sum
   int per_shift;      // log2 of a page's blocks, -1: no power of two
@@ -150,7 +151,6 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //    after the first tile, and no maximum is taken in the others.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
-constexpr int kGrain = 8;  // chunks: two a wave
 // Weights enter the products as fp16 times 2^kLift, so that small ones keep their bits.
 constexpr int kLift = 7;
 // A tile's sum of them that asks for the row's largest score anew: none is above fp16's range.
@@ -166,8 +166,8 @@ struct Part {
 
 __device__ inline int held(const Cache& c, int b) { return min(max(c.lens[b], 0), c.capacity()); }
 
-// `grain`: the least chunks of a part.  Every lane of a wave calls it; slot < 0: nothing to do.
-__device__ inline Part find_part(const Attn& a, int x, int z, int chunk, int grain) {
+// Every lane of a wave calls it; slot < 0: nothing to do.
+__device__ inline Part find_part(const Attn& a, int x, int z, int chunk) {
   const Cache& c = a.c;
   Part p;
   if (!a.dealt) {
@@ -187,7 +187,7 @@ __device__ inline Part find_part(const Attn& a, int x, int z, int chunk, int gra
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
   int n = lane < c.B ? max(1, (int)((float)mine * (float)(a.splits - c.B) / fmaxf(sum, 1.f) + 0.5f))
                      : 0;
-  n = min(n, max(1, (mine + grain - 1) / grain));
+  n = min(n, max(1, (mine + a.grain - 1) / a.grain));
   int end = n;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q4 = lane >> 4;
   const int h = blockIdx.y;
-  const Part part = find_part(a, blockIdx.x, blockIdx.z, kChunk, kGrain);
+  const Part part = find_part(a, blockIdx.x, blockIdx.z, kChunk);
   const int b = __builtin_amdgcn_readfirstlane(part.b);
   const int split = __builtin_amdgcn_readfirstlane(part.slot);
   if (split < 0) return;
@@ -880,7 +880,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
 }
 
 // How many parts sequence b has, as find_part deals them.
-__device__ inline int parts_of(const Attn& a, int b, int chunk, int grain) {
+__device__ inline int parts_of(const Attn& a, int b, int chunk) {
   if (!a.dealt) return a.splits;
   const Cache& c = a.c;
   const int lane = threadIdx.x & 63;
@@ -889,7 +889,7 @@ __device__ inline int parts_of(const Attn& a, int b, int chunk, int grain) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
   int n = max(1, (int)((float)mine * (float)(a.splits - c.B) / fmaxf(sum, 1.f) + 0.5f));
-  n = min(n, max(1, (mine + grain - 1) / grain));
+  n = min(n, max(1, (mine + a.grain - 1) / a.grain));
   return __shfl(n, b);
 }
 
@@ -905,7 +905,7 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
   int row0, n;
   c.rows(b, row0, n);
   const int rows = n * a.group;
-  const int parts = parts_of(a, b, kChunk, kGrain);
+  const int parts = parts_of(a, b, kChunk);
   if (a.dealt && parts == 1) return;  // written already
   const int64_t all = (int64_t)c.T * a.Hq;
   const int width = c.D / 4, groups = 256 / width / ways * ways, per = groups / ways;
@@ -1141,7 +1141,7 @@ __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, 
   int row0, n;
   c.rows(b, row0, n);
   const int rows = min(n * a.group, a.score_rows), len = held(c, b);
-  const int parts = parts_of(a, b, kChunk, kGrain);
+  const int parts = parts_of(a, b, kChunk);
   const int64_t all = (int64_t)c.T * a.Hq;
   if ((int)threadIdx.x < rows) {
     const int i = a.token_of(threadIdx.x);
@@ -1187,6 +1187,7 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(Attn a, Weights w, int
 // ------------------------------------------------------------------ host side
 struct Plan {
   bool few, dealt;
+  int grain;
   int splits, split_tokens, ways;  // ways: of join_parts
   int score_rows, score_tokens;
   int runs, run_rows;              // of attn_weights_kernel
@@ -1205,7 +1206,11 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t len = std::max<int64_t>(1, std::min<int64_t>(s->max_len, capacity));
   const int64_t tiles = p.few ? 1 : (rows + kRows - 1) / kRows;
   const int64_t units = tiles * c->heads * s->seqs;
-  const int step = p.few ? kGrain * kChunk : 4 * kTile;  // a whole number of stages
+  // The least part of few rows: a chunk a wave where that makes some but not many parts (3 to 14%
+  // faster from 600 to 8,000 tokens), two where one part could do (375 tokens of 160 heads: 9.2 us,
+  // 14.8 with two parts to join) or many would be (56,350 tokens of 2 heads: 25 us, 35 with 220).
+  p.grain = len > 8 * kChunk && len <= 256 * kChunk ? 4 : 8;
+  const int step = p.few ? p.grain * kChunk : 4 * kTile;  // a whole number of stages
   const int64_t most = (len + step - 1) / step;
   // two workgroups a CU run side by side
   const int64_t slots = 2 * (int64_t)fb_gpu::cu_count();
@@ -1345,6 +1350,7 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   a.splits = p.splits;
   a.split_tokens = p.split_tokens;
   a.dealt = p.dealt;
+  a.grain = p.grain;
   a.part = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.part);
   const int per = c->page / kBlock;
