@@ -149,6 +149,10 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //  - the sums are kept relative to a row's largest score of some earlier time.  It is looked for
 //    again only where the weights relative to it become too large, which their sum tells: rare
 //    after the first tile, and no maximum is taken in the others.
+// Two workgroups of four waves a CU, one round of them (more, smaller ones had more to join).
+// Measured: 2 sequences of up to 100,003 tokens, 64 query heads over 8 of 128 (0.4 GB): 75 us, 5.3
+// TB/s, and 9 to join; 16 of up to 8,192 with weights: 53 and 16 for joining and weights.  Short
+// ones wait for the chain length, table, codes, join: 777 tokens of 32 heads 8 us and 3.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
 // Weights enter the products as fp16 times 2^kLift, so that small ones keep their bits.
@@ -528,6 +532,10 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
 //  - the sums are brought up to date as above.
 // Heads and sequences vary fastest over the workgroups, then the tiles, the longest first: the
 // last ones to start are short, and where the heads are a multiple of 8 one XCD's L2 holds few.
+// Bound by VALU issue: a wave's 32 rows by 64 tokens take 476 instructions, 32 of them products; what
+// hides behind a product is four others.  Measured: a prompt of 4,096, 64 heads over 8 of 128, bf16:
+// 300 us, 920 TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads: 75 us, 470, for 384 workgroups have
+// the 512 places to themselves (five parts would fill them; joining those takes what it gains).
 // ---------------------------------------------------------------------------------
 constexpr int kRows = 128, kTile = 64;
 
@@ -952,11 +960,12 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
 // ---------------------------------------------------------------------------------
 // Accumulated weights of many rows: weights[t] += sum over the rows of exp(score - lse).  Workgroup =
 // (head and sequence, 256 tokens, a run of the rows).  Each wave holds 64 tokens' keys (32 of the
-// widest), decoded, as operands; the rows go to LDS, 128 at a time and straight from memory, and an operand that is read
-// there meets both blocks of keys (with one block the LDS reads took as long as the products).  A
-// lane's sums are of 16 tokens a block over the rows of its column, so nothing crosses lanes before
-// the end.  Runs of rows leave their sums apart, which
-// a last small kernel adds in order: no atomics.  Half the products of the attention itself.
+// widest), decoded, as operands; the rows go to LDS, 128 at a time and straight from memory, and an
+// operand that is read there meets both blocks of keys (with one block the LDS reads took as long as
+// the products).  A lane's sums are of 16 tokens a block over the rows of its column, so nothing
+// crosses lanes before the end.  Runs of rows leave their sums apart, which a last small kernel adds
+// in order: no atomics.  Half the products of the attention itself; one exponential a score bounds
+// it beside them.  Measured: a prompt of 4,096, 64 heads over 8 of 128: 265 us, 520 TFLOP/s.
 // ---------------------------------------------------------------------------------
 struct Weights {
   float* to;
@@ -1174,7 +1183,9 @@ __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, 
   }
 }
 
-// What is left after the parts: blocks x < joins join them, the others add the weights.
+// What is left after the parts: blocks x < joins join them, the others add the weights.  Bound by the
+// parts' bytes where there are many rows (2 parts of 980 rows of 24 heads of 128: 11 us), by latency
+// otherwise.
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void attn_finish_kernel(Attn a, Weights w, int joins, int ways) {
   const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -1239,11 +1250,13 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
     p.score_tokens = (w_tokens + kChunk - 1) / kChunk * kChunk;
     p.total += align256((size_t)s->seqs * c->heads * p.score_rows * p.score_tokens * 4);
   } else if (w_tokens > 0) {
-    // runs of rows until there are 6 workgroups for each place (a causal prompt leaves half of
-    // them empty), of 512 rows or more
+    // Runs of rows until there are 6 workgroups for each place (a causal prompt leaves half of
+    // them empty), of 512 rows or more; of one stage or more where that leaves places empty (82
+    // rows of 60 heads over 152 tokens: 35 us with 60 workgroups, 26 with 240).
     const int tokens = c->head_dim > 128 ? 4 * kBlock : 8 * kBlock;  // of a workgroup
     const int64_t wgs = (len + tokens - 1) / tokens * c->heads * s->seqs;
-    const int64_t runs = std::min((6 * slots + wgs - 1) / wgs, (rows + 511) / 512);
+    int64_t runs = std::min((6 * slots + wgs - 1) / wgs, (rows + 511) / 512);
+    if (runs * wgs < slots) runs = std::min((slots + wgs - 1) / wgs, (rows + 127) / 128);
     p.run_rows = (int)((rows + runs - 1) / runs + 127) / 128 * 128;  // whole stages
     p.runs = (int)((rows + p.run_rows - 1) / p.run_rows);
     p.score_tokens = w_tokens;
