@@ -1142,44 +1142,78 @@ __global__ __launch_bounds__(256) void attn_weights_join_kernel(Cache c, Weights
 }
 
 // Weights of few rows, from the scores that were written down: 4 tokens a thread.  Every row's sum
-// comes from its parts here too, so that this need not wait for their being joined.
+// comes from its parts here too, so that this need not wait for their being joined; the first 8 rows'
+// scores and the old weights are asked for before it, 16 threads take a row's parts.
 template <int DT, int DP>
 __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, int h, int b) {
+  constexpr int kFirst = 8;
+  __shared__ float part_m[16][16], part_l[16][16];
   __shared__ float lse2[16];
   const Cache& c = a.c;
   int row0, n;
   c.rows(b, row0, n);
   const int rows = min(n * a.group, a.score_rows), len = held(c, b);
-  const int parts = parts_of(a, b, kChunk);
   const int64_t all = (int64_t)c.T * a.Hq;
-  if ((int)threadIdx.x < rows) {
-    const int i = a.token_of(threadIdx.x);
-    const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (threadIdx.x - i * a.group);
-    float M = -__builtin_inff(), L = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[s * all + row].x);
-#pragma unroll 8
-    for (int s = 0; s < parts; ++s) {
-      const float2 ml = a.part_ml[s * all + row];
-      L += ml.y == 0.f ? 0.f : ml.y * exp2f_(ml.x - M);
-    }
-    lse2[threadIdx.x] = L == 0.f ? 0.f : M + __builtin_log2f(L);  // 0: sees nothing
-  }
-  __syncthreads();
   const int end = min(len, w.tokens);
   const float* const s0 = a.scores + ((int64_t)b * c.H + h) * a.score_rows * a.score_tokens;
   float* const to = w.to + b * w.seq + h * w.head;
-  for (int t = (x * 256 + threadIdx.x) * 4; t < end; t += xs * 1024) {
+  int t = (x * 256 + threadIdx.x) * 4;
+  f32x4 score[kFirst], old{0, 0, 0, 0};
+  const auto load = [&] {
+    if (t >= end) return;
+#pragma unroll
+    for (int row = 0; row < kFirst; ++row)
+      if (row < rows)
+        score[row] = *reinterpret_cast<const f32x4*>(s0 + (int64_t)row * a.score_tokens + t);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) old[k] = to[min(t + k, end - 1)];
+  };
+  load();
+  const int parts = parts_of(a, b, kChunk);
+  const int mine = threadIdx.x & 15, first = threadIdx.x >> 4;
+  float M = -__builtin_inff(), L = 0.f;
+  if (mine < rows) {
+    const int i = a.token_of(mine);
+    const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (mine - i * a.group);
+    for (int s = first; s < parts; s += 16) {
+      const float2 ml = a.part_ml[s * all + row];
+      if (ml.y == 0.f) continue;
+      const float to_m = fmaxf(M, ml.x);
+      L = L * exp2f_(M - to_m) + ml.y * exp2f_(ml.x - to_m);
+      M = to_m;
+    }
+  }
+  part_m[first][mine] = M;
+  part_l[first][mine] = L;
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {  // in a fixed order
+#pragma unroll
+    for (int s = 1; s < 16; ++s) M = fmaxf(M, part_m[s][mine]);
+    L = 0.f;
+#pragma unroll
+    for (int s = 0; s < 16; ++s)
+      L += part_l[s][mine] == 0.f ? 0.f : part_l[s][mine] * exp2f_(part_m[s][mine] - M);
+    lse2[mine] = L == 0.f ? 0.f : M + __builtin_log2f(L);  // 0: sees nothing
+  }
+  __syncthreads();
+  while (t < end) {
     f32x4 sum{0, 0, 0, 0};
+#pragma unroll
+    for (int row = 0; row < kFirst; ++row)
+      if (row < rows)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += exp2f_(score[row][k] - lse2[row]);  // unseen: 2^-inf
 #pragma unroll 4
-    for (int row = 0; row < rows; ++row) {
+    for (int row = kFirst; row < rows; ++row) {
       const f32x4 s = *reinterpret_cast<const f32x4*>(s0 + (int64_t)row * a.score_tokens + t);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[k] += exp2f_(s[k] - lse2[row]);  // unseen: 2^-inf
+      for (int k = 0; k < 4; ++k) sum[k] += exp2f_(s[k] - lse2[row]);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (t + k < end) to[t + k] += sum[k];
+      if (t + k < end) to[t + k] = old[k] + sum[k];
+    t += xs * 1024;
+    load();
   }
 }
 
