@@ -908,7 +908,7 @@ template <int DT>
 __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b) {
   using H = Half<DT>;
   __shared__ f32x4 part_v[256];
-  __shared__ float part_l[64];
+  __shared__ float part_m[64], part_l[64];
   const Cache& c = a.c;
   int row0, n;
   c.rows(b, row0, n);
@@ -924,28 +924,52 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
     const int64_t row = (int64_t)(row0 + i) * a.Hq + h * a.group + (r - i * a.group);
     float M = -__builtin_inff(), L = 0.f;
     f32x4 v{0, 0, 0, 0};
-    if (works) {
-#pragma unroll 8
-      for (int s = 0; s < parts; ++s) M = fmaxf(M, a.part_ml[s * all + row].x);
-#pragma unroll 4
-      for (int s = way; s < parts; s += ways) {
-        const float2 ml = a.part_ml[s * all + row];
-        const f32x4 w = *reinterpret_cast<const f32x4*>(a.part + (s * all + row) * c.D + d);
-        const float f = ml.y == 0.f ? 0.f : exp2f_(ml.x - M);
-        L += ml.y * f;
-        v += w * f;
+    constexpr int kAhead = 4;  // parts that are read at once
+    for (int s0 = way; works && s0 < parts; s0 += kAhead * ways) {
+      float2 ml[kAhead];
+      f32x4 w[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int s = s0 + j * ways, from = min(s, parts - 1);
+        ml[j] = a.part_ml[from * all + row];
+        w[j] = *reinterpret_cast<const f32x4*>(a.part + (from * all + row) * c.D + d);
+        if (s >= parts) ml[j].y = 0.f;
       }
+      float to = M;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) to = fmaxf(to, ml[j].y == 0.f ? M : ml[j].x);
+      const float f0 = M == to ? 1.f : exp2f_(M - to);
+      L *= f0;
+      v *= f0;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float f = ml[j].y == 0.f ? 0.f : exp2f_(ml[j].x - to);
+        L += ml[j].y * f;
+        v += w[j] * f;
+      }
+      M = to;
     }
     if (ways > 1) {
       __syncthreads();
       part_v[threadIdx.x] = v;
-      if (d == 0 && g < 64) part_l[g] = L;
+      if (d == 0 && g < 64) {
+        part_m[g] = M;
+        part_l[g] = L;
+      }
       __syncthreads();
-      if (works && way == 0)
+      if (works && way == 0) {
+        float to = M;
+        for (int w = 1; w < ways; ++w) to = fmaxf(to, part_m[g + w]);
+        const float f0 = M == to ? 1.f : exp2f_(M - to);
+        L *= f0;
+        v *= f0;
         for (int w = 1; w < ways; ++w) {
-          v += part_v[threadIdx.x + w * width];
-          L += part_l[g + w];
+          const float f = part_l[g + w] == 0.f ? 0.f : exp2f_(part_m[g + w] - to);
+          L += part_l[g + w] * f;
+          v += part_v[threadIdx.x + w * width] * f;
         }
+        M = to;
+      }
     }
     if (!works || way) continue;
     v *= L == 0.f ? 0.f : 1.f / L;
