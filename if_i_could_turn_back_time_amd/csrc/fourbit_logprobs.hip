@@ -154,7 +154,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   constexpr int V = Type<DT>::V;
   __shared__ float red[kWaves][3];
   __shared__ float lane_max[kWaves][64];
-  __shared__ unsigned bound;
   __shared__ int count, shares;
   __shared__ unsigned list_key[kList];
   __shared__ int list_id[kList];
@@ -257,19 +256,19 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   }
   if (!top) return;
 
-  if (wave == 0) {
+  // the bound, by every wave for itself and to 16 bits of the key: a little low costs candidates only
+  unsigned least = 0;
+  {
     float x = -inf;
+#pragma unroll
     for (int i = 0; i < kWaves; ++i) x = fmaxf(x, lane_max[i][lane]);
     const unsigned k = key_of(x);
-    int better = 0;  // lanes with a larger value, or an equal one and a lower number
-    for (int i = 0; i < 64; ++i) {
-      const unsigned o = (unsigned)__builtin_amdgcn_readlane((int)k, i);
-      better += o > k || (o == k && i < lane);
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+      const unsigned more = least | 1u << bit;
+      if (__popcll(__ballot(k >= more)) >= top) least = more;
     }
-    if (better == top - 1) bound = k;
   }
-  __syncthreads();
-  const unsigned least = bound;
   // NaN counts as the largest, but no maximum shows it: then every share is looked at
   const bool all = s.z != s.z;
   if (all || key_of(mine) >= least) share[atomicAdd(&shares, 1)] = tid;
@@ -365,6 +364,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
     const unsigned k = list_key[i];
     const int id = list_id[i];
     int better = 0;
+#pragma unroll 4
     for (int j = 0; j < found; ++j)
       better += list_key[j] > k || (list_key[j] == k && list_id[j] < id);
     if (better < top) {
