@@ -136,14 +136,35 @@ struct Sums {
     z *= f;
     R = to;
   }
-  __device__ void join(Sums o) {
-    const float to = fmaxf(R, o.R);
-    rebase(to);
-    o.rebase(to);
-    z += o.z;
-    w += o.w;
-  }
 };
+
+// The wave's sum and largest value, in every lane.
+template <int CTRL, int ROWS>
+__device__ inline float moved(float v, float old) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+      __builtin_bit_cast(int, old), __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+}
+__device__ inline float last_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ inline float wave_sum(float v) {
+  v += moved<0x111, 0xF>(v, 0.f);  // row_shr:1, 2, 4, 8
+  v += moved<0x112, 0xF>(v, 0.f);
+  v += moved<0x114, 0xF>(v, 0.f);
+  v += moved<0x118, 0xF>(v, 0.f);
+  v += moved<0x142, 0xA>(v, 0.f);  // row_bcast:15, 31
+  v += moved<0x143, 0xC>(v, 0.f);
+  return last_lane(v);
+}
+__device__ inline float wave_max(float v) {
+  v = fmaxf(v, moved<0x111, 0xF>(v, v));
+  v = fmaxf(v, moved<0x112, 0xF>(v, v));
+  v = fmaxf(v, moved<0x114, 0xF>(v, v));
+  v = fmaxf(v, moved<0x118, 0xF>(v, v));
+  v = fmaxf(v, moved<0x142, 0xA>(v, v));
+  v = fmaxf(v, moved<0x143, 0xC>(v, v));
+  return last_lane(v);
+}
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(
@@ -203,7 +224,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   }
   const float mine = m;
   lane_max[wave][lane] = m;
-  for (int o = 32; o; o >>= 1) s.join(Sums{__shfl_xor(s.R, o), __shfl_xor(s.z, o), __shfl_xor(s.w, o)});
+  s.rebase(wave_max(s.R));
+  s.z = wave_sum(s.z);
+  s.w = wave_sum(s.w);
   if (lane == 0) {
     red[wave][0] = s.R;
     red[wave][1] = s.z;
@@ -211,22 +234,29 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   }
   if (tid == 0) count = shares = 0;
   __syncthreads();
-  s = Sums{red[0][0], red[0][1], red[0][2]};
-  for (int i = 1; i < kWaves; ++i) s.join(Sums{red[i][0], red[i][1], red[i][2]});
+  float to = red[0][0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) to = fmaxf(to, red[i][0]);
+  s = Sums{to, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    Sums o{red[i][0], red[i][1], red[i][2]};
+    o.rebase(to);
+    s.z += o.z;
+    s.w += o.w;
+  }
   // Logits beyond 2^100, or nothing but -inf: relative to the largest itself, then scaled.
   float shift = 0.f;  // y = (x - shift) log2(e) - R
   if (!(s.z > 0.f) || __builtin_fabsf(s.R) >= kHuge) {
     m = -inf;
     for (int i = 0; i < kWaves; ++i) m = fmaxf(m, lane_max[i][lane]);
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = wave_max(m);
     if (__builtin_fabsf(m) < inf && s.z == s.z) {
       shift = m;
       s = Sums{0.f, 0.f, 0.f};
       row.walk([&](int, float x) { s.add((x - shift) * kLog2e); });
-      for (int o = 32; o; o >>= 1) {
-        s.z += __shfl_xor(s.z, o);
-        s.w += __shfl_xor(s.w, o);
-      }
+      s.z = wave_sum(s.z);
+      s.w = wave_sum(s.w);
       __syncthreads();
       if (lane == 0) {
         red[wave][1] = s.z;
