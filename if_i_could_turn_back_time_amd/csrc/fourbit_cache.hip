@@ -8,10 +8,25 @@ namespace {
 
 using namespace fbc;
 
+template <int CTRL, int ROWS>
+__device__ inline unsigned moved(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xF, false);
+}
+
+// The wave's largest value, in every lane.
+__device__ inline unsigned wave_max(unsigned v) {
+  v = max(v, moved<0x111, 0xF>(v));  // row_shr:1, 2, 4, 8
+  v = max(v, moved<0x112, 0xF>(v));
+  v = max(v, moved<0x114, 0xF>(v));
+  v = max(v, moved<0x118, 0xF>(v));
+  v = max(v, moved<0x142, 0xA>(v));  // row_bcast:15, 31
+  v = max(v, moved<0x143, 0xC>(v));
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // Largest of the workgroup's values; `lds` holds 4.  Every thread calls it, once for each `lds`.
 __device__ inline unsigned block_max(unsigned v, unsigned* lds) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+  v = wave_max(v);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   for (int w = 0; w < (int)blockDim.x / 64; ++w) v = max(v, lds[w]);
@@ -524,10 +539,8 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
   }
   if (__ballot(nan != 0) && (tid & 63) == 0) any_nan = 1;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    amax[0] = fmaxf(amax[0], __shfl_xor(amax[0], o));
-    amax[1] = fmaxf(amax[1], __shfl_xor(amax[1], o));
-  }
+  for (int x = 0; x < 2; ++x)  // not negative: in order as bits
+    amax[x] = __builtin_bit_cast(float, wave_max(__builtin_bit_cast(unsigned, amax[x])));
   if ((tid & 63) == 0) {
     red[0][tid >> 6] = amax[0];
     red[1][tid >> 6] = amax[1];
