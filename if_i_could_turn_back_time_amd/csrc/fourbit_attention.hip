@@ -161,14 +161,30 @@ constexpr int kLift = 7;
 constexpr float kMost = 32768.f;
 
 // Which sequence and part of it a workgroup has.  Up to 64 sequences are dealt out by their lengths:
-// of `a.splits` parts a sequence gets its share of all tokens, at least one, and its parts are of
-// one size, so that none of the parts that run side by side is much longer than the others.  More
-// sequences have a.splits parts each.
+// parts are about of one size, the least with which there are at most `a.splits` of them, so that
+// they all run side by side and none is much longer than the others.  More sequences have a.splits
+// parts each.
 struct Part {
   int b, first, last, parts, slot;  // chunks [first, last); place of its sums
 };
 
 __device__ inline int held(const Cache& c, int b) { return min(max(c.lens[b], 0), c.capacity()); }
+
+// The least size of a part (in chunks; found to a 32nd) with which lanes' `mine` chunks have at most
+// a.splits parts together, empty ones among them: one more would run after all the others.
+__device__ inline int part_size(const Attn& a, int mine) {
+  const int seqs = a.c.B;
+  const bool there = (int)(threadIdx.x & 63) < seqs;
+  const unsigned all = (unsigned)__builtin_amdgcn_readlane(sum_to_lane(mine), 63);
+  const unsigned places = (unsigned)max(a.splits - seqs / 2, 1);  // half a part a sequence is lost
+  int size = max((int)((all + places - 1) / places), a.grain);
+  for (;;) {
+    const int n = there ? max(1, (mine + size - 1) / size) : 0;
+    // (a.splits is at least seqs, so that one part each always does)
+    if (__builtin_amdgcn_readlane(sum_to_lane(n), 63) <= a.splits || size > 0x3000000) return size;
+    size += size / 32 + 1;
+  }
+}
 
 // Every lane of a wave calls it; slot < 0: nothing to do.
 __device__ inline Part find_part(const Attn& a, int x, int z, int chunk) {
@@ -185,28 +201,17 @@ __device__ inline Part find_part(const Attn& a, int x, int z, int chunk) {
   }
   const int lane = threadIdx.x & 63;
   const int mine = lane < c.B ? (held(c, lane) + chunk - 1) / chunk : 0;
-  // in chunks, as floats: exact enough to share by, the same in every wave
-  float sum = (float)mine;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-  int n = lane < c.B ? max(1, (int)((float)mine * (float)(a.splits - c.B) / fmaxf(sum, 1.f) + 0.5f))
-                     : 0;
-  n = min(n, max(1, (mine + a.grain - 1) / a.grain));
-  int end = n;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int before = __shfl_up(end, o);
-    if (lane >= o) end += before;
-  }
+  const int size = part_size(a, mine);
+  const int n = lane < c.B ? max(1, (mine + size - 1) / size) : 0, end = sum_to_lane(n);
   const unsigned long long past = __ballot(lane < c.B && end <= x);
   const int b = __popcll(past);
   p.b = min(b, c.B - 1);
   p.parts = __shfl(n, p.b);
   const int i = x - (__shfl(end, p.b) - p.parts), chunks = __shfl(mine, p.b);
   p.slot = b < c.B ? i : -1;
-  const int size = (chunks + p.parts - 1) / p.parts;
-  p.first = min(chunks, i * size);
-  p.last = min(chunks, p.first + size);
+  const int even = (chunks + p.parts - 1) / p.parts;  // no more than size
+  p.first = min(chunks, i * even);
+  p.last = min(chunks, p.first + even);
   return p;
 }
 
@@ -893,11 +898,8 @@ __device__ inline int parts_of(const Attn& a, int b, int chunk) {
   const Cache& c = a.c;
   const int lane = threadIdx.x & 63;
   const int mine = lane < c.B ? (held(c, lane) + chunk - 1) / chunk : 0;
-  float sum = (float)mine;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-  int n = max(1, (int)((float)mine * (float)(a.splits - c.B) / fmaxf(sum, 1.f) + 0.5f));
-  n = min(n, max(1, (mine + a.grain - 1) / a.grain));
+  const int size = part_size(a, mine);
+  const int n = max(1, (mine + size - 1) / size);
   return __shfl(n, b);
 }
 
@@ -1290,9 +1292,9 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   int parts = p.splits;  // of one sequence, at most
   if (p.few && s->seqs > 1 && s->seqs <= 64 && p.splits > 1) {
     p.dealt = true;
-    p.splits = s->seqs + (int)std::min<int64_t>(std::max<int64_t>(slots / c->heads, s->seqs),
-                                                most * s->seqs);
-    parts = (int)std::min<int64_t>(p.splits - s->seqs, (capacity + step - 1) / step) + 1;
+    p.splits = (int)std::min<int64_t>(std::max<int64_t>(slots / c->heads, s->seqs),
+                                      most * s->seqs);
+    parts = (int)std::min<int64_t>(p.splits, (capacity + step - 1) / step);
   }
   const size_t n = (size_t)s->tokens * q_heads;
   p.ways = 1;

@@ -278,17 +278,6 @@ constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
 constexpr int kCopies = 8;  // of a histogram of 256 bins: a lane adds to copy lane % kCopies
 constexpr int kCopy = 256 + 64 / kCopies;  // their bins are of different banks
 
-// Sum of v over this lane and those before it.
-__device__ inline int sum_to_lane(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
-  return v;
-}
-
 // Bits of a ballot of lanes before this one.
 __device__ inline int before_lane(unsigned long long bits) {
   return __builtin_amdgcn_mbcnt_hi((unsigned)(bits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)bits, 0));
