@@ -1279,22 +1279,24 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t units = tiles * c->heads * s->seqs;
   // The least part of few rows: a chunk a wave where that makes some but not many parts (3 to 14%
   // faster from 600 to 8,000 tokens), two where one part could do (375 tokens of 160 heads: 9.2 us,
-  // 14.8 with two parts to join) or many would be (56,350 tokens of 2 heads: 25 us, 35 with 220).
+  // 14.8 with two parts to join) or many would be (100,000 tokens of one head: 17.9 us, 21.2 with 390).
   p.grain = len > 8 * kChunk && len <= 256 * kChunk ? 4 : 8;
-  const int step = p.few ? p.grain * kChunk : 4 * kTile;  // a whole number of stages
-  const int64_t most = (len + step - 1) / step;
+  const int64_t least = p.few ? (int64_t)p.grain * kChunk : 4 * kTile;
+  const int step = p.few ? 4 * kChunk : 4 * kTile;  // a part is a whole number of rounds or stages
+  const int64_t most = (len + least - 1) / least;
   // two workgroups a CU run side by side
   const int64_t slots = 2 * (int64_t)fb_gpu::cu_count();
-  const int64_t want = std::max<int64_t>(1, slots / units);
-  const int64_t per = (most + std::min(want, most) - 1) / std::min(want, most);
+  const int64_t want = std::min(std::max<int64_t>(1, slots / units), most);
+  const int64_t steps = (len + step - 1) / step;
+  const int64_t per = std::max((steps + want - 1) / want, least / step);
   p.split_tokens = (int)(per * step);
-  p.splits = (int)((most + per - 1) / per);
+  p.splits = (int)((steps + per - 1) / per);
   int parts = p.splits;  // of one sequence, at most
   if (p.few && s->seqs > 1 && s->seqs <= 64 && p.splits > 1) {
     p.dealt = true;
     p.splits = (int)std::min<int64_t>(std::max<int64_t>(slots / c->heads, s->seqs),
                                       most * s->seqs);
-    parts = (int)std::min<int64_t>(p.splits, (capacity + step - 1) / step);
+    parts = (int)std::min<int64_t>(p.splits, (capacity + least - 1) / least);
   }
   const size_t n = (size_t)s->tokens * q_heads;
   p.ways = 1;
