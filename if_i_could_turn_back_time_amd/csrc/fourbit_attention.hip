@@ -150,8 +150,8 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //    again only where the weights relative to it become too large, which their sum tells: rare
 //    after the first tile, and no maximum is taken in the others.
 // Two workgroups of four waves a CU, one round of them (more, smaller ones had more to join).
-// Measured: 2 sequences of up to 100,003 tokens, 64 query heads over 8 of 128 (0.4 GB): 75 us, 5.3
-// TB/s, and 9 to join; 16 of up to 8,192 with weights: 53 and 16 for joining and weights.  Short
+// Measured: 2 sequences of up to 100,003 tokens, 64 query heads over 8 of 128 (0.4 GB): 76 us, 5.3
+// TB/s, and 6 to join; 16 of up to 8,192 with weights: 52 and 14 for joining and weights.  Short
 // ones wait for the chain length, table, codes, join: 777 tokens of 32 heads 8 us and 3.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;

@@ -111,7 +111,7 @@ struct NewTokens {
 // maximum, taken over their bits, and the codes.  Four tokens of a value's channel become one
 // word; a full block's words go through LDS to whole 16-token sides.  Earlier codes are read only
 // where the scale grows, and only a block that holds something not finite looks for it.  Bound by
-// memory: 4 sequences of up to 2,048 tokens, 8 heads of 128, bf16 (44 MB): 10.7 us, 4.1 TB/s; by its
+// memory: 4 sequences of up to 2,048 tokens, 8 heads of 128, bf16 (44 MB): 10.6 us, 4.1 TB/s; by its
 // launch for single tokens, 4.4 us.
 // ---------------------------------------------------------------------------------
 template <int DT>
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(
 // writes in one piece; it reads their bytes one by one, 16 bytes from its neighbours' (a cache that
 // turns values for the matrix cores is read whole where a quarter of it is kept).  Few blocks are
 // bound by the chain id, page, codes, so all codes of a thread are asked for together (1,024 of 4,096
-// tokens of 8 heads: 10 us); many by the first-level cache, which takes a wave's 64 strided bytes in
+// tokens of 32 heads: 10 us); many by the first-level cache, which takes a wave's 64 strided bytes in
 // 32 steps (16 sequences of up to 8,192 cut to 2,048: 52 us; 16-byte loads and a choice among
 // their words took 64 for their registers, keys and values in workgroups of their own 91).
 // ---------------------------------------------------------------------------------

@@ -13,8 +13,8 @@
 // values), those above the bound are taken and the equal ones in the order of their ids; where
 // even those above it are too many, a radix select over all 32 key bits takes their place.
 // One walk bounds it: 7 to 8 VALU instructions a value, fewer cycles than its bytes take.  Measured,
-// bf16: 1,024 rows of 131,072 with 20 alternatives 71 us, 3.8 TB/s; 2,048 of 32,000 38 us, 3.4;
-// 16 of 32,000 with 5 9 us, a row's latency on one CU.
+// bf16: 1,024 rows of 131,072 with 20 alternatives 65 us, 4.1 TB/s; 2,048 of 32,000 38 us, 3.4
+// (27 where the logits come out of the last-level cache); 16 of 32,000 with 5 8 us, a row's latency on one CU.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
