@@ -38,7 +38,10 @@ struct Attn {
   float* lse;         // or null
   int splits, split_tokens;
   bool dealt;         // see find_part
+  int chunk;          // tokens of a chunk: what parts are counted in
   int grain;          // chunks that a part has at least
+  int most;           // parts that a sequence has at most
+  int tiles;          // many rows: tiles of a sequence's rows that are dealt out; few: 0
   float* part;        // [splits][T * Hq][D]
   float2* part_ml;    // [splits][T * Hq]: what the sums are relative to (base 2), sum
   int per_shift;      // log2 of a page's blocks, -1: no power of two
@@ -155,32 +158,52 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 // ones wait for the chain length, table, codes, join: 777 tokens of 32 heads 8 us and 3.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
+constexpr int kRows = 128, kTile = 64;  // of the kernel for many rows
 // Weights enter the products as fp16 times 2^kLift, so that small ones keep their bits.
 constexpr int kLift = 7;
 // A tile's sum of them that asks for the row's largest score anew: none is above fp16's range.
 constexpr float kMost = 32768.f;
 
-// Which sequence and part of it a workgroup has.  Up to 64 sequences are dealt out by their lengths:
-// parts are about of one size, the least with which there are at most `a.splits` of them, so that
-// they all run side by side and none is much longer than the others.  More sequences have a.splits
-// parts each.
+// Which sequence, tile of its rows (many rows have several) and part of its tokens a workgroup has.
+// Up to 64 sequences are dealt out by their lengths: parts are about of one size, the least with
+// which there are at most `a.splits` of them for all tiles, so that they all run side by side and
+// none is much longer than the others.  More sequences have a.splits parts each.
 struct Part {
-  int b, first, last, parts, slot;  // chunks [first, last); place of its sums
+  int b, tile, first, last, parts, slot;  // chunks [first, last); place of its sums
 };
 
 __device__ inline int held(const Cache& c, int b) { return min(max(c.lens[b], 0), c.capacity()); }
 
-// The least size of a part (in chunks; found to a 32nd) with which lanes' `mine` chunks have at most
+// What lane b's sequence has to be dealt out, and its parts of `size` chunks.
+struct Load {
+  int chunks, tiles;
+  __device__ int parts(const Attn& a, int size) const {
+    return tiles ? min(max(1, (chunks + size - 1) / size), a.most) : 0;
+  }
+};
+
+__device__ inline Load load_of(const Attn& a, int b, int chunk) {
+  if (b >= a.c.B) return Load{0, 0};
+  Load x{(held(a.c, b) + chunk - 1) / chunk, 1};
+  if (a.tiles) {
+    int row0, n;
+    a.c.rows(b, row0, n);
+    x.tiles = min((n * a.group + kRows - 1) / kRows, a.tiles);
+  }
+  return x;
+}
+
+// The least size of a part (in chunks; found to a 32nd) with which the lanes' sequences have at most
 // a.splits parts together, empty ones among them: one more would run after all the others.
-__device__ inline int part_size(const Attn& a, int mine) {
-  const int seqs = a.c.B;
-  const bool there = (int)(threadIdx.x & 63) < seqs;
-  const unsigned all = (unsigned)__builtin_amdgcn_readlane(sum_to_lane(mine), 63);
-  const unsigned places = (unsigned)max(a.splits - seqs / 2, 1);  // half a part a sequence is lost
+__device__ inline int part_size(const Attn& a, Load mine) {
+  const int tiles = a.tiles ? __builtin_amdgcn_readlane(sum_to_lane(mine.tiles), 63) : a.c.B;
+  const unsigned all =
+      (unsigned)__builtin_amdgcn_readlane(sum_to_lane(mine.chunks * mine.tiles), 63);
+  const unsigned places = (unsigned)max(a.splits - tiles / 2, 1);  // half a part a tile is lost
   int size = max((int)((all + places - 1) / places), a.grain);
   for (;;) {
-    const int n = there ? max(1, (mine + size - 1) / size) : 0;
-    // (a.splits is at least seqs, so that one part each always does)
+    const int n = mine.parts(a, size) * mine.tiles;
+    // (a.splits is at least the tiles of all, so that one part each always does)
     if (__builtin_amdgcn_readlane(sum_to_lane(n), 63) <= a.splits || size > 0x3000000) return size;
     size += size / 32 + 1;
   }
@@ -190,6 +213,7 @@ __device__ inline int part_size(const Attn& a, int mine) {
 __device__ inline Part find_part(const Attn& a, int x, int z, int chunk) {
   const Cache& c = a.c;
   Part p;
+  p.tile = 0;
   if (!a.dealt) {
     p.b = z;
     p.slot = x;
@@ -200,16 +224,20 @@ __device__ inline Part find_part(const Attn& a, int x, int z, int chunk) {
     return p;
   }
   const int lane = threadIdx.x & 63;
-  const int mine = lane < c.B ? (held(c, lane) + chunk - 1) / chunk : 0;
-  const int size = part_size(a, mine);
-  const int n = lane < c.B ? max(1, (mine + size - 1) / size) : 0, end = sum_to_lane(n);
+  const Load mine = load_of(a, lane, chunk);
+  const int n = mine.parts(a, part_size(a, mine)), end = sum_to_lane(n * mine.tiles);
   const unsigned long long past = __ballot(lane < c.B && end <= x);
   const int b = __popcll(past);
   p.b = min(b, c.B - 1);
   p.parts = __shfl(n, p.b);
-  const int i = x - (__shfl(end, p.b) - p.parts), chunks = __shfl(mine, p.b);
+  const int chunks = __shfl(mine.chunks, p.b);
+  int i = x - (__shfl(end, p.b) - p.parts * __shfl(mine.tiles, p.b));
+  if (a.tiles && p.parts > 0) {
+    p.tile = i / p.parts;
+    i -= p.tile * p.parts;
+  }
   p.slot = b < c.B ? i : -1;
-  const int even = (chunks + p.parts - 1) / p.parts;  // no more than size
+  const int even = (chunks + p.parts - 1) / max(p.parts, 1);  // no more than size, or a.most of them
   p.first = min(chunks, i * even);
   p.last = min(chunks, p.first + even);
   return p;
@@ -539,11 +567,9 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
 // last ones to start are short, and where the heads are a multiple of 8 one XCD's L2 holds few.
 // Bound by VALU issue: a wave's 32 rows by 64 tokens take 476 instructions, 32 of them products; what
 // hides behind a product is four others.  Measured: a prompt of 4,096, 64 heads over 8 of 128, bf16:
-// 300 us, 920 TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads: 75 us, 470, for 384 workgroups have
-// the 512 places to themselves (five parts would fill them; joining those takes what it gains).
+// 300 us, 920 TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads, dealt out to 480 places of 512: 57
+// us, and 9 to join.
 // ---------------------------------------------------------------------------------
-constexpr int kRows = 128, kTile = 64;
-
 // Tokens that are staged at once: a barrier for each, so two tiles where LDS has room for it.
 template <int DP>
 constexpr int stage_tokens() {
@@ -571,7 +597,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, x2 = lane >> 5;
   const int h = blockIdx.x % c.H, bs = blockIdx.x / c.H;
-  const int b = bs / a.splits, split = bs - b * a.splits;
+  int b = bs / a.splits, split = bs - b * a.splits, parts = a.splits;
+  int tile0 = blockIdx.y, tile_step = gridDim.y, part_stages = a.split_tokens / ST;
+  if (a.dealt) {
+    const Part part = find_part(a, bs, 0, ST);
+    b = __builtin_amdgcn_readfirstlane(part.b);
+    split = __builtin_amdgcn_readfirstlane(part.slot);
+    if (split < 0) return;
+    parts = __builtin_amdgcn_readfirstlane(part.parts);
+    tile0 = __builtin_amdgcn_readfirstlane(part.tile);
+    tile_step = a.tiles;
+    const int stages = (held(c, b) + ST - 1) / ST;
+    part_stages = (stages + parts - 1) / parts;
+  }
   int row0, n;
   c.rows(b, row0, n);
   const int len = min(max(c.lens[b], 0), c.capacity());
@@ -605,7 +643,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   const auto v_at = [&](int i) { return EX ? v0 + i * 1024 : v_from(i); };
   const unsigned per = (unsigned)c.P / kBlock;
   const int32_t* const table = c.table + b * c.table_stride;
-  for (int ti = blockIdx.y; ti < tiles; ti += gridDim.y) {
+  for (int ti = tile0; ti < tiles; ti += tile_step) {
     const int tile = (tiles - 1 - ti) * kRows;  // the longest first
     const int row = tile + wave * 32 + r, i = a.token_of(row);
     const bool there = row < rows;
@@ -637,9 +675,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
     int E = kMinExp;                       // and their unit's exponent
     unsigned dead[(ND + 1) / 2] = {};      // bit 16 (d % 2) + k of d / 2: o[d][k] saw a NaN value
 
-    const int first = split * (a.split_tokens / ST);
+    const int first = split * part_stages;
     const int all = (most + ST - 1) / ST;
-    const int last = split + 1 == a.splits ? all : min(all, first + a.split_tokens / ST);
+    const int last = split + 1 == parts ? all : min(all, first + part_stages);
     // lane j has block j % SB of the next stage: its page as the table has it (read a stage ahead)
     // and place in the page
     int id, at;
@@ -866,7 +904,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
     if (there) {
       const int64_t orow = (int64_t)(row0 + i) * a.Hq + head;
       const float unit = exp2i(min(max(E - kLift, -126), 127)) *
-                         (a.splits == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+                         (parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -874,7 +912,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           const int ch = 32 * d + 2 * k + 4 * x2;
           if (ch >= D) continue;
           const f32x4 v = f32x4{o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]} * unit;
-          if (a.splits > 1) {
+          if (parts > 1) {
             *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * c.T * a.Hq + orow) * D + ch) = v;
           } else {
             const u32x2 w{(unsigned)H::round(v[0]) | (unsigned)H::round(v[1]) << 16,
@@ -883,7 +921,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           }
         }
       if (x2 == 0) {
-        if (a.splits > 1)
+        if (parts > 1)
           a.part_ml[(int64_t)split * c.T * a.Hq + orow] = float2{m, l};
         else if (a.lse)
           a.lse[orow] = l == 0.f ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
@@ -895,12 +933,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
 // How many parts sequence b has, as find_part deals them.
 __device__ inline int parts_of(const Attn& a, int b, int chunk) {
   if (!a.dealt) return a.splits;
-  const Cache& c = a.c;
-  const int lane = threadIdx.x & 63;
-  const int mine = lane < c.B ? (held(c, lane) + chunk - 1) / chunk : 0;
-  const int size = part_size(a, mine);
-  const int n = max(1, (mine + size - 1) / size);
-  return __shfl(n, b);
+  const Load mine = load_of(a, threadIdx.x & 63, chunk);
+  return __shfl(mine.parts(a, part_size(a, mine)), b);
 }
 
 // The parts' sums of a sequence's rows, in a fixed order.  D / 4 threads go over every `ways`-th part
@@ -915,7 +949,7 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
   int row0, n;
   c.rows(b, row0, n);
   const int rows = n * a.group;
-  const int parts = parts_of(a, b, kChunk);
+  const int parts = parts_of(a, b, a.chunk);
   if (a.dealt && parts == 1) return;  // written already
   const int64_t all = (int64_t)c.T * a.Hq;
   const int width = c.D / 4, groups = 256 / width / ways * ways, per = groups / ways;
@@ -1258,7 +1292,7 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(Attn a, Weights w, int
 // ------------------------------------------------------------------ host side
 struct Plan {
   bool few, dealt;
-  int grain;
+  int chunk, grain, most, tiles;
   int splits, split_tokens, ways;  // ways: of join_parts
   int score_rows, score_tokens;
   int runs, run_rows;              // of attn_weights_kernel
@@ -1281,22 +1315,35 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   // faster from 600 to 8,000 tokens), two where one part could do (375 tokens of 160 heads: 9.2 us,
   // 14.8 with two parts to join) or many would be (100,000 tokens of one head: 17.9 us, 21.2 with 390).
   p.grain = len > 8 * kChunk && len <= 256 * kChunk ? 4 : 8;
-  const int64_t least = p.few ? (int64_t)p.grain * kChunk : 4 * kTile;
+  p.chunk = kChunk;
+  if (!p.few) {
+    p.chunk = c->head_dim > 128 ? stage_tokens<256>() : stage_tokens<128>();
+    p.grain = 4 * kTile / p.chunk;
+  }
+  const int64_t least = (int64_t)p.grain * p.chunk;
   const int step = p.few ? 4 * kChunk : 4 * kTile;  // a part is a whole number of rounds or stages
   const int64_t most = (len + least - 1) / least;
-  // two workgroups a CU run side by side
-  const int64_t slots = 2 * (int64_t)fb_gpu::cu_count();
+  // two workgroups a CU run side by side, of many rows of more than 128 channels one (900 rows of 6,000
+  // tokens, 8 heads of 256: 122 us split for two, 101 so)
+  const int64_t slots = (p.few || c->head_dim <= 128 ? 2 : 1) * (int64_t)fb_gpu::cu_count();
   const int64_t want = std::min(std::max<int64_t>(1, slots / units), most);
   const int64_t steps = (len + step - 1) / step;
   const int64_t per = std::max((steps + want - 1) / want, least / step);
   p.split_tokens = (int)(per * step);
   p.splits = (int)((steps + per - 1) / per);
   int parts = p.splits;  // of one sequence, at most
-  if (p.few && s->seqs > 1 && s->seqs <= 64 && p.splits > 1) {
+  // Many rows are dealt out where parts are long: 2 x 333 rows of 4,001 tokens, 32 heads of 128, in
+  // parts of 2,048 77 us, dealt out 66; but 3 x 100 of 2,000, 32 heads over 8, in parts of 512 34.6 and
+  // 37.9, for the dealing and more parts to join.  A sequence has twice its even share at most, for
+  // what joining reads.
+  if (s->seqs > 1 && s->seqs <= 64 && p.splits > 1 &&
+      (p.few || (int64_t)p.split_tokens * c->head_dim >= 1024 * 128)) {
     p.dealt = true;
+    p.tiles = p.few ? 0 : (int)tiles;
+    p.most = p.few ? INT32_MAX : 2 * p.splits;
     p.splits = (int)std::min<int64_t>(std::max<int64_t>(slots / c->heads, s->seqs),
-                                      most * s->seqs);
-    parts = (int)std::min<int64_t>(p.splits, (capacity + least - 1) / least);
+                                      most * units / c->heads);
+    parts = (int)std::min({(int64_t)p.splits, (int64_t)p.most, (capacity + least - 1) / least});
   }
   const size_t n = (size_t)s->tokens * q_heads;
   p.ways = 1;
@@ -1344,9 +1391,9 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, Weights w, hipStrea
     hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, p.dealt ? 1 : a.c.B),
                        dim3(64 * few_waves<DP>()), 0, hs, a);
   } else {
-    const int64_t nx = (int64_t)a.c.H * a.c.B * p.splits;
+    const int64_t nx = (int64_t)a.c.H * (p.dealt ? 1 : a.c.B) * p.splits;
     if (nx > INT32_MAX) return FB_ERR_SHAPE;
-    const int64_t ny = std::min<int64_t>((rows + kRows - 1) / kRows, 65535);
+    const int64_t ny = p.dealt ? 1 : std::min<int64_t>((rows + kRows - 1) / kRows, 65535);
     hipLaunchKernelGGL((attn_many_kernel<DT, DP, EX>), dim3((unsigned)nx, (unsigned)ny), dim3(256),
                        0, hs, a);
   }
@@ -1425,7 +1472,10 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   a.splits = p.splits;
   a.split_tokens = p.split_tokens;
   a.dealt = p.dealt;
+  a.chunk = p.chunk;
   a.grain = p.grain;
+  a.most = p.most;
+  a.tiles = p.tiles;
   a.part = static_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.part);
   const int per = c->page / kBlock;

@@ -230,6 +230,18 @@ def test_several_tokens(dt, lens, new, heads, group, D, page):
     c.attend(new, group)
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("lens,new,heads,group,kw", [
+    ([1500, 0, 700, 40], [140, 0, 300, 33], 2, 1, {}), ([1500, 700], [140, 300], 2, 4, {"max_new": 40}),
+    ([1200, 90, 64, 400, 5], [20, 7, 30, 2, 9], 1, 3, {"max_len": 500})])
+def test_uneven_prompts(lens, new, heads, group, kw, D):
+    """Tiles of rows and parts of tokens dealt out by lengths: empty sequences, more tiles than the
+    bound says, longer ones than it says."""
+    print("uneven", lens, new, heads, group, kw, D, flush=True)
+    c = Case(lens, heads, D, 64, torch.bfloat16)
+    c.attend(new, group, **kw)
+
+
 @pytest.mark.parametrize("new", [[1, 1], [3, 1], [50, 21]])
 def test_bounds_change_speed_only(new):
     c = Case([900, 333], 2, 128, 64)
