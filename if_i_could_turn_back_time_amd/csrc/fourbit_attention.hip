@@ -152,7 +152,8 @@ __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x383838
 //  - the sums are kept relative to a row's largest score of some earlier time.  It is looked for
 //    again only where the weights relative to it become too large, which their sum tells: rare
 //    after the first tile, and no maximum is taken in the others.
-// Two workgroups of four waves a CU, one round of them (more, smaller ones had more to join).
+// Two workgroups of four waves a CU, one round of them (more, smaller ones had more to join); one
+// above 128 channels, for its registers.
 // Measured: 2 sequences of up to 100,003 tokens, 64 query heads over 8 of 128 (0.4 GB): 76 us, 5.3
 // TB/s, and 6 to join; 16 of up to 8,192 with weights: 52 and 14 for joining and weights.  Short
 // ones wait for the chain length, table, codes, join: 777 tokens of 32 heads 8 us and 3.
@@ -1323,9 +1324,9 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t least = (int64_t)p.grain * p.chunk;
   const int step = p.few ? 4 * kChunk : 4 * kTile;  // a part is a whole number of rounds or stages
   const int64_t most = (len + least - 1) / least;
-  // two workgroups a CU run side by side, of many rows of more than 128 channels one (900 rows of 6,000
-  // tokens, 8 heads of 256: 122 us split for two, 101 so)
-  const int64_t slots = (p.few || c->head_dim <= 128 ? 2 : 1) * (int64_t)fb_gpu::cu_count();
+  // Two workgroups a CU run side by side, of more than 128 channels one (900 rows of 6,000 tokens, 8
+  // heads of 256: 122 us split for two, 101 so; one of 60,000, 4 heads: 38 and 33).
+  const int64_t cus = fb_gpu::cu_count(), slots = c->head_dim <= 128 ? 2 * cus : cus;
   const int64_t want = std::min(std::max<int64_t>(1, slots / units), most);
   const int64_t steps = (len + step - 1) / step;
   const int64_t per = std::max((steps + want - 1) / want, least / step);
@@ -1359,13 +1360,13 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
     p.score_tokens = (w_tokens + kChunk - 1) / kChunk * kChunk;
     p.total += align256((size_t)s->seqs * c->heads * p.score_rows * p.score_tokens * 4);
   } else if (w_tokens > 0) {
-    // Runs of rows until there are 6 workgroups for each place (a causal prompt leaves half of
+    // Runs of rows until there are 12 workgroups a CU (a causal prompt leaves half of
     // them empty), of 512 rows or more; of one stage or more where that leaves places empty (82
     // rows of 60 heads over 152 tokens: 35 us with 60 workgroups, 26 with 240).
     const int tokens = c->head_dim > 128 ? 4 * kBlock : 8 * kBlock;  // of a workgroup
     const int64_t wgs = (len + tokens - 1) / tokens * c->heads * s->seqs;
-    int64_t runs = std::min((6 * slots + wgs - 1) / wgs, (rows + 511) / 512);
-    if (runs * wgs < slots) runs = std::min((slots + wgs - 1) / wgs, (rows + 127) / 128);
+    int64_t runs = std::min((12 * cus + wgs - 1) / wgs, (rows + 511) / 512);
+    if (runs * wgs < 2 * cus) runs = std::min((2 * cus + wgs - 1) / wgs, (rows + 127) / 128);
     p.run_rows = (int)((rows + runs - 1) / runs + 127) / 128 * 128;  // whole stages
     p.runs = (int)((rows + p.run_rows - 1) / p.run_rows);
     p.score_tokens = w_tokens;
