@@ -568,8 +568,8 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
 // last ones to start are short, and where the heads are a multiple of 8 one XCD's L2 holds few.
 // Bound by VALU issue: a wave's 32 rows by 64 tokens take 476 instructions, 32 of them products; what
 // hides behind a product is four others.  Measured: a prompt of 4,096, 64 heads over 8 of 128, bf16:
-// 300 us, 920 TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads, dealt out to 480 places of 512: 57
-// us, and 9 to join.
+// 300 us, 920 TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads, dealt out to 480 places of 512: 66
+// us, 11 of them for the join.
 // ---------------------------------------------------------------------------------
 // Tokens that are staged at once: a barrier for each, so two tiles where LDS has room for it.
 template <int DP>
