@@ -582,6 +582,10 @@ __device__ inline void load_to_lds(const uint8_t* from, uint8_t* to) {
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
+// Before the barrier behind which all waves read what these loads bring: every wave has to wait
+// for its own.  A barrier alone does not, and where else a wave waits the compiler decides.
+__device__ inline void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <int DT, int DP, bool EX>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a) {
   using H = Half<DT>;
@@ -710,6 +714,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
     }
     const auto run = [&](int st, const uint8_t* in_k, uint8_t* in_v, uint8_t* to_k,
                          uint8_t* to_v) __attribute__((always_inline)) {
+      wait_for_loads();
       __syncthreads();  // this stage has arrived; everyone is done with the other buffers
       const int stage_k = scale_k, stage_v = scale_v;
       if (st + 1 < last) fetch(to_k, to_v, st + 1);
@@ -1121,6 +1126,7 @@ __global__ __launch_bounds__(256, 2) void attn_weights_kernel(Attn a, Weights w)
       if (tid < ROWS)
         lse2[parity][tid] =
             next_lse == -__builtin_inff() ? __builtin_inff() : next_lse * kLog2e;
+      wait_for_loads();
       __syncthreads();  // these rows are there; everyone is done with the other buffer
       if (first + ROWS < to) fetch(other, first + ROWS);
 #pragma unroll 1
