@@ -58,6 +58,13 @@ struct Attn {
 
 __device__ inline float exp2f_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// What a block's sums of q and codes are multiplied by, for its scale's byte.  Positive and finite
+// whatever the byte, which may be of a block that nobody wrote: a masked score of -inf stays that.
+__device__ inline float key_scale(float scale2, int byte) {
+  return __builtin_amdgcn_fmed3f(scale2 * exp2i(min(max(byte - 127, -126), 127)), 0x1p-149f,
+                                 0x1.fffffep127f);
+}
+
 template <int DT>
 struct Half;
 template <>
@@ -366,7 +373,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
           s[j] = H::mfma16(H::decode(kf[j][p][2], kf[j][p][3]), qf[p][1], s[j]);
         }
       }
-      const float ks = a.scale2 * exp2i(min(max(sk - 127, -126), 127));
+      const float ks = key_scale(a.scale2, sk);
       const bool more = ch + NW < last;
       if (more) {
         place();
@@ -779,8 +786,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
       int ev[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int ek = __builtin_amdgcn_readlane(stage_k, 2 * part + y) - 127;
-        ks[y] = a.scale2 * exp2i(min(max(ek, -126), 127));
+        ks[y] = key_scale(a.scale2, __builtin_amdgcn_readlane(stage_k, 2 * part + y));
         ev[y] = t * kTile + y * kBlock < len
                     ? max(__builtin_amdgcn_readlane(stage_v, 2 * part + y) - 127, -126)
                     : kMinExp;
@@ -1093,7 +1099,7 @@ __global__ __launch_bounds__(256, 2) void attn_weights_kernel(Attn a, Weights w)
         kf[z][p][0] = H::decode(k[0], k[1]);
         kf[z][p][1] = H::decode(k[2], k[3]);
       }
-      ks[z] = a.scale2 * exp2i(min(max((int)c.ks[bi] - 127, -126), 127));
+      ks[z] = key_scale(a.scale2, c.ks[bi]);
 #pragma unroll
       for (int k = 0; k < 16; ++k) sum[z][k] = 0.f;
     }

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from if_i_could_turn_back_time_amd import KVCache, cache_append, cache_attention
+from test_gpu_cache import Case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -50,3 +51,22 @@ def test_weights_of_long_runs(D, group, n):
         assert bool(((w[0].double() - want).abs() <= err + 2.0 ** 10 * U * want).all())
         first = w if first is None else first
         assert torch.equal(first, w)
+
+
+# ------------------------------------------------------------------ tiny scales, unwritten blocks
+@pytest.mark.parametrize("fill", [0, 255])
+@pytest.mark.parametrize("scale", [1e-9, 1e-30])
+@pytest.mark.parametrize("new,group", [(1, 4), (5, 2), (5, 20)])
+def test_tiny_scale_beside_unwritten_blocks(new, group, scale, fill):
+    """Five tokens held: the rest of their chunk are blocks that hold any scale, and what is masked
+    there must not come up.  A block of zero keys has the least scale of all."""
+    def spoil(x):
+        x[:, 0, 1] = 0
+    c = Case([0], 2, 64, 64, parts=1)
+    c.append([0], [5], 1.0, spoil)
+    c.lens = [5]
+    used = c.cache.k_scale[c.table[0].long(), :, :1].clone()
+    c.cache.k_scale.fill_(fill)
+    c.cache.k_scale[c.table[0].long(), :, :1] = used
+    w = torch.zeros(1, 2, 128, device=DEV)
+    c.attend([new], group, scale=scale, weights=w)
