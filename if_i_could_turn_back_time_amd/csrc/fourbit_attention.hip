@@ -4,9 +4,9 @@
 // belong to one query row (a column of S^T) and the C layout of S^T is, with the cached tokens
 // dealt to the rows of K's operand in the right order, the B layout that P^T needs: no score ever
 // crosses lanes, except for the row maximum.  E4M3 codes are exact in fp16 and bf16, so products
-// of q and a code are exact in fp32; a block's scale joins after the sum, in fp32.  P enters as
-// fp16 (11 bits, relative to the row's largest score), times the block's scale of V relative to
-// the largest seen so far, which is a power of two.
+// of q and a code are exact in fp32; a block's scale of K joins after the sum, in fp32.  P enters as
+// fp16 (11 bits, relative to the row's largest score).  A block's scale of V joins where its codes
+// are decoded, relative to the unit that the sums are in (Unit).
 //
 // A sequence's rows are its (new token, query head of the group) pairs, token-major: with shared
 // heads a tile of rows reads a cached head once for the whole group.
@@ -76,13 +76,14 @@ struct Half<FB_DT_F16> {
   static __device__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  // 8 E4M3 codes, exactly
-  static __device__ x8 decode(unsigned lo, unsigned hi) {
+  // 8 E4M3 codes times a power of two: exactly from 2^-15 (a code's last bit is 2^-9, and
+  // subnormal operands count in the products) to 2^7
+  static __device__ x8 decode(unsigned lo, unsigned hi, float scale = 1.0f) {
     x8 r;
-    const h16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false);
-    const h16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
-    const h16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false);
-    const h16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
+    const h16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, scale, false);
+    const h16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, scale, true);
+    const h16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, scale, false);
+    const h16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, scale, true);
     r[0] = a[0], r[1] = a[1], r[2] = b[0], r[3] = b[1];
     r[4] = c[0], r[5] = c[1], r[6] = d[0], r[7] = d[1];
     return r;
@@ -145,6 +146,41 @@ __device__ inline unsigned nan_bytes(unsigned w) {
 
 // NaN codes as 1 (0x38), others as 0.
 __device__ inline unsigned nan_ones(unsigned w) { return nan_bytes(w) & 0x38383838u; }
+
+// The exponent of the unit that a wave's sums over the values are in.  It follows the blocks' scales
+// up and down, each time by an exact scaling of the sums, so that neither a weight nor a decoded
+// value loses bits to a block with another scale: two that are 2^22 apart share a unit, others take
+// turns.  A row leaves it when no later block is seen by it, so what comes behind a row never
+// touches its sums.  It stays within 2^60 of the largest it was, or sums could overflow: only
+// values 2^75 below the scale of a block that counted lose bits.
+struct Unit {
+  static constexpr int kUp = 7, kDown = 15;  // what decode takes
+  static constexpr int kFall = 60;
+  int now = -1000, top = -1000;
+
+  // A block's exponent as far as it is followed, and whether it can be decoded in this unit.
+  __device__ int reach(int e) const { return max(e, top - kFall - kDown); }
+  __device__ bool takes(int e) const { return (unsigned)(e - now + kDown) <= (unsigned)(kUp + kDown); }
+  // The unit for blocks of exponents e0 and e1; false: none takes both.
+  __device__ static bool shared(int e0, int e1, int& to) {
+    const int hi = max(e0, e1), apart = hi - min(e0, e1);
+    to = hi - max(apart - kDown, 0);
+    return apart <= kUp + kDown;
+  }
+  // The unit that move(to) ends in: `to`, or as near as can be.
+  __device__ int within(int to) const { return max(to, top - kFall); }
+  // Returns what the sums are multiplied by.
+  __device__ float move(int to) {
+    to = within(to);
+    const int by = now - to;  // at most kFall
+    now = to;
+    top = max(top, to);
+    return by < -126 ? 0.f : exp2i(by);
+  }
+  // What the codes of a block of exponent e are multiplied by in unit `u`: e - u is within
+  // [-kFall - kDown, kUp].
+  __device__ static float scale(int e, int u) { return exp2i(e - u); }
+};
 
 // ---------------------------------------------------------------------------------
 // Few rows (at most 16 a cached head and sequence: decoding).  Bound by reading the cache once,
@@ -264,7 +300,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
   constexpr int PASS = 64;  // channels joined at a time
   __shared__ float join[NW][16][PASS + 4];
   __shared__ float wave_m[NW][16], wave_l[NW][16];
-  __shared__ int wave_e[NW];
+  __shared__ int wave_e[NW][16];
   const Cache& c = a.c;
   const int D = EX ? DP : c.D;  // known: the loads' addresses differ by constants
   const int lane = threadIdx.x & 63;
@@ -290,6 +326,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     const int head = h * a.group + (row - i * a.group);
     const int sees = there ? min(max(len - n + i + 1, 0), len) : 0;
     const int least = min(max(len - n + a.token_of(tile) + 1, 0), len);  // of the tile's rows
+    const int most = min(max(len - n + a.token_of(min(tile + 16, rows) - 1) + 1, 0), len);
     typename H::x8 qf[NP][2];
 #pragma unroll
     for (int p = 0; p < NP; ++p)
@@ -303,7 +340,8 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
-    int E = kMinExp;                       // and their unit's exponent
+    Unit unit;
+    int E = unit.now;                      // the row's: of the last block that it saw
     unsigned dead[(ND + 7) / 8] = {};      // bit 4 (d % 8) + k of d / 8: o[d][k] saw a NaN value
 
     const int first = __builtin_amdgcn_readfirstlane(part.first);
@@ -395,23 +433,31 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
 #pragma unroll
         for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(to + 4 * j) = s[j] * ks;
       }
-      // of the lane's block, where it is held
-      const bool block_held = !masked || ch * kChunk + (q4 >> 1) * kBlock < len;
-      const int ev = block_held ? min(max(sv - 127, -126), 126) : kMinExp;
-      const int e = max(ev, __shfl_xor(ev, 32));
-      if (__any(e > E)) {  // the same for the wave
-        asm volatile("");
-        const float unit = exp2i(max(E - e, -126));
+      // of the lane's block, where a row sees it
+      const bool block_seen = !masked || ch * kChunk + (q4 >> 1) * kBlock < most;
+      const int e = unit.reach(block_seen ? sv - 127 : unit.now);
+      bool apart = false;
+      const auto move = [&](int to, int from) __attribute__((always_inline)) {
+        const bool sees_it = sees > from;
+        const float f = unit.move(to), mine = sees_it ? f : 1.f;
+        E = sees_it ? unit.now : E;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] *= unit;
-        E = e;
+        for (int d = 0; d < ND; ++d) o[d] *= mine;
+      };
+      int e0 = 0, e1 = 0;
+      if (__any(!unit.takes(e))) {
+        asm volatile("");
+        e0 = __builtin_amdgcn_readlane(e, 0);
+        e1 = ch * kChunk + kBlock < most ? __builtin_amdgcn_readlane(e, 32) : e0;
+        int to;
+        apart = !Unit::shared(e0, e1, to);
+        if (!apart) move(to, ch * kChunk);
       }
-      // the value block's scale joins in the exponent and leaves the sum again
-      const int fold = max(ev - E, -64);
+      const float vscale = Unit::scale(block_seen ? e : unit.now, unit.now);
       float sum;
       h16x8 pf[2];
       const auto weigh = [&]() __attribute__((always_inline)) {
-        const float shift = (float)(fold + kLift) - (m == -__builtin_inff() ? 0.f : m);
+        const float shift = (float)kLift - (m == -__builtin_inff() ? 0.f : m);
         sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -441,7 +487,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
         m = up;
         weigh();
       }
-      l = __builtin_fmaf(sum, exp2i(-fold - kLift), l);
+      l += sum;
       if (masked) {
         asm volatile("");
         unsigned nan = 0;
@@ -473,15 +519,33 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
           }
         }
       }
+      if (!apart) {
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        o[d] = F::mfma16(F::decode(vf[d][0], vf[d][1]), pf[0], o[d]);
-        o[d] = F::mfma16(F::decode(vf[d][2], vf[d][3]), pf[1], o[d]);
+        for (int d = 0; d < ND; ++d) {
+          o[d] = F::mfma16(F::decode(vf[d][0], vf[d][1], vscale), pf[0], o[d]);
+          o[d] = F::mfma16(F::decode(vf[d][2], vf[d][3], vscale), pf[1], o[d]);
+        }
+      } else {
+        // the blocks one after the other, each with the other's weights 0
+#pragma unroll 1
+        for (int y = 0; y < 2; ++y) {
+          const int ey = unit.reach(y ? e1 : e0);
+          move(ey, ch * kChunk + y * kBlock);
+          const float scale = Unit::scale(ey, unit.now);
+          const h16x8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+          const h16x8 p0 = (q4 >> 1) == y ? pf[0] : none, p1 = (q4 >> 1) == y ? pf[1] : none;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            o[d] = F::mfma16(F::decode(vf[d][0], vf[d][1], scale), p0, o[d]);
+            o[d] = F::mfma16(F::decode(vf[d][2], vf[d][3], scale), p1, o[d]);
+          }
+        }
       }
       if (more) load_v();
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    l *= exp2i(-kLift);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -493,12 +557,15 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     if (q4 == 0) {
       wave_m[wave][r] = m;
       wave_l[wave][r] = l;
+      wave_e[wave][r] = E;
     }
-    if (lane == 0) wave_e[wave] = E;
     __syncthreads();
-    int eM = wave_e[0];
+    const auto unit_of = [&](int rr) {  // the largest of the waves'
+      int x = wave_e[0][rr];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) eM = max(eM, wave_e[w]);
+      for (int w = 1; w < NW; ++w) x = max(x, wave_e[w][rr]);
+      return x;
+    };
     const auto largest = [&](int rr) {
       float x = wave_m[0][rr];
 #pragma unroll
@@ -508,7 +575,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     const auto share = [&](int w, int rr, float M) {
       return M == -__builtin_inff() ? 0.f : exp2f_(wave_m[w][rr] - M);
     };
-    const float mine = share(wave, r, largest(r)) * exp2i(max(E - eM, -126));
+    const float mine = __builtin_amdgcn_ldexpf(share(wave, r, largest(r)), E - unit_of(r));
     // of the row that this thread writes
     constexpr int TR = 4 * NW, E8 = PASS / TR;  // threads of a row, channels of a thread
     const int wr = threadIdx.x / TR, wi = a.token_of(tile + wr);
@@ -520,7 +587,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     const bool alone = part.parts == 1;  // no other part of the sequence: the result itself
     const int64_t orow = (int64_t)(row0 + wi) * a.Hq + h * a.group + (tile + wr - wi * a.group);
     const float out_scale =
-        exp2i(min(max(eM - kLift, -126), 127)) * (alone ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
+        exp2i(min(max(unit_of(wr) - kLift, -126), 127)) * (alone ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
 #pragma unroll
     for (int pass = 0; pass < DP / PASS; ++pass) {
       if (pass) __syncthreads();
@@ -684,7 +751,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[d][k] = 0.f;
     float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
-    int E = kMinExp;                       // and their unit's exponent
+    Unit unit;
+    int E = unit.now;                      // the row's: of the last block that it saw
     unsigned dead[(ND + 1) / 2] = {};      // bit 16 (d % 2) + k of d / 2: o[d][k] saw a NaN value
 
     const int first = split * part_stages;
@@ -730,8 +798,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
       const int t = st * (ST / kTile) + part;
       const uint8_t* const tk = in_k + part * kTile * DP;
       uint8_t* const tv = in_v + part * kTile * DP;
-      const auto values = [&](int i) {  // block i % 2, channels 32 (i / 2)..
-        return *reinterpret_cast<const u32x4*>(tv + ((2 * (i & 1) + x2) * DP + 32 * (i / 2) + r) * 16);
+      // What is read from LDS differs by constants and exchanged bits; the asm keeps the compiler from
+      // holding every address for the whole walk, which above 128 channels spills.
+      int k_piece = (r * NPC + exchange(r, x2)) * 16, v_piece = (x2 * DP + r) * 16;
+      asm volatile("" : "+v"(k_piece), "+v"(v_piece));
+      const auto values = [&](int i) {  // block i / ND, channels 32 (i % ND)..
+        return *reinterpret_cast<const u32x4*>(tv + v_piece + (2 * (i / ND) * DP + 32 * (i % ND)) * 16);
       };
       if (t * kTile + kTile > least_wg) {
         asm volatile("");
@@ -760,7 +832,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
             for (int k = 0; k < 16; ++k) bad[k] = 0.f;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              u32x4 w = values(2 * d + y);
+              u32x4 w = values(y * ND + d);
 #pragma unroll
               for (int u = 0; u < 4; ++u)
                 w[u] = nan_ones(w[u] & keep_bytes(y * kBlock + 4 * u, held));
@@ -783,15 +855,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
       }
       if (t * kTile >= wave_most) continue;  // the same for the wave
       float ks[2];
-      int ev[2];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
+      for (int y = 0; y < 2; ++y)
         ks[y] = key_scale(a.scale2, __builtin_amdgcn_readlane(stage_k, 2 * part + y));
-        ev[y] = t * kTile + y * kBlock < len
-                    ? max(__builtin_amdgcn_readlane(stage_v, 2 * part + y) - 127, -126)
-                    : kMinExp;
-        ev[y] = min(ev[y], 126);
-      }
       const bool masked = t * kTile + kTile > least;  // the same for the wave
       const int seen = sees - t * kTile - x2 * 16;    // tokens of the lane's part
       // Keys: piece i is 16 channels of block i % 2.  A piece is read two ahead of its products, and
@@ -804,8 +870,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
         for (int k = 0; k < 16; ++k) s[y][k] = 0.f;
       {
         const auto read = [&](int i) {
-          return *reinterpret_cast<const u32x4*>(
-              tk + (((i & 1) * 32 + r) * NPC + exchange(r, (i & ~1) + x2)) * 16);
+          return *reinterpret_cast<const u32x4*>(tk + (i & 1) * 32 * NPC * 16 +
+                                                 (k_piece ^ (i & ~1) * 16));
         };
         u32x4 w[2] = {read(0), read(1)};
         typename H::x8 lo = H::decode(w[0][0], w[0][1]), hi = H::decode(w[0][2], w[0][3]);
@@ -834,23 +900,29 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           for (int k = 0; k < 16; ++k)
             if (y * kBlock + k >= seen) s[y][k] = -__builtin_inff();
       }
-      const int e = max(ev[0], ev[1]);
-      if (e > E) {  // the same for the wave
-        asm volatile("");
-        const float unit = exp2i(max(E - e, -126));
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] *= unit;
-        E = e;
-      }
-      // the value block's scale joins in the exponent and leaves the sum again
-      const int fold[2] = {max(ev[0] - E, -64), max(ev[1] - E, -64)};
+      // The value blocks' unit, or one for each.  A row of the wave's sees the first; where none
+      // sees the second, its weights are 0.
+      const auto follow = [&](int e, int from) __attribute__((always_inline)) {
+        const float f = unit.move(e);
+        const bool sees_it = sees > from;
+        E = sees_it ? unit.now : E;
+        return sees_it ? f : 1.f;  // what the row's sums are multiplied by
+      };
+      const int e0 = unit.reach(__builtin_amdgcn_readlane(stage_v, 2 * part) - 127);
+      const bool turn = !unit.takes(e0);  // the same for the wave
+      float turned = 1.f;
+      if (turn) turned = follow(e0, t * kTile);
+      const int e1 = t * kTile + kBlock < wave_most
+                         ? unit.reach(__builtin_amdgcn_readlane(stage_v, 2 * part + 1) - 127)
+                         : unit.now;
+      const float vscale[2] = {Unit::scale(e0, unit.now),
+                               Unit::scale(e1, unit.takes(e1) ? unit.now : unit.within(e1))};
       float sum[2];
       h16x8 pf[2][2];
       const auto weigh = [&]() __attribute__((always_inline)) {
-        const float base = m == -__builtin_inff() ? 0.f : m;
+        const float shift = (float)kLift - (m == -__builtin_inff() ? 0.f : m);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const float shift = (float)(fold[y] + kLift) - base;
           sum[y] = 0.f;
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
@@ -861,7 +933,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
         }
       };
       weigh();
-      if (__any(m == -__builtin_inff() || fmaxf(sum[0], sum[1]) > kMost)) {
+      if (turn || __any(m == -__builtin_inff() || sum[0] + sum[1] > kMost)) {
         asm volatile("");
         float mx[2];
 #pragma unroll
@@ -873,28 +945,36 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
         float big = fmaxf(mx[0] * ks[0], mx[1] * ks[1]);  // the scales are positive
         big = fmaxf(big, __shfl_xor(big, 32));
         const float up = fmaxf(m, big);
-        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up);
+        const float alpha = up == -__builtin_inff() ? 0.f : exp2f_(m - up), both = alpha * turned;
         l *= alpha;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] *= alpha;
+        for (int d = 0; d < ND; ++d) o[d] *= both;
         m = up;
         weigh();
       }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) l = __builtin_fmaf(sum[y], exp2i(-fold[y] - kLift), l);
+      l += sum[0] + sum[1];
       {
-        h16x8 lo = F::decode(vw[0][0], vw[0][1]), hi = F::decode(vw[0][2], vw[0][3]);
+        h16x8 lo = F::decode(vw[0][0], vw[0][1], vscale[0]);
+        h16x8 hi = F::decode(vw[0][2], vw[0][3], vscale[0]);
 #pragma unroll
         for (int i = 0; i < 2 * ND; ++i) {
+          const int y = i / ND, d = i % ND;
+          const float scale = vscale[min(i + 1, 2 * ND - 1) / ND];
           h16x8 next_lo = lo, next_hi = hi;
           if (i + 2 < 2 * ND) vw[i & 1] = values(i + 2);
           const u32x4 n = vw[(i + 1) & 1];
+          if (i == ND && !unit.takes(e1)) {  // the same for the wave
+            asm volatile("");
+            const float f = follow(e1, t * kTile + kBlock);
+#pragma unroll
+            for (int z = 0; z < ND; ++z) o[z] *= f;
+          }
           __builtin_amdgcn_sched_barrier(0);
-          o[i / 2] = F::mfma32(lo, pf[i & 1][0], o[i / 2]);
-          if (i + 1 < 2 * ND) next_lo = F::decode(n[0], n[1]);
+          o[d] = F::mfma32(lo, pf[y][0], o[d]);
+          if (i + 1 < 2 * ND) next_lo = F::decode(n[0], n[1], scale);
           __builtin_amdgcn_sched_barrier(0);
-          o[i / 2] = F::mfma32(hi, pf[i & 1][1], o[i / 2]);
-          if (i + 1 < 2 * ND) next_hi = F::decode(n[2], n[3]);
+          o[d] = F::mfma32(hi, pf[y][1], o[d]);
+          if (i + 1 < 2 * ND) next_hi = F::decode(n[2], n[3], scale);
           __builtin_amdgcn_sched_barrier(0);
           lo = next_lo;
           hi = next_hi;
@@ -907,6 +987,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
       if (st + 1 < last) run(st + 1, lk1, lv1, lk0, lv0);
     }
     l += __shfl_xor(l, 32);
+    l *= exp2i(-kLift);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
       if (dead[d / 2])
@@ -915,15 +996,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           if (dead[d / 2] >> (16 * (d & 1) + k) & 1) o[d][k] = __builtin_nanf("");
     if (there) {
       const int64_t orow = (int64_t)(row0 + i) * a.Hq + head;
-      const float unit = exp2i(min(max(E - kLift, -126), 127)) *
-                         (parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+      const float factor = exp2i(min(max(E - kLift, -126), 127)) *
+                           (parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int k = 0; k < 16; k += 4) {
           const int ch = 32 * d + 2 * k + 4 * x2;
           if (ch >= D) continue;
-          const f32x4 v = f32x4{o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]} * unit;
+          const f32x4 v = f32x4{o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]} * factor;
           if (parts > 1) {
             *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * c.T * a.Hq + orow) * D + ch) = v;
           } else {

@@ -491,9 +491,10 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
  *          head and sequence q must then be 16-byte aligned, its strides too
  *   ws     256-byte aligned, fb_cache_attention_workspace_bytes (its contents are not kept)
  * A row that sees no token gets 0, with an lse of -inf.  Products are exact and summed in fp32;
- * attention weights enter the sum over v as fp16 (relative to the row's largest).  Page numbers
- * outside the pool and lengths beyond the table give undefined numbers, but nothing outside the
- * buffers is read. */
+ * attention weights enter the sum over v as fp16 (relative to the row's largest), whatever the
+ * scales of v's blocks.  (Values 2^75 times smaller than those of a block before them may be lost
+ * beside it, also where it has no weight.)  Page numbers outside the pool and lengths beyond the
+ * table give undefined numbers, but nothing outside the buffers is read. */
 int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, int64_t q_token,
                        int64_t q_head, int32_t q_heads, int32_t dtype, float scale, void* out,
                        float* lse, float* weights, int64_t w_seq, int64_t w_head,

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from if_i_could_turn_back_time_amd import KVCache, cache_append, cache_attention
+from oracle import cache_oracle as O
 from test_gpu_cache import Case
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +71,93 @@ def test_tiny_scale_beside_unwritten_blocks(new, group, scale, fill):
     c.cache.k_scale[c.table[0].long(), :, :1] = used
     w = torch.zeros(1, 2, 128, device=DEV)
     c.attend([new], group, scale=scale, weights=w)
+
+
+# ------------------------------------------------------------------ value scales far apart
+def _scaled(lens, heads, D, dt, gains, low, seed=0):
+    """Sequences whose value blocks (32 tokens) are gains[block % len] times as large; keys of the
+    blocks in ``low`` have a channel that makes their scores small where q's first is 8."""
+    c = Case([0] * len(lens), heads, D, 64, dt, parts=1, seed=seed)
+    per = -(-max(lens) // 64)
+    c.table = torch.arange(len(lens) * per, dtype=torch.int32, device=DEV).view(len(lens), per)
+    c.cache = KVCache.new(len(lens) * per, heads, D, 64, DEV)
+    for x in c.cache:
+        x.view(torch.uint8).fill_(0x7F)  # NaN codes, a scale of 1, where nobody writes
+    for start in range(0, max(lens), 32):
+        count = [max(0, min(32, n - start)) for n in lens]
+
+        def spoil(x, block=start // 32):
+            x[:, 0] = x[:, 0].clamp(-2, 2)
+            x[:, 0, :, 0] = -float(low.get(block % len(gains), 0))
+            x[:, 1] *= gains[block % len(gains)]
+        c.append([min(start, n) for n in lens], count, 1.0, spoil)
+    c.lens = list(lens)
+    return c
+
+
+def _strict(c, new, group, qdt, **kw):
+    """Attention within a bound that knows no value beyond its weight: each weight is off by 2^-11 of
+    itself, or by 2^-32 of the row's largest but no more than itself; sums are fp32 (as in
+    test_gpu_cache.py)."""
+    T, Hq = sum(new), c.heads * group
+    q = torch.randn(T, Hq, c.D, generator=c.g).clamp(-2, 2)
+    q[..., 0] = 8
+    q = q.to(qdt)
+    out = cache_attention(q.to(DEV), c.cache, c.table, _i32(*c.lens),
+                          _i32(0, *np.cumsum(new)), **kw)
+    q, out = q.double().numpy(), out.double().cpu().numpy()
+    ulp, least = (2.0 ** -11, 2.0 ** -25) if qdt == torch.float16 else (2.0 ** -8, 2.0 ** -134)
+    at = 0
+    for b, n in enumerate(new):
+        for h in range(c.heads):
+            k, v = c.k[b][h].values(), c.v[b][h].values()
+            t = len(k)
+            for j in range(h * group, (h + 1) * group):
+                o, _, p, mags, pv = O.attention(q[at:at + n, j], k, v, c.D ** -0.5)
+                d = (c.D + 24) * U * mags
+                rel = np.expm1(2 * d) + 8 * U * mags + 2.0 ** -11 + t * U
+                bound = rel[:, None] * pv + np.minimum(p, 2.0 ** -32) @ np.abs(v)
+                bound = bound + ulp * (np.abs(o) + bound) + least
+                got = out[at:at + n, j]
+                bad = ~(np.abs(got - o) <= bound)
+                assert not bad.any(), (b, h, j, np.argwhere(bad)[:4], got[bad][:4], o[bad][:4])
+        at += n
+
+
+GAINS = {
+    "a large block behind": ([1.0, 2.0 ** 40], {}),
+    "one whose weight is nothing": ([2.0 ** 40, 1.0, 1.0, 1.0], {0: 40}),
+    "one whose weight is little": ([1.0, 2.0 ** 40, 1.0], {1: 20}),
+    "within a unit": ([1.0, 2.0 ** 7, 2.0 ** -15, 2.0 ** -8], {1: 5}),
+    "just beyond it": ([1.0, 2.0 ** 8, 2.0 ** -15, 1.0, 2.0 ** -16], {}),
+    "up and down": ([2.0 ** -30, 2.0 ** 20, 2.0 ** -10, 0.0, 2.0 ** 25, 2.0 ** -35], {1: 60, 4: 60}),
+}
+
+
+@pytest.mark.parametrize("which", list(GAINS))
+@pytest.mark.parametrize("lens,new,heads,group,D", [
+    ([100, 290], [1, 1], 2, 4, 64), ([70, 131], [4, 3], 1, 3, 128), ([65, 200], [1, 2], 1, 5, 48),
+    ([333], [16], 1, 1, 256), ([700], [2], 1, 8, 128), ([130, 97], [70, 97], 2, 2, 64),
+    ([300, 33], [250, 33], 1, 3, 128), ([150], [120], 1, 1, 80), ([170], [140], 1, 2, 256)])
+def test_value_scales_far_apart(which, lens, new, heads, group, D):
+    """The values of a block with another scale cost no other token's weight a bit, whether the
+    block comes before or behind, in the same tile or for rows that do not see it."""
+    print(which, lens, new, heads, group, D, flush=True)
+    gains, low = GAINS[which]
+    c = _scaled(lens, heads, D, torch.float32, gains, low)
+    _strict(c, new, group, torch.bfloat16)
+
+
+@pytest.mark.parametrize("new,group", [([1], 4), ([3], 4), ([120], 2)])
+def test_fp16_values_far_apart(new, group):
+    """The extremes of fp16 side by side, with fp16 queries."""
+    c = _scaled([190], 2, 128, torch.float16, [1e-3, 1.5e4, 1e-3, 1e-5], {1: 60})
+    _strict(c, new, group, torch.float16)
+
+
+@pytest.mark.parametrize("new", [[1], [40]])
+def test_value_scales_far_apart_in_parts(new):
+    """A long cache, so that parts and waves with units of their own are joined."""
+    gains = [1.0] * 40 + [2.0 ** 35] + [2.0 ** -12] * 30 + [2.0 ** -30]
+    c = _scaled([5000], 1, 64, torch.float32, gains, {40: 60})
+    _strict(c, new, 2, torch.bfloat16)
