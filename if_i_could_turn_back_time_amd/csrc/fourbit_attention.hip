@@ -132,6 +132,23 @@ __device__ inline typename Half<DT>::x8 load_q(const Attn& a, bool there, int64_
   return __builtin_bit_cast(typename Half<DT>::x8, w);
 }
 
+// Rows in front of the first sequence's and behind the last one's get what a row gets that sees
+// nothing.  Workgroup x of xs writes some of head h's.
+__device__ inline void rows_of_none(const Attn& a, int h, int x, int xs) {
+  const Cache& c = a.c;
+  if (!c.cu) return;
+  const int before = min(max(c.cu[0], 0), c.T);
+  const int behind = c.T - min(max(c.cu[c.B], before), c.T), none = before + behind;
+  const int pieces = a.group * c.D / 8;  // 16 bytes each: D is a multiple of 16
+  for (int i = x; i < none; i += xs) {
+    const int64_t row = (int64_t)(i < before ? i : c.T - none + i) * a.Hq + h * a.group;
+    u32x4* const to = reinterpret_cast<u32x4*>(static_cast<unsigned short*>(a.out) + row * c.D);
+    for (int p = threadIdx.x; p < pieces; p += blockDim.x) to[p] = u32x4{0, 0, 0, 0};
+    if (a.lse)
+      for (int p = threadIdx.x; p < a.group; p += blockDim.x) a.lse[row + p] = -__builtin_inff();
+  }
+}
+
 // The bytes of the 4 codes from `at` on that lie before `limit`.
 __device__ inline unsigned keep_bytes(int at, int limit) {
   const int n = limit - at;
@@ -307,6 +324,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q4 = lane >> 4;
   const int h = blockIdx.y;
+  rows_of_none(a, h, blockIdx.x + gridDim.x * blockIdx.z, gridDim.x * gridDim.z);
   const Part part = find_part(a, blockIdx.x, blockIdx.z, kChunk);
   const int b = __builtin_amdgcn_readfirstlane(part.b);
   const int split = __builtin_amdgcn_readfirstlane(part.slot);
@@ -676,6 +694,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, x2 = lane >> 5;
   const int h = blockIdx.x % c.H, bs = blockIdx.x / c.H;
+  rows_of_none(a, h, bs + gridDim.x / c.H * blockIdx.y, gridDim.x / c.H * gridDim.y);
   int b = bs / a.splits, split = bs - b * a.splits, parts = a.splits;
   int tile0 = blockIdx.y, tile_step = gridDim.y, part_stages = a.split_tokens / ST;
   if (a.dealt) {
@@ -1480,7 +1499,7 @@ int check_attention(const fb_cache_t* c, const fb_seqs_t* s, int32_t q_heads, Ca
 
 template <int DT, int DP, bool EX>
 int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, Weights w, hipStream_t hs) {
-  const int64_t rows = (int64_t)std::min(s->max_new, s->tokens) * a.group;
+  const int64_t rows = (int64_t)std::max(1, std::min(s->max_new, s->tokens)) * a.group;
   if (p.few) {
     hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, p.dealt ? 1 : a.c.B),
                        dim3(64 * few_waves<DP>()), 0, hs, a);
@@ -1537,7 +1556,7 @@ int fb_cache_attention(const fb_cache_t* c, const fb_seqs_t* s, const void* q, i
   if (st != FB_OK) return st;
   if (dtype != FB_DT_F16 && dtype != FB_DT_BF16) return FB_ERR_DTYPE;
   if (!(scale > 0.f) || !(scale < 1e30f)) return FB_ERR_VALUE;
-  if (s->tokens == 0 || s->max_new == 0) return FB_OK;
+  if (s->tokens == 0) return FB_OK;
   if (!q || !out || (weights && !lse)) return FB_ERR_NULL;
   if (weights && w_tokens < 1) return FB_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(q) & 1u) || (reinterpret_cast<uintptr_t>(out) & 15u) ||

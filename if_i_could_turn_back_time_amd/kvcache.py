@@ -105,7 +105,8 @@ def cache_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: 
 
     ``lens`` (int32 [sequences]) counts the tokens held, the new ones among them: row i of a
     sequence's n new rows sees the first ``lens - n + i + 1`` tokens.  A row that sees none gets
-    0 (and an lse of -inf).  A value of a token that a row does not see never reaches it, NaN or
+    0 (and an lse of -inf), and so does one that is no sequence's (in front of ``cu_seqlens[0]`` or
+    from its last entry on, as in a batch padded for a graph).  A value of a token that a row does not see never reaches it, NaN or
     not.  ``cu_seqlens`` and ``max_new`` as for :func:`cache_append` (``max_new`` too small
     changes speed only, except that ``weights`` may miss the rows beyond it); ``max_len``: about
     the longest length, by which the work is split.

@@ -462,7 +462,8 @@ typedef struct {
   int32_t seqs;          /* 1 .. 65535                                                     */
   int32_t max_pages;
   int32_t tokens;        /* rows of x or q in all                                          */
-  int32_t max_new;       /* at least the most new tokens of one sequence                   */
+  int32_t max_new;       /* at least the most new tokens of one sequence; what a smaller one
+                            does, each function says                                       */
   int32_t max_len;       /* about the most tokens a sequence holds: how work is split goes
                             by it, the result does not                                     */
 } fb_seqs_t;
@@ -487,10 +488,12 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
  *   lse    fp32 [tokens, q_heads] or NULL: log of the sum of exp(scale * q.k)
  *   weights fp32 [seqs, heads, >= max_len] or NULL: weights[b, h, t] grows by the attention
  *          weight that token t got from all rows and query heads of this call (needs lse; rows
- *          beyond max_new may be missed here, and only here).  With more than 16 rows a cached
+ *          beyond max_new may be missed here, and only here: elsewhere a max_new too small, 0 too,
+ *          changes speed only).  With more than 16 rows a cached
  *          head and sequence q must then be 16-byte aligned, its strides too
  *   ws     256-byte aligned, fb_cache_attention_workspace_bytes (its contents are not kept)
- * A row that sees no token gets 0, with an lse of -inf.  Products are exact and summed in fp32;
+ * A row that sees no token, or that is no sequence's (in front of cu[0] or from cu[seqs] on), gets
+ * 0, with an lse of -inf.  Products are exact and summed in fp32;
  * attention weights enter the sum over v as fp16 (relative to the row's largest), whatever the
  * scales of v's blocks.  (Values 2^75 times smaller than those of a block before them may be lost
  * beside it, also where it has no weight.)  Page numbers outside the pool and lengths beyond the

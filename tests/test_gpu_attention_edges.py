@@ -161,3 +161,46 @@ def test_value_scales_far_apart_in_parts(new):
     gains = [1.0] * 40 + [2.0 ** 35] + [2.0 ** -12] * 30 + [2.0 ** -30]
     c = _scaled([5000], 1, 64, torch.float32, gains, {40: 60})
     _strict(c, new, 2, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ bounds and rows of no sequence
+def _poison(*shapes):
+    """Leaves NaN in the memory that the allocator hands out next."""
+    x = [torch.full(shape, float("nan"), dtype=dt, device=DEV) for shape, dt in shapes]
+    del x
+
+
+@pytest.mark.parametrize("new,group,lens", [([1, 1], 4, [900, 333]), ([50, 21], 4, [900, 333]),
+                                            ([20], 1, [40]), ([3], 20, [2000])])
+def test_max_new_of_nothing(new, group, lens):
+    """max_new too small, 0 as well, changes speed only."""
+    c = Case(lens, 2, 128, 64)
+    T = sum(new)
+    for kw in ({"max_new": 0}, {"max_new": 0, "max_len": 0}):
+        _poison(((T, 2 * group, 128), torch.bfloat16), ((T, 2 * group), torch.float32))
+        c.attend(new, group, **kw)
+
+
+@pytest.mark.parametrize("new,group,lens,kw", [
+    ([1, 1], 4, [900, 333], {}), ([1, 1, 1], 2, [40, 7, 90], {"max_new": 1}), ([60, 21], 4, [900, 333], {}),
+    ([150, 0, 130], 1, [1500, 10, 700], {"max_new": 150, "max_len": 1500}), ([0, 0], 2, [5, 6], {}),
+    ([300], 8, [300], {"max_new": 300})])
+@pytest.mark.parametrize("before,behind", [(0, 7), (3, 0), (2, 150)])
+def test_rows_of_no_sequence(new, group, lens, kw, before, behind):
+    """A padded batch: the rows that are no sequence's get 0 and -inf, the others what they get
+    without them, bit for bit where the work is split alike."""
+    heads, D, T = 2, 64, sum(new)
+    c = Case(lens, heads, D, 64)
+    q = torch.randn(before + T + behind, heads * group, D, generator=c.g).bfloat16().to(DEV)
+    cu = _i32(0, *np.cumsum(new))
+    inner = q[before:before + T]
+    kw = {"max_new": max(new), **kw}
+    want, want_lse = cache_attention(inner, c.cache, c.table, _i32(*lens), cu, return_lse=True, **kw)
+    for _ in range(3):
+        _poison((q.shape, q.dtype), (q.shape[:2], torch.float32))
+        out, lse = cache_attention(q, c.cache, c.table, _i32(*lens), cu + before, return_lse=True,
+                                   **kw)
+        assert torch.equal(out[before:before + T], want)
+        assert torch.equal(lse[before:before + T], want_lse)
+        for rows in (slice(0, before), slice(before + T, None)):
+            assert bool((out[rows] == 0).all()) and bool((lse[rows] == -torch.inf).all())
