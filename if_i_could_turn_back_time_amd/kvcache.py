@@ -66,8 +66,10 @@ class KVCache(NamedTuple):
         v = self.v[at].float().transpose(-1, -2).reshape(n, H, P, D)
         out = []
         for x, s in ((k, self.k_scale), (v, self.v_scale)):
-            e = (s[at].int() - 127).repeat_interleave(BLOCK, 2)[..., None]
-            out.append(torch.ldexp(x, e).transpose(0, 1).reshape(H, n * P, D)[:, :length])
+            s = s[at].int().repeat_interleave(BLOCK, 2)[..., None]
+            # 2^(s - 127) from its bits: torch.ldexp takes a power, which the GPU rounds
+            scale = torch.where(s > 0, s << 23, 1 << 22).int().view(torch.float32)
+            out.append((x * scale).transpose(0, 1).reshape(H, n * P, D)[:, :length])
         return out[0], out[1]
 
 

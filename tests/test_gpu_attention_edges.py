@@ -204,3 +204,20 @@ def test_rows_of_no_sequence(new, group, lens, kw, before, behind):
         assert torch.equal(lse[before:before + T], want_lse)
         for rows in (slice(0, before), slice(before + T, None)):
             assert bool((out[rows] == 0).all()) and bool((lse[rows] == -torch.inf).all())
+
+
+# ------------------------------------------------------------------ reading the cache back
+def test_read_is_exact():
+    """Every code at every scale whose products fp32 holds, as numpy's ldexp has it."""
+    cache = KVCache.new(250, 1, 16, 32, DEV)
+    codes = torch.arange(512, device=DEV).to(torch.uint8).view(32, 16)
+    cache.k.view(torch.uint8)[:] = codes
+    cache.v.view(torch.uint8)[:] = codes.view(2, 16, 16).transpose(1, 2)
+    cache.k_scale[:, 0, 0] = torch.arange(250, device=DEV).to(torch.uint8)
+    cache.v_scale.copy_(cache.k_scale)
+    k, v = cache.read(torch.arange(250, device=DEV, dtype=torch.int32), 250 * 32)
+    with np.errstate(over="ignore", under="ignore"):
+        want = np.ldexp(codes.view(torch.float8_e4m3fn).float().cpu().numpy()[None],
+                        np.arange(-127, 123)[:, None, None])
+    for got in (k, v):
+        np.testing.assert_array_equal(got.view(250, 32, 16).cpu().numpy(), want)
