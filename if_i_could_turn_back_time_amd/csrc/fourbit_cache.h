@@ -12,7 +12,7 @@ namespace fbc {
 
 constexpr int kBlock = 32;     // tokens of one scale
 constexpr int kSide = 16;      // tokens of one channel side by side in v
-constexpr int kMinExp = -100;  // of a block's scale: keeps every product of scales normal
+constexpr int kMinExp = -100;  // of a block's scale; a block of zeros has it
 constexpr int kMaxDim = 256;
 
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));

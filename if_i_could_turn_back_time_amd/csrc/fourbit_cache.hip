@@ -421,6 +421,10 @@ __device__ inline float largest(const float (&v)[8]) {
   return m;
 }
 
+// A token's scale over its new block's: 0 times it is 0, however far apart they are (what is not 0 is
+// at most 448 times the new one).
+__device__ inline float rescale(float from, float inv) { return fminf(from * inv, 0x1p126f); }
+
 // WIDE: D is a multiple of 64, so a wave's rows of values are of one side and its tokens uniform.
 // BIG: D is above 128.
 template <bool WIDE, bool BIG>
@@ -552,7 +556,7 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
   for (int i = 0; i < KC; ++i) {
     const int e = tid + 256 * i;
     if (e >= total) continue;
-    const float f = from_scale[0][e / pieces] * inv[0];
+    const float f = rescale(from_scale[0][e / pieces], inv[0]);
     float v[8];
     decode8(key[i], v);
 #pragma unroll
@@ -570,7 +574,7 @@ __global__ __launch_bounds__(256, BIG ? 4 : 8) void evict_move_kernel(Cache c, C
       float v[8];
       decode8(u32x2{value[i][2 * half], value[i][2 * half + 1]}, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= f[half * 8 + j] * inv[1];
+      for (int j = 0; j < 8; ++j) v[j] *= rescale(f[half * 8 + j], inv[1]);
       w[half] = finite ? encode8_finite(v) : encode8(v);
     }
     *reinterpret_cast<u32x4*>(to.v + bi * kBlock * c.D + e * kSide) =

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from if_i_could_turn_back_time_amd import KVCache, cache_append, cache_attention
+from if_i_could_turn_back_time_amd import (KVCache, cache_append, cache_attention,
+                                           cache_evict)
 from oracle import cache_oracle as O
 from test_gpu_cache import Case
 
@@ -221,3 +222,38 @@ def test_read_is_exact():
                         np.arange(-127, 123)[:, None, None])
     for got in (k, v):
         np.testing.assert_array_equal(got.view(250, 32, 16).cpu().numpy(), want)
+
+
+# ------------------------------------------------------------------ eviction across scales
+@pytest.mark.parametrize("D", [64, 80, 256])
+@pytest.mark.parametrize("big", [2.0 ** 28, 2.0 ** 100, 3e38])
+def test_evict_zeros_from_large_blocks(D, big):
+    """Tokens of zeros, of tiny values and of NaN leave blocks of large ones for blocks of their own."""
+    n, heads, page = 200, 2, 64
+
+    def spoil(x):
+        x.clamp_(-1, 1)
+        x *= big
+        x[::2] = 0                    # zeros in blocks of large values
+        x[64:96] = 0                  # and a block of them
+        x[96:128:2] = 1e-30
+        x[130, 0, 0, 3] = x[132, 1, 1, 5] = float("nan")
+    c = Case([0], heads, D, page, torch.float32, parts=1)
+    need = -(-n // page)
+    c.cache = KVCache.new(2 * need, heads, D, page, DEV)
+    c.table = torch.arange(need, dtype=torch.int32, device=DEV)[None]
+    c.append([0], [n], 1.0, spoil)
+    c.lens = [n]
+    c.check_codes()
+    w = torch.zeros(1, heads, n, device=DEV)
+    w[..., ::2] = 1  # the even ones stay
+    new_table = torch.arange(need, 2 * need, dtype=torch.int32, device=DEV)[None]
+    r = cache_evict(c.cache, c.table, _i32(n), w, 105, 9, new_table, max_len=n)
+    k, v = c.cache.read(new_table[0], 105)
+    for h in range(heads):
+        ids = r.kept[0, h].cpu().numpy()
+        np.testing.assert_array_equal(ids, O.evict(w[0, h].cpu().numpy(), 105, 9))
+        for got, old in ((k[h], c.k[0][h]), (v[h], c.v[0][h])):
+            cut = O.Tokens(D)
+            cut.append(old.values()[ids])
+            np.testing.assert_array_equal(got.double().cpu().numpy(), cut.values())
