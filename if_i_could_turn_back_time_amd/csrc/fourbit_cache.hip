@@ -102,6 +102,7 @@ struct NewTokens {
   const void *k, *v;
   int64_t k_token, k_head, v_token, v_head;
   bool k_vec, v_vec;
+  int most;  // of a sequence
 };
 
 // ---------------------------------------------------------------------------------
@@ -124,6 +125,7 @@ __global__ __launch_bounds__(256) void cache_append_kernel(Cache c, NewTokens x)
   const int b = bh / c.H, h = bh - b * c.H;
   int row0, n;
   c.rows(b, row0, n);
+  n = min(n, x.most);
   const int start = c.lens[b];
   if (start < 0 || n < 1) return;
   const int64_t end64 = (int64_t)start + n;
@@ -607,7 +609,8 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
   const int64_t nx = (int64_t)s->seqs * c->heads * 2;
   if (ny > 65535 || nx > INT32_MAX) return FB_ERR_SHAPE;
   const NewTokens x{k,      v,      k_token, k_head, v_token,
-                    v_head, vec16(k, k_token, k_head, bytes), vec16(v, v_token, v_head, bytes)};
+                    v_head, vec16(k, k_token, k_head, bytes), vec16(v, v_token, v_head, bytes),
+                    s->max_new};
   const dim3 grid((unsigned)nx, (unsigned)ny), threads((unsigned)(c->head_dim + 63) / 64 * 64);
   hipStream_t hs = static_cast<hipStream_t>(stream);
   if (dtype == FB_DT_F16)

@@ -88,7 +88,8 @@ def cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, table: torch.
 
     ``cu_seqlens`` (int32 [sequences + 1]): sequence b's tokens are rows ``cu_seqlens[b]`` to
     ``cu_seqlens[b + 1]``; without it there is one token a sequence.  ``max_new``: the most new
-    tokens of one sequence (more are not written); by default all of them could be one's.
+    tokens of one sequence (those behind its first ``max_new`` are not written); by default all
+    of them could be one's.
 
     A block's scale is the least power of two (from 2^-100 up) that brings its values within
     E4M3's range; values are rounded to nearest even, non-finite ones are held as NaN.  A block

@@ -471,8 +471,8 @@ typedef struct {
 /* Writes new keys and values into the cache: sequence b's at lens[b], lens[b] + 1, ... (lens:
  * the tokens held before the call).  A block that holds earlier tokens keeps the larger of its
  * scale and the new tokens' own; where it grows, the earlier codes are rounded to the new scale.
- * Slots behind the new tokens are left as they are.  Tokens beyond a sequence's last page or
- * of pages outside the pool are not written.
+ * Slots behind the new tokens are left as they are.  A sequence's tokens beyond its first max_new,
+ * beyond its last page or of pages outside the pool are not written.
  *   k, v  [tokens, heads, D] of dtype FB_DT_F16, BF16 or F32; strides in elements, the last
  *         dimension contiguous; element-aligned pointers */
 int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int64_t k_token,

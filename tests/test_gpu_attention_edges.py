@@ -257,3 +257,19 @@ def test_evict_zeros_from_large_blocks(D, big):
             cut = O.Tokens(D)
             cut.append(old.values()[ids])
             np.testing.assert_array_equal(got.double().cpu().numpy(), cut.values())
+
+
+# ------------------------------------------------------------------ appending no more than max_new
+@pytest.mark.parametrize("max_new", [0, 1, 2, 31, 33, 40])
+def test_append_writes_no_more_than_max_new(max_new):
+    """Of 40 tokens a sequence the first max_new come into the cache and into the scales."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(80, 2, 64, device=DEV, generator=g) * torch.linspace(1, 90, 80, device=DEV)[:, None, None]
+    table, start = _i32(0, 1, 2, 3, 4, 5).view(2, 3), _i32(30, 7)
+    got, want = (KVCache.new(6, 2, 64, 32, DEV) for _ in range(2))
+    cache_append(got, x, x, table, start, _i32(0, 40, 80), max_new=max_new)
+    n = min(max_new, 40)
+    y = torch.cat([x[:n], x[40:40 + n]])
+    cache_append(want, y, y, table, start, _i32(0, n, 2 * n))
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
