@@ -1256,12 +1256,15 @@ __global__ __launch_bounds__(256, 2) void attn_weights_kernel(Attn a, Weights w)
 #pragma unroll
           for (int z = 0; z < KB; ++z) s[z] = H::mfma32(kf[z][i / 2][i & 1], now, s[z]);
         }
-        const float l = lse2[parity][row];
+        float l = lse2[parity][row];
         // the tile's least row against the wave's last token, its last against the run's end
         const bool masked = a.token_of(first + y * 32) + len - n + 1 < t0 + KB * kBlock ||
                             first + y * 32 + 32 > to;
         if (masked) {
           asm volatile("");  // a branch, not selects in every tile
+          // a row of NaN gives nothing to what it does not see either: its scores have the NaN
+          const float lost = l == l ? 0.f : l;
+          l = l == l ? l : 0.f;
           const int seen = first + row < to
                                ? len - n + a.token_of(first + row) + 1 - t0 - 4 * x2
                                : INT32_MIN;
@@ -1269,7 +1272,7 @@ __global__ __launch_bounds__(256, 2) void attn_weights_kernel(Attn a, Weights w)
           for (int z = 0; z < KB; ++z)
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-              if (z * kBlock + 8 * (k / 4) + k % 4 >= seen) s[z][k] = -__builtin_inff();
+              s[z][k] = z * kBlock + 8 * (k / 4) + k % 4 < seen ? s[z][k] + lost : -__builtin_inff();
         }
 #pragma unroll
         for (int z = 0; z < KB; ++z)
@@ -1371,16 +1374,26 @@ __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, 
   __syncthreads();
   while (t < end) {
     f32x4 sum{0, 0, 0, 0};
+    if (t + 4 <= len - n + 1) {  // every row sees them
 #pragma unroll
-    for (int row = 0; row < kFirst; ++row)
-      if (row < rows)
+      for (int row = 0; row < kFirst; ++row)
+        if (row < rows)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] += exp2f_(score[row][k] - lse2[row]);  // unseen: 2^-inf
+          for (int k = 0; k < 4; ++k) sum[k] += exp2f_(score[row][k] - lse2[row]);
 #pragma unroll 4
-    for (int row = kFirst; row < rows; ++row) {
-      const f32x4 s = *reinterpret_cast<const f32x4*>(s0 + (int64_t)row * a.score_tokens + t);
+      for (int row = kFirst; row < rows; ++row) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(s0 + (int64_t)row * a.score_tokens + t);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[k] += exp2f_(s[k] - lse2[row]);
+        for (int k = 0; k < 4; ++k) sum[k] += exp2f_(s[k] - lse2[row]);
+      }
+    } else {  // seldom; a row of NaN gives nothing to what it does not see either
+#pragma unroll 1
+      for (int row = 0; row < rows; ++row) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(s0 + (int64_t)row * a.score_tokens + t);
+        const int sees = len - n + a.token_of(row) + 1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += t + k < sees ? exp2f_(s[k] - lse2[row]) : 0.f;
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)

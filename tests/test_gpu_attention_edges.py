@@ -273,3 +273,25 @@ def test_append_writes_no_more_than_max_new(max_new):
     cache_append(want, y, y, table, start, _i32(0, n, 2 * n))
     for a, b in zip(got, want):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ weights beside a row of NaN
+@pytest.mark.parametrize("new,group,D", [(4, 2, 64), (3, 4, 128), (9, 4, 64), (60, 2, 128), (150, 1, 256),
+                                         (90, 20, 64)])
+def test_weights_beside_a_row_of_nan(new, group, D):
+    """A query of NaN makes NaN of the weights of the tokens that it sees, and of no others: those
+    get what the later rows give them."""
+    n, heads, bad = 400, 2, new // 2
+    c = Case([n], heads, D, 64)
+    q = torch.randn(new, heads * group, D, generator=c.g).bfloat16().to(DEV)
+    cu, lens = _i32(0, new), _i32(n)
+    spoilt = q.clone()
+    spoilt[bad, :, 1] = float("nan")
+    w, later = (torch.zeros(1, heads, n, device=DEV) for _ in range(2))
+    cache_attention(spoilt, c.cache, c.table, lens, cu, weights=w, max_len=n)
+    cache_attention(q[bad + 1:], c.cache, c.table, lens, _i32(0, new - bad - 1), weights=later, max_len=n)
+    seen = n - new + bad + 1
+    assert bool(w[..., :seen].isnan().all())
+    # the same rows' weights, summed in another order: at most 2^12 of them
+    got, want = w[0, :, seen:].double(), later[0, :, seen:].double()
+    assert bool(((got - want).abs() <= 2.0 ** 13 * U * want).all())
