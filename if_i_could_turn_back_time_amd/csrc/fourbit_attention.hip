@@ -42,8 +42,8 @@ struct Attn {
   int grain;          // chunks that a part has at least
   int most;           // parts that a sequence has at most
   int tiles;          // many rows: tiles of a sequence's rows that are dealt out; few: 0
-  float* part;        // [splits][T * Hq][D]
-  float2* part_ml;    // [splits][T * Hq]: what the sums are relative to (base 2), sum
+  float* part;        // [splits][T * Hq][D]: averages over a part, which are no larger than v
+  float2* part_ml;    // [splits][T * Hq]: what the weights' sum is relative to (base 2), the sum
   int per_shift;      // log2 of a page's blocks, -1: no power of two
   float* scores;      // or null: [B][H][score_rows][score_tokens], base 2
   int score_rows, score_tokens;
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_f
     const bool alone = part.parts == 1;  // no other part of the sequence: the result itself
     const int64_t orow = (int64_t)(row0 + wi) * a.Hq + h * a.group + (tile + wr - wi * a.group);
     const float out_scale =
-        exp2i(min(max(unit_of(wr) - kLift, -126), 127)) * (alone ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
+        exp2i(min(max(unit_of(wr) - kLift, -126), 127)) * (L == 0.f ? 0.f : 1.f / L);
 #pragma unroll
     for (int pass = 0; pass < DP / PASS; ++pass) {
       if (pass) __syncthreads();
@@ -1015,8 +1015,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
           if (dead[d / 2] >> (16 * (d & 1) + k) & 1) o[d][k] = __builtin_nanf("");
     if (there) {
       const int64_t orow = (int64_t)(row0 + i) * a.Hq + head;
-      const float factor = exp2i(min(max(E - kLift, -126), 127)) *
-                           (parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+      const float factor = exp2i(min(max(E - kLift, -126), 127)) * (l == 0.f ? 0.f : 1.f / l);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -1057,6 +1056,8 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
   using H = Half<DT>;
   __shared__ f32x4 part_v[256];
   __shared__ float part_m[64], part_l[64];
+  // The weights' sums are held 2^24 times smaller: times averages near fp32's range they would pass it.
+  constexpr float kBelow = 24.f;
   const Cache& c = a.c;
   int row0, n;
   c.rows(b, row0, n);
@@ -1091,9 +1092,9 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
       v *= f0;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const float f = ml[j].y == 0.f ? 0.f : exp2f_(ml[j].x - to);
-        L += ml[j].y * f;
-        v += w[j] * f;
+        const float g = ml[j].y == 0.f ? 0.f : ml[j].y * exp2f_(ml[j].x - to - kBelow);
+        L += g;
+        v += w[j] * g;
       }
       M = to;
     }
@@ -1125,7 +1126,7 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
                   (unsigned)H::round(v[2]) | (unsigned)H::round(v[3]) << 16};
     *reinterpret_cast<u32x2*>(static_cast<unsigned short*>(a.out) + row * c.D + d) = w;
     if (d == 0 && a.lse)
-      a.lse[row] = L == 0.f ? -__builtin_inff() : (M + __builtin_log2f(L)) * kLn2;
+      a.lse[row] = L == 0.f ? -__builtin_inff() : (M + (__builtin_log2f(L) + kBelow)) * kLn2;
   }
 }
 

@@ -295,3 +295,18 @@ def test_weights_beside_a_row_of_nan(new, group, D):
     # the same rows' weights, summed in another order: at most 2^12 of them
     got, want = w[0, :, seen:].double(), later[0, :, seen:].double()
     assert bool(((got - want).abs() <= 2.0 ** 13 * U * want).all())
+
+
+# ------------------------------------------------------------------ values near fp32's range
+@pytest.mark.parametrize("lens,new,group", [([6000], [1], 4), ([5000, 300], [1, 1], 1), ([4000], [3], 8),
+                                            ([3000], [40], 2), ([6000, 2500], [30, 41], 2)])
+def test_large_values_in_parts(lens, new, group):
+    """Values of 2^120 to 2^126, all of one sign: no sum over a part or over the parts may overflow."""
+    c = _scaled(lens, 2, 64, torch.float32, [2.0 ** 122, 2.0 ** 124], {})
+    for side in c.v:
+        assert all(np.abs(v.values()).max() < 2.0 ** 127 for v in side)
+    c.cache.v.view(torch.uint8).bitwise_and_(0x7F)
+    for side in c.v:
+        for v in side:
+            v.codes = np.abs(v.codes)
+    _strict(c, new, group, torch.bfloat16)
