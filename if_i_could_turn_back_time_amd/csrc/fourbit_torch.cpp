@@ -251,6 +251,13 @@ void no_grad_through(std::initializer_list<at::Tensor> ts, const char* what) {
     if (t.requires_grad()) throw std::runtime_error(what);
 }
 
+// What these calls write in place raises its version, as torch's own operators do, so that a graph
+// that saved it notices.
+void written(std::initializer_list<at::Tensor> ts) {
+  for (const at::Tensor& t : ts)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 fb_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
                     const at::Tensor& vs) {
   want_plain(k, k, "cache: tensors on a ROCm GPU are needed");
@@ -361,6 +368,7 @@ void cache_append(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& 
   c10::DeviceGuard guard(ck.device());
   check(fb_cache_append(&c, &s, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                         v.stride(1), dt, stream_of(ck)));
+  written({ck, cv, cks, cvs});
 }
 
 std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
@@ -414,6 +422,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
       out.data_ptr(), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, wp,
       wp ? weights->stride(0) : 0, wp ? weights->stride(1) : 0,
       wp ? (int32_t)weights->size(2) : 0, ptr_or_null(ws, need), need, stream_of(ck)));
+  if (wp) written({*weights});
   return {out, want_lse ? std::optional<at::Tensor>(lse) : std::nullopt};
 }
 
@@ -452,6 +461,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cache_evict(
                        (int32_t)new_table.size(1), static_cast<int32_t*>(kept.data_ptr()),
                        static_cast<float*>(nw.data_ptr()), static_cast<int32_t*>(nl.data_ptr()),
                        stream_of(ck)));
+  written({ck, cv, cks, cvs});
   return {kept, nl, nw};
 }
 

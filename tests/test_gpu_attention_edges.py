@@ -310,3 +310,30 @@ def test_large_values_in_parts(lens, new, group):
         for v in side:
             v.codes = np.abs(v.codes)
     _strict(c, new, group, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ what torch knows of these calls
+def test_in_place_writes_raise_versions():
+    c = Case([90], 2, 64, 64)
+    lens = _i32(90)
+    w = torch.zeros(1, 2, 128, device=DEV)
+    p = torch.ones(1, 2, 128, device=DEV, requires_grad=True)
+    product = w * p  # keeps w
+    before = [x._version for x in c.cache]
+    q = torch.randn(1, 4, 64, device=DEV, dtype=torch.bfloat16)
+    cache_attention(q, c.cache, c.table, lens)
+    assert [x._version for x in c.cache] == before
+    cache_attention(q, c.cache, c.table, lens, weights=w, max_len=90)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        product.sum().backward()
+    assert [x._version for x in c.cache] == before
+    cache_append(c.cache, q[:, :2], q[:, 2:], c.table, lens)
+    assert all(x._version > v for x, v in zip(c.cache, before))
+    before = [x._version for x in c.cache]
+    spare = _i32(*[i for i in range(5) if i not in c.table[0].tolist()][:1])[None]
+    cache_evict(c.cache, c.table, lens, w, 40, 8, spare, max_len=90)
+    assert all(x._version > v for x, v in zip(c.cache, before))
+    with torch.inference_mode():
+        cache = KVCache.new(2, 2, 64, 64, DEV)
+    cache_append(cache, q[:, :2], q[:, 2:], _i32(0, 1)[None], _i32(0))  # has no version, and works
+    assert bool((cache.k_scale[0, :, 0] > 0).all())
