@@ -258,6 +258,17 @@ void written(std::initializer_list<at::Tensor> ts) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// A trace, or a mode that records or replaces torch's operators, would hold the results as constants
+// or buffers that nobody fills.
+void not_recorded() {
+  using Key = c10::impl::TorchDispatchModeKey;
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer) ||
+      Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FUNCTIONAL))
+    throw std::runtime_error("this call is no torch operator: it cannot be traced or recorded (a HIP "
+                             "graph can capture it)");
+}
+
 fb_cache_t cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
                     const at::Tensor& vs) {
   want_plain(k, k, "cache: tensors on a ROCm GPU are needed");
@@ -352,6 +363,7 @@ void cache_append(const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& 
                   const at::Tensor& cvs, const at::Tensor& k, const at::Tensor& v,
                   const at::Tensor& table, const at::Tensor& start,
                   const std::optional<at::Tensor>& cu, std::optional<int64_t> max_new) {
+  not_recorded();
   const fb_cache_t c = cache_of(ck, cv, cks, cvs);
   want_plain(k, ck, "k and v must be tensors on the cache's GPU");
   want_plain(v, ck, "k and v must be tensors on the cache's GPU");
@@ -377,6 +389,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> cache_attention(
     const std::optional<at::Tensor>& cu, std::optional<int64_t> max_new,
     std::optional<int64_t> max_len, std::optional<double> scale,
     const std::optional<at::Tensor>& weights, bool want_lse) {
+  not_recorded();
   const fb_cache_t c = cache_of(ck, cv, cks, cvs);
   want_plain(given, ck, "q must be a tensor on the cache's GPU");
   no_grad_through({given}, "attention over the cache has no gradient: call it under torch.no_grad() "
@@ -430,6 +443,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> cache_evict(
     const at::Tensor& ck, const at::Tensor& cv, const at::Tensor& cks, const at::Tensor& cvs,
     const at::Tensor& table, const at::Tensor& lens, const at::Tensor& weights, int64_t keep,
     int64_t recent, const at::Tensor& new_table, std::optional<int64_t> max_len) {
+  not_recorded();
   const fb_cache_t c = cache_of(ck, cv, cks, cvs);
   want(weights.dim() == 3, "weights must be float32 [sequences, heads, tokens]");
   const fb_seqs_t s = seqs_of(table, lens, std::nullopt, table.size(0), std::nullopt,
@@ -520,6 +534,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
 
 std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& tokens,
                                        int64_t top) {
+  not_recorded();
   want(logits.defined() && plain(logits), "logits must be a tensor on a ROCm GPU");
   want_plain(tokens, logits, "tokens must be a tensor on the logits' GPU");
   want(dtype_code(logits.scalar_type()) >= 0, "logits must be float16, bfloat16 or float32");

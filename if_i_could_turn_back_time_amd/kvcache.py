@@ -7,7 +7,8 @@ bytes of a 16-bit cache.  They lie in pages that all sequences share: a sequence
 the pages its row of an int32 ``table`` names, in order, and its length is an entry of an int32
 tensor on the GPU.  Who owns which page is the program's business.  Nothing on the GPU is read
 back, so every call can be captured in a HIP graph (``torch.cuda.graph``) and replayed while the
-tables and lengths change.
+tables and lengths change.  The calls are no torch operators: tracing and recording them
+(``torch.jit.trace``, ``make_fx``) is refused.
 
     cache = KVCache.new(pages=512, heads=8, head_dim=128)
     cache_append(cache, k, v, table, held)                  # one new token a sequence

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from if_i_could_turn_back_time_amd import (KVCache, cache_append, cache_attention,
-                                           cache_evict)
+                                           cache_evict, token_logprobs)
 from oracle import cache_oracle as O
 from test_gpu_cache import Case
 
@@ -337,3 +337,37 @@ def test_in_place_writes_raise_versions():
         cache = KVCache.new(2, 2, 64, 64, DEV)
     cache_append(cache, q[:, :2], q[:, 2:], _i32(0, 1)[None], _i32(0))  # has no version, and works
     assert bool((cache.k_scale[0, :, 0] > 0).all())
+
+
+def _calls():
+    c = Case([90], 2, 64, 64)
+    lens = _i32(90)
+    spare = _i32(*[i for i in range(5) if i not in c.table[0].tolist()][:1])[None]
+    w = torch.rand(1, 2, 128, device=DEV)
+    tok = torch.zeros(1, dtype=torch.long, device=DEV)
+    q = torch.randn(1, 4, 64, device=DEV, dtype=torch.bfloat16)
+    return q, (lambda q: cache_attention(q, c.cache, c.table, lens),
+               lambda q: cache_append(c.cache, q[:, :2], q[:, 2:], c.table, lens) or q,
+               lambda q: cache_evict(c.cache, c.table, lens, w, 40, 8, spare, max_len=90).weights,
+               lambda q: token_logprobs(q.flatten(1), tok).logprob)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_recording_is_refused(which):
+    """A trace would hold what the call gave once, a recorded graph an empty buffer."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    q, calls = _calls()
+    call = calls[which]
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(call, (q,), check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(q)
+    call(q)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_fake_tensors_are_refused(which):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    q, calls = _calls()
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises((RuntimeError, ValueError)):
+        calls[which](q)
