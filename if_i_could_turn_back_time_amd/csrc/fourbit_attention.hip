@@ -304,16 +304,13 @@ __device__ inline Part find_part(const Attn& a, int x, int z, int chunk) {
   return p;
 }
 
-template <int DP>
-constexpr int few_waves() {
-  return 4;
-}
+constexpr int kFewWaves = 4;
 
 template <int DT, int DP, bool EX>
-__global__ __launch_bounds__(64 * few_waves<DP>(), DP > 128 ? 1 : 2) void attn_few_kernel(Attn a) {
+__global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : 2) void attn_few_kernel(Attn a) {
   using H = Half<DT>;
   using F = Half<FB_DT_F16>;
-  constexpr int NP = DP / 64, ND = DP / 16, NW = few_waves<DP>();
+  constexpr int NP = DP / 64, ND = DP / 16, NW = kFewWaves;
   constexpr int PASS = 64;  // channels joined at a time
   __shared__ float join[NW][16][PASS + 4];
   __shared__ float wave_m[NW][16], wave_l[NW][16];
@@ -1321,7 +1318,6 @@ __global__ __launch_bounds__(256) void attn_weights_join_kernel(Cache c, Weights
 // Weights of few rows, from the scores that were written down: 4 tokens a thread.  Every row's sum
 // comes from its parts here too, so that this need not wait for their being joined; the first 8 rows'
 // scores and the old weights are asked for before it, 16 threads take a row's parts.
-template <int DT, int DP>
 __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, int h, int b) {
   constexpr int kFirst = 8;
   __shared__ float part_m[16][16], part_l[16][16];
@@ -1407,13 +1403,13 @@ __device__ void add_few_weights(const Attn& a, const Weights& w, int x, int xs, 
 // What is left after the parts: blocks x < joins join them, the others add the weights.  Bound by the
 // parts' bytes where there are many rows (2 parts of 980 rows of 24 heads of 128: 11 us), by latency
 // otherwise.
-template <int DT, int DP>
+template <int DT>
 __global__ __launch_bounds__(256) void attn_finish_kernel(Attn a, Weights w, int joins, int ways) {
   const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   if (x < joins)
     join_parts<DT>(a, ways, x, joins, h, b);
   else
-    add_few_weights<DT, DP>(a, w, x - joins, gridDim.x - joins, h, b);
+    add_few_weights(a, w, x - joins, gridDim.x - joins, h, b);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1516,7 +1512,7 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, Weights w, hipStrea
   const int64_t rows = (int64_t)std::max(1, std::min(s->max_new, s->tokens)) * a.group;
   if (p.few) {
     hipLaunchKernelGGL((attn_few_kernel<DT, DP, EX>), dim3(p.splits, a.c.H, p.dealt ? 1 : a.c.B),
-                       dim3(64 * few_waves<DP>()), 0, hs, a);
+                       dim3(64 * kFewWaves), 0, hs, a);
   } else {
     const int64_t nx = (int64_t)a.c.H * (p.dealt ? 1 : a.c.B) * p.splits;
     if (nx > INT32_MAX) return FB_ERR_SHAPE;
@@ -1531,7 +1527,7 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, Weights w, hipStrea
   const int joins = p.part ? (int)std::min<int64_t>((rows + per - 1) / per, 1 << 20) : 0;
   const int adds = a.scores ? (int)((len + 1023) / 1024) : 0;
   if (joins + adds) {
-    hipLaunchKernelGGL((attn_finish_kernel<DT, DP>), dim3(joins + adds, a.c.H, a.c.B), dim3(256), 0,
+    hipLaunchKernelGGL(attn_finish_kernel<DT>, dim3(joins + adds, a.c.H, a.c.B), dim3(256), 0,
                        hs, a, w, joins, p.ways);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
