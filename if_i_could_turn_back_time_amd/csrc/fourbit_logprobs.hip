@@ -502,10 +502,18 @@ int fb_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int64_t
   if (misaligned({logprob, entropy, top_logprobs, stats}, 3) || misaligned({token, top_ids}, 7))
     return FB_ERR_ALIGN;
   hipStream_t hs = static_cast<hipStream_t>(stream);
+  const int64_t row_bytes = stride * (dtype == FB_DT_F32 ? 4 : 2);
   const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(kThreads), 0, hs, logits, stride, vocab,
-                       token, top, logprob, entropy, top_logprobs, top_ids, stats);
-    return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+    // a grid has fewer than 2^32 threads in a direction: beyond that rows would go missing
+    constexpr int64_t kMost = 1 << 22;
+    for (int64_t r = 0; r < rows; r += kMost) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(rows - r, kMost)), dim3(kThreads), 0, hs,
+                         static_cast<const char*>(logits) + r * row_bytes, stride, vocab, token + r,
+                         top, logprob + r, entropy + r, top ? top_logprobs + r * top : nullptr,
+                         top ? top_ids + r * top : nullptr, stats ? stats + 3 * r : nullptr);
+      if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+    }
+    return FB_OK;
   };
   return dtype == FB_DT_F16    ? go(logprobs_kernel<FB_DT_F16>)
          : dtype == FB_DT_BF16 ? go(logprobs_kernel<FB_DT_BF16>)
