@@ -1515,7 +1515,7 @@ int launch(const Attn& a, const Plan& p, const fb_seqs_t* s, Weights w, hipStrea
                        dim3(64 * kFewWaves), 0, hs, a);
   } else {
     const int64_t nx = (int64_t)a.c.H * (p.dealt ? 1 : a.c.B) * p.splits;
-    if (nx > INT32_MAX) return FB_ERR_SHAPE;
+    if (!fits_grid(nx, 256) || (w.to && !fits_grid((int64_t)a.c.H * a.c.B, 256))) return FB_ERR_SHAPE;
     const int64_t ny = p.dealt ? 1 : std::min<int64_t>((rows + kRows - 1) / kRows, 65535);
     hipLaunchKernelGGL((attn_many_kernel<DT, DP, EX>), dim3((unsigned)nx, (unsigned)ny), dim3(256),
                        0, hs, a);

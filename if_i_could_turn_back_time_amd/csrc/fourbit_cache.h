@@ -81,6 +81,10 @@ inline int check_cache(const fb_cache_t* c, const fb_seqs_t* s, Cache& k) {
   return FB_OK;
 }
 
+// Host: whether `groups` workgroups of `threads` can be launched in one direction.  Their threads are
+// counted in 32 bits: beyond that some would not run.
+inline bool fits_grid(int64_t groups, int threads) { return groups * threads <= UINT32_MAX; }
+
 // 2^e for e in [-126, 127].
 __device__ inline float exp2i(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }
 

@@ -607,11 +607,12 @@ int fb_cache_append(const fb_cache_t* c, const fb_seqs_t* s, const void* k, int6
   // blocks that max_new tokens can touch from any start on
   const int64_t ny = ((int64_t)std::min(s->max_new, s->tokens) + kBlock - 2) / kBlock + 1;
   const int64_t nx = (int64_t)s->seqs * c->heads * 2;
-  if (ny > 65535 || nx > INT32_MAX) return FB_ERR_SHAPE;
+  const int nt = (c->head_dim + 63) / 64 * 64;
+  if (ny > 65535 || !fits_grid(nx, nt)) return FB_ERR_SHAPE;
   const NewTokens x{k,      v,      k_token, k_head, v_token,
                     v_head, vec16(k, k_token, k_head, bytes), vec16(v, v_token, v_head, bytes),
                     s->max_new};
-  const dim3 grid((unsigned)nx, (unsigned)ny), threads((unsigned)(c->head_dim + 63) / 64 * 64);
+  const dim3 grid((unsigned)nx, (unsigned)ny), threads((unsigned)nt);
   hipStream_t hs = static_cast<hipStream_t>(stream);
   if (dtype == FB_DT_F16)
     hipLaunchKernelGGL(cache_append_kernel<FB_DT_F16>, grid, threads, 0, hs, kc, x);
@@ -641,7 +642,7 @@ int fb_cache_evict(const fb_cache_t* c, const fb_seqs_t* s, const float* weights
   to.table_stride = new_stride;
   to.max_pages = new_pages;
   const int64_t nx = ((int64_t)keep + kBlock - 1) / kBlock;
-  if (nx > INT32_MAX) return FB_ERR_SHAPE;
+  if (!fits_grid(nx, 256)) return FB_ERR_SHAPE;
   hipStream_t hs = static_cast<hipStream_t>(stream);
   const auto select = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(c->heads, s->seqs), dim3(kSelect), 0, hs, kc, weights, w_seq,

@@ -467,6 +467,8 @@ typedef struct {
   int32_t max_len;       /* about the most tokens a sequence holds: how work is split goes
                             by it, the result does not                                     */
 } fb_seqs_t;
+/* A call whose sequences and heads (or kept tokens) ask for more than 2^32 - 1 threads in one
+ * direction of a launch is refused (FB_ERR_SHAPE). */
 
 /* Writes new keys and values into the cache: sequence b's at lens[b], lens[b] + 1, ... (lens:
  * the tokens held before the call).  A block that holds earlier tokens keeps the larger of its
