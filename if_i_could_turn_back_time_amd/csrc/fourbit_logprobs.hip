@@ -5,6 +5,9 @@
 // w = sum 2^y y come from one walk over the row:  log p_i = ln 2 (y_i - log2 z), entropy =
 // ln 2 (log2 z - w / z).  Each thread has its own R, raised when a value passes it by 2^kSlack; a
 // whole R is subtracted without rounding (one fma) and threads are joined by exact powers of two.
+// That holds while R, itself rounded from a product, is within 8 of it: between -2^27 (where it
+// starts, so that anything lower counts as 0) and 2^27.  Rows beyond are walked again relative to
+// their largest value.
 // The alternatives: lane l's largest value over all waves is one of 64 different values of the
 // row, so the top-th largest of these 64 bounds the row's top-th largest from below.  Only threads
 // whose own largest reaches the bound hold candidates (about as many as are wanted), and only
@@ -120,7 +123,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 24.f;     // a thread's sums stay below 2^24 * its values
 constexpr float kLow = -200.f;     // 2^y is 0 from here on, and y itself may be -inf
-constexpr float kHuge = 1.2676506e30f;  // 2^100: logits beyond it would overflow in base 2
+constexpr float kFar = 0x1p27f;    // of R, see above
+constexpr float kHuge = 0x1p100f;  // keeps a difference of two R finite
 
 // Sums of 2^y and 2^y y relative to R.
 struct Sums {
@@ -190,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   const bool given = t >= 0 && t < vocab;
   const float at_token = given ? (float)row.p[t] : 0.f;
   float m = -inf;  // the thread's largest value
-  Sums s{-kHuge, 0.f, 0.f};
+  Sums s{-kFar, 0.f, 0.f};
   const auto raise = [&](float x) {  // to a whole number near x
     const float to = fminf(__builtin_rintf(x * kLog2e), 3e38f);
     if (to > s.R + kSlack) s.rebase(to);
@@ -245,13 +249,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
     s.z += o.z;
     s.w += o.w;
   }
-  // Logits beyond 2^100, or nothing but -inf: relative to the largest itself, then scaled.
+  // Far from 0, or nothing but -inf: relative to the largest itself, then scaled.  (The sums may be
+  // NaN for being far; of a row that holds a NaN they come out so again.)
   float shift = 0.f;  // y = (x - shift) log2(e) - R
-  if (!(s.z > 0.f) || __builtin_fabsf(s.R) >= kHuge) {
+  if (!(s.z > 0.f) || __builtin_fabsf(s.R) >= kFar) {
     m = -inf;
     for (int i = 0; i < kWaves; ++i) m = fmaxf(m, lane_max[i][lane]);
     m = wave_max(m);
-    if (__builtin_fabsf(m) < inf && s.z == s.z) {
+    if (__builtin_fabsf(m) < inf) {
       shift = m;
       s = Sums{0.f, 0.f, 0.f};
       row.walk([&](int, float x) { s.add((x - shift) * kLog2e); });
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
       }
     }
   }
-  if (s.z == inf) s.z = __builtin_nanf("");  // of a logit of +inf
+  if (m == inf || s.z == inf) s.z = __builtin_nanf("");  // of a logit of +inf
   const float log2z = __builtin_log2f(s.z);
   const auto logp = [&](float x) {
     return s.z == 0.f ? -inf : kLn2 * (__builtin_fmaf(x - shift, kLog2e, -s.R) - log2z);
