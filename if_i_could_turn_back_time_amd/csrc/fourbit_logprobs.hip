@@ -278,7 +278,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(
   if (m == inf || s.z == inf) s.z = __builtin_nanf("");  // of a logit of +inf
   const float log2z = __builtin_log2f(s.z);
   const auto logp = [&](float x) {
-    return s.z == 0.f ? -inf : kLn2 * (__builtin_fmaf(x - shift, kLog2e, -s.R) - log2z);
+    const float y = __builtin_fmaf(x - shift, kLog2e, -s.R) - log2z;
+    // a masked logit of the type's least value passes the range in base 2 only
+    return s.z == 0.f ? -inf : y < -kHuge ? (x - shift) - kLn2 * (s.R + log2z) : kLn2 * y;
   };
   if (tid == 0) {
     logprob[r] = given ? logp(at_token) : 0.f;

@@ -42,7 +42,7 @@ def test_masks_of_any_size(dt, V):
     """Forbidden tokens given as large negative numbers: alone at first in a thread's walk, and with
     an ordinary logit behind them."""
     g = torch.Generator().manual_seed(V)
-    masks = [-1e8, -1e9, -1e10, -3e10, -1e12, -7e13, -1e15, -1e20, -3e25, -1e29, -1e30]
+    masks = [-1e8, -1e9, -1e10, -3e10, -1e12, -7e13, -1e15, -1e20, -3e25, -1e29, -1e30, -3.38e38]
     x = torch.randn(len(masks), V, generator=g)
     for i, mask in enumerate(masks):
         x[i, torch.rand(V, generator=g) < 0.9] = mask * (1 + 0.01 * torch.rand((), generator=g))
