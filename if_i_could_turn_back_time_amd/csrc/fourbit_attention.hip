@@ -224,6 +224,18 @@ constexpr int kRows = 128, kTile = 64;  // of the kernel for many rows
 constexpr int kLift = 7;
 // A tile's sum of them that asks for the row's largest score anew: none is above fp16's range.
 constexpr float kMost = 32768.f;
+// From here on a row's largest score, rounded, can be units away from itself, and its weight anything:
+// such rows are weighed anew by rounded scores, of which the largest is equal to it.
+constexpr float kFar = 4194304.f;
+
+__device__ inline bool is_far(float m) {
+  return __builtin_fabsf(m) >= kFar && m != -__builtin_inff();
+}
+// The weight's exponent, relative to m, for a sum of q and codes and their block's scale.
+__device__ inline float exponent(float s, float ks, float m, float shift) {
+#pragma clang fp contract(off)
+  return is_far(m) ? (s * ks - m) + (float)kLift : __builtin_fmaf(s, ks, shift);
+}
 
 // Which sequence, tile of its rows (many rows have several) and part of its tokens a workgroup has.
 // Up to 64 sequences are dealt out by their lengths: parts are about of one size, the least with
@@ -355,6 +367,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : 2) void attn_few_ker
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
+    bool far = false;                      // whether a row's m is
     Unit unit;
     int E = unit.now;                      // the row's: of the last block that it saw
     unsigned dead[(ND + 7) / 8] = {};      // bit 4 (d % 8) + k of d / 8: o[d][k] saw a NaN value
@@ -471,20 +484,21 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : 2) void attn_few_ker
       const float vscale = Unit::scale(block_seen ? e : unit.now, unit.now);
       float sum;
       h16x8 pf[2];
-      const auto weigh = [&]() __attribute__((always_inline)) {
+      const auto weigh = [&](auto anew) __attribute__((always_inline)) {
         const float shift = (float)kLift - (m == -__builtin_inff() ? 0.f : m);
         sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float p = exp2f_(__builtin_fmaf(s[j][k], ks, shift));
+            const float p = exp2f_(anew ? exponent(s[j][k], ks, m, shift)
+                                        : __builtin_fmaf(s[j][k], ks, shift));
             sum += p;
             pf[j / 2][4 * (j & 1) + k] = (_Float16)p;
           }
       };
-      weigh();
-      if (__any(m == -__builtin_inff() || sum > kMost)) {
+      weigh(std::false_type{});
+      if (far || __any(m == -__builtin_inff() || sum > kMost)) {
         asm volatile("");
         float big = s[0][0];
 #pragma unroll
@@ -500,7 +514,8 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : 2) void attn_few_ker
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= alpha;
         m = up;
-        weigh();
+        far = __any(is_far(m));
+        weigh(std::true_type{});
       }
       l += sum;
       if (masked) {
@@ -767,6 +782,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[d][k] = 0.f;
     float m = -__builtin_inff(), l = 0.f;  // m: what the sums are relative to
+    bool far = false;                      // whether a row's m is
     Unit unit;
     int E = unit.now;                      // the row's: of the last block that it saw
     unsigned dead[(ND + 1) / 2] = {};      // bit 16 (d % 2) + k of d / 2: o[d][k] saw a NaN value
@@ -935,21 +951,22 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
                                Unit::scale(e1, unit.takes(e1) ? unit.now : unit.within(e1))};
       float sum[2];
       h16x8 pf[2][2];
-      const auto weigh = [&]() __attribute__((always_inline)) {
+      const auto weigh = [&](auto anew) __attribute__((always_inline)) {
         const float shift = (float)kLift - (m == -__builtin_inff() ? 0.f : m);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           sum[y] = 0.f;
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float p = exp2f_(__builtin_fmaf(s[y][k], ks[y], shift));
+            const float p = exp2f_(anew ? exponent(s[y][k], ks[y], m, shift)
+                                        : __builtin_fmaf(s[y][k], ks[y], shift));
             sum[y] += p;
             pf[y][k / 8][k & 7] = (_Float16)p;
           }
         }
       };
-      weigh();
-      if (turn || __any(m == -__builtin_inff() || sum[0] + sum[1] > kMost)) {
+      weigh(std::false_type{});
+      if (turn || far || __any(m == -__builtin_inff() || sum[0] + sum[1] > kMost)) {
         asm volatile("");
         float mx[2];
 #pragma unroll
@@ -966,7 +983,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void attn_many_kernel(Attn a
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] *= both;
         m = up;
-        weigh();
+        far = __any(is_far(m));
+        weigh(std::true_type{});
       }
       l += sum[0] + sum[1];
       {
@@ -1226,10 +1244,14 @@ __global__ __launch_bounds__(256, 2) void attn_weights_kernel(Attn a, Weights w)
     };
     const auto stage = [&](int first, const uint8_t* buf, uint8_t* other, int parity)
         __attribute__((always_inline)) {
-      // a row that sees nothing gives no weight
-      if (tid < ROWS)
-        lse2[parity][tid] =
-            next_lse == -__builtin_inff() ? __builtin_inff() : next_lse * kLog2e;
+      // A row that sees nothing gives no weight.  One far from 0 (see kFar) has what its sum's rounding
+      // may hide added, so that no weight is above 1.
+      if (tid < ROWS) {
+        const float l = next_lse * kLog2e;
+        lse2[parity][tid] = next_lse == -__builtin_inff() ? __builtin_inff()
+                            : is_far(l)                   ? l + __builtin_fabsf(l) * 0x1p-21f
+                                                          : l;
+      }
       wait_for_loads();
       __syncthreads();  // these rows are there; everyone is done with the other buffer
       if (first + ROWS < to) fetch(other, first + ROWS);

@@ -371,3 +371,33 @@ def test_fake_tensors_are_refused(which):
     q, calls = _calls()
     with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises((RuntimeError, ValueError)):
         calls[which](q)
+
+
+# ------------------------------------------------------------------ scores far from 0
+@pytest.mark.parametrize("size", [1e8, 1e9, 1e10, 1e12, 1e20])
+@pytest.mark.parametrize("new,group,lens", [(1, 4, 300), (3, 4, 70), (60, 2, 300), (1, 2, 4000)])
+def test_scores_of_any_size(new, group, lens, size):
+    """Scores so large that fp32 holds them to many units: the weights are those of one token or of a
+    few, and the outputs lie between the least and the largest value that a row sees."""
+    c = Case([0], 2, 64, 64, torch.bfloat16, parts=1)
+    c.table = torch.arange(-(-lens // 64), dtype=torch.int32, device=DEV)[None]
+    c.cache = KVCache.new(c.table.shape[1], 2, 64, 64, DEV)
+
+    def spoil(x):
+        x[:, 0] *= size
+    c.append([0], [lens], 1.0, spoil)
+    q = torch.randn(new, 2 * group, 64, generator=c.g).bfloat16().to(DEV)
+    w = torch.zeros(1, 2, lens, device=DEV)
+    out, lse = cache_attention(q, c.cache, c.table, _i32(lens), _i32(0, new), weights=w, max_len=lens,
+                               return_lse=True)
+    assert bool(((w >= 0) & (w <= new * group * 1.01)).all())
+    out = out.double().cpu().numpy()
+    assert bool(lse.isfinite().all())
+    for h in range(2):
+        v = c.v[0][h].values()
+        for i in range(new):
+            seen = v[:lens - new + 1 + i]
+            lo, hi = seen.min(0), seen.max(0)
+            slack = 2.0 ** -7 * np.maximum(np.abs(lo), np.abs(hi))  # rounding to 16 bits, and of sums
+            got = out[i, h * group:(h + 1) * group]
+            assert (got >= lo - slack).all() and (got <= hi + slack).all()
