@@ -216,7 +216,9 @@ struct Unit {
 // above 128 channels, for its registers.
 // Measured: 2 sequences of up to 100,003 tokens, 64 query heads over 8 of 128 (0.4 GB): 76 us, 5.3
 // TB/s, and 6 to join; 16 of up to 8,192 with weights: 52 and 14 for joining and weights.  Short
-// ones wait for the chain length, table, codes, join: 777 tokens of 32 heads 8 us and 3.
+// ones wait for the chain length, table, codes, join: 777 tokens of 32 heads 8 us and 3.  A head is
+// worked on at 64, 128 or 256 channels: 4 sequences of up to 8,000, 32 heads over 8, take 14.7 us with
+// 64, 17.3 with 80, 19.9 with 128, 27.5 with 144, 32.0 with 256.
 // ---------------------------------------------------------------------------------
 constexpr int kChunk = 64;
 constexpr int kRows = 128, kTile = 64;  // of the kernel for many rows
@@ -670,10 +672,13 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : 2) void attn_few_ker
 //  - the sums are brought up to date as above.
 // Heads and sequences vary fastest over the workgroups, then the tiles, the longest first: the
 // last ones to start are short, and where the heads are a multiple of 8 one XCD's L2 holds few.
-// Bound by VALU issue: a wave's 32 rows by 64 tokens take 476 instructions, 32 of them products; what
-// hides behind a product is four others.  Measured: a prompt of 4,096, 64 heads over 8 of 128, bf16:
-// 300 us, 920 TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads, dealt out to 480 places of 512: 66
-// us, 11 of them for the join.
+// Bound by VALU issue: a wave's 32 rows by 64 tokens take 451 instructions, 355 of them vector and 32
+// products; what hides behind a product is four others.  128 of them decode, which each of the four
+// waves does for itself.  Measured: a prompt of 4,096, 64 heads over 8 of 128, bf16: 292 us, 940
+// TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads, dealt out to 480 places of 512: 65 us, 11 of them
+// for the join.  Above 128 channels the registers are all taken, and 80 (256) or 252 bytes (others) of
+// what the branches for rare tiles hold are spilled: 900 rows of 6,000 of 8 heads 45.5 us with 128
+// channels, 82 with 256, 133 with 192, which are worked on as 256 at run-time strides.
 // ---------------------------------------------------------------------------------
 // Tokens that are staged at once: a barrier for each, so two tiles where LDS has room for it.
 template <int DP>
@@ -1152,8 +1157,9 @@ __device__ void join_parts(const Attn& a, int ways, int x, int xs, int h, int b)
 // operand that is read there meets both blocks of keys (with one block the LDS reads took as long as
 // the products).  A lane's sums are of 16 tokens a block over the rows of its column, so nothing
 // crosses lanes before the end.  Runs of rows leave their sums apart, which a last small kernel adds
-// in order: no atomics.  Half the products of the attention itself; one exponential a score bounds
-// it beside them.  Measured: a prompt of 4,096, 64 heads over 8 of 128: 265 us, 520 TFLOP/s.
+// in order: no atomics.  Half the products of the attention itself.  Measured: a prompt of 4,096, 64
+// heads over 8 of 128: 215 us, 640 TFLOP/s (5 more for the last kernel); what it waits for beside the
+// products and one exponential a score was not looked into.
 // ---------------------------------------------------------------------------------
 struct Weights {
   float* to;
@@ -1456,9 +1462,10 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int64_t len = std::max<int64_t>(1, std::min<int64_t>(s->max_len, capacity));
   const int64_t tiles = p.few ? 1 : (rows + kRows - 1) / kRows;
   const int64_t units = tiles * c->heads * s->seqs;
-  // The least part of few rows: a chunk a wave where that makes some but not many parts (3 to 14%
-  // faster from 600 to 8,000 tokens), two where one part could do (375 tokens of 160 heads: 9.2 us,
-  // 14.8 with two parts to join) or many would be (100,000 tokens of one head: 17.9 us, 21.2 with 390).
+  // The least part of few rows: a chunk a wave where that makes some but not many parts (one sequence
+  // of 8 heads: 2,000 tokens 10.4 us, 12.6 with two; 8,000 11.1 and 12.7; 16,384 14.0 and 13.8, of one
+  // head 11.7 and 13.1), two where one part could do (375 tokens of 160 heads: 9.2 us, 14.8 with two
+  // parts to join) or many would be (100,000 tokens of one head: 17.9 us, 21.2 with 390).
   p.grain = len > 8 * kChunk && len <= 256 * kChunk ? 4 : 8;
   p.chunk = kChunk;
   if (!p.few) {
@@ -1469,7 +1476,7 @@ Plan plan(const fb_cache_t* c, const fb_seqs_t* s, int q_heads, int w_tokens) {
   const int step = p.few ? 4 * kChunk : 4 * kTile;  // a part is a whole number of rounds or stages
   const int64_t most = (len + least - 1) / least;
   // Two workgroups a CU run side by side, of more than 128 channels one (900 rows of 6,000 tokens, 8
-  // heads of 256: 122 us split for two, 101 so; one of 60,000, 4 heads: 38 and 33).
+  // heads of 256: 101 us split for two, 82 so; one of 60,000, 4 heads: 39 and 34).
   const int64_t cus = fb_gpu::cu_count(), slots = c->head_dim <= 128 ? 2 * cus : cus;
   const int64_t want = std::min(std::max<int64_t>(1, slots / units), most);
   const int64_t steps = (len + step - 1) / step;

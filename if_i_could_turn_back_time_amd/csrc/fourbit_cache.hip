@@ -404,12 +404,12 @@ __global__ __launch_bounds__(kSelect) void evict_select_kernel(
 // Second half: the kept tokens to their new pages.  Workgroup = (one new block, head, sequence),
 // as an append of 32 tokens that are decoded from the cache.  Keys: 8 channels of a token a thread,
 // as they lie.  Values: a thread has one channel of 16 new tokens, a side of the new block, which it
-// writes in one piece; it reads their bytes one by one, 16 bytes from its neighbours' (a cache that
-// turns values for the matrix cores is read whole where a quarter of it is kept).  Few blocks are
+// writes in one piece; it reads their bytes one by one, 16 bytes from its neighbours'.  Few blocks are
 // bound by the chain id, page, codes, so all codes of a thread are asked for together (1,024 of 4,096
-// tokens of 32 heads: 10 us); many by the first-level cache, which takes a wave's 64 strided bytes in
-// 32 steps (16 sequences of up to 8,192 cut to 2,048: 52 us; 16-byte loads and a choice among
-// their words took 64 for their registers, keys and values in workgroups of their own 91).
+// tokens of 32 heads: 9 us); many by the values' strided bytes, 32 accesses of the first-level cache for
+// 64 lanes, which is busy two thirds of the time (16 sequences of up to 8,192 cut to 2,048, 79 MB
+// fetched for 67 MB kept: 46 to 50 us; 16-byte loads and a choice among their words took 64 for their
+// registers, keys and values in workgroups of their own 91).
 // ---------------------------------------------------------------------------------
 // The codes of a word that are NaN: their top bits.
 __device__ inline unsigned nan_codes(unsigned w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }

@@ -113,7 +113,9 @@ def cache_attention(q: torch.Tensor, cache: KVCache, table: torch.Tensor, lens: 
     from its last entry on, as in a batch padded for a graph).  A value of a token that a row does not see never reaches it, NaN or
     not.  ``cu_seqlens`` and ``max_new`` as for :func:`cache_append` (``max_new`` too small
     changes speed only, except that ``weights`` may miss the rows beyond it); ``max_len``: about
-    the longest length, by which the work is split.
+    the longest length, by which the work is split.  One sequence, and more than 64, should have it
+    close: 8,000 tokens of 32 heads take 18 us under their own length and 118 under 131,072 (2 to 64
+    sequences are dealt out by their lengths).
 
     ``weights`` (fp32 [sequences, heads, at least max_len]): grows in place by the attention
     weight that each held token got in this call, summed over rows and query heads; what
