@@ -676,9 +676,9 @@ __global__ __launch_bounds__(64 * kFewWaves, DP > 128 ? 1 : 2) void attn_few_ker
 // products; what hides behind a product is four others.  128 of them decode, which each of the four
 // waves does for itself.  Measured: a prompt of 4,096, 64 heads over 8 of 128, bf16: 292 us, 940
 // TFLOP/s; 2 x 333 rows of 4,001 tokens, 32 heads, dealt out to 480 places of 512: 65 us, 11 of them
-// for the join.  Above 128 channels the registers are all taken, and 80 (256) or 252 bytes (others) of
-// what the branches for rare tiles hold are spilled: 900 rows of 6,000 of 8 heads 45.5 us with 128
-// channels, 82 with 256, 133 with 192, which are worked on as 256 at run-time strides.
+// for the join.  Above 128 channels the registers are all taken, and 80 (256) or 252 bytes (others) are
+// spilled, with 256 none of them between the products of a tile: 900 rows of 6,000 of 8 heads 45.5 us
+// with 128 channels, 82 with 256, 133 with 192, which are worked on as 256 at run-time strides.
 // ---------------------------------------------------------------------------------
 // Tokens that are staged at once: a barrier for each, so two tiles where LDS has room for it.
 template <int DP>
