@@ -11,7 +11,10 @@ from .jenks import (bias_mask, jenks2, linear_mask, module_bias, module_conv,  #
                     module_weights)
 from .kvcache import (Evicted, KVCache, cache_append, cache_attention,  # noqa: F401
                       cache_evict)
-from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
+from .logprobs import (HeadLogprobs, TokenLogprobs, head_logprobs,  # noqa: F401
+                       token_logprobs)
+from .embedding import token_embedding  # noqa: F401
+from .residual import ResidualNorm, residual_norm  # noqa: F401
 from . import _capi  # noqa: F401
 
 __all__ = ["PackedWeight", "QuantLinear", "fp4_mfma_shared", "fwht_block_for", "packed_k",
@@ -19,4 +22,5 @@ __all__ = ["PackedWeight", "QuantLinear", "fp4_mfma_shared", "fwht_block_for", "
            "quantize_module", "adaround_levels", "pack_quantized_linears", "replace_forward",
            "jenks2", "linear_mask", "bias_mask", "module_weights", "module_bias",
            "module_conv", "KVCache", "cache_append", "cache_attention", "cache_evict", "Evicted",
-           "token_logprobs", "TokenLogprobs"]
+           "token_logprobs", "TokenLogprobs",
+           "head_logprobs", "HeadLogprobs", "token_embedding", "residual_norm", "ResidualNorm"]

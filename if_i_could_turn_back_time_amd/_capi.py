@@ -46,6 +46,10 @@ EXPORTED = (
     "fb_grad_bias_workspace_bytes",
     "fb_cache_append", "fb_cache_attention", "fb_cache_attention_workspace_bytes",
     "fb_cache_evict", "fb_token_logprobs", "fb_token_logprobs_grad",
+    "fb_embed", "fb_embed_grad", "fb_embed_grad_workspace_bytes",
+    "fb_residual_norm", "fb_residual_norm_grad", "fb_residual_norm_grad_workspace_bytes",
+    "fb_head_logprobs", "fb_head_logprobs_workspace_bytes", "fb_head_logprobs_grad",
+    "fb_head_logprobs_grad_workspace_bytes",
 )
 
 
@@ -68,6 +72,14 @@ class FbSeqs(ctypes.Structure):
                 ("max_new", ctypes.c_int32), ("max_len", ctypes.c_int32)]
 
 
+class FbNorm(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "branch", "gate", "weight", "branch_weight")]
+    _fields_ += [(n, ctypes.c_int64) for n in ("x_stride", "branch_stride", "rows", "gate_rows")]
+    _fields_ += [(n, ctypes.c_int32) for n in ("width", "dtype", "weight_dtype",
+                                               "branch_weight_dtype", "gate_dtype")]
+    _fields_ += [(n, ctypes.c_float) for n in ("scale", "eps")]
+
+
 _lib = None
 
 
@@ -84,6 +96,7 @@ def lib() -> ctypes.CDLL:
     vp, i32, sz = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t
     sp = ctypes.POINTER(FbShape)
     i64, cp, qp = ctypes.c_int64, ctypes.POINTER(FbCache), ctypes.POINTER(FbSeqs)
+    np_ = ctypes.POINTER(FbNorm)
     sigs = {
         "fb_abi_version": (i32, []),
         "fb_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -141,6 +154,19 @@ def lib() -> ctypes.CDLL:
                                              vp]),
         "fb_token_logprobs_grad": (ctypes.c_int, [vp, i32, i64, i64, i32, vp, i32, vp, vp, vp, vp,
                                                   vp, vp, vp, vp]),
+        "fb_embed": (ctypes.c_int, [vp, i64, i32, i32, i32, vp, i64, ctypes.c_float, vp, vp]),
+        "fb_embed_grad": (ctypes.c_int, [vp, i64, i32, i32, i32, vp, i64, ctypes.c_float, vp, vp,
+                                         sz, vp]),
+        "fb_embed_grad_workspace_bytes": (sz, [i64, i32, i32]),
+        "fb_residual_norm": (ctypes.c_int, [np_, vp, vp, vp, vp]),
+        "fb_residual_norm_grad": (ctypes.c_int, [np_, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+        "fb_residual_norm_grad_workspace_bytes": (sz, [np_]),
+        "fb_head_logprobs": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i32, i32, vp, vp, vp, vp,
+                                            vp, sz, vp]),
+        "fb_head_logprobs_workspace_bytes": (sz, [i64, i32, i32]),
+        "fb_head_logprobs_grad": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i32, i32, vp, vp, vp,
+                                                 vp, vp, vp, vp, vp, sz, vp]),
+        "fb_head_logprobs_grad_workspace_bytes": (sz, [i64, i32, i32, i32, i32]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)

@@ -94,6 +94,9 @@ def build(verbose: bool = False) -> Path:
     cache_o = BUILD / "fourbit_cache.o"
     attn_o = BUILD / "fourbit_attention.o"
     logp_o = BUILD / "fourbit_logprobs.o"
+    embed_o = BUILD / "fourbit_embed.o"
+    norm_o = BUILD / "fourbit_norm.o"
+    head_o = BUILD / "fourbit_head.o"
     trace_o = BUILD / "fourbit_gemv_trace.o"
     trace_ilp_o = BUILD / "fourbit_gemv_ilp_trace.o"
     steps = [
@@ -109,6 +112,9 @@ def build(verbose: bool = False) -> Path:
         [_hipcc(), *HIP_FLAGS, *inc, "-c", str(CSRC / "fourbit_attention.hip"), "-o",
          str(attn_o)],
         [_hipcc(), *HIP_FLAGS, *inc, "-c", str(CSRC / "fourbit_logprobs.hip"), "-o", str(logp_o)],
+        [_hipcc(), *HIP_FLAGS, *inc, "-c", str(CSRC / "fourbit_embed.hip"), "-o", str(embed_o)],
+        [_hipcc(), *HIP_FLAGS, *inc, "-c", str(CSRC / "fourbit_norm.hip"), "-o", str(norm_o)],
+        [_hipcc(), *HIP_FLAGS, *inc, "-c", str(CSRC / "fourbit_head.hip"), "-o", str(head_o)],
         # the GPU packer must round every fp64 operation as the host packer does
         [_hipcc(), *HIP_FLAGS, "-ffp-contract=off", *inc, "-c", str(CSRC / "fourbit_pack.hip"),
          "-o", str(pack_o)],
@@ -134,7 +140,8 @@ def build(verbose: bool = False) -> Path:
         tmp = lib.with_suffix(".so.tmp")
         link = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", str(host_o),
                 *map(str, kern_os), str(gemm_o), str(grad_o), str(pack_o), str(jenks2_o),
-                str(cache_o), str(attn_o), str(logp_o), "-o", str(tmp), "-lpthread"]
+                str(cache_o), str(attn_o), str(logp_o), str(embed_o), str(norm_o), str(head_o),
+                "-o", str(tmp), "-lpthread"]
         if verbose:
             print(" ".join(link), flush=True)
         _run(link)

@@ -1,0 +1,798 @@
+// Log probabilities of given tokens, and entropies, under a head of 16-bit weights, whose logits are
+// never kept; and the gradients of the hidden states and of the weights.
+//
+//   l = x W^T,  logprob = l[token] - log sum exp l,  entropy = -sum p log p
+//   G[r, v] = g_r [v = token_r] - p (g_r + h_r (log p + entropy_r)),  grad_x = G W,  grad_w = G^T x
+//
+// Four products on the matrix cores, all by product_kernel:
+//   kStats    a tile of logits is reduced where it was summed, to (largest, sum of exponentials, sum of
+//             exponentials times distance) for each of its rows; head_join makes a row's results of them.
+//   kGradient the same logits again, bit for bit (a logit's products are added in the same order
+//             whatever the tile), turned into G, rounded to the weights' type, for a piece of the
+//             vocabulary: 1 GiB of G at most.
+//   kProduct  grad_x: G times W over the vocabulary, pieces and parts of which are added in fp32;
+//             grad_w: G^T times x over the rows.
+// G in 16 bits costs each of its values half a step; products and all sums are fp32.  In fp16 each
+// row of G has a power of two of its own that brings it near the type's largest values, and grad_w's
+// x one that takes it off again.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "fourbit.h"
+#include "fourbit_decode.h"
+
+namespace fb_gpu {
+__attribute__((visibility("hidden"))) int cu_count();
+}  // namespace fb_gpu
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLow = -200.f;  // exp of it is 0, and its product with a sum stays finite
+constexpr int kChunk = 64;      // contraction values staged at a time
+
+enum Mode { kStats, kGradient, kProduct };
+
+struct ProductArgs {
+  const uint8_t* p;  // the side whose index is contiguous in the result
+  const uint8_t* q;
+  int64_t ldp, ldq;  // elements
+  int np, nq, k;
+  int tiles_p, tiles_q;
+  int chunks;        // of a part
+  // kStats
+  float *pm, *pz, *pw;  // [tiles_p * WP, nq]
+  float* given;         // [nq]: the given token's logit
+  const int64_t* token;
+  int v0;  // p's first row is this token
+  // kGradient
+  const float *rowmax, *log2z;  // stats [nq, 2]: the first and the second
+  const float *entropy, *g_logprob, *g_entropy, *scale;
+  uint16_t* g;
+  int64_t ldg;
+  int vocab;
+  // kProduct
+  void* out;       // [nq, np] of 16 bits, or null
+  float* acc;      // [parts, nq, np] otherwise
+  int add;         // to what acc holds
+  const float* out_scale;  // null, or of one value
+  const float* row_scale;  // null, or [nq]
+};
+
+// One operand's tile of T values by kChunk of the contraction in LDS, T / 8 requests of 1 KiB.
+// Rows of the contraction side by side (TR = false): [T][64], a row's eight 16-byte units permuted by
+// its number, so that the 16 lanes that LDS serves at a time read 16 different ones.
+// The contraction along memory's rows (TR): [64][T], 32 bytes of 16 values permuted by the row, read
+// by the transposing LDS reads: 16 lanes read 4 rows of 16 values and get a column of 4 each.
+template <bool TR, int T, int WAVES>
+struct Side {
+  static constexpr int kRequests = (T / 8 + WAVES - 1) / WAVES;
+  static constexpr bool kEven = T / 8 % WAVES == 0;
+  unsigned off[kRequests];  // of this lane's request j
+  int ku;                   // TR = false: the lane's first contraction value (of even requests)
+  unsigned rd;              // where this lane reads
+  __device__ void init(int wave, int lane, int64_t ld) {
+    ku = 0;
+#pragma unroll
+    for (int j = 0; j < kRequests; ++j) {
+      const int i = wave * kRequests + j;
+      if constexpr (TR) {
+        constexpr int PER = T / 8;  // lanes of a row
+        const int k = i * (64 / PER) + lane / PER;
+        const int f = (k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2);
+        const int w = ((lane % PER) >> 1) ^ f;
+        off[j] = (unsigned)(k * ld + w * 16 + (lane & 1) * 8) * 2u;
+      } else {
+        const int row = i * 8 + (lane >> 3);
+        const int u = (lane & 7) ^ ((row >> 1) & 7);
+        off[j] = (unsigned)(row * ld + u * 8) * 2u;
+        if (j == 0) ku = u * 8;
+      }
+    }
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (TR) {
+      const int f = (r >> 2) | (((g ^ (g >> 1)) & 1) << 2);
+      rd = (8 * g + (r >> 2)) * (2 * T) + f * 32 + (r & 3) * 8;
+    } else {
+      rd = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+    }
+  }
+  // Requests chunk c of the tile at t0.
+  __device__ void stage(const uint8_t* base, int64_t ld, int n, int k, int t0, int c, int wave,
+                        uint8_t* buf) const {
+    const int rows = min(T, n - t0), left = k - c * kChunk;
+    rsrc_t rs;  // up to the last whole unit of 8 values
+    if constexpr (TR)
+      rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(base) + ((int64_t)c * kChunk * ld + t0) * 2, (short)0,
+          (int)(((min(left, kChunk) - 1) * ld + ((rows + 7) & ~7)) * 2), kRsrcWord3);
+    else
+      rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base) + (int64_t)t0 * ld * 2,
+                                             (short)0, (int)(((rows - 1) * ld + ((k + 7) & ~7)) * 2),
+                                             kRsrcWord3);
+#pragma unroll
+    for (int j = 0; j < kRequests; ++j) {
+      const int i = wave * kRequests + j;
+      if (!kEven && i >= T / 8) break;
+      unsigned o = off[j];
+      if constexpr (!TR) {
+        // requests of a wave differ by 8 rows, which changes the unit by 4
+        const int kv = j & 1 ? ku ^ 32 : ku;
+        o = kv < left ? o + (unsigned)c * (kChunk * 2) : kXOutOfRange;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_byte*)(buf + i * 1024), 16, o, 0, 0, 0);
+    }
+  }
+  // The matrix operand of 16 values (tile i) and contraction values 32 s .. 32 s + 31.
+  __device__ u32x4 read(const uint8_t* buf, int i, int s) const {
+    if constexpr (TR) {
+      typedef __attribute__((address_space(3))) s16x4* lds4;
+      const uint8_t* at = buf + (rd ^ (i * 32)) + s * 32 * 2 * T;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * 2 * T));
+      const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+      return u32x4{a.x, a.y, b.x, b.y};
+    } else {
+      return *reinterpret_cast<const u32x4*>(buf + (rd ^ (s * 64)) + i * 2048);
+    }
+  }
+};
+
+// Workgroup barrier once this wave has received all that it asked for.  Builtins, because the compiler
+// counts them: after waits it cannot see it has every LDS read wait for the requests before it.
+__device__ inline void arrive() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int DT>
+__device__ inline unsigned pack2(float a, float b) {
+  if constexpr (DT == FB_DT_F16)
+    return __builtin_bit_cast(unsigned short, (_Float16)a) |
+           (unsigned)__builtin_bit_cast(unsigned short, (_Float16)b) << 16;
+  else
+    return __builtin_bit_cast(unsigned short, (__bf16)a) |
+           (unsigned)__builtin_bit_cast(unsigned short, (__bf16)b) << 16;
+}
+
+// A tile of TP x TQ of p q^T, WP x WQ waves.
+template <int DT, bool PT, bool QT, int TP, int TQ, int WP, int WQ, int MODE>
+__global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) {
+  constexpr int WAVES = WP * WQ;
+  constexpr int RP = TP / WP / 16, RQ = TQ / WQ / 16;
+  __shared__ __align__(1024) uint8_t p0[TP * 128], p1[TP * 128], q0[TQ * 128], q1[TQ * 128];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wp = wave % WP, wq = wave / WP;
+
+  // Workgroups go round-robin over the 8 XCDs: each takes a contiguous run of tiles, 4 of q by many
+  // of p at a time, which share operands in its L2.
+  int id = blockIdx.x;
+  {
+    const int n = gridDim.x >> 3, r = gridDim.x & 7, xcd = id & 7, i = id >> 3;
+    id = (xcd < r ? xcd * (n + 1) : r * (n + 1) + (xcd - r) * n) + i;
+  }
+  const int per = a.tiles_p * a.tiles_q, part = id / per;
+  id -= part * per;
+  const int group = id / (4 * a.tiles_p), gq = min(4, a.tiles_q - group * 4);
+  const int in = id - group * 4 * a.tiles_p;
+  const int tp = in / gq, tq = group * 4 + in % gq;
+  const int tp0 = tp * TP, tq0 = tq * TQ;
+  const int c0 = part * a.chunks;
+  const int n = min(a.chunks, (a.k + kChunk - 1) / kChunk - c0);
+
+  Side<PT, TP, WAVES> sp;
+  Side<QT, TQ, WAVES> sq;
+  sp.init(wave, lane, a.ldp);
+  sq.init(wave, lane, a.ldq);
+  const auto request = [&](int c, uint8_t* pb, uint8_t* qb) {
+    sp.stage(a.p, a.ldp, a.np, a.k, tp0, c0 + c, wave, pb);
+    sq.stage(a.q, a.ldq, a.nq, a.k, tq0, c0 + c, wave, qb);
+  };
+  f32x4 acc[RP][RQ];
+#pragma unroll
+  for (int i = 0; i < RP; ++i)
+#pragma unroll
+    for (int j = 0; j < RQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 pa[2][RP], qa[2][RQ];
+  // Item i of what a half chunk reads: one of p first, then q, then the rest of p.
+  const auto read = [&](const uint8_t* pb, const uint8_t* qb, int s, int to, int i) {
+    if (i >= 1 && i <= RQ)
+      qa[to][i - 1] = sq.read(qb, wq * RQ + i - 1, s);
+    else
+      pa[to][i ? i - RQ : 0] = sp.read(pb, wp * RP + (i ? i - RQ : 0), s);
+  };
+  // The products of a half chunk, with the next one's operands read between them.
+  const auto half = [&](const uint8_t* pb, const uint8_t* qb, int s, int from) {
+    constexpr int G = RP > 2 ? RP - 2 : 1, I = RP + RQ;
+#pragma unroll
+    for (int i = 0; i < RP; ++i) {
+#pragma unroll
+      for (int t = i * I / G; t < (i + 1) * I / G && t < I; ++t) read(pb, qb, s, from ^ 1, t);
+#pragma unroll
+      for (int j = 0; j < RQ; ++j) acc[i][j] = mfma<DT>(pa[from][i], qa[from][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const auto step = [&](int c, uint8_t* pb, uint8_t* qb, const uint8_t* pn, const uint8_t* qn) {
+    half(pb, qb, 1, 0);
+    // the next chunk is there, and no wave reads this one any more
+    arrive();
+    if (c + 2 < n) request(c + 2, pb, qb);
+    half(pn, qn, 0, 1);
+  };
+  if (n > 0) {
+    request(0, p0, q0);
+    arrive();
+    if (n > 1) request(1, p1, q1);
+#pragma unroll
+    for (int i = 0; i < RP + RQ; ++i) read(p0, q0, 0, 0, i);
+    for (int c = 0; c < n; c += 2) {
+      step(c, p0, q0, p1, q1);
+      if (c + 1 < n) step(c + 1, p1, q1, p0, q0);
+    }
+  }
+
+  // lane: q's row lane % 16 of tile j, p's rows 4 (lane / 16) .. + 3 of tile i
+  const int pl = tp0 + wp * (TP / WP) + (lane >> 4) * 4;
+  const int ql = tq0 + wq * (TQ / WQ) + (lane & 15);
+  if constexpr (MODE == kStats) {
+    const bool whole = tp0 + TP <= a.np;
+#pragma unroll
+    for (int j = 0; j < RQ; ++j) {
+      const int r = ql + j * 16;
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < RP; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!whole && pl + i * 16 + e >= a.np) acc[i][j][e] = -__builtin_inff();
+          m = fmaxf(m, acc[i][j][e]);
+        }
+      }
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const float to = m == -__builtin_inff() ? 0.f : m;
+      float z = 0.f, w = 0.f;
+#pragma unroll
+      for (int i = 0; i < RP; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d = acc[i][j][e] - to, x = __builtin_amdgcn_exp2f(d * kLog2e);
+          z += x;
+          w = __builtin_fmaf(x, fmaxf(d, kLow), w);
+        }
+      z += __shfl_xor(z, 16);
+      w += __shfl_xor(w, 16);
+      z += __shfl_xor(z, 32);
+      w += __shfl_xor(w, 32);
+      if (r < a.nq) {
+        const int64_t t = a.token[r] - a.v0 - pl;  // from this lane's first token on
+        if (t >= 0 && t < TP && (t & 15) < 4) {
+#pragma unroll
+          for (int i = 0; i < RP; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t == i * 16 + e && pl + i * 16 + e < a.np) a.given[r] = acc[i][j][e];
+        }
+        if (lane < 16) {
+          const int64_t at = (int64_t)(tp * WP + wp) * a.nq + r;
+          a.pm[at] = m;
+          a.pz[at] = z;
+          a.pw[at] = w;
+        }
+      }
+    }
+  } else if constexpr (MODE == kGradient) {
+#pragma unroll
+    for (int j = 0; j < RQ; ++j) {
+      const int r = ql + j * 16;
+      if (r >= a.nq) continue;
+      const int64_t token = a.token[r];
+      const bool any = token >= 0 && token < a.vocab;
+      const float g = any && a.g_logprob ? a.g_logprob[r] : 0.f;
+      const float ge = a.g_entropy ? a.g_entropy[r] : 0.f;
+      const float m = a.rowmax[2 * r], l2z = a.log2z[2 * r], up = a.scale[r];
+      const float all = -up * (g + (a.g_entropy ? ge * a.entropy[r] : 0.f));
+      const float slope = -up * ge * kLn2;
+      const int t = any ? (int)(token - a.v0) - pl : -1;
+      uint16_t* const row = a.g + (int64_t)r * a.ldg + pl;
+#pragma unroll
+      for (int i = 0; i < RP; ++i) {
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = __builtin_fmaf(acc[i][j][e] - m, kLog2e, -l2z);
+          float v = __builtin_amdgcn_exp2f(y) * __builtin_fmaf(slope, fmaxf(y, kLow), all);
+          if (t == i * 16 + e) v = __builtin_fmaf(up, g, v);
+          o[e] = up == 0.f || pl + i * 16 + e >= a.np ? 0.f : v;
+        }
+        if (pl + i * 16 < a.ldg)
+          *reinterpret_cast<uint2*>(row + i * 16) =
+              make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+      }
+    }
+  } else {
+    const float all = a.out_scale ? a.out_scale[0] : 1.f;
+    const bool vec = (a.np & 3) == 0;
+#pragma unroll
+    for (int j = 0; j < RQ; ++j) {
+      const int r = ql + j * 16;
+      if (r >= a.nq) continue;
+      const float up = a.row_scale && !a.acc ? a.row_scale[r] : all;
+#pragma unroll
+      for (int i = 0; i < RP; ++i) {
+        const int at = pl + i * 16;
+        const f32x4 v = acc[i][j];
+        if (a.acc) {
+          float* const dst = a.acc + ((int64_t)part * a.nq + r) * a.np + at;
+          if (vec && at < a.np) {
+            f32x4 s = v;
+            if (a.add) s += *reinterpret_cast<const f32x4*>(dst);
+            *reinterpret_cast<f32x4*>(dst) = s;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (at + e < a.np) dst[e] = a.add ? dst[e] + v[e] : v[e];
+          }
+        } else {
+          uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)r * a.np + at;
+          const unsigned lo = pack2<DT>(v[0] * up, v[1] * up), hi = pack2<DT>(v[2] * up, v[3] * up);
+          if (vec && at < a.np) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+          } else {
+            if (at < a.np) dst[0] = (uint16_t)lo;
+            if (at + 1 < a.np) dst[1] = (uint16_t)(lo >> 16);
+            if (at + 2 < a.np) dst[2] = (uint16_t)hi;
+            if (at + 3 < a.np) dst[3] = (uint16_t)(hi >> 16);
+          }
+        }
+      }
+    }
+  }
+}
+
+// A row's results from its parts' (m, z, w): 16 rows by 16 threads each.
+__global__ __launch_bounds__(256) void head_join(const float* __restrict__ pm,
+                                                 const float* __restrict__ pz,
+                                                 const float* __restrict__ pw, int parts, int rows,
+                                                 const float* __restrict__ given,
+                                                 const int64_t* __restrict__ token, int vocab,
+                                                 float* __restrict__ logprob,
+                                                 float* __restrict__ entropy,
+                                                 float* __restrict__ stats) {
+  __shared__ float red[3][16][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, r = blockIdx.x * 16 + x;
+  float m = -__builtin_inff(), z = 0.f, w = 0.f;
+  const auto add = [&](float m2, float z2, float w2) {
+    if (z2 == 0.f) return;
+    const float to = fmaxf(m, m2), d1 = m - to, d2 = m2 - to;
+    const float f1 = z == 0.f ? 0.f : __builtin_amdgcn_exp2f(d1 * kLog2e);
+    const float f2 = __builtin_amdgcn_exp2f(d2 * kLog2e);
+    w = f1 * __builtin_fmaf(fmaxf(d1, kLow), z, w) + f2 * __builtin_fmaf(fmaxf(d2, kLow), z2, w2);
+    z = f1 * z + f2 * z2;
+    m = to;
+  };
+  if (r < rows)
+#pragma unroll 4
+    for (int p = y; p < parts; p += 16) {
+      const int64_t at = (int64_t)p * rows + r;
+      add(pm[at], pz[at], pw[at]);
+    }
+  red[0][y][x] = m;
+  red[1][y][x] = z;
+  red[2][y][x] = w;
+  __syncthreads();
+  if (y || r >= rows) return;
+  for (int i = 1; i < 16; ++i) add(red[0][i][x], red[1][i][x], red[2][i][x]);
+  const int64_t t = token[r];
+  const bool none = z == 0.f;
+  const float l2z = __builtin_log2f(z);
+  const bool any = t >= 0 && t < vocab;
+  logprob[r] = !any ? 0.f : none ? -__builtin_inff() : given[r] - m - kLn2 * l2z;
+  entropy[r] = none ? 0.f : __builtin_fmaf(kLn2, l2z, -w / z);
+  if (stats) {
+    stats[2 * r] = none ? 0.f : m;
+    stats[2 * r + 1] = none ? __builtin_inff() : l2z;
+  }
+}
+
+// What bounds |G| in row r: 0 where no gradient comes in.
+__device__ inline float row_bound(int64_t r, const int64_t* token, int vocab, const float* g,
+                                  const float* ge) {
+  const int64_t t = token[r];
+  float b = g && t >= 0 && t < vocab ? __builtin_fabsf(g[r]) : 0.f;
+  if (ge) b += 24.f * __builtin_fabsf(ge[r]);  // 1 + log of the largest vocabulary
+  return b;
+}
+// The least exponent with bound <= 2^e.
+__device__ inline int bound_exp(float b) {
+  const int e = (int)(__builtin_bit_cast(unsigned, b) >> 23) - 126;
+  return e < -100 ? -100 : e > 127 ? 127 : e;
+}
+constexpr int kF16Exp = 14;
+
+// fp16: *top = the largest row's exponent.
+__global__ __launch_bounds__(1024) void head_top(const int64_t* __restrict__ token, int vocab,
+                                                 const float* __restrict__ g,
+                                                 const float* __restrict__ ge, int rows,
+                                                 float* __restrict__ top) {
+  __shared__ int red[1024];
+  int e = -100;
+  for (int r = threadIdx.x; r < rows; r += 1024) e = max(e, bound_exp(row_bound(r, token, vocab, g, ge)));
+  red[threadIdx.x] = e;
+  __syncthreads();
+  for (int s = 512; s; s >>= 1) {
+    if ((int)threadIdx.x < s) red[threadIdx.x] = max(red[threadIdx.x], red[threadIdx.x + s]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) top[0] = __builtin_ldexpf(1.f, red[0] - kF16Exp);
+}
+
+// A row's power of two and x as grad_w takes it: times what brings the row's G back to the scale of
+// the largest row's, 0 where the row has no gradient (whatever x holds there).
+template <int DT>
+__global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, int64_t ldx, int K8,
+                                                 const int64_t* __restrict__ token, int vocab,
+                                                 const float* __restrict__ g,
+                                                 const float* __restrict__ ge,
+                                                 const float* __restrict__ top,
+                                                 float* __restrict__ scale, float* __restrict__ undo,
+                                                 uint8_t* __restrict__ xs) {
+  const int64_t r = blockIdx.x;
+  const float b = row_bound(r, token, vocab, g, ge);
+  float up = b == 0.f ? 0.f : 1.f, down = up;
+  if constexpr (DT == FB_DT_F16) {
+    if (b != 0.f) {
+      const int e = kF16Exp - bound_exp(b);
+      up = __builtin_ldexpf(1.f, e);
+      down = __builtin_ldexpf(1.f, -e);
+    }
+  }
+  if (threadIdx.x == 0) {
+    scale[r] = up;
+    undo[r] = down;
+  }
+  if (!xs) return;
+  const float f = DT == FB_DT_F16 && b != 0.f ? down / top[0] : up;
+  const u32x4* const src = reinterpret_cast<const u32x4*>(x + r * ldx * 2);
+  u32x4* const dst = reinterpret_cast<u32x4*>(xs + r * K8 * 16);
+  for (int i = threadIdx.x; i < K8; i += 256) {
+    u32x4 v = b == 0.f ? u32x4{0, 0, 0, 0} : src[i];
+    if constexpr (DT == FB_DT_F16) {
+      if (f != 1.f) {
+        half8_t h = __builtin_bit_cast(half8_t, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = (_Float16)((float)h[e] * f);
+        v = __builtin_bit_cast(u32x4, h);
+      }
+    }
+    dst[i] = v;
+  }
+}
+
+// out = the parts' sums added in their order, times the row's power of two, rounded once.
+template <int DT>
+__global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, int parts, int rows,
+                                                int K, const float* __restrict__ undo,
+                                                uint16_t* __restrict__ out) {
+  const int64_t n = (int64_t)rows * K, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  if ((K & 3) == 0) {
+    f32x4 s = *reinterpret_cast<const f32x4*>(acc + i);
+    for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(acc + p * n + i);
+    s *= undo[i / K];
+    *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]));
+  } else {
+    for (int64_t at = i; at < n && at < i + 4; ++at) {
+      float s = acc[at];
+      for (int p = 1; p < parts; ++p) s += acc[p * n + at];
+      out[at] = (uint16_t)pack2<DT>(s * undo[at / K], 0.f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------
+constexpr int64_t kMostG = 1ll << 30;       // bytes of G at once
+constexpr int64_t kMostRows = 1 << 24;
+constexpr int64_t kStatRows = 1 << 14;      // rows of logits whose parts are held at once
+
+struct Shape {
+  int tp, tq, wp;
+  int slots;  // workgroups of a CU
+};
+constexpr Shape kShapes[] = {{256, 256, 2, 1}, {128, 128, 2, 2}, {128, 64, 4, 2}, {128, 16, 4, 4}};
+
+int pick_shape(int64_t np, int64_t nq, int cus) {
+  if (nq <= 16) return 3;
+  if (nq <= 64) return 2;
+  const int64_t big = ((np + 255) / 256) * ((nq + 255) / 256);
+  return nq <= 128 || big * 4 < cus * 3 ? 1 : 0;
+}
+
+template <int DT, bool PT, bool QT, int MODE>
+int launch_product(ProductArgs a, int shape, int parts, hipStream_t hs) {
+  const Shape s = kShapes[shape];
+  a.tiles_p = (a.np + s.tp - 1) / s.tp;
+  a.tiles_q = (a.nq + s.tq - 1) / s.tq;
+  a.chunks = ((a.k + kChunk - 1) / kChunk + parts - 1) / parts;
+  const int64_t grid = (int64_t)a.tiles_p * a.tiles_q * parts;
+  if (grid > (1 << 22)) return FB_ERR_SHAPE;
+  const auto go = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), 0, hs, a);
+    return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+  };
+  if (shape == 0) return go(product_kernel<DT, PT, QT, 256, 256, 2, 4, MODE>, 512);
+  if (shape == 1) return go(product_kernel<DT, PT, QT, 128, 128, 2, 2, MODE>, 256);
+  if constexpr (!QT) {
+    if (shape == 2) return go(product_kernel<DT, PT, QT, 128, 64, 4, 1, MODE>, 256);
+    return go(product_kernel<DT, PT, QT, 128, 16, 4, 1, MODE>, 256);
+  }
+  return FB_ERR_SHAPE;
+}
+
+size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+struct StatPlan {
+  int64_t rows;  // at once
+  int shape, parts;
+  size_t part_bytes, bytes;
+};
+StatPlan stat_plan(int64_t rows, int vocab, int cus) {
+  StatPlan p{};
+  p.rows = std::min(rows, kStatRows);
+  p.shape = pick_shape(vocab, p.rows, cus);
+  const Shape s = kShapes[p.shape];
+  p.parts = (vocab + s.tp - 1) / s.tp * s.wp;
+  p.part_bytes = up256((size_t)p.parts * p.rows * 4);
+  p.bytes = 3 * p.part_bytes + up256(p.rows * 4);
+  return p;
+}
+
+struct GradPlan {
+  int64_t piece;  // tokens of the vocabulary at once
+  int gshape, xshape, wshape, parts;
+  bool acc;
+  size_t at_scale, at_undo, at_top, at_x, at_g, at_acc, bytes;
+};
+GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
+  GradPlan p{};
+  const int64_t v256 = ((int64_t)vocab + 255) / 256 * 256;
+  p.piece = std::min(v256, std::max<int64_t>(256, kMostG / (rows * 2) / 256 * 256));
+  p.gshape = pick_shape(std::min<int64_t>(p.piece, vocab), rows, cus);
+  p.xshape = pick_shape(K, rows, cus);
+  p.wshape = (int64_t)((K + 255) / 256) * ((p.piece + 255) / 256) * 4 < cus * 3 ? 1 : 0;
+  p.parts = 1;
+  if (gx) {
+    const int64_t chunks = p.piece / kChunk;
+    double best = 0;
+    for (int sh = p.xshape; sh <= std::max(1, p.xshape); ++sh) {
+      const Shape s = kShapes[sh];
+      const int64_t tiles = (K + s.tp - 1) / s.tp * ((rows + s.tq - 1) / s.tq);
+      const int64_t slots = (int64_t)cus * s.slots;
+      for (int n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, chunks); ++n) {
+        if (n > 1 && (int64_t)n * rows * K * 4 > kMostG) break;
+        // chunks in a row, each costing its tile's products; parts their sums' traffic
+        const double t = (double)((tiles * n + slots - 1) / slots) * ((chunks + n - 1) / n) *
+                             (s.tp * s.tq * s.slots / 65536.0 + 0.05) +
+                         (n > 1 ? n * (double)rows * K * 8 / 4e6 : 0.0);
+        if (best == 0 || t < best) {
+          best = t;
+          p.parts = n;
+          p.xshape = sh;
+        }
+      }
+    }
+  }
+  const int64_t per = (p.piece / kChunk + p.parts - 1) / p.parts;
+  p.parts = (int)((p.piece / kChunk + per - 1) / per);
+  p.acc = gx && (p.parts > 1 || p.piece < v256);
+  size_t at = 0;
+  const auto take = [&](size_t n) {
+    const size_t was = at;
+    at += up256(n);
+    return was;
+  };
+  p.at_scale = take(rows * 4);
+  p.at_undo = take(rows * 4);
+  p.at_top = take(4);
+  p.at_x = take(gw ? (size_t)rows * ((K + 7) / 8) * 16 : 0);
+  p.at_g = take((size_t)rows * p.piece * 2);
+  p.at_acc = take(p.acc ? (size_t)p.parts * rows * K * 4 : 0);
+  p.bytes = at;
+  return p;
+}
+
+bool bad_align(std::initializer_list<const void*> ps, unsigned mask) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) & mask) return true;
+  return false;
+}
+
+int head_check(int32_t dtype, int64_t rows, int32_t K, int32_t vocab, int64_t ldx, int64_t ldw) {
+  if (dtype != FB_DT_F16 && dtype != FB_DT_BF16) return FB_ERR_DTYPE;
+  const int64_t k8 = ((int64_t)K + 7) / 8 * 8;
+  if (rows < 0 || rows > kMostRows || K < 1 || K > (1 << 20) || vocab < 1 || vocab > (1 << 24) ||
+      ldx < k8 || ldw < k8 || ldx > (1 << 20) || ldw > (1 << 20))
+    return FB_ERR_SHAPE;
+  if ((ldx | ldw) & 7) return FB_ERR_ALIGN;
+  return FB_OK;
+}
+
+template <int DT>
+int run_stats(ProductArgs a, const StatPlan& p, int64_t rows, int32_t vocab, float* logprob,
+              float* entropy, float* stats, uint8_t* ws, hipStream_t hs) {
+  for (int64_t r = 0; r < rows; r += p.rows) {
+    ProductArgs b = a;
+    b.q = a.q + r * a.ldq * 2;
+    b.nq = (int)std::min(rows - r, p.rows);
+    b.token = a.token + r;
+    b.pm = reinterpret_cast<float*>(ws);
+    b.pz = reinterpret_cast<float*>(ws + p.part_bytes);
+    b.pw = reinterpret_cast<float*>(ws + 2 * p.part_bytes);
+    b.given = reinterpret_cast<float*>(ws + 3 * p.part_bytes);
+    const int st = launch_product<DT, false, false, kStats>(b, p.shape, 1, hs);
+    if (st != FB_OK) return st;
+    hipLaunchKernelGGL(head_join, dim3((b.nq + 15) / 16), dim3(256), 0, hs, b.pm, b.pz, b.pw, p.parts,
+                       b.nq, b.given, b.token, vocab, logprob + r, entropy + r,
+                       stats ? stats + 2 * r : nullptr);
+    if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+  }
+  return FB_OK;
+}
+
+template <int DT>
+int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, int32_t vocab,
+             void* grad_x, void* grad_w, uint8_t* ws, hipStream_t hs) {
+  float* const scale = reinterpret_cast<float*>(ws + p.at_scale);
+  float* const undo = reinterpret_cast<float*>(ws + p.at_undo);
+  float* const top = reinterpret_cast<float*>(ws + p.at_top);
+  uint8_t* const xs = ws + p.at_x;
+  float* const acc = reinterpret_cast<float*>(ws + p.at_acc);
+  const int K8 = (K + 7) / 8;
+  if (DT == FB_DT_F16)
+    hipLaunchKernelGGL(head_top, dim3(1), dim3(1024), 0, hs, in.token, vocab, in.g_logprob,
+                       in.g_entropy, (int)rows, top);
+  hipLaunchKernelGGL(head_rows<DT>, dim3((unsigned)rows), dim3(256), 0, hs, in.q, in.ldq, K8,
+                     in.token, vocab, in.g_logprob, in.g_entropy, top, scale, undo,
+                     grad_w ? xs : nullptr);
+  if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+  for (int64_t v = 0; v < vocab; v += p.piece) {
+    const int nv = (int)std::min<int64_t>(p.piece, vocab - v);
+    ProductArgs g = in;
+    g.p = in.p + v * in.ldp * 2;
+    g.np = nv;
+    g.nq = (int)rows;
+    g.k = K8 * 8;
+    g.v0 = (int)v;
+    g.scale = scale;
+    g.g = reinterpret_cast<uint16_t*>(ws + p.at_g);
+    g.ldg = ((int64_t)nv + 63) / 64 * 64;
+    g.vocab = vocab;
+    int st = launch_product<DT, false, false, kGradient>(g, p.gshape, 1, hs);
+    if (st != FB_OK) return st;
+    if (grad_x) {
+      ProductArgs b{};
+      b.p = in.p + v * in.ldp * 2;
+      b.ldp = in.ldp;
+      b.np = K;
+      b.q = ws + p.at_g;
+      b.ldq = g.ldg;
+      b.nq = (int)rows;
+      b.k = nv;
+      b.out = grad_x;
+      b.acc = p.acc ? acc : nullptr;
+      b.add = v > 0;
+      b.row_scale = undo;
+      st = launch_product<DT, true, false, kProduct>(b, p.xshape, p.parts, hs);
+      if (st != FB_OK) return st;
+    }
+    if (grad_w) {
+      ProductArgs b{};
+      b.p = xs;
+      b.ldp = K8 * 8;
+      b.np = K;
+      b.q = ws + p.at_g;
+      b.ldq = g.ldg;
+      b.nq = nv;
+      b.k = (int)rows;
+      b.out = static_cast<uint8_t*>(grad_w) + v * K * 2;
+      b.out_scale = DT == FB_DT_F16 ? top : nullptr;
+      st = launch_product<DT, true, true, kProduct>(b, p.wshape, 1, hs);
+      if (st != FB_OK) return st;
+    }
+  }
+  if (p.acc) {
+    const int64_t n = ((int64_t)rows * K + 1023) / 1024;
+    if (n > (1 << 23)) return FB_ERR_SHAPE;
+    hipLaunchKernelGGL(head_sum<DT>, dim3((unsigned)n), dim3(256), 0, hs, acc, p.parts, (int)rows, K,
+                       undo, static_cast<uint16_t*>(grad_x));
+    if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+  }
+  return FB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fb_head_logprobs_workspace_bytes(int64_t rows, int32_t K, int32_t vocab) {
+  if (rows < 1 || rows > kMostRows || K < 1 || vocab < 1) return 0;
+  return stat_plan(rows, vocab, fb_gpu::cu_count()).bytes;
+}
+
+int fb_head_logprobs(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int32_t dtype,
+                     int64_t rows, int32_t K, int32_t vocab, const int64_t* token, float* logprob,
+                     float* entropy, float* stats, void* ws, size_t ws_bytes, void* stream) {
+  const int st = head_check(dtype, rows, K, vocab, x_stride, w_stride);
+  if (st != FB_OK) return st;
+  if (rows == 0) return FB_OK;
+  if (!x || !w || !token || !logprob || !entropy || !ws) return FB_ERR_NULL;
+  if (bad_align({x, w}, 15) || bad_align({token}, 7) || bad_align({logprob, entropy, stats}, 3) ||
+      bad_align({ws}, 255))
+    return FB_ERR_ALIGN;
+  const StatPlan p = stat_plan(rows, vocab, fb_gpu::cu_count());
+  if (ws_bytes < p.bytes) return FB_ERR_WORKSPACE;
+  ProductArgs a{};
+  a.p = static_cast<const uint8_t*>(w);
+  a.ldp = w_stride;
+  a.np = vocab;
+  a.q = static_cast<const uint8_t*>(x);
+  a.ldq = x_stride;
+  a.k = (K + 7) / 8 * 8;
+  a.token = token;
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  return dtype == FB_DT_F16 ? run_stats<FB_DT_F16>(a, p, rows, vocab, logprob, entropy, stats,
+                                                   static_cast<uint8_t*>(ws), hs)
+                            : run_stats<FB_DT_BF16>(a, p, rows, vocab, logprob, entropy, stats,
+                                                    static_cast<uint8_t*>(ws), hs);
+}
+
+size_t fb_head_logprobs_grad_workspace_bytes(int64_t rows, int32_t K, int32_t vocab,
+                                             int32_t want_x, int32_t want_w) {
+  if (rows < 1 || rows > kMostRows || K < 1 || vocab < 1) return 0;
+  return grad_plan(rows, K, vocab, want_x, want_w, fb_gpu::cu_count()).bytes;
+}
+
+int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
+                          int32_t dtype, int64_t rows, int32_t K, int32_t vocab,
+                          const int64_t* token, const float* stats, const float* entropy,
+                          const float* g_logprob, const float* g_entropy, void* grad_x, void* grad_w,
+                          void* ws, size_t ws_bytes, void* stream) {
+  const int st = head_check(dtype, rows, K, vocab, x_stride, w_stride);
+  if (st != FB_OK) return st;
+  if (rows == 0 || (!grad_x && !grad_w)) return FB_OK;
+  if (!x || !w || !token || !stats || (g_entropy && !entropy) || !ws) return FB_ERR_NULL;
+  if (bad_align({x, w}, 15) || bad_align({token}, 7) || bad_align({grad_x, grad_w}, 7) ||
+      bad_align({stats, entropy, g_logprob, g_entropy}, 3) || bad_align({ws}, 255))
+    return FB_ERR_ALIGN;
+  const GradPlan p = grad_plan(rows, K, vocab, grad_x, grad_w, fb_gpu::cu_count());
+  if (ws_bytes < p.bytes) return FB_ERR_WORKSPACE;
+  ProductArgs a{};
+  a.p = static_cast<const uint8_t*>(w);
+  a.ldp = w_stride;
+  a.q = static_cast<const uint8_t*>(x);
+  a.ldq = x_stride;
+  a.token = token;
+  a.rowmax = stats;
+  a.log2z = stats + 1;
+  a.entropy = entropy;
+  a.g_logprob = g_logprob;
+  a.g_entropy = g_entropy;
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  return dtype == FB_DT_F16
+             ? run_grad<FB_DT_F16>(a, p, rows, K, vocab, grad_x, grad_w, static_cast<uint8_t*>(ws), hs)
+             : run_grad<FB_DT_BF16>(a, p, rows, K, vocab, grad_x, grad_w, static_cast<uint8_t*>(ws), hs);
+}
+
+}  // extern "C"

@@ -567,6 +567,514 @@ std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tenso
   return r;
 }
 
+// ---------------------------------------------------------------------------------
+// Embedding, the seam between blocks, and log probabilities under a head: what embedding.py,
+// residual.py and logprobs.py call.
+// ---------------------------------------------------------------------------------
+void first_derivative(const char* what) {
+  if (at::GradMode::is_enabled()) throw std::runtime_error(what);
+}
+
+// x as [rows, width], the values of a row side by side and rows a whole stride apart: a view where
+// that can be, else a copy.
+at::Tensor as_rows(const at::Tensor& x) {
+  at::Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  if ((r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < 0)) r = r.contiguous();
+  return r;
+}
+int64_t row_stride(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// tokens as contiguous int64 [rows].
+at::Tensor flat_tokens(const at::Tensor& tokens) {
+  return tokens.reshape({-1}).to(at::kLong).contiguous();
+}
+void want_tokens(const at::Tensor& tokens, const at::Tensor& like) {
+  want_plain(tokens, like, "tokens must be a tensor on the weight's GPU");
+  want(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt,
+       "tokens must be int64 or int32");
+}
+
+at::Tensor embedding_forward(const at::Tensor& w, const at::Tensor& token, double scale) {
+  c10::DeviceGuard guard(w.device());
+  at::Tensor out = at::empty({token.size(0), w.size(1)}, w.options());
+  check(fb_embed(w.data_ptr(), row_stride(w), dtype_code(w.scalar_type()), (int32_t)w.size(0),
+                 (int32_t)w.size(1), static_cast<const int64_t*>(token.data_ptr()), token.size(0),
+                 (float)scale, out.data_ptr(), stream_of(w)));
+  return out;
+}
+
+struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& w,
+                            const at::Tensor& token, double scale) {
+    ctx->save_for_backward({token});
+    ctx->saved_data["vocab"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    return embedding_forward(w, token, scale);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    first_derivative("token_embedding has no second derivative");
+    const at::Tensor token = ctx->get_saved_variables()[0];
+    const at::Tensor g = as_rows(grads[0]);
+    const int64_t V = ctx->saved_data["vocab"].toInt(), K = g.size(1), M = g.size(0);
+    c10::DeviceGuard guard(g.device());
+    at::Tensor gw = at::empty({V, K}, g.options().memory_format(at::MemoryFormat::Contiguous));
+    const size_t need = fb_embed_grad_workspace_bytes(M, (int32_t)V, (int32_t)K);
+    const at::Tensor ws = need ? scratch(need, g) : at::Tensor();
+    check(fb_embed_grad(g.data_ptr(), row_stride(g), dtype_code(g.scalar_type()), (int32_t)V,
+                        (int32_t)K, static_cast<const int64_t*>(token.data_ptr()), M,
+                        (float)ctx->saved_data["scale"].toDouble(), gw.data_ptr(),
+                        ptr_or_null(ws, need), need, stream_of(g)));
+    return {gw, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor token_embedding(const at::Tensor& tokens, const at::Tensor& weight, double scale) {
+  not_recorded();
+  want(weight.defined() && plain(weight), "weight must be a tensor on a ROCm GPU");
+  want_tokens(tokens, weight);
+  want(dtype_code(weight.scalar_type()) >= 0, "weight must be float16, bfloat16 or float32");
+  want(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(1) >= 1 &&
+           weight.size(0) <= (1 << 30) && weight.size(1) <= (1 << 20),
+       "weight must be [vocab, width], a width of at most 2^20");
+  want(std::isfinite(scale), "scale must be finite");
+  want(tokens.numel() <= (1 << 30), "too many tokens");
+  const at::Tensor t = flat_tokens(tokens), w = as_rows(weight);
+  const at::Tensor out = at::GradMode::is_enabled() && w.requires_grad()
+                             ? TokenEmbedding::apply(w, t, scale)
+                             : embedding_forward(w, t, scale);
+  auto sizes = tokens.sizes().vec();
+  sizes.push_back(weight.size(1));
+  return out.view(sizes);
+}
+
+fb_norm_t norm_of(const at::Tensor& x, const at::Tensor& branch, const at::Tensor& gate,
+                  const at::Tensor& weight, const at::Tensor& branch_weight, int64_t gate_rows,
+                  double scale, double eps) {
+  fb_norm_t n{};
+  n.x = x.data_ptr();
+  n.x_stride = row_stride(x);
+  n.rows = x.size(0);
+  n.width = (int32_t)x.size(1);
+  n.dtype = dtype_code(x.scalar_type());
+  n.weight = weight.data_ptr();
+  n.weight_dtype = dtype_code(weight.scalar_type());
+  if (branch.defined()) {
+    n.branch = branch.data_ptr();
+    n.branch_stride = row_stride(branch);
+  }
+  if (gate.defined()) {
+    n.gate = gate.data_ptr();
+    n.gate_dtype = dtype_code(gate.scalar_type());
+    n.gate_rows = gate_rows;
+  }
+  if (branch_weight.defined()) {
+    n.branch_weight = branch_weight.data_ptr();
+    n.branch_weight_dtype = dtype_code(branch_weight.scalar_type());
+  }
+  n.scale = (float)scale;
+  n.eps = (float)eps;
+  return n;
+}
+
+// stream, normed, stats of x [rows, width].
+std::vector<at::Tensor> norm_forward(const fb_norm_t& n, const at::Tensor& x, const at::Tensor& branch,
+                                     bool stats) {
+  c10::DeviceGuard guard(x.device());
+  const auto like = x.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor h = branch.defined() ? at::empty(x.sizes(), like) : x;
+  at::Tensor y = at::empty(x.sizes(), like);
+  at::Tensor st = stats ? at::empty({x.size(0), 2}, x.options().dtype(at::kFloat)) : at::Tensor();
+  if (x.size(0) == 0) return {h, y, st};
+  check(fb_residual_norm(&n, branch.defined() ? h.data_ptr() : nullptr, y.data_ptr(),
+                         stats ? static_cast<float*>(st.data_ptr()) : nullptr, stream_of(x)));
+  return {h, y, st};
+}
+
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const at::Tensor& x,
+                                                const std::optional<at::Tensor>& given_branch,
+                                                const std::optional<at::Tensor>& given_gate,
+                                                const at::Tensor& weight,
+                                                const std::optional<at::Tensor>& given_branch_weight,
+                                                int64_t gate_rows, double scale, double eps) {
+    const at::Tensor branch = given_branch.value_or(at::Tensor()),
+                     gate = given_gate.value_or(at::Tensor()),
+                     branch_weight = given_branch_weight.value_or(at::Tensor());
+    const fb_norm_t n = norm_of(x, branch, gate, weight, branch_weight, gate_rows, scale, eps);
+    const auto r = norm_forward(n, x, branch, true);
+    ctx->save_for_backward({x, branch, gate, weight, branch_weight, r[2]});
+    ctx->saved_data["gate_rows"] = gate_rows;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    // without a branch the stream is x, as a result, so that its gradient is added here, in fp32
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    first_derivative("residual_norm has no second derivative");
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &branch = s[1], &gate = s[2], &weight = s[3], &bw = s[4];
+    const fb_norm_t n = norm_of(x, branch, gate, weight, bw, ctx->saved_data["gate_rows"].toInt(),
+                                ctx->saved_data["scale"].toDouble(),
+                                ctx->saved_data["eps"].toDouble());
+    c10::DeviceGuard guard(x.device());
+    at::Tensor gh = grads[0], gy = grads[1];
+    if (gy.defined()) gy = gy.contiguous();
+    if (gh.defined()) gh = gh.contiguous();
+    at::Tensor out[5];
+    const at::Tensor* of[5] = {&x, &branch, &gate, &weight, &bw};
+    for (int i = 0, edge = 0; i < 5; ++i)  // autograd counts the inputs that there are
+      if (of[i]->defined() && ctx->needs_input_grad(edge++))
+        out[i] = at::empty(of[i]->sizes(),
+                           of[i]->options().memory_format(at::MemoryFormat::Contiguous));
+    if (x.size(0) == 0)
+      for (at::Tensor& t : out)
+        if (t.defined()) t.zero_();
+    const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const size_t need = fb_residual_norm_grad_workspace_bytes(&n);
+    const at::Tensor ws = need ? scratch(need, x) : at::Tensor();
+    if (x.size(0))
+      check(fb_residual_norm_grad(&n, static_cast<const float*>(s[5].data_ptr()), ptr(gh), ptr(gy),
+                                  ptr(out[0]), ptr(out[1]), ptr(out[3]), ptr(out[4]), ptr(out[2]),
+                                  ptr_or_null(ws, need), need, stream_of(x)));
+    return {out[0], out[1], out[2], out[3], out[4], at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// stream, normed.
+std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::Tensor& weight,
+                                                 const std::optional<at::Tensor>& branch,
+                                                 const std::optional<at::Tensor>& gate, double scale,
+                                                 const std::optional<at::Tensor>& branch_weight,
+                                                 double eps) {
+  not_recorded();
+  want(x.defined() && plain(x), "x must be a tensor on a ROCm GPU");
+  want(dtype_code(x.scalar_type()) >= 0, "x must be float16, bfloat16 or float32");
+  want(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 32768,
+       "x must be [..., width], a width of at most 32768");
+  const int64_t d = x.size(-1);
+  const auto vector = [&](const at::Tensor& t, const char* what) {
+    want_plain(t, x, what);
+    want(t.dim() == 1 && t.size(0) == d &&
+             (t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat),
+         what);
+  };
+  vector(weight, "weight must be [width], of x's dtype or float32");
+  if (branch_weight) vector(*branch_weight, "branch_weight must be [width], of x's dtype or float32");
+  want(branch || (!gate && !branch_weight), "gate and branch_weight need a branch");
+  want(std::isfinite(scale) && std::isfinite(eps) && eps >= 0,
+       "scale must be finite, eps finite and not negative");
+  const int64_t M = x.numel() / d;
+  want(M <= INT32_MAX, "too many rows");
+  at::Tensor b, g;
+  int64_t gate_rows = 1;
+  if (branch) {
+    want_plain(*branch, x, "branch must be a tensor on x's GPU");
+    want(branch->sizes() == x.sizes() && branch->scalar_type() == x.scalar_type(),
+         "branch must have x's shape and dtype");
+    b = as_rows(*branch);
+  }
+  if (gate) {
+    want_plain(*gate, x, "gate must be a tensor on x's GPU");
+    want(gate->scalar_type() == x.scalar_type() || gate->scalar_type() == at::kFloat,
+         "gate must be of x's dtype or float32");
+    const char* what = "gate must be [width], or have x's shape but for leading dimensions of 1 from some "
+                       "one on to the last but one (expand others)";
+    want(gate->dim() >= 1 && gate->dim() <= x.dim() && gate->size(-1) == d, what);
+    g = *gate;
+    while (g.dim() < x.dim()) g = g.unsqueeze(0);
+    // of the leading dimensions the gate has the first k, and one of all others: rows that follow each
+    // other share one of its rows
+    int64_t k = 0, rows = 1;
+    while (k + 1 < x.dim() && g.size(k) == x.size(k)) rows *= x.size(k++);
+    for (int64_t i = k; i + 1 < x.dim(); ++i) want(g.size(i) == 1, what);
+    g = g.reshape({rows, d}).contiguous();
+    gate_rows = std::max<int64_t>(1, rows ? M / rows : 1);
+  }
+  const at::Tensor x2 = as_rows(x), w = weight.contiguous();
+  const at::Tensor bw = branch_weight ? branch_weight->contiguous() : at::Tensor();
+  std::vector<at::Tensor> r;
+  const auto grad = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (grad(x2) || grad(b) || grad(g) || grad(w) || grad(bw))) {
+    const auto maybe = [](const at::Tensor& t) {
+      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
+    };
+    r = ResidualNorm::apply(x2, maybe(b), maybe(g), w, maybe(bw), gate_rows, scale, eps);
+  } else {
+    r = norm_forward(norm_of(x2, b, g, w, bw, gate_rows, scale, eps), x2, b, false);
+    if (!b.defined()) return {x, r[1].view(x.sizes())};
+  }
+  return {r[0].view_as(x), r[1].view(x.sizes())};
+}
+
+// A 16-bit matrix as the head's products take it: 16-byte aligned, rows a multiple of 8 values apart,
+// with zeros up to the next multiple of 8 values of a row.
+at::Tensor head_side(const at::Tensor& t) {
+  const int64_t K = t.size(1);
+  if (K % 8 == 0 && row_stride(t) % 8 == 0 && row_stride(t) >= K && row_stride(t) <= (1 << 20) &&
+      !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u))
+    return t;
+  const int64_t ld = (K + 127) / 128 * 128;
+  const at::Tensor c = t.contiguous();
+  at::Tensor out = at::empty({t.size(0), ld}, c.options());
+  const int dt = dtype_code(t.scalar_type());
+  check(fb_cast_rows(c.data_ptr(), dt, (int32_t)t.size(0), (int32_t)K, out.data_ptr(), dt, (int32_t)ld,
+                     stream_of(t)));
+  return out;
+}
+
+// logprob, entropy, stats.
+std::vector<at::Tensor> head_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& token) {
+  c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
+  const auto f = x.options().dtype(at::kFloat);
+  at::Tensor lp = at::empty({M}, f), ent = at::empty({M}, f), st = at::empty({M, 2}, f);
+  if (M == 0) return {lp, ent, st};
+  const at::Tensor xs = head_side(x), ws_ = head_side(w);
+  const size_t need = fb_head_logprobs_workspace_bytes(M, (int32_t)K, (int32_t)V);
+  const at::Tensor ws = scratch(need, x);
+  check(fb_head_logprobs(xs.data_ptr(), row_stride(xs), ws_.data_ptr(), row_stride(ws_),
+                         dtype_code(x.scalar_type()), M, (int32_t)K, (int32_t)V,
+                         static_cast<const int64_t*>(token.data_ptr()),
+                         static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()),
+                         static_cast<float*>(st.data_ptr()), ws.data_ptr(), need, stream_of(x)));
+  return {lp, ent, st};
+}
+
+const float* f32_of(const at::Tensor& t) {
+  return t.defined() ? static_cast<const float*>(t.data_ptr()) : nullptr;
+}
+
+struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const at::Tensor& x, const at::Tensor& w,
+                                                const at::Tensor& token) {
+    const auto r = head_forward(x, w, token);
+    ctx->save_for_backward({x, w, token, r[1], r[2]});
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    first_derivative("head_logprobs has no second derivative");
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &w = s[1], &token = s[2], &ent = s[3], &st = s[4];
+    c10::DeviceGuard guard(x.device());
+    at::Tensor g[2];
+    for (int i = 0; i < 2; ++i)
+      if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
+    const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
+    at::Tensor gx, gw;
+    if (ctx->needs_input_grad(0))
+      gx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+    if (ctx->needs_input_grad(1)) {
+      gw = at::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
+      if (M == 0) gw.zero_();
+    }
+    if (M) {
+      const at::Tensor xs = head_side(x), ws_ = head_side(w);
+      const size_t need = fb_head_logprobs_grad_workspace_bytes(M, (int32_t)K, (int32_t)V,
+                                                                gx.defined(), gw.defined());
+      const at::Tensor ws = scratch(need, x);
+      check(fb_head_logprobs_grad(
+          xs.data_ptr(), row_stride(xs), ws_.data_ptr(), row_stride(ws_), dtype_code(x.scalar_type()),
+          M, (int32_t)K, (int32_t)V, static_cast<const int64_t*>(token.data_ptr()), f32_of(st),
+          f32_of(ent), f32_of(g[0]), f32_of(g[1]), gx.defined() ? gx.data_ptr() : nullptr,
+          gw.defined() ? gw.data_ptr() : nullptr, ws.data_ptr(), need, stream_of(x)));
+    }
+    return {gx, gw, at::Tensor()};
+  }
+};
+
+// A packed head: its logits are fb_gemv's or fb_gemm's, in fp32, for as many rows at once as they take
+// half a GiB.
+constexpr int64_t kMostLogits = 1 << 27;
+
+struct Packed {
+  at::Tensor wdev;
+  int64_t N, K, fmt, fwht;
+  bool f16_exact;
+};
+
+fb_shape_t packed_shape(const Packed& p, int64_t rows, int xdt, int ydt) {
+  fb_shape_t s{};
+  s.N = (int32_t)p.N;
+  s.K = (int32_t)((p.K + 127) / 128 * 128);
+  s.B = (int32_t)rows;
+  s.group = p.fmt == FB_FMT_E2M1 ? 32 : 128;
+  s.fmt = (int32_t)p.fmt;
+  s.fwht_block = (int32_t)p.fwht;
+  s.x_dtype = xdt;
+  s.y_dtype = ydt;
+  return s;
+}
+
+// x [M, K] as the kernels take it: fp16 for GF4 and rotations, else fp16 or bf16, rows of the packed K.
+at::Tensor packed_rows(const Packed& p, const at::Tensor& x) {
+  const int xdt = dtype_code(x.scalar_type());
+  int kdt = xdt == FB_DT_F32 ? FB_DT_BF16 : xdt;
+  if (p.fmt != FB_FMT_E2M1 || p.fwht) kdt = FB_DT_F16;
+  want(p.fmt != FB_FMT_E2M1 || kdt != FB_DT_F16 || p.f16_exact,
+       "the head's E2M1 scales do not decode exactly to float16: pass bfloat16 hidden states");
+  const int64_t kp = (p.K + 127) / 128 * 128;
+  const at::Tensor c = x.contiguous();
+  if (kdt == xdt && kp == p.K && !(reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u)) return c;
+  at::Tensor out = at::empty({x.size(0), kp}, x.options().dtype(kdt == FB_DT_F16 ? at::kHalf : at::kBFloat16));
+  check(fb_cast_rows(c.data_ptr(), xdt, (int32_t)x.size(0), (int32_t)p.K, out.data_ptr(), kdt, (int32_t)kp,
+                     stream_of(x)));
+  return out;
+}
+
+// fp32 logits of rows r .. r + n - 1 of xk into y [>= n, N].
+void packed_logits(const Packed& p, const at::Tensor& xk, int64_t r, int64_t n, const at::Tensor& y) {
+  fb_shape_t s = packed_shape(p, n, dtype_code(xk.scalar_type()), FB_DT_F32);
+  const void* x = static_cast<const char*>(xk.data_ptr()) + r * xk.size(1) * 2;
+  if (n <= kMaxGemvBatch) {
+    const size_t need = fb_workspace_bytes(&s);
+    const at::Tensor ws = need ? scratch(need, xk) : at::Tensor();
+    check(fb_gemv(p.wdev.data_ptr(), x, y.data_ptr(), &s, ptr_or_null(ws, need), need, stream_of(xk)));
+  } else {
+    const size_t need = fb_gemm_workspace_bytes(&s);
+    const at::Tensor ws = need ? scratch(need, xk) : at::Tensor();
+    check(fb_gemm(p.wdev.data_ptr(), x, y.data_ptr(), &s, nullptr, 0, ptr_or_null(ws, need), need,
+                  stream_of(xk)));
+  }
+}
+
+int64_t packed_piece(const Packed& p, int64_t M) {
+  return std::min(M, std::max<int64_t>(16, std::min<int64_t>(kMostLogits / p.N, kGradRows) / 16 * 16));
+}
+
+std::vector<at::Tensor> packed_forward(const Packed& p, const at::Tensor& x, const at::Tensor& token) {
+  c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0);
+  const auto f = x.options().dtype(at::kFloat);
+  at::Tensor lp = at::empty({M}, f), ent = at::empty({M}, f), st = at::empty({M, 3}, f);
+  if (M == 0) return {lp, ent, st};
+  const at::Tensor xk = packed_rows(p, x);
+  const int64_t step = packed_piece(p, M);
+  const at::Tensor y = at::empty({step, p.N}, f);
+  for (int64_t r = 0; r < M; r += step) {
+    const int64_t n = std::min(step, M - r);
+    packed_logits(p, xk, r, n, y);
+    check(fb_token_logprobs(y.data_ptr(), FB_DT_F32, p.N, n, (int32_t)p.N,
+                            static_cast<const int64_t*>(token.data_ptr()) + r, 0,
+                            static_cast<float*>(lp.data_ptr()) + r,
+                            static_cast<float*>(ent.data_ptr()) + r, nullptr, nullptr,
+                            static_cast<float*>(st.data_ptr()) + 3 * r, stream_of(x)));
+  }
+  return {lp, ent, st};
+}
+
+struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
+                                                const at::Tensor& x, const at::Tensor& wdev,
+                                                const at::Tensor& token, int64_t N, int64_t K,
+                                                int64_t fmt, int64_t fwht, bool f16_exact) {
+    const Packed p{wdev, N, K, fmt, fwht, f16_exact};
+    const auto r = packed_forward(p, x, token);
+    ctx->save_for_backward({x, wdev, token, r[1], r[2]});
+    ctx->saved_data["head"] = std::vector<int64_t>{N, K, fmt, fwht, f16_exact};
+    ctx->set_materialize_grads(false);
+    return {r[0], r[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    first_derivative("head_logprobs has no second derivative");
+    const auto s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &token = s[2], &ent = s[3], &st = s[4];
+    const auto h = ctx->saved_data["head"].toIntVector();
+    const Packed p{s[1], h[0], h[1], h[2], h[3], (bool)h[4]};
+    c10::DeviceGuard guard(x.device());
+    at::Tensor g[2];
+    for (int i = 0; i < 2; ++i)
+      if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
+    const int64_t M = x.size(0), kp = (p.K + 127) / 128 * 128;
+    at::Tensor gx = at::empty({M, kp}, x.options().memory_format(at::MemoryFormat::Contiguous));
+    const int xdt = dtype_code(x.scalar_type());
+    if (M) {
+      const at::Tensor xk = packed_rows(p, x);
+      const int64_t step = packed_piece(p, M);
+      const auto f = x.options().dtype(at::kFloat);
+      const at::Tensor y = at::empty({step, p.N}, f), gl = at::empty({step, p.N}, f);
+      fb_shape_t sh = packed_shape(p, step, FB_DT_F16, FB_DT_F32);
+      const size_t need = fb_grad_x_workspace_bytes(&sh, p.f16_exact);
+      want(need, "a packed head of this many rows has no gradient");
+      const at::Tensor ws = scratch(need, x);
+      for (int64_t r = 0; r < M; r += step) {
+        const int64_t n = std::min(step, M - r);
+        packed_logits(p, xk, r, n, y);
+        check(fb_token_logprobs_grad(
+            y.data_ptr(), FB_DT_F32, p.N, n, (int32_t)p.N,
+            static_cast<const int64_t*>(token.data_ptr()) + r, 0, nullptr, f32_of(st) + 3 * r,
+            f32_of(ent) + r, g[0].defined() ? f32_of(g[0]) + r : nullptr,
+            g[1].defined() ? f32_of(g[1]) + r : nullptr, nullptr, gl.data_ptr(), stream_of(x)));
+        sh.B = (int32_t)n;
+        check(fb_grad_x(p.wdev.data_ptr(), gl.data_ptr(), static_cast<char*>(gx.data_ptr()) + r * kp * gx.element_size(),
+                        &sh, xdt, p.f16_exact, ws.data_ptr(), need, stream_of(x)));
+      }
+    }
+    if (kp != p.K) gx = gx.narrow(1, 0, p.K).contiguous();
+    return {gx, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+// x [..., K] and tokens [...]: x's rows, the tokens, after the checks that both kinds of heads share.
+std::pair<at::Tensor, at::Tensor> head_inputs(const at::Tensor& x, const at::Tensor& tokens, int64_t K,
+                                              const at::Tensor& like) {
+  not_recorded();
+  want(x.defined() && plain(x), "hidden must be a tensor on a ROCm GPU");
+  want(x.device() == like.device(), "all tensors must be on one GPU");
+  want_tokens(tokens, x);
+  want(x.dim() >= 1 && x.size(-1) == K, "hidden must be [..., width] with the head's width");
+  want(tokens.sizes() == x.sizes().slice(0, x.dim() - 1),
+       "tokens must have hidden's shape without the last dimension");
+  want(tokens.numel() <= (1 << 24), "too many tokens");
+  return {as_rows(x), flat_tokens(tokens)};
+}
+
+// logprob, entropy.
+std::tuple<at::Tensor, at::Tensor> head_logprobs(const at::Tensor& hidden, const at::Tensor& weight,
+                                                 const at::Tensor& tokens) {
+  want(weight.defined() && plain(weight), "the head must be a tensor on a ROCm GPU or packed");
+  want(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(0) <= (1 << 24) && weight.size(1) >= 1 &&
+           weight.size(1) <= (1 << 20),
+       "the head's weight must be [vocab, width], a width of at most 2^20, a vocabulary of at most 2^24");
+  const auto [x, t] = head_inputs(hidden, tokens, weight.size(1), weight);
+  want((x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16) &&
+           x.scalar_type() == weight.scalar_type(),
+       "hidden and the head's weight must both be float16 or both bfloat16");
+  const at::Tensor w = as_rows(weight);
+  std::vector<at::Tensor> r;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))
+    r = HeadLogprobs::apply(x, w, t);
+  else
+    r = head_forward(x, w, t);
+  return {r[0].view(tokens.sizes()), r[1].view(tokens.sizes())};
+}
+
+std::tuple<at::Tensor, at::Tensor> packed_head_logprobs(const at::Tensor& hidden, const at::Tensor& wdev,
+                                                        const at::Tensor& tokens, int64_t N, int64_t K,
+                                                        int64_t fmt, int64_t fwht, bool f16_exact) {
+  want(wdev.defined() && plain(wdev), "the packed head must be on a ROCm GPU");
+  const auto [x, t] = head_inputs(hidden, tokens, K, wdev);
+  want(dtype_code(x.scalar_type()) >= 0, "hidden must be float16, bfloat16 or float32");
+  const Packed p{wdev, N, K, fmt, fwht, f16_exact};
+  const fb_shape_t s = packed_shape(p, 1, FB_DT_F16, FB_DT_F32);
+  want(fb_device_bytes(&s) && (size_t)wdev.numel() >= fb_device_bytes(&s) && s.K <= kMaxGemmK,
+       "the packed head is not of its format's size");
+  std::vector<at::Tensor> r;
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    r = PackedHeadLogprobs::apply(x, wdev, t, N, K, fmt, fwht, f16_exact);
+  else
+    r = packed_forward(p, x, t);
+  return {r[0].view(tokens.sizes()), r[1].view(tokens.sizes())};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_fourbit_torch, m) {
@@ -578,4 +1086,8 @@ PYBIND11_MODULE(_fourbit_torch, m) {
   m.def("cache_attention", &cache_attention);
   m.def("cache_evict", &cache_evict);
   m.def("token_logprobs", &token_logprobs);
+  m.def("token_embedding", &token_embedding);
+  m.def("residual_norm", &residual_norm);
+  m.def("head_logprobs", &head_logprobs);
+  m.def("packed_head_logprobs", &packed_head_logprobs);
 }

@@ -556,6 +556,92 @@ int fb_token_logprobs_grad(const void* logits, int32_t dtype, int64_t stride, in
                            const float* g_logprob, const float* g_entropy, const float* g_top,
                            void* grad, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * The two ends of a decoder of packed linear layers and the seams between its blocks.  No
+ * counterpart in the reference.
+ * ------------------------------------------------------------------------------- */
+
+/* Embedding: out[i] = scale * w[token[i]], 0 for a token outside [0, vocab).
+ *   w      [vocab, K] of dtype FB_DT_F16, BF16 or F32, rows w_stride elements apart
+ *   token  int64 [rows];  out [rows, K] of the same dtype, contiguous */
+int fb_embed(const void* w, int64_t w_stride, int32_t dtype, int32_t vocab, int32_t K,
+             const int64_t* token, int64_t rows, float scale, void* out, void* stream);
+
+/* Its gradient: grad[v] = scale * the sum of the rows of g whose token is v, all of [vocab, K], in
+ * fp32 and in an order that the tokens alone decide, rounded once.
+ *   g     [rows, K] of dtype, rows g_stride elements apart
+ *   grad  [vocab, K] of dtype, contiguous, 16-byte aligned
+ *   ws    256-byte aligned, fb_embed_grad_workspace_bytes (its contents are not kept) */
+int fb_embed_grad(const void* g, int64_t g_stride, int32_t dtype, int32_t vocab, int32_t K,
+                  const int64_t* token, int64_t rows, float scale, void* grad, void* ws,
+                  size_t ws_bytes, void* stream);
+size_t fb_embed_grad_workspace_bytes(int64_t rows, int32_t vocab, int32_t K);
+
+/* The seam between two blocks: h = x + scale * gate * b' with b' = branch * rsqrt(mean branch^2 + eps)
+ * * branch_weight (the branch itself where branch_weight is NULL), y = h * rsqrt(mean h^2 + eps) *
+ * weight, row by row, in fp32; h and y are rounded once each.  Without a branch h is x. */
+typedef struct {
+  const void* x;              /* [rows, width] of dtype, rows x_stride elements apart          */
+  const void* branch;         /* the same, or NULL                                              */
+  const void* gate;           /* [ceil(rows / gate_rows), width], or NULL (1); needs a branch:
+                                 gate_rows consecutive rows share one of its rows               */
+  const void* weight;         /* [width]                                                        */
+  const void* branch_weight;  /* [width] or NULL; needs a branch                                */
+  int64_t x_stride, branch_stride;
+  int64_t rows;               /* 0 .. 2^31 - 1                                                  */
+  int64_t gate_rows;          /* 1 .. 2^31 - 1                                                  */
+  int32_t width;              /* 1 .. 32768                                                     */
+  int32_t dtype;              /* FB_DT_F16, BF16 or F32, of x, branch and the results           */
+  int32_t weight_dtype, branch_weight_dtype, gate_dtype;  /* dtype or FB_DT_F32                 */
+  float scale, eps;           /* eps >= 0                                                       */
+} fb_norm_t;
+
+/*   h, y   [rows, width] of dtype, contiguous (h: with a branch)
+ *   stats  fp32 [rows, 2]: the two rsqrt, what the gradient needs; NULL: not wanted */
+int fb_residual_norm(const fb_norm_t* n, void* h, void* y, float* stats, void* stream);
+
+/* Its gradient from g_h and g_y (contiguous [rows, width] of dtype, or NULL: 0).  Any of the results
+ * may be NULL: grad_x and grad_branch [rows, width] of dtype, grad_weight, grad_branch_weight and
+ * grad_gate of the shapes and types of what they belong to.  Sums over rows are in fp32 and in an order
+ * that the sizes alone decide.
+ *   ws  256-byte aligned, fb_residual_norm_grad_workspace_bytes (its contents are not kept) */
+int fb_residual_norm_grad(const fb_norm_t* n, const float* stats, const void* g_h, const void* g_y,
+                          void* grad_x, void* grad_branch, void* grad_weight,
+                          void* grad_branch_weight, void* grad_gate, void* ws, size_t ws_bytes,
+                          void* stream);
+size_t fb_residual_norm_grad_workspace_bytes(const fb_norm_t* n);
+
+/* fb_token_logprobs of the logits x . w^T, without their being kept: log probabilities of the given
+ * tokens and entropies of their distributions.
+ *   x      [rows, K], w [vocab, K] of dtype FB_DT_F16 or BF16, 16-byte aligned, rows a multiple of 8
+ *          elements apart, at least K rounded up to 8; where K is no multiple of 8, the values between
+ *          are read and must be 0 in both
+ *   token, logprob, entropy  as for fb_token_logprobs
+ *   stats  fp32 [rows, 2]: (a, b) with log p = logit - a - ln 2 b, what the gradient needs; NULL: not
+ *          wanted
+ *   ws     256-byte aligned, fb_head_logprobs_workspace_bytes (its contents are not kept)
+ * Products are exact and summed in fp32.  K up to 2^20, vocab up to 2^24, rows up to 2^24. */
+int fb_head_logprobs(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int32_t dtype,
+                     int64_t rows, int32_t K, int32_t vocab, const int64_t* token, float* logprob,
+                     float* entropy, float* stats, void* ws, size_t ws_bytes, void* stream);
+size_t fb_head_logprobs_workspace_bytes(int64_t rows, int32_t K, int32_t vocab);
+
+/* The gradient: with G[r, v] as fb_token_logprobs_grad's (no alternatives), grad_x = G w and
+ * grad_w = G^T x.  The logits are computed again, a piece of the vocabulary at a time; G enters the
+ * products rounded to dtype (fp16: times a power of two of its row).  A row whose g are 0, or that has
+ * no token and no g_entropy, adds nothing to grad_w whatever its x holds.
+ *   stats, entropy     as fb_head_logprobs wrote them
+ *   g_*                fp32 [rows], or NULL (taken as 0)
+ *   grad_x, grad_w     [rows, K], [vocab, K] of dtype, contiguous, 8-byte aligned; NULL: not wanted
+ *   ws                 256-byte aligned, fb_head_logprobs_grad_workspace_bytes with which are wanted */
+int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
+                          int32_t dtype, int64_t rows, int32_t K, int32_t vocab,
+                          const int64_t* token, const float* stats, const float* entropy,
+                          const float* g_logprob, const float* g_entropy, void* grad_x, void* grad_w,
+                          void* ws, size_t ws_bytes, void* stream);
+size_t fb_head_logprobs_grad_workspace_bytes(int64_t rows, int32_t K, int32_t vocab,
+                                             int32_t want_x, int32_t want_w);
+
 #ifdef __cplusplus
 }
 #endif
