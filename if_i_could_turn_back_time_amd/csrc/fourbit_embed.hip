@@ -6,7 +6,7 @@
 // The gradient sorts the places by token (stably, so that a token's places keep their order): then a
 // token's rows are a run.  Runs are summed in fp32 and in a fixed order, whatever the device does:
 // kShare sorted places that lie within one run are summed by themselves first (a padding or stop token
-// may have most of the batch), and the run's workgroup adds those sums and the places before and
+// may have most of the batch), and a long run's wave adds those sums and the places before and
 // behind them.  The table's zeros, most of the bytes, are written beside the sort.  Up to
 // kSmall places are sorted in one workgroup's LDS, 6 bits a pass; more by passes of 8 bits over memory.
 // Bound by memory: the table's gradient written, and the rows read, once.
@@ -16,77 +16,14 @@
 #include <cstdint>
 
 #include "fourbit.h"
+#include "fourbit_rows.h"
+#include "fourbit_tokens.h"
 
 namespace fb_gpu {
 __attribute__((visibility("hidden"))) int cu_count();
 }  // namespace fb_gpu
 
 namespace {
-
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));  // rows of odd widths begin anywhere
-
-template <int DT>
-struct Of;
-template <>
-struct Of<FB_DT_F32> {
-  using T = float;
-  static constexpr int V = 4;
-};
-template <>
-struct Of<FB_DT_F16> {
-  using T = _Float16;
-  static constexpr int V = 8;
-};
-template <>
-struct Of<FB_DT_BF16> {
-  using T = __bf16;
-  static constexpr int V = 8;
-};
-
-template <int DT>
-__device__ inline void load(const void* p, int64_t at, int n, float (&o)[Of<DT>::V]) {
-  using T = typename Of<DT>::T;
-  constexpr int V = Of<DT>::V;
-  const T* s = static_cast<const T*>(p) + at;
-  if (n >= V) {
-    const u32x4 w = *reinterpret_cast<const u32x4_any*>(s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if constexpr (DT == FB_DT_F32) {
-        const unsigned u = w[i];
-        o[i] = __builtin_bit_cast(float, u);
-      } else {
-        const unsigned u = w[i / 2];
-        if constexpr (DT == FB_DT_F16)
-          o[i] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u >> (16 * (i & 1))));
-        else
-          o[i] = __builtin_bit_cast(float, i & 1 ? u & 0xFFFF0000u : u << 16);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = i < n ? (float)s[i] : 0.f;
-  }
-}
-template <int DT>
-__device__ inline void store(void* p, int64_t at, int n, const float (&v)[Of<DT>::V]) {
-  using T = typename Of<DT>::T;
-  constexpr int V = Of<DT>::V;
-  T* d = static_cast<T*>(p) + at;
-  if (n >= V) {
-    T o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = (T)v[i];
-    u32x4 w;
-    __builtin_memcpy(&w, o, 16);
-    *reinterpret_cast<u32x4_any*>(d) = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) d[i] = (T)v[i];
-  }
-}
 
 // Workgroup: `across` threads of a row's vectors, 256 / across rows.
 template <int DT>
@@ -103,7 +40,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const void* __restrict__ w, 
     const int64_t t = token[r];
     float v[V];
     if (t >= 0 && t < vocab) {
-      load<DT>(w, t * stride + at, K - at, v);
+      load<DT>(w, t * stride, at, K - at, v);
 #pragma unroll
       for (int i = 0; i < V; ++i) v[i] *= scale;
     } else {
@@ -116,7 +53,6 @@ __global__ __launch_bounds__(256) void embed_kernel(const void* __restrict__ w, 
 
 constexpr int kSmall = 16384;  // places of one workgroup's sort
 constexpr int kSmallBits = 18;
-constexpr int kShare = 32;     // sorted places of a sum of their own
 
 __device__ inline unsigned key_of(int64_t t, int vocab) {
   return t >= 0 && t < vocab ? (unsigned)t : (unsigned)vocab;  // the others, together, last
@@ -134,6 +70,16 @@ __device__ inline unsigned long long same_digit(unsigned digit, bool on) {
   return m;
 }
 
+// Zeros, by 256 threads of each of `groups` workgroups.  As many as there are CUs, and plain stores: 1 GiB
+// in 165 us (6.5 TB/s), with 1,024 threads 188, with non-temporal stores of 512 such workgroups 225.
+__device__ inline void clear(u32x4* to, int64_t units, uint8_t* tail, int tail_bytes, int group,
+                             int groups) {
+  if (threadIdx.x >= 256) return;
+  for (int64_t i = (int64_t)group * 256 + threadIdx.x; i < units; i += (int64_t)groups * 256)
+    to[i] = u32x4{0, 0, 0, 0};
+  if (group == 0 && (int)threadIdx.x < tail_bytes) tail[threadIdx.x] = 0;
+}
+
 // Workgroup 0 sorts up to kSmall places by token: key and place in one word.  The others clear the
 // gradient, whose zeros need not wait.
 __global__ __launch_bounds__(1024) void embed_sort_small(const int64_t* __restrict__ token, int rows,
@@ -143,11 +89,7 @@ __global__ __launch_bounds__(1024) void embed_sort_small(const int64_t* __restri
                                                          u32x4* __restrict__ grad, int64_t units,
                                                          uint8_t* __restrict__ tail, int tail_bytes) {
   if (blockIdx.x) {
-    const u32x4 zero{0, 0, 0, 0};
-    const int64_t step = (int64_t)(gridDim.x - 1) * 1024;
-    for (int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; i < units; i += step)
-      __builtin_nontemporal_store(zero, grad + i);
-    if (blockIdx.x == 1 && (int)threadIdx.x < tail_bytes) tail[threadIdx.x] = 0;
+    clear(grad, units, tail, tail_bytes, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   constexpr int WAVES = 16, BINS = 64;
@@ -216,9 +158,7 @@ __global__ __launch_bounds__(256) void embed_keys(const int64_t* __restrict__ to
   const int64_t step = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
   for (int64_t i = i0; i < rows; i += step)
     item[i] = make_uint2(key_of(token[i], vocab), (unsigned)i);
-  const u32x4 zero{0, 0, 0, 0};
-  for (int64_t i = i0; i < units; i += step) __builtin_nontemporal_store(zero, grad + i);
-  if (i0 < tail_bytes) tail[i0] = 0;
+  clear(grad, units, tail, tail_bytes, blockIdx.x, gridDim.x);
 }
 
 __global__ __launch_bounds__(256) void embed_count(const uint2* __restrict__ item, int64_t rows,
@@ -310,6 +250,8 @@ __global__ __launch_bounds__(256) void embed_move(const uint2* __restrict__ item
 }
 
 // ---- sums over the sorted places ----
+constexpr int kShare = 16;  // sorted places of a sum of their own
+
 struct SumArgs {
   const unsigned *key, *place;
   const void* g;
@@ -319,101 +261,168 @@ struct SumArgs {
   float* part;  // [rows / kShare, K]
   void* grad;
 };
+constexpr int kVecs = 2;  // 16-byte pieces of a row a lane
 
-// Adds rows from .. to - 1 of the sorted places to s, four in flight.
-template <int DT>
-__device__ inline void add_rows(const SumArgs& a, int64_t from, int64_t to, int at,
-                                float (&s)[Of<DT>::V]) {
+// Adds the n rows whose places lanes l0 .. l0 + n - 1 hold to s, U in flight.
+template <int DT, int U>
+__device__ inline void add_rows(const SumArgs& a, unsigned place, int l0, int n, int at,
+                                float (&s)[kVecs][Of<DT>::V]) {
   constexpr int V = Of<DT>::V;
-  int64_t i = from;
-  for (; i + 4 <= to; i += 4) {
-    float v[4][V];
+  for (int i = 0; i < n; i += U) {
+    u32x4 w[U][kVecs];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load<DT>(a.g, (int64_t)a.place[i + j] * a.g_stride + at, a.K - at, v[j]);
+    for (int j = 0; j < U; ++j) {
+      const int64_t r = __builtin_amdgcn_readlane((int)place, min(l0 + i + j, 63));
+      if (i + j < n)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] += v[j][e];
-  }
-  for (; i < to; ++i) {
-    float v[V];
-    load<DT>(a.g, (int64_t)a.place[i] * a.g_stride + at, a.K - at, v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) s[e] += v[e];
-  }
-}
-
-// How many of the n <= kShare sorted places from `from` on have key k, which none before has not.
-__device__ inline int run_length(const SumArgs& a, int64_t from, int64_t n, unsigned k) {
-  int c = 0;
-#pragma unroll
-  for (int j = 0; j < kShare; ++j)
-    if (j < n && from + j < a.rows) c += a.key[from + j] == k;
-  return c;
-}
-
-// Shares of kShare sorted places that are one token's.
-template <int DT>
-__global__ __launch_bounds__(256) void embed_shares(SumArgs a, int across) {
-  constexpr int V = Of<DT>::V;
-  const int x = threadIdx.x % across, y = threadIdx.x / across, per = 256 / across;
-  const int at = (blockIdx.x * across + x) * V;
-  if (at >= a.K) return;
-  const int64_t shares = a.rows / kShare;
-  for (int64_t c = (int64_t)blockIdx.y * per + y; c < shares; c += (int64_t)gridDim.y * per) {
-    const unsigned k = a.key[c * kShare];
-    if (k == (unsigned)a.vocab || k != a.key[c * kShare + kShare - 1]) continue;
-    float s[V] = {};
-    add_rows<DT>(a, c * kShare, (c + 1) * kShare, at, s);
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (at + e < a.K) a.part[c * a.K + at + e] = s[e];
-  }
-}
-
-// The run that begins at a sorted place, if one does.
-template <int DT>
-__global__ __launch_bounds__(256) void embed_runs(SumArgs a, int across) {
-  constexpr int V = Of<DT>::V;
-  const int x = threadIdx.x % across, y = threadIdx.x / across, per = 256 / across;
-  const int at = (blockIdx.x * across + x) * V;
-  if (at >= a.K) return;
-  for (int64_t i = (int64_t)blockIdx.y * per + y; i < a.rows; i += (int64_t)gridDim.y * per) {
-    const unsigned k = a.key[i];
-    if (k == (unsigned)a.vocab || (i && a.key[i - 1] == k)) continue;
-    float s[V] = {};
-    const int64_t share = (i + kShare - 1) / kShare;  // the first whole one
-    int64_t end = i + run_length(a, i, share * kShare - i, k);
-    add_rows<DT>(a, i, end, at, s);
-    if (end == share * kShare) {
-      int64_t c = share;
-      for (; (c + 1) * kShare <= a.rows && a.key[(c + 1) * kShare - 1] == k; ++c)
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (at + e < a.K) s[e] += a.part[c * a.K + at + e];
-      end = c * kShare + run_length(a, c * kShare, kShare, k);
-      add_rows<DT>(a, c * kShare, end, at, s);
+        for (int k = 0; k < kVecs; ++k)
+          w[j][k] = raw<DT>(a.g, r * a.g_stride, at + k * 64 * V, a.K - at - k * 64 * V);
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e] *= a.scale;
-    store<DT>(a.grad, (int64_t)k * a.K + at, a.K - at, s);
+    for (int j = 0; j < U; ++j) {
+      if (i + j >= n) break;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        float v[V];
+        unpack<DT>(settled<DT>(w[j][k], at + k * 64 * V, a.K - at - k * 64 * V), v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[k][e] += v[e];
+      }
+    }
   }
 }
 
-// ---------------------------------------------------------------------------------
-// host side
-// ---------------------------------------------------------------------------------
-constexpr int64_t kMostRows = 1ll << 30;
-
-int elem(int32_t dtype) { return dtype == FB_DT_F32 ? 4 : 2; }
-
-int embed_check(int32_t dtype, int64_t stride, int64_t rows, int32_t vocab, int32_t K) {
-  if (dtype != FB_DT_F16 && dtype != FB_DT_BF16 && dtype != FB_DT_F32) return FB_ERR_DTYPE;
-  if (rows < 0 || rows > kMostRows || vocab < 1 || vocab > (1 << 30) || K < 1 || K > (1 << 20) ||
-      stride < 0)
-    return FB_ERR_SHAPE;
-  return FB_OK;
+// Shares of kShare sorted places that are one token's, a wave (and its columns) each.
+template <int DT>
+__global__ __launch_bounds__(256) void token_shares(SumArgs a) {
+  constexpr int V = Of<DT>::V;
+  const int lane = threadIdx.x & 63, at = (blockIdx.x * kVecs * 64 + lane) * V;
+  const int64_t shares = a.rows / kShare;
+  for (int64_t c = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); c < shares;
+       c += (int64_t)gridDim.y * 4) {
+    const int64_t i = c * kShare + min(lane, kShare - 1);
+    const unsigned k = a.key[i], place = a.place[i];
+    const unsigned k0 = __builtin_amdgcn_readfirstlane(k);
+    if (k0 == (unsigned)a.vocab || k0 != (unsigned)__builtin_amdgcn_readlane((int)k, kShare - 1)) continue;
+    float s[kVecs][V] = {};
+    add_rows<DT, 8>(a, place, 0, kShare, at, s);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (at + j * 64 * V + e < a.K) a.part[c * a.K + at + j * 64 * V + e] = s[j][e];
+  }
 }
+
+template <int DT>
+__device__ inline void store_run(const SumArgs& a, unsigned k, int at, float (&s)[kVecs][Of<DT>::V]) {
+  constexpr int V = Of<DT>::V;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[j][e] *= a.scale;
+    const int col = at + j * 64 * V;
+    if (col < a.K) store<DT>(a.grad, (int64_t)k * a.K + col, a.K - col, s[j]);
+  }
+}
+
+// The run of fewer than kLong places that begins at a sorted place, if one does, a wave (and its columns)
+// each.
+constexpr int kLong = 32;
+template <int DT>
+__global__ __launch_bounds__(256) void token_runs(SumArgs a) {
+  constexpr int V = Of<DT>::V;
+  const int lane = threadIdx.x & 63, at = (blockIdx.x * kVecs * 64 + lane) * V;
+  const unsigned none = 0xFFFFFFFFu;
+  for (int64_t i = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); i < a.rows;
+       i += (int64_t)gridDim.y * 4) {
+    const unsigned before = i ? a.key[i - 1] : none;
+    const unsigned key = i + lane < a.rows ? a.key[i + lane] : none;
+    const unsigned place = i + lane < a.rows ? a.place[i + lane] : 0;
+    const unsigned k = __builtin_amdgcn_readfirstlane(key);
+    if (k == (unsigned)a.vocab || __builtin_amdgcn_readfirstlane(before) == k) continue;
+    const unsigned long long other = __ballot(key != k || lane >= kLong);
+    if (__builtin_ctzll(other) == kLong) continue;
+    float s[kVecs][V] = {};
+    add_rows<DT, 8>(a, place, 0, __builtin_ctzll(other), at, s);
+    store_run<DT>(a, k, at, s);
+  }
+}
+
+// The longer runs, 16 waves each: every wave adds a row before the first whole share, each 16th of the
+// shares and a row behind the last, and the waves' sums are joined in pairs.  A run is its first place's
+// that kLong divides, of which it has one.  (By one wave, runs of 270 rows took 50 us.)
+template <int DT>
+__global__ __launch_bounds__(1024) void token_long_runs(SumArgs a) {
+  constexpr int V = Of<DT>::V;
+  __shared__ float red[8][kVecs * V][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int at = (blockIdx.x * kVecs * 64 + lane) * V;
+  for (int64_t q = (int64_t)blockIdx.y * kLong; q < a.rows; q += (int64_t)gridDim.y * kLong) {
+    const unsigned k = a.key[q];
+    // places before q of this run, fewer than kLong where it is the run's first such place
+    const unsigned long long same = __ballot(q - 1 - lane >= 0 && a.key[max(q - 1 - lane, (int64_t)0)] == k);
+    const int ahead = ~same ? __builtin_ctzll(~same) : 64;
+    const int64_t start = q - ahead;
+    if (k == (unsigned)a.vocab || ahead >= kLong || start + kLong > a.rows ||
+        a.key[start + kLong - 1] != k)
+      continue;
+    float s[kVecs][V] = {};
+    int64_t c = (start + kShare - 1) / kShare;
+    const auto row = [&](int64_t i) { add_rows<DT, 1>(a, a.place[i], 0, 1, at, s); };
+    if (start + wave < c * kShare) row(start + wave);
+    for (bool more = true; more;) {  // 64 shares at a time
+      const int64_t last = (c + lane + 1) * kShare - 1;
+      const unsigned long long end = __ballot(last >= a.rows || a.key[min(last, a.rows - 1)] != k);
+      const int n = end ? __builtin_ctzll(end) : 64;
+      u32x4 v[4][kVecs][V / 4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int p = 0; p < kVecs; ++p)
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const int col = at + p * 64 * V + e;
+            v[j][p][e / 4] = wave + 16 * j < n
+                                 ? raw<FB_DT_F32>(a.part, (c + wave + 16 * j) * a.K, col, a.K - col)
+                                 : u32x4{0, 0, 0, 0};
+          }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int p = 0; p < kVecs; ++p)
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const int col = at + p * 64 * V + e;
+            float o[4];
+            unpack<FB_DT_F32>(settled<FB_DT_F32>(v[j][p][e / 4], col, a.K - col), o);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) s[p][e + m] += o[m];
+          }
+      c += n;
+      more = n == 64;
+    }
+    const int64_t rest = c * kShare + wave;
+    if (rest < a.rows && a.key[rest] == k) row(rest);
+    for (int half = 8; half; half >>= 1) {
+      if (wave >= half && wave < 2 * half)
+#pragma unroll
+        for (int p = 0; p < kVecs; ++p)
+#pragma unroll
+          for (int e = 0; e < V; ++e) red[wave - half][p * V + e][lane] = s[p][e];
+      __syncthreads();
+      if (wave < half)
+#pragma unroll
+        for (int p = 0; p < kVecs; ++p)
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[p][e] += red[wave][p * V + e][lane];
+      __syncthreads();
+    }
+    if (wave == 0) store_run<DT>(a, k, at, s);
+  }
+}
+
+inline int elem(int32_t dtype) { return dtype == FB_DT_F32 ? 4 : 2; }
 
 // Threads of a row: a power of two that its vectors fill, 256 at most.
 int across_of(int K, int32_t dtype) {
@@ -428,6 +437,33 @@ dim3 grid_of(int K, int32_t dtype, int64_t rows) {
   return dim3((K + across * V - 1) / (across * V), (unsigned)std::min<int64_t>(y, 65535));
 }
 
+template <int DT>
+int run_sums(const SumArgs& a, hipStream_t hs) {
+  constexpr int kColumns = 64 * kVecs * Of<DT>::V;
+  const auto grid = [&](int64_t n) {
+    return dim3((a.K + kColumns - 1) / kColumns, (unsigned)std::min<int64_t>((n + 3) / 4, 65535));
+  };
+  hipLaunchKernelGGL(token_runs<DT>, grid(a.rows), dim3(256), 0, hs, a);
+  if (a.rows >= kLong) {
+    hipLaunchKernelGGL(token_shares<DT>, grid(a.rows / kShare), dim3(256), 0, hs, a);
+    hipLaunchKernelGGL(token_long_runs<DT>, grid((a.rows + kLong - 1) / kLong * 4), dim3(1024), 0, hs, a);
+  }
+  return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+}
+
+// ---------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------
+constexpr int64_t kMostRows = 1ll << 30;
+
+int embed_check(int32_t dtype, int64_t stride, int64_t rows, int32_t vocab, int32_t K) {
+  if (dtype != FB_DT_F16 && dtype != FB_DT_BF16 && dtype != FB_DT_F32) return FB_ERR_DTYPE;
+  if (rows < 0 || rows > kMostRows || vocab < 1 || vocab > (1 << 30) || K < 1 || K > (1 << 20) ||
+      stride < 0)
+    return FB_ERR_SHAPE;
+  return FB_OK;
+}
+
 int bits_of(int32_t vocab) {  // of the keys 0 .. vocab
   int b = 1;
   while (b < 31 && vocab >> b) ++b;
@@ -437,43 +473,67 @@ bool small_sort(int64_t rows, int32_t vocab) { return rows <= kSmall && bits_of(
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
-struct EmbedPlan {
+struct SortPlan {
   int tiles;
-  size_t at_key, at_place, at_part, at_item[2], at_count, bytes;
+  size_t at_item[2], at_count, bytes;
 };
-EmbedPlan embed_plan(int64_t rows, int32_t vocab, int32_t K) {
-  EmbedPlan p{};
-  size_t at = 0;
-  const auto take = [&](size_t n) {
-    const size_t was = at;
-    at += up256(n);
-    return was;
-  };
-  p.at_key = take(rows * 4);
-  p.at_place = take(rows * 4);
-  p.at_part = take((size_t)(rows / kShare) * K * 4);
-  if (!small_sort(rows, vocab)) {
-    p.tiles = (int)((rows + kTile - 1) / kTile);
-    p.at_item[0] = take(rows * 8);
-    p.at_item[1] = take(rows * 8);
-    p.at_count = take((size_t)p.tiles * kBins * 4);
-  }
-  p.bytes = at;
+SortPlan sort_plan(int64_t rows, int32_t vocab) {
+  SortPlan p{};
+  if (small_sort(rows, vocab)) return p;
+  p.tiles = (int)((rows + kTile - 1) / kTile);
+  p.at_item[1] = up256(rows * 8);
+  p.at_count = 2 * p.at_item[1];
+  p.bytes = p.at_count + up256((size_t)p.tiles * kBins * 4);
   return p;
 }
 
-template <int DT>
-int run_sums(const SumArgs& a, int across, hipStream_t hs) {
-  const int32_t dt = DT;
-  if (a.rows >= kShare)
-    hipLaunchKernelGGL(embed_shares<DT>, grid_of(a.K, dt, a.rows / kShare), dim3(256), 0, hs, a, across);
-  hipLaunchKernelGGL(embed_runs<DT>, grid_of(a.K, dt, a.rows), dim3(256), 0, hs, a, across);
-  return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+struct EmbedPlan {
+  size_t at_place, at_part, at_sort, bytes;
+};
+EmbedPlan embed_plan(int64_t rows, int32_t vocab, int32_t K) {
+  EmbedPlan p{};
+  p.at_place = up256(rows * 4);
+  p.at_part = 2 * p.at_place;
+  p.at_sort = p.at_part + up256((size_t)(rows / kShare) * K * 4);
+  p.bytes = p.at_sort + sort_plan(rows, vocab).bytes;
+  return p;
 }
 
 bool off(const void* p, unsigned mask) { return reinterpret_cast<uintptr_t>(p) & mask; }
 
 }  // namespace
+
+size_t fb_gpu::sort_bytes(int64_t rows, int32_t vocab) { return sort_plan(rows, vocab).bytes; }
+
+int fb_gpu::sort_tokens(const int64_t* token, int64_t rows, int32_t vocab, unsigned* key,
+                        unsigned* place, void* clear, int64_t bytes, void* ws, hipStream_t hs) {
+  const SortPlan p = sort_plan(rows, vocab);
+  const int64_t units = bytes / 16;
+  u32x4* const zeros = static_cast<u32x4*>(clear);
+  uint8_t* const tail = static_cast<uint8_t*>(clear) + units * 16;
+  const int bits = bits_of(vocab), cus = cu_count();
+  if (small_sort(rows, vocab)) {
+    const int64_t fill = std::min<int64_t>(units / 1024 + 1, cus);
+    hipLaunchKernelGGL(embed_sort_small, dim3((unsigned)(1 + fill)), dim3(1024), 0, hs, token, (int)rows,
+                       vocab, bits, key, place, zeros, units, tail, (int)(bytes & 15));
+    return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+  }
+  uint8_t* const w = static_cast<uint8_t*>(ws);
+  uint2* const item[2] = {reinterpret_cast<uint2*>(w), reinterpret_cast<uint2*>(w + p.at_item[1])};
+  unsigned* const count = reinterpret_cast<unsigned*>(w + p.at_count);
+  hipLaunchKernelGGL(embed_keys, dim3(cus), dim3(256), 0, hs, token, rows, vocab, item[0], zeros,
+                     units, tail, (int)(bytes & 15));
+  int from = 0;
+  for (int shift = 0; shift < bits; shift += 8, from ^= 1) {
+    const bool last = shift + 8 >= bits;
+    hipLaunchKernelGGL(embed_count, dim3(p.tiles), dim3(256), 0, hs, item[from], rows, shift, count,
+                       p.tiles);
+    hipLaunchKernelGGL(embed_scan, dim3(1), dim3(1024), 0, hs, count, p.tiles * kBins);
+    hipLaunchKernelGGL(embed_move, dim3(p.tiles), dim3(256), 0, hs, item[from], rows, shift, count,
+                       p.tiles, item[from ^ 1], last ? key : nullptr, last ? place : nullptr);
+  }
+  return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+}
 
 extern "C" {
 
@@ -513,40 +573,25 @@ int fb_embed_grad(const void* g, int64_t g_stride, int32_t dtype, int32_t vocab,
   if (ws_bytes < p.bytes) return FB_ERR_WORKSPACE;
   hipStream_t hs = static_cast<hipStream_t>(stream);
   uint8_t* const w = static_cast<uint8_t*>(ws);
-  const int64_t bytes = (int64_t)vocab * K * elem(dtype), units = bytes / 16;
-  uint8_t* const tail = static_cast<uint8_t*>(grad) + units * 16;
-  u32x4* const zeros = static_cast<u32x4*>(grad);
-  unsigned* const key = reinterpret_cast<unsigned*>(w + p.at_key);
+  unsigned* const key = reinterpret_cast<unsigned*>(w);
   unsigned* const place = reinterpret_cast<unsigned*>(w + p.at_place);
-  const int bits = bits_of(vocab), cus = fb_gpu::cu_count();
-  if (small_sort(rows, vocab)) {
-    const int64_t fill = std::min<int64_t>((units + 4095) / 4096 + 1, 2 * cus);
-    hipLaunchKernelGGL(embed_sort_small, dim3((unsigned)(1 + fill)), dim3(1024), 0, hs, token, (int)rows,
-                       vocab, bits, key, place, zeros, units, tail, (int)(bytes & 15));
-  } else {
-    uint2* item[2] = {reinterpret_cast<uint2*>(w + p.at_item[0]),
-                      reinterpret_cast<uint2*>(w + p.at_item[1])};
-    unsigned* const count = reinterpret_cast<unsigned*>(w + p.at_count);
-    hipLaunchKernelGGL(embed_keys, dim3(8 * cus), dim3(256), 0, hs, token, rows, vocab, item[0], zeros,
-                       units, tail, (int)(bytes & 15));
-    int from = 0;
-    for (int shift = 0; shift < bits; shift += 8, from ^= 1) {
-      const bool last = shift + 8 >= bits;
-      hipLaunchKernelGGL(embed_count, dim3(p.tiles), dim3(256), 0, hs, item[from], rows, shift, count,
-                         p.tiles);
-      hipLaunchKernelGGL(embed_scan, dim3(1), dim3(1024), 0, hs, count, p.tiles * kBins);
-      hipLaunchKernelGGL(embed_move, dim3(p.tiles), dim3(256), 0, hs, item[from], rows, shift, count,
-                         p.tiles, item[from ^ 1], last ? key : nullptr, last ? place : nullptr);
-    }
-  }
-  if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
-  if (rows == 0) return FB_OK;
-  SumArgs a{key, place, g, g_stride, rows, vocab, K, scale,
-            reinterpret_cast<float*>(w + p.at_part), grad};
-  const int across = across_of(K, dtype);
-  return dtype == FB_DT_F16    ? run_sums<FB_DT_F16>(a, across, hs)
-         : dtype == FB_DT_BF16 ? run_sums<FB_DT_BF16>(a, across, hs)
-                               : run_sums<FB_DT_F32>(a, across, hs);
+  const int rc = fb_gpu::sort_tokens(token, rows, vocab, key, place, grad,
+                                     (int64_t)vocab * K * elem(dtype), w + p.at_sort, hs);
+  if (rc != FB_OK || rows == 0) return rc;
+  SumArgs a{};
+  a.key = key;
+  a.place = place;
+  a.g = g;
+  a.g_stride = g_stride;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.K = K;
+  a.scale = scale;
+  a.part = reinterpret_cast<float*>(w + p.at_part);
+  a.grad = grad;
+  return dtype == FB_DT_F16    ? run_sums<FB_DT_F16>(a, hs)
+         : dtype == FB_DT_BF16 ? run_sums<FB_DT_BF16>(a, hs)
+                               : run_sums<FB_DT_F32>(a, hs);
 }
 
 }  // extern "C"

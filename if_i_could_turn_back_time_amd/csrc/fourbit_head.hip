@@ -12,9 +12,11 @@
 //             vocabulary: 1 GiB of G at most.
 //   kProduct  grad_x: G times W over the vocabulary, pieces and parts of which are added in fp32;
 //             grad_w: G^T times x over the rows.
-// G in 16 bits costs each of its values half a step; products and all sums are fp32.  In fp16 each
-// row of G has a power of two of its own that brings it near the type's largest values, and grad_w's
-// x one that takes it off again.
+// G in 16 bits costs each of its values half a step; products and all sums are fp32.  One value of a row
+// stands out, the given token's, and its half step alone would be as large as the result's own rounding:
+// what it lost is kept in fp32 and goes into both results, times its row of W (head_sum) or of x (grad_w's
+// tiles end with the rows whose token they hold, which a sort by token finds).  In fp16 each row of G has a power of two of
+// its own that brings it near the type's largest values, and grad_w's x one that takes it off again.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -22,6 +24,7 @@
 
 #include "fourbit.h"
 #include "fourbit_decode.h"
+#include "fourbit_tokens.h"
 
 namespace fb_gpu {
 __attribute__((visibility("hidden"))) int cu_count();
@@ -30,6 +33,7 @@ __attribute__((visibility("hidden"))) int cu_count();
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));  // rows of odd widths begin anywhere
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -46,7 +50,7 @@ struct ProductArgs {
   int tiles_p, tiles_q;
   int chunks;        // of a part
   // kStats
-  float *pm, *pz, *pw;  // [tiles_p * WP, nq]
+  float *pm, *pz, *pw;  // [tiles_p, nq]
   float* given;         // [nq]: the given token's logit
   const int64_t* token;
   int v0;  // p's first row is this token
@@ -56,13 +60,21 @@ struct ProductArgs {
   uint16_t* g;
   int64_t ldg;
   int vocab;
+  float* lost;  // [nq]: what the given token's value lost in rounding
   // kProduct
-  void* out;       // [nq, np] of 16 bits, or null
-  float* acc;      // [parts, nq, np] otherwise
-  int add;         // to what acc holds
+  void* out;   // [nq, np] of 16 bits, or null
+  float* acc;  // [parts, nq, np] otherwise
+  int add;     // to what acc holds
   const float* out_scale;  // null, or of one value
-  const float* row_scale;  // null, or [nq]
+  // and for QT: the rows by token (key, place), from which of them on each 128 tokens' lie, and what to
+  // add of each
+  const unsigned *key, *place, *start;
+  int starts;
 };
+
+// By what the 32-byte units of contraction row k are permuted (TR, below): the rows that 32 lanes read
+// at a time, 0 to 3 and 8 to 11 of 16 or 4 to 7 and 12 to 15, get all of 0 to 7.
+__device__ inline int row_mask(int k) { return (k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2); }
 
 // One operand's tile of T values by kChunk of the contraction in LDS, T / 8 requests of 1 KiB.
 // Rows of the contraction side by side (TR = false): [T][64], a row's eight 16-byte units permuted by
@@ -84,8 +96,7 @@ struct Side {
       if constexpr (TR) {
         constexpr int PER = T / 8;  // lanes of a row
         const int k = i * (64 / PER) + lane / PER;
-        const int f = (k & 3) | ((((k >> 3) ^ (k >> 4)) & 1) << 2);
-        const int w = ((lane % PER) >> 1) ^ f;
+        const int w = ((lane % PER) >> 1) ^ row_mask(k);
         off[j] = (unsigned)(k * ld + w * 16 + (lane & 1) * 8) * 2u;
       } else {
         const int row = i * 8 + (lane >> 3);
@@ -96,8 +107,8 @@ struct Side {
     }
     const int r = lane & 15, g = lane >> 4;
     if constexpr (TR) {
-      const int f = (r >> 2) | (((g ^ (g >> 1)) & 1) << 2);
-      rd = (8 * g + (r >> 2)) * (2 * T) + f * 32 + (r & 3) * 8;
+      const int k = 8 * g + (r >> 2);
+      rd = k * (2 * T) + row_mask(k) * 32 + (r & 3) * 8;
     } else {
       rd = r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
     }
@@ -161,6 +172,26 @@ __device__ inline unsigned pack2(float a, float b) {
     return __builtin_bit_cast(unsigned short, (__bf16)a) |
            (unsigned)__builtin_bit_cast(unsigned short, (__bf16)b) << 16;
 }
+
+template <int DT>
+__device__ inline float rounded(float v) {
+  if constexpr (DT == FB_DT_F16) return (float)(_Float16)v;
+  else return (float)(__bf16)v;
+}
+
+// Sums of exp(l - m) and of exp(l - m) (l - m).
+struct Sums {
+  float m = -__builtin_inff(), z = 0.f, w = 0.f;
+  __device__ void add(float m2, float z2, float w2) {
+    if (z2 == 0.f) return;  // of nothing but -inf
+    const float to = fmaxf(m, m2), d1 = m - to, d2 = m2 - to;
+    const float f1 = z == 0.f ? 0.f : __builtin_amdgcn_exp2f(d1 * kLog2e);
+    const float f2 = __builtin_amdgcn_exp2f(d2 * kLog2e);
+    w = f1 * __builtin_fmaf(fmaxf(d1, kLow), z, w) + f2 * __builtin_fmaf(fmaxf(d2, kLow), z2, w2);
+    z = f1 * z + f2 * z2;
+    m = to;
+  }
+};
 
 // A tile of TP x TQ of p q^T, WP x WQ waves.
 template <int DT, bool PT, bool QT, int TP, int TQ, int WP, int WQ, int MODE>
@@ -241,11 +272,98 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
     }
   }
 
+  if constexpr (MODE == kProduct && QT) {
+    // What the rows' given tokens lost, of the tokens in this tile: 64 rows at a time as one more chunk,
+    // with one value of q in each.
+    const int s0 = a.start[min((a.v0 + tq0) / 128, a.starts)];
+    const int s1 = a.start[min((a.v0 + tq0 + TQ) / 128, a.starts)];
+    for (int at = s0; at < s1; at += kChunk) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < TQ * 8; i += WAVES * 64)
+        reinterpret_cast<u32x4*>(q0)[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < sp.kRequests; ++j) {
+        constexpr int PER = TP / 8;
+        const int i = wave * sp.kRequests + j, k = i * (64 / PER) + lane / PER;
+        const int w = ((lane % PER) >> 1) ^ row_mask(k);
+        const int64_t col = tp0 + w * 16 + (lane & 1) * 8;
+        const int64_t row = a.place[min(at + k, s1 - 1)];
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(a.p + (row * a.ldp +
+                                                                   (col < a.ldp ? col : 0)) * 2),
+            (__attribute__((address_space(3))) void*)(p0 + i * 1024), 16, 0, 0);
+      }
+      __syncthreads();
+      const int k = threadIdx.x;
+      if (k < kChunk && at + k < s1) {
+        const int v = (int)a.key[at + k] - a.v0 - tq0;
+        reinterpret_cast<uint16_t*>(q0)[k * TQ + ((v >> 4) ^ row_mask(k)) * 16 + (v & 15)] =
+            (uint16_t)pack2<DT>(a.lost[a.place[at + k]], 0.f);
+      }
+      arrive();
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int i = 0; i < RP + RQ; ++i) read(p0, q0, s, 0, i);
+#pragma unroll
+        for (int i = 0; i < RP; ++i)
+#pragma unroll
+          for (int j = 0; j < RQ; ++j) acc[i][j] = mfma<DT>(pa[0][i], qa[0][j], acc[i][j]);
+      }
+    }
+  }
+
   // lane: q's row lane % 16 of tile j, p's rows 4 (lane / 16) .. + 3 of tile i
   const int pl = tp0 + wp * (TP / WP) + (lane >> 4) * 4;
   const int ql = tq0 + wq * (TQ / WQ) + (lane & 15);
+
+  // 16-bit results go through LDS, a wave's part of the tile each, so that a store writes whole runs of a
+  // row: straight from the accumulators (32 bytes of 16 rows each) they took 92 of 486 us of grad_w of
+  // 2048 x 32000 x 4096.  The 16-byte units of a row are permuted by its number.
+  constexpr int kUnits = RP * 2, kWaveBytes = RP * RQ * 512, kPer = TP * 128 / kWaveBytes;
+  static_assert(kPer >= 1 && (kPer >= WAVES || (TP == TQ && kPer * 4 >= WAVES)), "all waves' parts fit");
+  uint8_t* const mine_lds = (wave / kPer == 0   ? p0
+                             : wave / kPer == 1 ? p1
+                             : wave / kPer == 2 ? q0
+                                                : q1) +
+                            wave % kPer * kWaveBytes;
+  const auto put = [&](int i, int j, unsigned lo, unsigned hi) {
+    const int row = j * 16 + (lane & 15), u = i * 2 + (lane >> 5);
+    *reinterpret_cast<uint2*>(mine_lds + row * (kUnits * 16) + ((u ^ (row & (kUnits - 1))) << 4) +
+                              ((lane >> 4) & 1) * 8) = make_uint2(lo, hi);
+  };
+  const auto put_one = [&](int i, int j, int e, uint16_t v) {
+    const int row = j * 16 + (lane & 15), u = i * 2 + (lane >> 5);
+    *reinterpret_cast<uint16_t*>(mine_lds + row * (kUnits * 16) + ((u ^ (row & (kUnits - 1))) << 4) +
+                                 ((lane >> 4) & 1) * 8 + e * 2) = v;
+  };
+  // The wave's part to rows of `out`, ld values apart, of which the first n columns and rows are there.
+  const auto write = [&](void* out, int64_t ld, int n, int rows) {
+    constexpr int R = 64 / kUnits;  // rows of a store
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < RQ * 16 / R; ++k) {
+      const int row = k * R + lane / kUnits, u = lane % kUnits;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(mine_lds + row * (kUnits * 16) +
+                                                      ((u ^ (row & (kUnits - 1))) << 4));
+      const int64_t r = tq0 + wq * (TQ / WQ) + row;
+      const int c = tp0 + wp * (TP / WP) + u * 8;
+      uint16_t* const to = static_cast<uint16_t*>(out) + r * ld + c;
+      if (r < rows && c + 8 <= n) {
+        *reinterpret_cast<u32x4_any*>(to) = v;
+      } else if (r < rows) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < n) to[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+      }
+    }
+  };
+  if constexpr (MODE != kStats) __syncthreads();  // no wave reads a tile any more
   if constexpr (MODE == kStats) {
     const bool whole = tp0 + TP <= a.np;
+    float* const part = reinterpret_cast<float*>(p0);  // [WP, TQ, 3]
+    static_assert(WP * TQ * 12 <= TP * 128, "the waves' sums take the place of a tile");
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < RQ; ++j) {
       const int r = ql + j * 16;
@@ -283,126 +401,170 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
             for (int e = 0; e < 4; ++e)
               if (t == i * 16 + e && pl + i * 16 + e < a.np) a.given[r] = acc[i][j][e];
         }
-        if (lane < 16) {
-          const int64_t at = (int64_t)(tp * WP + wp) * a.nq + r;
-          a.pm[at] = m;
-          a.pz[at] = z;
-          a.pw[at] = w;
-        }
+      }
+      if (lane < 16) {
+        float* const to_wave = part + ((wp * TQ) + r - tq0) * 3;
+        to_wave[0] = m;
+        to_wave[1] = z;
+        to_wave[2] = w;
       }
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < TQ && tq0 + i < a.nq; i += WAVES * 64) {
+      Sums t;
+#pragma unroll
+      for (int w = 0; w < WP; ++w) {
+        const float* const v = part + (w * TQ + i) * 3;
+        t.add(v[0], v[1], v[2]);
+      }
+      const int64_t at = (int64_t)tp * a.nq + tq0 + i;
+      a.pm[at] = t.m;
+      a.pz[at] = t.z;
+      a.pw[at] = t.w;
+    }
   } else if constexpr (MODE == kGradient) {
+    const bool whole = tp0 + TP <= a.np;
+    const auto rows = [&](auto with_entropy) {
+      constexpr bool ENT = decltype(with_entropy)::value;
 #pragma unroll
     for (int j = 0; j < RQ; ++j) {
-      const int r = ql + j * 16;
-      if (r >= a.nq) continue;
+      const int r = min(ql + j * 16, a.nq - 1);
+      const bool mine = ql + j * 16 < a.nq;
       const int64_t token = a.token[r];
       const bool any = token >= 0 && token < a.vocab;
       const float g = any && a.g_logprob ? a.g_logprob[r] : 0.f;
-      const float ge = a.g_entropy ? a.g_entropy[r] : 0.f;
+      const float ge = ENT ? a.g_entropy[r] : 0.f;
       const float m = a.rowmax[2 * r], l2z = a.log2z[2 * r], up = a.scale[r];
-      const float all = -up * (g + (a.g_entropy ? ge * a.entropy[r] : 0.f));
+      const float all = -up * (g + (ENT ? ge * a.entropy[r] : 0.f));
       const float slope = -up * ge * kLn2;
-      const int t = any ? (int)(token - a.v0) - pl : -1;
-      uint16_t* const row = a.g + (int64_t)r * a.ldg + pl;
+      const auto value = [&](float l) {
+        const float y = __builtin_fmaf(l - m, kLog2e, -l2z), p = __builtin_amdgcn_exp2f(y);
+        return p * (ENT ? __builtin_fmaf(slope, fmaxf(y, kLow), all) : all);
+      };
+      // a row without a gradient is 0 whatever its logits are
+      const unsigned keep = up == 0.f ? 0u : ~0u;
 #pragma unroll
       for (int i = 0; i < RP; ++i) {
         float o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float y = __builtin_fmaf(acc[i][j][e] - m, kLog2e, -l2z);
-          float v = __builtin_amdgcn_exp2f(y) * __builtin_fmaf(slope, fmaxf(y, kLow), all);
-          if (t == i * 16 + e) v = __builtin_fmaf(up, g, v);
-          o[e] = up == 0.f || pl + i * 16 + e >= a.np ? 0.f : v;
+          o[e] = value(acc[i][j][e]);
+          if (!whole && pl + i * 16 + e >= a.np) o[e] = 0.f;
         }
-        if (pl + i * 16 < a.ldg)
-          *reinterpret_cast<uint2*>(row + i * 16) =
-              make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+        put(i, j, pack2<DT>(o[0], o[1]) & keep, pack2<DT>(o[2], o[3]) & keep);
+      }
+      const int64_t t = token - a.v0 - pl;  // the given token, from this lane's first one on
+      if (any && keep && t >= 0 && t < RP * 16 && (t & 15) < 4) {
+#pragma unroll
+        for (int i = 0; i < RP; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t == i * 16 + e) {
+              const float v = __builtin_fmaf(up, g, value(acc[i][j][e]));
+              put_one(i, j, e, (uint16_t)pack2<DT>(v, 0.f));
+              if (mine) a.lost[r] = v - rounded<DT>(v);
+            }
       }
     }
+    };
+    if (a.g_entropy)
+      rows(std::true_type{});
+    else
+      rows(std::false_type{});
+    write(a.g, a.ldg, (int)a.ldg, a.nq);
   } else {
-    const float all = a.out_scale ? a.out_scale[0] : 1.f;
-    const bool vec = (a.np & 3) == 0;
+    if (a.acc) {
+      const bool vec = (a.np & 3) == 0;
 #pragma unroll
-    for (int j = 0; j < RQ; ++j) {
-      const int r = ql + j * 16;
-      if (r >= a.nq) continue;
-      const float up = a.row_scale && !a.acc ? a.row_scale[r] : all;
+      for (int j = 0; j < RQ; ++j) {
+        const int r = ql + j * 16;
+        if (r >= a.nq) continue;
 #pragma unroll
-      for (int i = 0; i < RP; ++i) {
-        const int at = pl + i * 16;
-        const f32x4 v = acc[i][j];
-        if (a.acc) {
+        for (int i = 0; i < RP; ++i) {
+          const int at = pl + i * 16;
           float* const dst = a.acc + ((int64_t)part * a.nq + r) * a.np + at;
           if (vec && at < a.np) {
-            f32x4 s = v;
+            f32x4 s = acc[i][j];
             if (a.add) s += *reinterpret_cast<const f32x4*>(dst);
             *reinterpret_cast<f32x4*>(dst) = s;
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (at + e < a.np) dst[e] = a.add ? dst[e] + v[e] : v[e];
-          }
-        } else {
-          uint16_t* const dst = static_cast<uint16_t*>(a.out) + (int64_t)r * a.np + at;
-          const unsigned lo = pack2<DT>(v[0] * up, v[1] * up), hi = pack2<DT>(v[2] * up, v[3] * up);
-          if (vec && at < a.np) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-          } else {
-            if (at < a.np) dst[0] = (uint16_t)lo;
-            if (at + 1 < a.np) dst[1] = (uint16_t)(lo >> 16);
-            if (at + 2 < a.np) dst[2] = (uint16_t)hi;
-            if (at + 3 < a.np) dst[3] = (uint16_t)(hi >> 16);
+              if (at + e < a.np) dst[e] = a.add ? dst[e] + acc[i][j][e] : acc[i][j][e];
           }
         }
       }
+    } else {
+      const float up = a.out_scale ? a.out_scale[0] : 1.f;
+#pragma unroll
+      for (int j = 0; j < RQ; ++j)
+#pragma unroll
+        for (int i = 0; i < RP; ++i) {
+          const f32x4 v = acc[i][j] * up;
+          put(i, j, pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
+        }
+      write(a.out, a.np, a.np, a.nq);
     }
   }
 }
 
-// A row's results from its parts' (m, z, w): 16 rows by 16 threads each.
-__global__ __launch_bounds__(256) void head_join(const float* __restrict__ pm,
-                                                 const float* __restrict__ pz,
-                                                 const float* __restrict__ pw, int parts, int rows,
-                                                 const float* __restrict__ given,
-                                                 const int64_t* __restrict__ token, int vocab,
-                                                 float* __restrict__ logprob,
-                                                 float* __restrict__ entropy,
-                                                 float* __restrict__ stats) {
-  __shared__ float red[3][16][17];
+// A row's results from its parts: 16 rows by 64 threads each.
+__global__ __launch_bounds__(1024) void head_join(const float* __restrict__ pm,
+                                                  const float* __restrict__ pz,
+                                                  const float* __restrict__ pw, int parts, int rows,
+                                                  const float* __restrict__ given,
+                                                  const int64_t* __restrict__ token, int vocab,
+                                                  float* __restrict__ logprob,
+                                                  float* __restrict__ entropy,
+                                                  float* __restrict__ stats) {
+  __shared__ float red[3][64][17];
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4, r = blockIdx.x * 16 + x;
-  float m = -__builtin_inff(), z = 0.f, w = 0.f;
-  const auto add = [&](float m2, float z2, float w2) {
-    if (z2 == 0.f) return;
-    const float to = fmaxf(m, m2), d1 = m - to, d2 = m2 - to;
-    const float f1 = z == 0.f ? 0.f : __builtin_amdgcn_exp2f(d1 * kLog2e);
-    const float f2 = __builtin_amdgcn_exp2f(d2 * kLog2e);
-    w = f1 * __builtin_fmaf(fmaxf(d1, kLow), z, w) + f2 * __builtin_fmaf(fmaxf(d2, kLow), z2, w2);
-    z = f1 * z + f2 * z2;
-    m = to;
-  };
-  if (r < rows)
-#pragma unroll 4
-    for (int p = y; p < parts; p += 16) {
+  Sums s;
+  for (int p0 = y; p0 < parts; p0 += 256) {
+    float m[4], z[4], w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int p = p0 + j * 64;
       const int64_t at = (int64_t)p * rows + r;
-      add(pm[at], pz[at], pw[at]);
+      const bool on = p < parts && r < rows;
+      m[j] = on ? pm[at] : 0.f;
+      z[j] = on ? pz[at] : 0.f;
+      w[j] = on ? pw[at] : 0.f;
     }
-  red[0][y][x] = m;
-  red[1][y][x] = z;
-  red[2][y][x] = w;
-  __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s.add(m[j], z[j], w[j]);
+  }
+  // halves, so that the order is the same whatever the machine does
+  for (int half = 32; half >= 1; half >>= 1) {
+    if (y >= half && y < 2 * half) {
+      red[0][y][x] = s.m;
+      red[1][y][x] = s.z;
+      red[2][y][x] = s.w;
+    }
+    __syncthreads();
+    if (y < half) s.add(red[0][y + half][x], red[1][y + half][x], red[2][y + half][x]);
+  }
   if (y || r >= rows) return;
-  for (int i = 1; i < 16; ++i) add(red[0][i][x], red[1][i][x], red[2][i][x]);
   const int64_t t = token[r];
-  const bool none = z == 0.f;
-  const float l2z = __builtin_log2f(z);
+  const bool none = s.z == 0.f;
+  const float l2z = __builtin_log2f(s.z);
   const bool any = t >= 0 && t < vocab;
-  logprob[r] = !any ? 0.f : none ? -__builtin_inff() : given[r] - m - kLn2 * l2z;
-  entropy[r] = none ? 0.f : __builtin_fmaf(kLn2, l2z, -w / z);
+  logprob[r] = !any ? 0.f : none ? -__builtin_inff() : given[r] - s.m - kLn2 * l2z;
+  entropy[r] = none ? 0.f : __builtin_fmaf(kLn2, l2z, -s.w / s.z);
   if (stats) {
-    stats[2 * r] = none ? 0.f : m;
+    stats[2 * r] = none ? 0.f : s.m;
     stats[2 * r + 1] = none ? __builtin_inff() : l2z;
   }
+}
+
+// start[i] = the first sorted place of a token from 128 i on, for i up to `tiles` (beyond the last).
+__global__ __launch_bounds__(256) void head_starts(const unsigned* __restrict__ key, int rows,
+                                                   int vocab, int tiles, unsigned* __restrict__ start) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i > rows) return;
+  const auto tile = [&](int at) { return key[at] >= (unsigned)vocab ? tiles : (int)(key[at] / 128); };
+  const int from = i ? tile(i - 1) + 1 : 0, to = i < rows ? tile(i) : tiles;
+  for (int t = from; t <= to; ++t) start[t] = i;
 }
 
 // What bounds |G| in row r: 0 where no gradient comes in.
@@ -446,7 +608,7 @@ __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, 
                                                  const float* __restrict__ ge,
                                                  const float* __restrict__ top,
                                                  float* __restrict__ scale, float* __restrict__ undo,
-                                                 uint8_t* __restrict__ xs) {
+                                                 float* __restrict__ lost, uint8_t* __restrict__ xs) {
   const int64_t r = blockIdx.x;
   const float b = row_bound(r, token, vocab, g, ge);
   float up = b == 0.f ? 0.f : 1.f, down = up;
@@ -460,6 +622,7 @@ __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, 
   if (threadIdx.x == 0) {
     scale[r] = up;
     undo[r] = down;
+    lost[r] = 0.f;
   }
   if (!xs) return;
   const float f = DT == FB_DT_F16 && b != 0.f ? down / top[0] : up;
@@ -479,23 +642,40 @@ __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, 
   }
 }
 
-// out = the parts' sums added in their order, times the row's power of two, rounded once.
+// out = (the parts' sums added in their order + what the given token's value lost times its row of W)
+// times the row's power of two, rounded once.
 template <int DT>
 __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, int parts, int rows,
                                                 int K, const float* __restrict__ undo,
+                                                const float* __restrict__ lost,
+                                                const int64_t* __restrict__ token, int vocab,
+                                                const uint16_t* __restrict__ w, int64_t ldw,
                                                 uint16_t* __restrict__ out) {
   const int64_t n = (int64_t)rows * K, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  const auto value = [](unsigned h) {
+    if constexpr (DT == FB_DT_F16) return (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+    else return __builtin_bit_cast(float, h << 16);
+  };
   if (i >= n) return;
   if ((K & 3) == 0) {
+    const int64_t r = i / K, t = token[r];
     f32x4 s = *reinterpret_cast<const f32x4*>(acc + i);
     for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(acc + p * n + i);
-    s *= undo[i / K];
+    const float l = lost[r];
+    if (l != 0.f && t >= 0 && t < vocab) {
+      const uint2 v = *reinterpret_cast<const uint2*>(w + t * ldw + (i - r * K));
+      s += f32x4{l * value(v.x & 0xFFFFu), l * value(v.x >> 16), l * value(v.y & 0xFFFFu),
+                 l * value(v.y >> 16)};
+    }
+    s *= undo[r];
     *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]));
   } else {
     for (int64_t at = i; at < n && at < i + 4; ++at) {
+      const int64_t r = at / K, t = token[r];
       float s = acc[at];
       for (int p = 1; p < parts; ++p) s += acc[p * n + at];
-      out[at] = (uint16_t)pack2<DT>(s * undo[at / K], 0.f);
+      if (lost[r] != 0.f && t >= 0 && t < vocab) s += lost[r] * value(w[t * ldw + (at - r * K)]);
+      out[at] = (uint16_t)pack2<DT>(s * undo[r], 0.f);
     }
   }
 }
@@ -507,17 +687,32 @@ constexpr int64_t kMostG = 1ll << 30;       // bytes of G at once
 constexpr int64_t kMostRows = 1 << 24;
 constexpr int64_t kStatRows = 1 << 14;      // rows of logits whose parts are held at once
 
+// Tiles to choose from, with what a workgroup of each takes in us: a chunk of the contraction with all
+// of a CU's workgroups running and with one, where the contraction lies along rows and where (TR) not, and
+// the rest.  Fitted to timings of the four products of 2048 x 32000 x 4096, 1024 x 32000 x 4096, 4096 x
+// 131072 x 4096 and 777 x 50001 x 1000.
 struct Shape {
-  int tp, tq, wp;
-  int slots;  // workgroups of a CU
+  int tp, tq, slots;  // workgroups of a CU
+  double full, alone, full_tr, alone_tr, rest;
 };
-constexpr Shape kShapes[] = {{256, 256, 2, 1}, {128, 128, 2, 2}, {128, 64, 4, 2}, {128, 16, 4, 4}};
+constexpr Shape kShapes[] = {{256, 256, 1, 1.55, 1.55, 1.5, 1.5, 9},
+                             {128, 128, 2, 0.95, 0.75, 1.13, 0.85, 7},
+                             {128, 64, 2, 0.8, 0.6, 0.9, 0.7, 6},
+                             {128, 16, 4, 0.8, 0.4, 0.8, 0.4, 5}};
 
-int pick_shape(int64_t np, int64_t nq, int cus) {
+double product_us(int shape, bool tr, int64_t np, int64_t nq, int64_t k, int parts, int cus) {
+  const Shape& s = kShapes[shape];
+  const int64_t wgs = (np + s.tp - 1) / s.tp * ((nq + s.tq - 1) / s.tq) * parts, slots = cus * s.slots;
+  const int64_t chunks = ((k + kChunk - 1) / kChunk + parts - 1) / parts, left = wgs % slots;
+  const double full = tr ? s.full_tr : s.full, alone = tr ? s.alone_tr : s.alone;
+  return wgs / slots * (chunks * full + s.rest) +
+         (left ? chunks * (left <= cus ? alone : full) + s.rest : 0.0);
+}
+
+int pick_shape(bool tr, int64_t np, int64_t nq, int64_t k, int cus) {
   if (nq <= 16) return 3;
   if (nq <= 64) return 2;
-  const int64_t big = ((np + 255) / 256) * ((nq + 255) / 256);
-  return nq <= 128 || big * 4 < cus * 3 ? 1 : 0;
+  return nq <= 128 || product_us(1, tr, np, nq, k, 1, cus) < product_us(0, tr, np, nq, k, 1, cus);
 }
 
 template <int DT, bool PT, bool QT, int MODE>
@@ -548,12 +743,12 @@ struct StatPlan {
   int shape, parts;
   size_t part_bytes, bytes;
 };
-StatPlan stat_plan(int64_t rows, int vocab, int cus) {
+StatPlan stat_plan(int64_t rows, int K, int vocab, int cus) {
   StatPlan p{};
   p.rows = std::min(rows, kStatRows);
-  p.shape = pick_shape(vocab, p.rows, cus);
+  p.shape = pick_shape(false, vocab, p.rows, K, cus);
   const Shape s = kShapes[p.shape];
-  p.parts = (vocab + s.tp - 1) / s.tp * s.wp;
+  p.parts = (vocab + s.tp - 1) / s.tp;
   p.part_bytes = up256((size_t)p.parts * p.rows * 4);
   p.bytes = 3 * p.part_bytes + up256(p.rows * 4);
   return p;
@@ -562,41 +757,35 @@ StatPlan stat_plan(int64_t rows, int vocab, int cus) {
 struct GradPlan {
   int64_t piece;  // tokens of the vocabulary at once
   int gshape, xshape, wshape, parts;
-  bool acc;
-  size_t at_scale, at_undo, at_top, at_x, at_g, at_acc, bytes;
+  size_t at_scale, at_undo, at_lost, at_top, at_x, at_g, at_acc;
+  size_t at_key, at_place, at_start, at_sort, bytes;
 };
 GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
   GradPlan p{};
   const int64_t v256 = ((int64_t)vocab + 255) / 256 * 256;
   p.piece = std::min(v256, std::max<int64_t>(256, kMostG / (rows * 2) / 256 * 256));
-  p.gshape = pick_shape(std::min<int64_t>(p.piece, vocab), rows, cus);
-  p.xshape = pick_shape(K, rows, cus);
-  p.wshape = (int64_t)((K + 255) / 256) * ((p.piece + 255) / 256) * 4 < cus * 3 ? 1 : 0;
+  const int64_t most = std::min<int64_t>(p.piece, vocab);
+  p.gshape = pick_shape(false, most, rows, K, cus);
+  p.wshape = product_us(1, true, K, most, rows, 1, cus) < product_us(0, true, K, most, rows, 1, cus);
   p.parts = 1;
   if (gx) {
-    const int64_t chunks = p.piece / kChunk;
+    const int64_t chunks = (most + kChunk - 1) / kChunk;
+    const int least = rows <= 16 ? 3 : rows <= 64 ? 2 : rows <= 128 ? 1 : 0;
     double best = 0;
-    for (int sh = p.xshape; sh <= std::max(1, p.xshape); ++sh) {
-      const Shape s = kShapes[sh];
-      const int64_t tiles = (K + s.tp - 1) / s.tp * ((rows + s.tq - 1) / s.tq);
-      const int64_t slots = (int64_t)cus * s.slots;
-      for (int n = 1; n <= 64 && n * 4 <= std::max<int64_t>(4, chunks); ++n) {
+    for (int shape = least; shape <= std::max(1, least); ++shape)
+      for (int n = 1; n <= 64 && n <= chunks; ++n) {
         if (n > 1 && (int64_t)n * rows * K * 4 > kMostG) break;
-        // chunks in a row, each costing its tile's products; parts their sums' traffic
-        const double t = (double)((tiles * n + slots - 1) / slots) * ((chunks + n - 1) / n) *
-                             (s.tp * s.tq * s.slots / 65536.0 + 0.05) +
-                         (n > 1 ? n * (double)rows * K * 8 / 4e6 : 0.0);
-        if (best == 0 || t < best) {
-          best = t;
+        // and the parts' sums, written and read at 5 TB/s
+        const double us = product_us(shape, true, K, rows, most, n, cus) + n * (double)rows * K * 8 / 5e6;
+        if (best == 0 || us < best) {
+          best = us;
           p.parts = n;
-          p.xshape = sh;
+          p.xshape = shape;
         }
       }
-    }
+    const int64_t per = (chunks + p.parts - 1) / p.parts;
+    p.parts = (int)((chunks + per - 1) / per);
   }
-  const int64_t per = (p.piece / kChunk + p.parts - 1) / p.parts;
-  p.parts = (int)((p.piece / kChunk + per - 1) / per);
-  p.acc = gx && (p.parts > 1 || p.piece < v256);
   size_t at = 0;
   const auto take = [&](size_t n) {
     const size_t was = at;
@@ -605,10 +794,17 @@ GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
   };
   p.at_scale = take(rows * 4);
   p.at_undo = take(rows * 4);
+  p.at_lost = take(rows * 4);
   p.at_top = take(4);
   p.at_x = take(gw ? (size_t)rows * ((K + 7) / 8) * 16 : 0);
   p.at_g = take((size_t)rows * p.piece * 2);
-  p.at_acc = take(p.acc ? (size_t)p.parts * rows * K * 4 : 0);
+  p.at_acc = take(gx ? (size_t)p.parts * rows * K * 4 : 0);
+  if (gw) {
+    p.at_key = take(rows * 4);
+    p.at_place = take(rows * 4);
+    p.at_start = take(((size_t)vocab / 128 + 2) * 4);
+    p.at_sort = take(fb_gpu::sort_bytes(rows, vocab));
+  }
   p.bytes = at;
   return p;
 }
@@ -643,7 +839,7 @@ int run_stats(ProductArgs a, const StatPlan& p, int64_t rows, int32_t vocab, flo
     b.given = reinterpret_cast<float*>(ws + 3 * p.part_bytes);
     const int st = launch_product<DT, false, false, kStats>(b, p.shape, 1, hs);
     if (st != FB_OK) return st;
-    hipLaunchKernelGGL(head_join, dim3((b.nq + 15) / 16), dim3(256), 0, hs, b.pm, b.pz, b.pw, p.parts,
+    hipLaunchKernelGGL(head_join, dim3((b.nq + 15) / 16), dim3(1024), 0, hs, b.pm, b.pz, b.pw, p.parts,
                        b.nq, b.given, b.token, vocab, logprob + r, entropy + r,
                        stats ? stats + 2 * r : nullptr);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
@@ -656,6 +852,7 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
              void* grad_x, void* grad_w, uint8_t* ws, hipStream_t hs) {
   float* const scale = reinterpret_cast<float*>(ws + p.at_scale);
   float* const undo = reinterpret_cast<float*>(ws + p.at_undo);
+  float* const lost = reinterpret_cast<float*>(ws + p.at_lost);
   float* const top = reinterpret_cast<float*>(ws + p.at_top);
   uint8_t* const xs = ws + p.at_x;
   float* const acc = reinterpret_cast<float*>(ws + p.at_acc);
@@ -664,9 +861,20 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
     hipLaunchKernelGGL(head_top, dim3(1), dim3(1024), 0, hs, in.token, vocab, in.g_logprob,
                        in.g_entropy, (int)rows, top);
   hipLaunchKernelGGL(head_rows<DT>, dim3((unsigned)rows), dim3(256), 0, hs, in.q, in.ldq, K8,
-                     in.token, vocab, in.g_logprob, in.g_entropy, top, scale, undo,
+                     in.token, vocab, in.g_logprob, in.g_entropy, top, scale, undo, lost,
                      grad_w ? xs : nullptr);
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+  unsigned* const key = reinterpret_cast<unsigned*>(ws + p.at_key);
+  unsigned* const place = reinterpret_cast<unsigned*>(ws + p.at_place);
+  unsigned* const start = reinterpret_cast<unsigned*>(ws + p.at_start);
+  const int starts = (vocab + 127) / 128;
+  if (grad_w) {
+    const int st = fb_gpu::sort_tokens(in.token, rows, vocab, key, place, nullptr, 0, ws + p.at_sort, hs);
+    if (st != FB_OK) return st;
+    hipLaunchKernelGGL(head_starts, dim3((unsigned)(rows / 256 + 1)), dim3(256), 0, hs, key, (int)rows,
+                       vocab, starts, start);
+    if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
+  }
   for (int64_t v = 0; v < vocab; v += p.piece) {
     const int nv = (int)std::min<int64_t>(p.piece, vocab - v);
     ProductArgs g = in;
@@ -679,6 +887,7 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
     g.g = reinterpret_cast<uint16_t*>(ws + p.at_g);
     g.ldg = ((int64_t)nv + 63) / 64 * 64;
     g.vocab = vocab;
+    g.lost = lost;
     int st = launch_product<DT, false, false, kGradient>(g, p.gshape, 1, hs);
     if (st != FB_OK) return st;
     if (grad_x) {
@@ -690,10 +899,8 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
       b.ldq = g.ldg;
       b.nq = (int)rows;
       b.k = nv;
-      b.out = grad_x;
-      b.acc = p.acc ? acc : nullptr;
+      b.acc = acc;
       b.add = v > 0;
-      b.row_scale = undo;
       st = launch_product<DT, true, false, kProduct>(b, p.xshape, p.parts, hs);
       if (st != FB_OK) return st;
     }
@@ -708,15 +915,22 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
       b.k = (int)rows;
       b.out = static_cast<uint8_t*>(grad_w) + v * K * 2;
       b.out_scale = DT == FB_DT_F16 ? top : nullptr;
+      b.v0 = (int)v;
+      b.key = key;
+      b.place = place;
+      b.start = start;
+      b.starts = starts;
+      b.lost = lost;
       st = launch_product<DT, true, true, kProduct>(b, p.wshape, 1, hs);
       if (st != FB_OK) return st;
     }
   }
-  if (p.acc) {
+  if (grad_x) {
     const int64_t n = ((int64_t)rows * K + 1023) / 1024;
     if (n > (1 << 23)) return FB_ERR_SHAPE;
     hipLaunchKernelGGL(head_sum<DT>, dim3((unsigned)n), dim3(256), 0, hs, acc, p.parts, (int)rows, K,
-                       undo, static_cast<uint16_t*>(grad_x));
+                       undo, lost, in.token, vocab, reinterpret_cast<const uint16_t*>(in.p), in.ldp,
+                       static_cast<uint16_t*>(grad_x));
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
   return FB_OK;
@@ -728,7 +942,7 @@ extern "C" {
 
 size_t fb_head_logprobs_workspace_bytes(int64_t rows, int32_t K, int32_t vocab) {
   if (rows < 1 || rows > kMostRows || K < 1 || vocab < 1) return 0;
-  return stat_plan(rows, vocab, fb_gpu::cu_count()).bytes;
+  return stat_plan(rows, K, vocab, fb_gpu::cu_count()).bytes;
 }
 
 int fb_head_logprobs(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int32_t dtype,
@@ -741,7 +955,7 @@ int fb_head_logprobs(const void* x, int64_t x_stride, const void* w, int64_t w_s
   if (bad_align({x, w}, 15) || bad_align({token}, 7) || bad_align({logprob, entropy, stats}, 3) ||
       bad_align({ws}, 255))
     return FB_ERR_ALIGN;
-  const StatPlan p = stat_plan(rows, vocab, fb_gpu::cu_count());
+  const StatPlan p = stat_plan(rows, K, vocab, fb_gpu::cu_count());
   if (ws_bytes < p.bytes) return FB_ERR_WORKSPACE;
   ProductArgs a{};
   a.p = static_cast<const uint8_t*>(w);

@@ -17,6 +17,7 @@
 #include <cstdint>
 
 #include "fourbit.h"
+#include "fourbit_rows.h"
 
 namespace fb_gpu {
 __attribute__((visibility("hidden"))) int cu_count();
@@ -24,80 +25,16 @@ __attribute__((visibility("hidden"))) int cu_count();
 
 namespace {
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));  // rows of odd widths begin anywhere
-
+// load and store of a vector that may be fp32 instead.
 template <int DT>
-struct Of;
-template <>
-struct Of<FB_DT_F32> {
-  using T = float;
-  static constexpr int V = 4;
-};
-template <>
-struct Of<FB_DT_F16> {
-  using T = _Float16;
-  static constexpr int V = 8;
-};
-template <>
-struct Of<FB_DT_BF16> {
-  using T = __bf16;
-  static constexpr int V = 8;
-};
-
-// V values from p on, of which the first `n` are there (0 beyond them).
-template <int DT>
-__device__ inline void load(const void* p, int64_t at, int n, float (&o)[Of<DT>::V]) {
-  using T = typename Of<DT>::T;
+__device__ inline void load_vec(const void* p, int f32, int64_t from, int at, int n,
+                                float (&o)[Of<DT>::V]) {
   constexpr int V = Of<DT>::V;
-  const T* s = static_cast<const T*>(p) + at;
-  if (n >= V) {
-    const u32x4 w = *reinterpret_cast<const u32x4_any*>(s);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if constexpr (DT == FB_DT_F32) {
-        const unsigned u = w[i];
-        o[i] = __builtin_bit_cast(float, u);
-      } else {
-        const unsigned u = w[i / 2];
-        if constexpr (DT == FB_DT_F16)
-          o[i] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u >> (16 * (i & 1))));
-        else
-          o[i] = __builtin_bit_cast(float, i & 1 ? u & 0xFFFF0000u : u << 16);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = i < n ? (float)s[i] : 0.f;
-  }
-}
-template <int DT>
-__device__ inline void store(void* p, int64_t at, int n, const float (&v)[Of<DT>::V]) {
-  using T = typename Of<DT>::T;
-  constexpr int V = Of<DT>::V;
-  T* d = static_cast<T*>(p) + at;
-  if (n >= V) {
-    T o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = (T)v[i];
-    u32x4 w;
-    __builtin_memcpy(&w, o, 16);
-    *reinterpret_cast<u32x4_any*>(d) = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) d[i] = (T)v[i];
-  }
-}
-// The same of a vector that may be fp32 instead.
-template <int DT>
-__device__ inline void load_vec(const void* p, int f32, int64_t at, int n, float (&o)[Of<DT>::V]) {
-  constexpr int V = Of<DT>::V;
-  if (DT == FB_DT_F32 || !f32) return load<DT>(p, at, n, o);
+  if (DT == FB_DT_F32 || !f32) return load<DT>(p, from, at, n, o);
 #pragma unroll
   for (int h = 0; h < V; h += 4) {
     float v[4];
-    load<FB_DT_F32>(p, at + h, n - h, v);
+    load<FB_DT_F32>(p, from, at + h, n - h, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[h + i] = v[i];
   }
@@ -110,6 +47,16 @@ __device__ inline void store_vec(void* p, int f32, int64_t at, int n, const floa
   for (int h = 0; h < V; h += 4) {
     const float v[4] = {o[h], o[h + 1], o[h + 2], o[h + 3]};
     store<FB_DT_F32>(p, at + h, n - h, v);
+  }
+}
+
+// V fp32 values to p[at] on, of d.
+template <int V>
+__device__ inline void store_part(float* p, int at, int d, const float (&v)[V]) {
+#pragma unroll
+  for (int h = 0; h < V; h += 4) {
+    const float o[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+    store<FB_DT_F32>(p, at + h, d - at - h, o);
   }
 }
 
@@ -174,19 +121,26 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * T + t) * V;
-    load_vec<DT>(a.n.weight, a.wf32, at, d - at, w[j]);
-    if (a.n.branch_weight) load_vec<DT>(a.n.branch_weight, a.bf32, at, d - at, wb[j]);
+    load_vec<DT>(a.n.weight, a.wf32, 0, at, d - at, w[j]);
+    if (a.n.branch_weight) load_vec<DT>(a.n.branch_weight, a.bf32, 0, at, d - at, wb[j]);
   }
   const float inv = 1.f / (float)d;
   for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.n.rows; r0 += (int64_t)gridDim.x * G) {
     const int64_t r = min(r0 + group, a.n.rows - 1);  // all groups take part in the barriers
     const bool mine = r0 + group < a.n.rows;
     float x[NV][V], b[NV][V], r1 = 0.f;
+    u32x4 xr[NV], br[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      load<DT>(a.n.x, r * a.n.x_stride + at, d - at, x[j]);
-      if (a.n.branch) load<DT>(a.n.branch, r * a.n.branch_stride + at, d - at, b[j]);
+      xr[j] = raw<DT>(a.n.x, r * a.n.x_stride, at, d - at);
+      if (a.n.branch) br[j] = raw<DT>(a.n.branch, r * a.n.branch_stride, at, d - at);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = (j * T + t) * V;
+      unpack<DT>(settled<DT>(xr[j], at, d - at), x[j]);
+      if (a.n.branch) unpack<DT>(settled<DT>(br[j], at, d - at), b[j]);
     }
     if (a.n.branch) {
       if (a.n.branch_weight) {
@@ -207,7 +161,7 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
       for (int j = 0; j < NV; ++j) {
         const int at = (j * T + t) * V;
         float g[V];
-        if (a.n.gate) load_vec<DT>(a.n.gate, a.gf32, g0 + at, d - at, g);
+        if (a.n.gate) load_vec<DT>(a.n.gate, a.gf32, g0, at, d - at, g);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           x[j][i] = __builtin_fmaf(a.n.gate ? a.n.scale * g[i] : a.n.scale, b[j][i], x[j][i]);
@@ -237,10 +191,31 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
   }
 }
 
+// 16 bytes of a row's values, or the two pieces that as many take in fp32.
+struct Raw2 {
+  u32x4 lo, hi;
+};
+template <int DT>
+__device__ inline Raw2 raw_vec(const void* p, int f32, int64_t from, int at, int n) {
+  if (DT == FB_DT_F32 || !f32) return {raw<DT>(p, from, at, n), u32x4{0, 0, 0, 0}};
+  return {raw<FB_DT_F32>(p, from, at, n), raw<FB_DT_F32>(p, from, at + 4, n - 4)};
+}
+template <int DT>
+__device__ inline void unpack_vec(const Raw2& r, int f32, int at, int n, float (&o)[Of<DT>::V]) {
+  if (DT == FB_DT_F32 || !f32) return unpack<DT>(settled<DT>(r.lo, at, n), o);
+  const u32x4 lo = settled<FB_DT_F32>(r.lo, at, n), hi = settled<FB_DT_F32>(r.hi, at + 4, n - 4);
+#pragma unroll
+  for (int i = 0; i < Of<DT>::V; ++i) {
+    const unsigned u = i < 4 ? lo[i & 3] : hi[i & 3];
+    o[i] = __builtin_bit_cast(float, u);
+  }
+}
+
 // A unit is the rows_per_unit consecutive rows of a group of threads, which keeps their sums for the
 // weights and, over runs of rows that share a gate, for the gate.  A gate whose rows are all one
 // unit's is written; else the unit leaves its part, in place 0 where the gate's first row of it is the
-// unit's first, in place 1 otherwise (its last gate).
+// unit's first, in place 1 otherwise (its last gate).  A row is asked for while the one before it is
+// worked on, and kept as it came: what is needed again after the sums is unpacked again.
 template <int DT, int T, int NV>
 __global__ __launch_bounds__(kBlock<T>) void norm_grad_kernel(NormArgs a) {
   constexpr int V = Of<DT>::V, G = kBlock<T> / T;
@@ -250,119 +225,127 @@ __global__ __launch_bounds__(kBlock<T>) void norm_grad_kernel(NormArgs a) {
   const int64_t first = (int64_t)unit * a.rows_per_unit;
   const int64_t end = min(first + a.rows_per_unit, a.n.rows);
   const bool branch = a.n.branch, post = a.n.branch_weight, gate = a.n.gate;
-  float sw[NV][V], swb[NV][V], sg[NV][V];
+  if (first >= end) return;  // the whole group
+  float sw[NV][V], swb[NV][V], sg[NV][V], w[NV][V], wb[NV][V];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+  for (int j = 0; j < NV; ++j) {
+    const int at = (j * T + t) * V;
+    load_vec<DT>(a.n.weight, a.wf32, 0, at, d - at, w[j]);
+    if (post) load_vec<DT>(a.n.branch_weight, a.bf32, 0, at, d - at, wb[j]);
 #pragma unroll
     for (int i = 0; i < V; ++i) sw[j][i] = swb[j][i] = sg[j][i] = 0.f;
+  }
   const float inv = 1.f / (float)d;
   int64_t gi = gate ? first / a.n.gate_rows : 0;
+  int64_t left = gate ? (gi + 1) * a.n.gate_rows - first : 0;  // rows of this gate from here on
   int turn = 0;
-  for (int64_t k = 0; k < a.rows_per_unit; ++k) {
-    const int64_t r = first + k;
-    if (r >= end) break;  // the same for the whole group
-    const float r1 = a.stats[2 * r], r2 = a.stats[2 * r + 1];
-    float x[NV][V], b[NV][V], gy[NV][V], u[NV][V];  // u: dh + r2 dn
-    float s[3] = {0.f, 0.f, 0.f};
+  u32x4 x[NV], b[NV], gy[NV], gh[NV];
+  Raw2 g[NV];
+  float r1, r2;
+  const auto fetch = [&](int64_t r, int64_t of) {
+    r1 = a.stats[2 * r];
+    r2 = a.stats[2 * r + 1];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      load<DT>(a.n.x, r * a.n.x_stride + at, d - at, x[j]);
-      if (branch) load<DT>(a.n.branch, r * a.n.branch_stride + at, d - at, b[j]);
-      if (a.dy) load<DT>(a.dy, r * d + at, d - at, gy[j]);
-      if (a.dh) load<DT>(a.dh, r * d + at, d - at, u[j]);
+      x[j] = raw<DT>(a.n.x, r * a.n.x_stride, at, d - at);
+      if (branch) b[j] = raw<DT>(a.n.branch, r * a.n.branch_stride, at, d - at);
+      if (gate) g[j] = raw_vec<DT>(a.n.gate, a.gf32, of * d, at, d - at);
+      gy[j] = gh[j] = u32x4{0, 0, 0, 0};
+      if (a.dy) gy[j] = raw<DT>(a.dy, r * d, at, d - at);
+      if (a.dh) gh[j] = raw<DT>(a.dh, r * d, at, d - at);
     }
+  };
+  fetch(first, gi);
+  for (int64_t r = first; r < end; ++r) {
+    float n[NV][V], u[NV][V], nb[NV][V], f[NV][V];  // u: dh + r2 dn, f: scale gate
+    float s[3] = {0.f, 0.f, 0.f};
+    const float ra = r1, rb = r2;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      float w[V], wb[V], g[V];
-      load_vec<DT>(a.n.weight, a.wf32, at, d - at, w);
-      if (post) load_vec<DT>(a.n.branch_weight, a.bf32, at, d - at, wb);
-      if (gate) load_vec<DT>(a.n.gate, a.gf32, gi * d + at, d - at, g);
+      float xx[V], dy[V];
+      unpack<DT>(settled<DT>(x[j], at, d - at), xx);
+      unpack<DT>(settled<DT>(gy[j], at, d - at), dy);
+      unpack<DT>(settled<DT>(gh[j], at, d - at), u[j]);
+      if (branch) {
+        unpack<DT>(settled<DT>(b[j], at, d - at), nb[j]);
+        if (gate) unpack_vec<DT>(g[j], a.gf32, at, d - at, f[j]);
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         float q = 0.f;
         if (branch) {
-          if (post) b[j][i] *= r1;  // n_b
-          const float f = gate ? a.n.scale * g[i] : a.n.scale;
-          q = post ? f * wb[i] * b[j][i] : f * b[j][i];
+          if (post) nb[j][i] *= ra;
+          f[j][i] = gate ? a.n.scale * f[j][i] : a.n.scale;
+          q = post ? f[j][i] * wb[j][i] * nb[j][i] : f[j][i] * nb[j][i];
         }
-        const float n = (x[j][i] + q) * r2;
-        const float dy = a.dy ? gy[j][i] : 0.f, dn = dy * w[i];
-        u[j][i] = __builtin_fmaf(r2, dn, a.dh ? u[j][i] : 0.f);
-        x[j][i] = n;
-        sw[j][i] = __builtin_fmaf(dy, n, sw[j][i]);
-        s[0] = __builtin_fmaf(dn, n, s[0]);
-        if (post) {
-          s[1] = __builtin_fmaf(u[j][i], q, s[1]);
-          s[2] = __builtin_fmaf(n, q, s[2]);
-        }
+        n[j][i] = (xx[i] + q) * rb;
+        const float dn = dy[i] * w[j][i];
+        u[j][i] = __builtin_fmaf(rb, dn, u[j][i]);
+        sw[j][i] = __builtin_fmaf(dy[i], n[j][i], sw[j][i]);
+        s[0] = __builtin_fmaf(dn, n[j][i], s[0]);
+        s[1] = __builtin_fmaf(u[j][i], q, s[1]);
+        s[2] = __builtin_fmaf(n[j][i], q, s[2]);
       }
     }
+    const int64_t of = gi;
+    const bool flush = gate && (--left == 0 || r + 1 == end);
+    if (gate && left == 0) {
+      ++gi;
+      left = a.n.gate_rows;
+    }
+    if (r + 1 < end) fetch(r + 1, gi);
     group_sum<T>(s, red[turn ^= 1]);
-    const float m1 = s[0] * inv * r2;               // dx = u - m1 n
-    const float m2 = (s[1] - m1 * s[2]) * inv;      // mean of wb g t n_b
+    const float m1 = s[0] * inv * rb;           // dx = u - m1 n
+    const float m2 = (s[1] - m1 * s[2]) * inv;  // mean of wb g t n_b
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = u[j][i] = __builtin_fmaf(-m1, x[j][i], u[j][i]);
-      if (a.dx) store<DT>(a.dx, r * d + at, d - at, o);
+      for (int i = 0; i < V; ++i) u[j][i] = __builtin_fmaf(-m1, n[j][i], u[j][i]);
+      if (a.dx) store<DT>(a.dx, r * d + at, d - at, u[j]);
       if (branch) {
-        float wb[V], g[V];
-        if (post) load_vec<DT>(a.n.branch_weight, a.bf32, at, d - at, wb);
-        if (gate) load_vec<DT>(a.n.gate, a.gf32, gi * d + at, d - at, g);
+        float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float tt = a.n.scale * u[j][i], nb = b[j][i];
-          sg[j][i] = __builtin_fmaf(tt, post ? wb[i] * nb : nb, sg[j][i]);
-          const float f = gate ? tt * g[i] : tt;
-          o[i] = f;
+          if (gate)
+            sg[j][i] = __builtin_fmaf(a.n.scale * u[j][i], post ? wb[j][i] * nb[j][i] : nb[j][i], sg[j][i]);
+          const float tf = u[j][i] * f[j][i];  // g t
+          o[i] = tf;
           if (post) {
-            swb[j][i] = __builtin_fmaf(f, nb, swb[j][i]);
-            o[i] = r1 * __builtin_fmaf(-m2, nb, f * wb[i]);
+            swb[j][i] = __builtin_fmaf(tf, nb[j][i], swb[j][i]);
+            o[i] = ra * __builtin_fmaf(-m2, nb[j][i], tf * wb[j][i]);
           }
         }
         if (a.db) store<DT>(a.db, r * d + at, d - at, o);
       }
     }
-    if (gate) {
-      const int64_t g0 = gi * a.n.gate_rows, g1 = min(g0 + a.n.gate_rows, a.n.rows);
-      if (r + 1 == g1 || r + 1 == end) {
-        const bool whole = g0 >= first && g1 <= end;
-        if (a.dgate) {
+    if (flush) {
+      const int64_t g0 = of * a.n.gate_rows, g1 = min(g0 + a.n.gate_rows, a.n.rows);
+      const bool whole = g0 >= first && g1 <= end;
+      if (a.dgate) {
 #pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const int at = (j * T + t) * V;
-            if (whole) {
-              store_vec<DT>(a.dgate, a.gf32, gi * d + at, d - at, sg[j]);
-            } else {
-              float* const p = a.pg + ((int64_t)unit * 2 + (g0 > first)) * d;
-#pragma unroll
-              for (int i = 0; i < V; ++i)
-                if (at + i < d) p[at + i] = sg[j][i];
-            }
+        for (int j = 0; j < NV; ++j) {
+          const int at = (j * T + t) * V;
+          if (whole) {
+            store_vec<DT>(a.dgate, a.gf32, of * d + at, d - at, sg[j]);
+          } else {
+            store_part(a.pg + ((int64_t)unit * 2 + (g0 > first)) * d, at, d, sg[j]);
           }
         }
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) sg[j][i] = 0.f;
-        gi += r + 1 == g1;
       }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) sg[j][i] = 0.f;
     }
   }
-  if (first >= a.n.rows) return;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * T + t) * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (at + i < d) {
-        if (a.dw) a.pw[(int64_t)unit * d + at + i] = sw[j][i];
-        if (a.dwb) a.pwb[(int64_t)unit * d + at + i] = swb[j][i];
-      }
+    if (a.dw) store_part(a.pw + (int64_t)unit * d, at, d, sw[j]);
+    if (a.dwb) store_part(a.pwb + (int64_t)unit * d, at, d, swb[j]);
   }
 }
 
@@ -474,11 +457,17 @@ Split split_of(int width) {
     if (width <= t * 16) return {t, 16};
   return {1024, 32};
 }
+// The gradient keeps three sums for each value: half as many of them a thread.
+Split grad_split_of(int width) {
+  for (int t = 64; t <= 512; t *= 2)
+    if (width <= t * 8) return {t, 8};
+  if (width <= 8192) return {512, 16};
+  return {1024, width <= 16384 ? 16 : 32};
+}
 
-// Units of the gradient: two rounds of workgroups at most, or the parts' sums cost as much as rows.
+// Units of the gradient: as many as fill the device once, for each leaves sums to be added.
 int rows_per_unit(const fb_norm_t* n, int cus) {
-  const Split s = split_of(n->width);
-  const int64_t units = (int64_t)cus * std::max(1, 512 / s.threads);
+  const int64_t units = (int64_t)cus * std::min(8, std::max(1, 1024 / grad_split_of(n->width).threads));
   return (int)std::max<int64_t>(1, (n->rows + units - 1) / units);
 }
 
@@ -498,43 +487,49 @@ NormPlan norm_plan(const fb_norm_t* n, int cus) {
   return p;
 }
 
-template <int DT, typename F>
-int with_split(int width, F&& go) {
-  constexpr int V = Of<DT>::V;
-  const Split s = split_of(width);
-  if (s.values == 8) return go(std::integral_constant<int, 64>{}, std::integral_constant<int, 8 / V>{});
-  if (s.values == 32)
-    return go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 32 / V>{});
-  constexpr std::integral_constant<int, 16 / V> nv{};
-  switch (s.threads) {
-    case 64: return go(std::integral_constant<int, 64>{}, nv);
-    case 128: return go(std::integral_constant<int, 128>{}, nv);
-    case 256: return go(std::integral_constant<int, 256>{}, nv);
-    case 512: return go(std::integral_constant<int, 512>{}, nv);
-    default: return go(std::integral_constant<int, 1024>{}, nv);
-  }
-}
-
+template <int T, int VALUES, int DT>
+struct Config {
+  static constexpr int kThreads = T, kVecs = VALUES / Of<DT>::V;
+};
 template <int DT>
 int run_norm(const NormArgs& a, hipStream_t hs) {
-  return with_split<DT>(a.n.width, [&](auto t, auto nv) {
-    constexpr int T = decltype(t)::value, NV = decltype(nv)::value, G = kBlock<T> / T;
+  const auto go = [&](auto c) {
+    constexpr int T = decltype(c)::kThreads, NV = decltype(c)::kVecs, G = kBlock<T> / T;
     const int64_t groups = (a.n.rows + G - 1) / G;
     const int64_t most = (int64_t)fb_gpu::cu_count() * (2048 / kBlock<T>);
     hipLaunchKernelGGL((norm_kernel<DT, T, NV>), dim3((unsigned)std::min(groups, most)),
                        dim3(kBlock<T>), 0, hs, a);
     return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
-  });
+  };
+  const Split s = split_of(a.n.width);
+  if (s.values == 8) return go(Config<64, 8, DT>{});
+  if (s.values == 32) return go(Config<1024, 32, DT>{});
+  switch (s.threads) {
+    case 64: return go(Config<64, 16, DT>{});
+    case 128: return go(Config<128, 16, DT>{});
+    case 256: return go(Config<256, 16, DT>{});
+    case 512: return go(Config<512, 16, DT>{});
+    default: return go(Config<1024, 16, DT>{});
+  }
 }
 
 template <int DT>
 int run_norm_grad(const NormArgs& a, hipStream_t hs) {
-  const int st = with_split<DT>(a.n.width, [&](auto t, auto nv) {
-    constexpr int T = decltype(t)::value, NV = decltype(nv)::value, G = kBlock<T> / T;
+  const auto go = [&](auto c) {
+    constexpr int T = decltype(c)::kThreads, NV = decltype(c)::kVecs, G = kBlock<T> / T;
     hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV>), dim3((unsigned)((a.units + G - 1) / G)),
                        dim3(kBlock<T>), 0, hs, a);
     return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
-  });
+  };
+  const Split s = grad_split_of(a.n.width);
+  int st;
+  if (s.values == 32) st = go(Config<1024, 32, DT>{});
+  else if (s.threads == 1024) st = go(Config<1024, 16, DT>{});
+  else if (s.values == 16) st = go(Config<512, 16, DT>{});
+  else if (s.threads == 512) st = go(Config<512, 8, DT>{});
+  else if (s.threads == 256) st = go(Config<256, 8, DT>{});
+  else if (s.threads == 128) st = go(Config<128, 8, DT>{});
+  else st = go(Config<64, 8, DT>{});
   if (st != FB_OK) return st;
   int64_t gates = 0;
   if (a.dgate && a.n.gate_rows > 1) gates = (a.n.rows + a.n.gate_rows - 1) / a.n.gate_rows;
