@@ -49,7 +49,8 @@ EXPORTED = (
     "fb_embed", "fb_embed_grad", "fb_embed_grad_workspace_bytes",
     "fb_residual_norm", "fb_residual_norm_grad", "fb_residual_norm_grad_workspace_bytes",
     "fb_head_logprobs", "fb_head_logprobs_workspace_bytes", "fb_head_logprobs_grad",
-    "fb_head_logprobs_grad_workspace_bytes",
+    "fb_head_logprobs_grad_workspace_bytes", "fb_packed_head_grad",
+    "fb_packed_head_grad_workspace_bytes",
 )
 
 
@@ -166,6 +167,8 @@ def lib() -> ctypes.CDLL:
         "fb_head_logprobs_workspace_bytes": (sz, [i64, i32, i32]),
         "fb_head_logprobs_grad": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i32, i32, vp, vp, vp,
                                                  vp, vp, vp, vp, vp, sz, vp]),
+        "fb_packed_head_grad": (ctypes.c_int, [vp, vp, sp, vp, vp, vp, vp, vp, vp, i32, vp, sz, vp]),
+        "fb_packed_head_grad_workspace_bytes": (sz, [sp]),
         "fb_head_logprobs_grad_workspace_bytes": (sz, [i64, i32, i32, i32, i32]),
     }
     for name, (res, args) in sigs.items():

@@ -24,6 +24,7 @@
 
 #include "fourbit.h"
 #include "fourbit_decode.h"
+#include "fourbit_layout.h"
 #include "fourbit_tokens.h"
 
 namespace fb_gpu {
@@ -55,7 +56,8 @@ struct ProductArgs {
   const int64_t* token;
   int v0;  // p's first row is this token
   // kGradient
-  const float *rowmax, *log2z;  // stats [nq, 2]: the first and the second
+  const float* stats;  // [nq, 2] as head_join writes them, or (three) [nq, 3] as fb_token_logprobs does
+  int three;
   const float *entropy, *g_logprob, *g_entropy, *scale;
   uint16_t* g;
   int64_t ldg;
@@ -434,7 +436,17 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
       const bool any = token >= 0 && token < a.vocab;
       const float g = any && a.g_logprob ? a.g_logprob[r] : 0.f;
       const float ge = ENT ? a.g_entropy[r] : 0.f;
-      const float m = a.rowmax[2 * r], l2z = a.log2z[2 * r], up = a.scale[r];
+      float m, l2z;  // log2 p = (l - m) log2(e) - l2z
+      if (a.three) {
+        // (l - a) log2(e) - R - b, relative to a logit near the largest instead
+        const float off = a.stats[3 * r + 1] * kLn2;
+        m = a.stats[3 * r] + off;
+        l2z = a.stats[3 * r + 2] + __builtin_fmaf(-off, kLog2e, a.stats[3 * r + 1]);
+      } else {
+        m = a.stats[2 * r];
+        l2z = a.stats[2 * r + 1];
+      }
+      const float up = a.scale[r];
       const float all = -up * (g + (ENT ? ge * a.entropy[r] : 0.f));
       const float slope = -up * ge * kLn2;
       const auto value = [&](float l) {
@@ -567,6 +579,39 @@ __global__ __launch_bounds__(256) void head_starts(const unsigned* __restrict__ 
   for (int t = from; t <= to; ++t) start[t] = i;
 }
 
+// A packed weight in 16 bits, [N, K], a block of 16 rows by 512 columns a wave: lane L has row L % 16 of
+// its 128 columns L / 16.  Through LDS, so that rows are written 1 KiB at a time.
+template <int FMT, int DT>
+__global__ __launch_bounds__(256) void head_decode(const uint8_t* __restrict__ w, int N, int K, int spans,
+                                                   int64_t blocks, uint16_t* __restrict__ out) {
+  constexpr int BB = FMT == FB_FMT_GF4 ? fb::kGf4BlockBytes : fb::kE2m1BlockBytes;
+  __shared__ __align__(16) u32x4 rows[4][16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, item = lane >> 4;
+  const int64_t b = (int64_t)blockIdx.x * 4 + wave;
+  if (b >= blocks) return;
+  Rec<FMT> r;
+  load_rec_global<FMT>(w + b * BB, lane, r);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      u32x4 v;
+      if constexpr (FMT == FB_FMT_GF4)
+        v = gf4_decode8(r.nib[c][d], r.t0, r.t1);
+      else
+        v = e2m1_decode8<DT>(r.nib[c][d],
+                             __builtin_bit_cast(float, ((r.t0.x >> (8 * c)) & 0xFFu) << 23));
+      rows[wave][row][(item * 16 + c * 4 + d) ^ row] = v;
+    }
+  asm volatile("" ::: "memory");
+  const int64_t n0 = b / spans * 16;
+  const int col = (int)(b % spans) * 512 + lane * 8;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (n0 + i < N && col < K)
+      *reinterpret_cast<u32x4*>(out + (n0 + i) * K + col) = rows[wave][i][lane ^ i];
+}
+
 // What bounds |G| in row r: 0 where no gradient comes in.
 __device__ inline float row_bound(int64_t r, const int64_t* token, int vocab, const float* g,
                                   const float* ge) {
@@ -650,7 +695,7 @@ __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, i
                                                 const float* __restrict__ lost,
                                                 const int64_t* __restrict__ token, int vocab,
                                                 const uint16_t* __restrict__ w, int64_t ldw,
-                                                uint16_t* __restrict__ out) {
+                                                void* __restrict__ out, int odt) {
   const int64_t n = (int64_t)rows * K, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   const auto value = [](unsigned h) {
     if constexpr (DT == FB_DT_F16) return (float)__builtin_bit_cast(_Float16, (unsigned short)h);
@@ -668,14 +713,14 @@ __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, i
                  l * value(v.y >> 16)};
     }
     s *= undo[r];
-    *reinterpret_cast<uint2*>(out + i) = make_uint2(pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3]));
+    store4(out, i, s, odt);
   } else {
     for (int64_t at = i; at < n && at < i + 4; ++at) {
       const int64_t r = at / K, t = token[r];
       float s = acc[at];
       for (int p = 1; p < parts; ++p) s += acc[p * n + at];
       if (lost[r] != 0.f && t >= 0 && t < vocab) s += lost[r] * value(w[t * ldw + (at - r * K)]);
-      out[at] = (uint16_t)pack2<DT>(s * undo[r], 0.f);
+      store_y(out, at, s * undo[r], odt);
     }
   }
 }
@@ -849,7 +894,7 @@ int run_stats(ProductArgs a, const StatPlan& p, int64_t rows, int32_t vocab, flo
 
 template <int DT>
 int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, int32_t vocab,
-             void* grad_x, void* grad_w, uint8_t* ws, hipStream_t hs) {
+             void* grad_x, int32_t grad_x_dtype, void* grad_w, uint8_t* ws, hipStream_t hs) {
   float* const scale = reinterpret_cast<float*>(ws + p.at_scale);
   float* const undo = reinterpret_cast<float*>(ws + p.at_undo);
   float* const lost = reinterpret_cast<float*>(ws + p.at_lost);
@@ -930,7 +975,7 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
     if (n > (1 << 23)) return FB_ERR_SHAPE;
     hipLaunchKernelGGL(head_sum<DT>, dim3((unsigned)n), dim3(256), 0, hs, acc, p.parts, (int)rows, K,
                        undo, lost, in.token, vocab, reinterpret_cast<const uint16_t*>(in.p), in.ldp,
-                       static_cast<uint16_t*>(grad_x));
+                       grad_x, grad_x_dtype);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
   return FB_OK;
@@ -998,15 +1043,74 @@ int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_
   a.q = static_cast<const uint8_t*>(x);
   a.ldq = x_stride;
   a.token = token;
-  a.rowmax = stats;
-  a.log2z = stats + 1;
+  a.stats = stats;
   a.entropy = entropy;
   a.g_logprob = g_logprob;
   a.g_entropy = g_entropy;
   hipStream_t hs = static_cast<hipStream_t>(stream);
   return dtype == FB_DT_F16
-             ? run_grad<FB_DT_F16>(a, p, rows, K, vocab, grad_x, grad_w, static_cast<uint8_t*>(ws), hs)
-             : run_grad<FB_DT_BF16>(a, p, rows, K, vocab, grad_x, grad_w, static_cast<uint8_t*>(ws), hs);
+             ? run_grad<FB_DT_F16>(a, p, rows, K, vocab, grad_x, dtype, grad_w, static_cast<uint8_t*>(ws),
+                                   hs)
+             : run_grad<FB_DT_BF16>(a, p, rows, K, vocab, grad_x, dtype, grad_w, static_cast<uint8_t*>(ws),
+                                    hs);
+}
+
+size_t fb_packed_head_grad_workspace_bytes(const fb_shape_t* s) {
+  if (!s || s->B < 1 || s->B > kMostRows || fb_validate(s) != FB_OK) return 0;
+  return up256((size_t)s->N * s->K * 2) +
+         grad_plan(s->B, s->K, s->N, true, false, fb_gpu::cu_count()).bytes;
+}
+
+int fb_packed_head_grad(const void* wdev, const void* x, const fb_shape_t* s, const int64_t* token,
+                        const float* stats, const float* entropy, const float* g_logprob,
+                        const float* g_entropy, void* grad_x, int32_t grad_x_dtype, void* ws,
+                        size_t ws_bytes, void* stream) {
+  if (!s || !wdev || !x || !token || !stats || (g_entropy && !entropy) || !grad_x || !ws)
+    return FB_ERR_NULL;
+  int st = fb_validate(s);
+  if (st != FB_OK) return st;
+  if (s->fwht_block) return FB_ERR_FWHT;
+  if (s->x_dtype != FB_DT_F16 && s->x_dtype != FB_DT_BF16) return FB_ERR_DTYPE;
+  if (s->fmt == FB_FMT_GF4 && s->x_dtype != FB_DT_F16) return FB_ERR_DTYPE;
+  if (grad_x_dtype != FB_DT_F16 && grad_x_dtype != FB_DT_BF16 && grad_x_dtype != FB_DT_F32)
+    return FB_ERR_DTYPE;
+  st = head_check(s->x_dtype, s->B, s->K, s->N, s->K, s->K);
+  if (st != FB_OK) return st;
+  if (bad_align({wdev, x, grad_x}, 15) || bad_align({token}, 7) ||
+      bad_align({stats, entropy, g_logprob, g_entropy}, 3) || bad_align({ws}, 255))
+    return FB_ERR_ALIGN;
+  const size_t decoded = up256((size_t)s->N * s->K * 2);
+  const GradPlan p = grad_plan(s->B, s->K, s->N, true, false, fb_gpu::cu_count());
+  if (ws_bytes < decoded + p.bytes) return FB_ERR_WORKSPACE;
+  hipStream_t hs = static_cast<hipStream_t>(stream);
+  const int spans = (s->K / 128 + 3) / 4;
+  const int64_t blocks = (int64_t)((s->N + 15) / 16) * spans;
+  if ((blocks + 3) / 4 > (1 << 23)) return FB_ERR_SHAPE;
+  const auto decode = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((blocks + 3) / 4)), dim3(256), 0, hs,
+                       static_cast<const uint8_t*>(wdev), s->N, s->K, spans, blocks,
+                       static_cast<uint16_t*>(ws));
+    return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
+  };
+  st = s->fmt == FB_FMT_GF4         ? decode(head_decode<FB_FMT_GF4, FB_DT_F16>)
+       : s->x_dtype == FB_DT_F16 ? decode(head_decode<FB_FMT_E2M1, FB_DT_F16>)
+                                 : decode(head_decode<FB_FMT_E2M1, FB_DT_BF16>);
+  if (st != FB_OK) return st;
+  ProductArgs a{};
+  a.p = static_cast<const uint8_t*>(ws);
+  a.ldp = s->K;
+  a.q = static_cast<const uint8_t*>(x);
+  a.ldq = s->K;
+  a.token = token;
+  a.stats = stats;
+  a.three = 1;
+  a.entropy = entropy;
+  a.g_logprob = g_logprob;
+  a.g_entropy = g_entropy;
+  uint8_t* const rest = static_cast<uint8_t*>(ws) + decoded;
+  return s->x_dtype == FB_DT_F16
+             ? run_grad<FB_DT_F16>(a, p, s->B, s->K, s->N, grad_x, grad_x_dtype, nullptr, rest, hs)
+             : run_grad<FB_DT_BF16>(a, p, s->B, s->K, s->N, grad_x, grad_x_dtype, nullptr, rest, hs);
 }
 
 }  // extern "C"

@@ -594,9 +594,13 @@ void want_tokens(const at::Tensor& tokens, const at::Tensor& like) {
        "tokens must be int64 or int32");
 }
 
-at::Tensor embedding_forward(const at::Tensor& w, const at::Tensor& token, double scale) {
-  c10::DeviceGuard guard(w.device());
-  at::Tensor out = at::empty({token.size(0), w.size(1)}, w.options());
+// The shape that is the caller's is given to results where they are made: a view of one that is
+// differentiated would be a node of its own.
+at::Tensor embedding_forward(const at::Tensor& weight, const at::Tensor& token, at::IntArrayRef sizes,
+                             double scale) {
+  c10::DeviceGuard guard(weight.device());
+  const at::Tensor w = as_rows(weight);
+  at::Tensor out = at::empty(sizes, w.options().memory_format(at::MemoryFormat::Contiguous));
   check(fb_embed(w.data_ptr(), row_stride(w), dtype_code(w.scalar_type()), (int32_t)w.size(0),
                  (int32_t)w.size(1), static_cast<const int64_t*>(token.data_ptr()), token.size(0),
                  (float)scale, out.data_ptr(), stream_of(w)));
@@ -605,11 +609,11 @@ at::Tensor embedding_forward(const at::Tensor& w, const at::Tensor& token, doubl
 
 struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& w,
-                            const at::Tensor& token, double scale) {
+                            const at::Tensor& token, const std::vector<int64_t>& sizes, double scale) {
     ctx->save_for_backward({token});
     ctx->saved_data["vocab"] = w.size(0);
     ctx->saved_data["scale"] = scale;
-    return embedding_forward(w, token, scale);
+    return embedding_forward(w, token, sizes, scale);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
@@ -625,7 +629,7 @@ struct TokenEmbedding : torch::autograd::Function<TokenEmbedding> {
                         (int32_t)K, static_cast<const int64_t*>(token.data_ptr()), M,
                         (float)ctx->saved_data["scale"].toDouble(), gw.data_ptr(),
                         ptr_or_null(ws, need), need, stream_of(g)));
-    return {gw, at::Tensor(), at::Tensor()};
+    return {gw, at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
@@ -639,13 +643,12 @@ at::Tensor token_embedding(const at::Tensor& tokens, const at::Tensor& weight, d
        "weight must be [vocab, width], a width of at most 2^20");
   want(std::isfinite(scale), "scale must be finite");
   want(tokens.numel() <= (1 << 30), "too many tokens");
-  const at::Tensor t = flat_tokens(tokens), w = as_rows(weight);
-  const at::Tensor out = at::GradMode::is_enabled() && w.requires_grad()
-                             ? TokenEmbedding::apply(w, t, scale)
-                             : embedding_forward(w, t, scale);
+  const at::Tensor t = flat_tokens(tokens);
   auto sizes = tokens.sizes().vec();
   sizes.push_back(weight.size(1));
-  return out.view(sizes);
+  return at::GradMode::is_enabled() && weight.requires_grad()
+             ? TokenEmbedding::apply(weight, t, sizes, scale)
+             : embedding_forward(weight, t, sizes, scale);
 }
 
 fb_norm_t norm_of(const at::Tensor& x, const at::Tensor& branch, const at::Tensor& gate,
@@ -677,16 +680,34 @@ fb_norm_t norm_of(const at::Tensor& x, const at::Tensor& branch, const at::Tenso
   return n;
 }
 
-// stream, normed, stats of x [rows, width].
-std::vector<at::Tensor> norm_forward(const fb_norm_t& n, const at::Tensor& x, const at::Tensor& branch,
-                                     bool stats) {
+// The inputs of a call as the kernels take them; what is not given is undefined.
+struct NormInputs {
+  at::Tensor x, branch, gate, weight, branch_weight;  // rows, rows, rows, vectors
+  int64_t gate_rows;
+  double scale, eps;
+  fb_norm_t c() const { return norm_of(x, branch, gate, weight, branch_weight, gate_rows, scale, eps); }
+};
+NormInputs norm_inputs(const at::Tensor& x, const std::optional<at::Tensor>& branch,
+                       const std::optional<at::Tensor>& gate, const at::Tensor& weight,
+                       const std::optional<at::Tensor>& branch_weight, int64_t gate_rows, double scale,
+                       double eps) {
+  NormInputs n{as_rows(x), {}, {}, weight.contiguous(), {}, gate_rows, scale, eps};
+  if (branch) n.branch = as_rows(*branch);
+  if (gate) n.gate = gate->reshape({-1, x.size(-1)}).contiguous();
+  if (branch_weight) n.branch_weight = branch_weight->contiguous();
+  return n;
+}
+
+// stream, normed (of x's shape), stats.
+std::vector<at::Tensor> norm_forward(const NormInputs& n, const at::Tensor& x, bool stats) {
   c10::DeviceGuard guard(x.device());
   const auto like = x.options().memory_format(at::MemoryFormat::Contiguous);
-  at::Tensor h = branch.defined() ? at::empty(x.sizes(), like) : x;
+  at::Tensor h = n.branch.defined() ? at::empty(x.sizes(), like) : x;
   at::Tensor y = at::empty(x.sizes(), like);
-  at::Tensor st = stats ? at::empty({x.size(0), 2}, x.options().dtype(at::kFloat)) : at::Tensor();
-  if (x.size(0) == 0) return {h, y, st};
-  check(fb_residual_norm(&n, branch.defined() ? h.data_ptr() : nullptr, y.data_ptr(),
+  at::Tensor st = stats ? at::empty({n.x.size(0), 2}, x.options().dtype(at::kFloat)) : at::Tensor();
+  if (x.numel() == 0) return {h, y, st};
+  const fb_norm_t c = n.c();
+  check(fb_residual_norm(&c, n.branch.defined() ? h.data_ptr() : nullptr, y.data_ptr(),
                          stats ? static_cast<float*>(st.data_ptr()) : nullptr, stream_of(x)));
   return {h, y, st};
 }
@@ -694,20 +715,19 @@ std::vector<at::Tensor> norm_forward(const fb_norm_t& n, const at::Tensor& x, co
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
                                                 const at::Tensor& x,
-                                                const std::optional<at::Tensor>& given_branch,
-                                                const std::optional<at::Tensor>& given_gate,
+                                                const std::optional<at::Tensor>& branch,
+                                                const std::optional<at::Tensor>& gate,
                                                 const at::Tensor& weight,
-                                                const std::optional<at::Tensor>& given_branch_weight,
+                                                const std::optional<at::Tensor>& branch_weight,
                                                 int64_t gate_rows, double scale, double eps) {
-    const at::Tensor branch = given_branch.value_or(at::Tensor()),
-                     gate = given_gate.value_or(at::Tensor()),
-                     branch_weight = given_branch_weight.value_or(at::Tensor());
-    const fb_norm_t n = norm_of(x, branch, gate, weight, branch_weight, gate_rows, scale, eps);
-    const auto r = norm_forward(n, x, branch, true);
-    ctx->save_for_backward({x, branch, gate, weight, branch_weight, r[2]});
+    const NormInputs n = norm_inputs(x, branch, gate, weight, branch_weight, gate_rows, scale, eps);
+    const auto r = norm_forward(n, x, true);
+    ctx->save_for_backward({n.x, n.branch, n.gate, n.weight, n.branch_weight, r[2]});
     ctx->saved_data["gate_rows"] = gate_rows;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["eps"] = eps;
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    if (gate) ctx->saved_data["gate"] = gate->sizes().vec();
     ctx->set_materialize_grads(false);
     // without a branch the stream is x, as a result, so that its gradient is added here, in fp32
     return {r[0], r[1]};
@@ -716,30 +736,32 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
                                                  torch::autograd::variable_list grads) {
     first_derivative("residual_norm has no second derivative");
     const auto s = ctx->get_saved_variables();
-    const at::Tensor &x = s[0], &branch = s[1], &gate = s[2], &weight = s[3], &bw = s[4];
-    const fb_norm_t n = norm_of(x, branch, gate, weight, bw, ctx->saved_data["gate_rows"].toInt(),
-                                ctx->saved_data["scale"].toDouble(),
-                                ctx->saved_data["eps"].toDouble());
+    const NormInputs n{s[0], s[1], s[2], s[3], s[4], ctx->saved_data["gate_rows"].toInt(),
+                       ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble()};
+    const at::Tensor& x = n.x;
     c10::DeviceGuard guard(x.device());
     at::Tensor gh = grads[0], gy = grads[1];
     if (gy.defined()) gy = gy.contiguous();
     if (gh.defined()) gh = gh.contiguous();
     at::Tensor out[5];
-    const at::Tensor* of[5] = {&x, &branch, &gate, &weight, &bw};
-    for (int i = 0, edge = 0; i < 5; ++i)  // autograd counts the inputs that there are
-      if (of[i]->defined() && ctx->needs_input_grad(edge++))
-        out[i] = at::empty(of[i]->sizes(),
-                           of[i]->options().memory_format(at::MemoryFormat::Contiguous));
-    if (x.size(0) == 0)
-      for (at::Tensor& t : out)
-        if (t.defined()) t.zero_();
-    const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-    const size_t need = fb_residual_norm_grad_workspace_bytes(&n);
-    const at::Tensor ws = need ? scratch(need, x) : at::Tensor();
-    if (x.size(0))
-      check(fb_residual_norm_grad(&n, static_cast<const float*>(s[5].data_ptr()), ptr(gh), ptr(gy),
+    const at::Tensor* of[5] = {&n.x, &n.branch, &n.gate, &n.weight, &n.branch_weight};
+    for (int i = 0, edge = 0; i < 5; ++i) {  // autograd counts the inputs that there are
+      if (!of[i]->defined() || !ctx->needs_input_grad(edge++)) continue;
+      const auto sizes = i < 2    ? ctx->saved_data["sizes"].toIntVector()
+                         : i == 2 ? ctx->saved_data["gate"].toIntVector()
+                                  : of[i]->sizes().vec();
+      out[i] = at::empty(sizes, of[i]->options().memory_format(at::MemoryFormat::Contiguous));
+      if (x.size(0) == 0) out[i].zero_();
+    }
+    if (x.size(0)) {
+      const auto ptr = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      const fb_norm_t c = n.c();
+      const size_t need = fb_residual_norm_grad_workspace_bytes(&c);
+      const at::Tensor ws = scratch(need, x);
+      check(fb_residual_norm_grad(&c, static_cast<const float*>(s[5].data_ptr()), ptr(gh), ptr(gy),
                                   ptr(out[0]), ptr(out[1]), ptr(out[3]), ptr(out[4]), ptr(out[2]),
-                                  ptr_or_null(ws, need), need, stream_of(x)));
+                                  ws.data_ptr(), need, stream_of(x)));
+    }
     return {out[0], out[1], out[2], out[3], out[4], at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
@@ -769,14 +791,12 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::
        "scale must be finite, eps finite and not negative");
   const int64_t M = x.numel() / d;
   want(M <= INT32_MAX, "too many rows");
-  at::Tensor b, g;
-  int64_t gate_rows = 1;
   if (branch) {
     want_plain(*branch, x, "branch must be a tensor on x's GPU");
     want(branch->sizes() == x.sizes() && branch->scalar_type() == x.scalar_type(),
          "branch must have x's shape and dtype");
-    b = as_rows(*branch);
   }
+  int64_t gate_rows = 1;
   if (gate) {
     want_plain(*gate, x, "gate must be a tensor on x's GPU");
     want(gate->scalar_type() == x.scalar_type() || gate->scalar_type() == at::kFloat,
@@ -784,30 +804,23 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::
     const char* what = "gate must be [width], or have x's shape but for leading dimensions of 1 from some "
                        "one on to the last but one (expand others)";
     want(gate->dim() >= 1 && gate->dim() <= x.dim() && gate->size(-1) == d, what);
-    g = *gate;
-    while (g.dim() < x.dim()) g = g.unsqueeze(0);
     // of the leading dimensions the gate has the first k, and one of all others: rows that follow each
     // other share one of its rows
+    const int64_t missing = x.dim() - gate->dim();
+    const auto size = [&](int64_t i) { return i < missing ? 1 : gate->size(i - missing); };
     int64_t k = 0, rows = 1;
-    while (k + 1 < x.dim() && g.size(k) == x.size(k)) rows *= x.size(k++);
-    for (int64_t i = k; i + 1 < x.dim(); ++i) want(g.size(i) == 1, what);
-    g = g.reshape({rows, d}).contiguous();
+    while (k + 1 < x.dim() && size(k) == x.size(k)) rows *= x.size(k++);
+    for (int64_t i = k; i + 1 < x.dim(); ++i) want(size(i) == 1, what);
     gate_rows = std::max<int64_t>(1, rows ? M / rows : 1);
   }
-  const at::Tensor x2 = as_rows(x), w = weight.contiguous();
-  const at::Tensor bw = branch_weight ? branch_weight->contiguous() : at::Tensor();
+  const auto grad = [](const std::optional<at::Tensor>& t) { return t && t->requires_grad(); };
   std::vector<at::Tensor> r;
-  const auto grad = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
-  if (at::GradMode::is_enabled() && (grad(x2) || grad(b) || grad(g) || grad(w) || grad(bw))) {
-    const auto maybe = [](const at::Tensor& t) {
-      return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt;
-    };
-    r = ResidualNorm::apply(x2, maybe(b), maybe(g), w, maybe(bw), gate_rows, scale, eps);
-  } else {
-    r = norm_forward(norm_of(x2, b, g, w, bw, gate_rows, scale, eps), x2, b, false);
-    if (!b.defined()) return {x, r[1].view(x.sizes())};
-  }
-  return {r[0].view_as(x), r[1].view(x.sizes())};
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || grad(branch) ||
+                                     grad(gate) || grad(branch_weight)))
+    r = ResidualNorm::apply(x, branch, gate, weight, branch_weight, gate_rows, scale, eps);
+  else
+    r = norm_forward(norm_inputs(x, branch, gate, weight, branch_weight, gate_rows, scale, eps), x, false);
+  return {r[0], r[1]};
 }
 
 // A 16-bit matrix as the head's products take it: 16-byte aligned, rows a multiple of 8 values apart,
@@ -826,12 +839,13 @@ at::Tensor head_side(const at::Tensor& t) {
   return out;
 }
 
-// logprob, entropy, stats.
-std::vector<at::Tensor> head_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& token) {
+// logprob, entropy (of the tokens' shape), stats for rows x.
+std::vector<at::Tensor> head_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& token,
+                                     at::IntArrayRef sizes) {
   c10::DeviceGuard guard(x.device());
   const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
-  const auto f = x.options().dtype(at::kFloat);
-  at::Tensor lp = at::empty({M}, f), ent = at::empty({M}, f), st = at::empty({M, 2}, f);
+  const auto f = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor lp = at::empty(sizes, f), ent = at::empty(sizes, f), st = at::empty({M, 2}, f);
   if (M == 0) return {lp, ent, st};
   const at::Tensor xs = head_side(x), ws_ = head_side(w);
   const size_t need = fb_head_logprobs_workspace_bytes(M, (int32_t)K, (int32_t)V);
@@ -850,10 +864,13 @@ const float* f32_of(const at::Tensor& t) {
 
 struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
-                                                const at::Tensor& x, const at::Tensor& w,
-                                                const at::Tensor& token) {
-    const auto r = head_forward(x, w, token);
+                                                const at::Tensor& hidden, const at::Tensor& weight,
+                                                const at::Tensor& token,
+                                                const std::vector<int64_t>& sizes) {
+    const at::Tensor x = as_rows(hidden), w = as_rows(weight);
+    const auto r = head_forward(x, w, token, sizes);
     ctx->save_for_backward({x, w, token, r[1], r[2]});
+    ctx->saved_data["sizes"] = hidden.sizes().vec();
     ctx->set_materialize_grads(false);
     return {r[0], r[1]};
   }
@@ -869,7 +886,8 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
     const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
     at::Tensor gx, gw;
     if (ctx->needs_input_grad(0))
-      gx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+      gx = at::empty(ctx->saved_data["sizes"].toIntVector(),
+                     x.options().memory_format(at::MemoryFormat::Contiguous));
     if (ctx->needs_input_grad(1)) {
       gw = at::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
       if (M == 0) gw.zero_();
@@ -885,7 +903,7 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
           f32_of(ent), f32_of(g[0]), f32_of(g[1]), gx.defined() ? gx.data_ptr() : nullptr,
           gw.defined() ? gw.data_ptr() : nullptr, ws.data_ptr(), need, stream_of(x)));
     }
-    return {gx, gw, at::Tensor()};
+    return {gx, gw, at::Tensor(), at::Tensor()};
   }
 };
 
@@ -896,7 +914,7 @@ constexpr int64_t kMostLogits = 1 << 27;
 struct Packed {
   at::Tensor wdev;
   int64_t N, K, fmt, fwht;
-  bool f16_exact;
+  bool f16_exact, bf16_exact;
 };
 
 fb_shape_t packed_shape(const Packed& p, int64_t rows, int xdt, int ydt) {
@@ -948,11 +966,12 @@ int64_t packed_piece(const Packed& p, int64_t M) {
   return std::min(M, std::max<int64_t>(16, std::min<int64_t>(kMostLogits / p.N, kGradRows) / 16 * 16));
 }
 
-std::vector<at::Tensor> packed_forward(const Packed& p, const at::Tensor& x, const at::Tensor& token) {
+std::vector<at::Tensor> packed_forward(const Packed& p, const at::Tensor& x, const at::Tensor& token,
+                                       at::IntArrayRef sizes) {
   c10::DeviceGuard guard(x.device());
   const int64_t M = x.size(0);
-  const auto f = x.options().dtype(at::kFloat);
-  at::Tensor lp = at::empty({M}, f), ent = at::empty({M}, f), st = at::empty({M, 3}, f);
+  const auto f = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor lp = at::empty(sizes, f), ent = at::empty(sizes, f), st = at::empty({M, 3}, f);
   if (M == 0) return {lp, ent, st};
   const at::Tensor xk = packed_rows(p, x);
   const int64_t step = packed_piece(p, M);
@@ -971,13 +990,17 @@ std::vector<at::Tensor> packed_forward(const Packed& p, const at::Tensor& x, con
 
 struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
-                                                const at::Tensor& x, const at::Tensor& wdev,
-                                                const at::Tensor& token, int64_t N, int64_t K,
-                                                int64_t fmt, int64_t fwht, bool f16_exact) {
-    const Packed p{wdev, N, K, fmt, fwht, f16_exact};
-    const auto r = packed_forward(p, x, token);
+                                                const at::Tensor& hidden, const at::Tensor& wdev,
+                                                const at::Tensor& token,
+                                                const std::vector<int64_t>& sizes, int64_t N, int64_t K,
+                                                int64_t fmt, int64_t fwht, bool f16_exact,
+                                                bool bf16_exact) {
+    const Packed p{wdev, N, K, fmt, fwht, f16_exact, bf16_exact};
+    const at::Tensor x = as_rows(hidden);
+    const auto r = packed_forward(p, x, token, sizes);
+    ctx->saved_data["sizes"] = hidden.sizes().vec();
     ctx->save_for_backward({x, wdev, token, r[1], r[2]});
-    ctx->saved_data["head"] = std::vector<int64_t>{N, K, fmt, fwht, f16_exact};
+    ctx->saved_data["head"] = std::vector<int64_t>{N, K, fmt, fwht, f16_exact, bf16_exact};
     ctx->set_materialize_grads(false);
     return {r[0], r[1]};
   }
@@ -987,7 +1010,7 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
     const auto s = ctx->get_saved_variables();
     const at::Tensor &x = s[0], &token = s[2], &ent = s[3], &st = s[4];
     const auto h = ctx->saved_data["head"].toIntVector();
-    const Packed p{s[1], h[0], h[1], h[2], h[3], (bool)h[4]};
+    const Packed p{s[1], h[0], h[1], h[2], h[3], (bool)h[4], (bool)h[5]};
     c10::DeviceGuard guard(x.device());
     at::Tensor g[2];
     for (int i = 0; i < 2; ++i)
@@ -995,8 +1018,18 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
     const int64_t M = x.size(0), kp = (p.K + 127) / 128 * 128;
     at::Tensor gx = at::empty({M, kp}, x.options().memory_format(at::MemoryFormat::Contiguous));
     const int xdt = dtype_code(x.scalar_type());
-    if (M) {
-      const at::Tensor xk = packed_rows(p, x);
+    const at::Tensor xk = M ? packed_rows(p, x) : at::Tensor();
+    // the weight in 16 bits, as x, where it is exact there and not rotated; else in fp32 terms
+    const bool exact = p.fmt != FB_FMT_E2M1 || !M || (xk.scalar_type() == at::kHalf ? p.f16_exact : p.bf16_exact);
+    if (M && !p.fwht && exact) {
+      fb_shape_t sh = packed_shape(p, M, dtype_code(xk.scalar_type()), FB_DT_F32);
+      const size_t need = fb_packed_head_grad_workspace_bytes(&sh);
+      const at::Tensor ws = scratch(need, x);
+      check(fb_packed_head_grad(p.wdev.data_ptr(), xk.data_ptr(), &sh,
+                                static_cast<const int64_t*>(token.data_ptr()), f32_of(st), f32_of(ent),
+                                f32_of(g[0]), f32_of(g[1]), gx.data_ptr(), xdt, ws.data_ptr(), need,
+                                stream_of(x)));
+    } else if (M) {
       const int64_t step = packed_piece(p, M);
       const auto f = x.options().dtype(at::kFloat);
       const at::Tensor y = at::empty({step, p.N}, f), gl = at::empty({step, p.N}, f);
@@ -1018,13 +1051,13 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
       }
     }
     if (kp != p.K) gx = gx.narrow(1, 0, p.K).contiguous();
-    return {gx, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor()};
+    return {gx.view(ctx->saved_data["sizes"].toIntVector()), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
-// x [..., K] and tokens [...]: x's rows, the tokens, after the checks that both kinds of heads share.
-std::pair<at::Tensor, at::Tensor> head_inputs(const at::Tensor& x, const at::Tensor& tokens, int64_t K,
+// x [..., K] and tokens [...]: the flat tokens, after the checks that both kinds of heads share.
+at::Tensor head_tokens(const at::Tensor& x, const at::Tensor& tokens, int64_t K,
                                               const at::Tensor& like) {
   not_recorded();
   want(x.defined() && plain(x), "hidden must be a tensor on a ROCm GPU");
@@ -1034,7 +1067,7 @@ std::pair<at::Tensor, at::Tensor> head_inputs(const at::Tensor& x, const at::Ten
   want(tokens.sizes() == x.sizes().slice(0, x.dim() - 1),
        "tokens must have hidden's shape without the last dimension");
   want(tokens.numel() <= (1 << 24), "too many tokens");
-  return {as_rows(x), flat_tokens(tokens)};
+  return flat_tokens(tokens);
 }
 
 // logprob, entropy.
@@ -1044,35 +1077,32 @@ std::tuple<at::Tensor, at::Tensor> head_logprobs(const at::Tensor& hidden, const
   want(weight.dim() == 2 && weight.size(0) >= 1 && weight.size(0) <= (1 << 24) && weight.size(1) >= 1 &&
            weight.size(1) <= (1 << 20),
        "the head's weight must be [vocab, width], a width of at most 2^20, a vocabulary of at most 2^24");
-  const auto [x, t] = head_inputs(hidden, tokens, weight.size(1), weight);
-  want((x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16) &&
-           x.scalar_type() == weight.scalar_type(),
+  const at::Tensor t = head_tokens(hidden, tokens, weight.size(1), weight);
+  want((hidden.scalar_type() == at::kHalf || hidden.scalar_type() == at::kBFloat16) &&
+           hidden.scalar_type() == weight.scalar_type(),
        "hidden and the head's weight must both be float16 or both bfloat16");
-  const at::Tensor w = as_rows(weight);
-  std::vector<at::Tensor> r;
-  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))
-    r = HeadLogprobs::apply(x, w, t);
-  else
-    r = head_forward(x, w, t);
-  return {r[0].view(tokens.sizes()), r[1].view(tokens.sizes())};
+  const auto r = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())
+                     ? HeadLogprobs::apply(hidden, weight, t, tokens.sizes().vec())
+                     : head_forward(as_rows(hidden), as_rows(weight), t, tokens.sizes());
+  return {r[0], r[1]};
 }
 
 std::tuple<at::Tensor, at::Tensor> packed_head_logprobs(const at::Tensor& hidden, const at::Tensor& wdev,
                                                         const at::Tensor& tokens, int64_t N, int64_t K,
-                                                        int64_t fmt, int64_t fwht, bool f16_exact) {
+                                                        int64_t fmt, int64_t fwht, bool f16_exact,
+                                                        bool bf16_exact) {
   want(wdev.defined() && plain(wdev), "the packed head must be on a ROCm GPU");
-  const auto [x, t] = head_inputs(hidden, tokens, K, wdev);
-  want(dtype_code(x.scalar_type()) >= 0, "hidden must be float16, bfloat16 or float32");
-  const Packed p{wdev, N, K, fmt, fwht, f16_exact};
+  const at::Tensor t = head_tokens(hidden, tokens, K, wdev);
+  want(dtype_code(hidden.scalar_type()) >= 0, "hidden must be float16, bfloat16 or float32");
+  const Packed p{wdev, N, K, fmt, fwht, f16_exact, bf16_exact};
   const fb_shape_t s = packed_shape(p, 1, FB_DT_F16, FB_DT_F32);
   want(fb_device_bytes(&s) && (size_t)wdev.numel() >= fb_device_bytes(&s) && s.K <= kMaxGemmK,
        "the packed head is not of its format's size");
-  std::vector<at::Tensor> r;
-  if (at::GradMode::is_enabled() && x.requires_grad())
-    r = PackedHeadLogprobs::apply(x, wdev, t, N, K, fmt, fwht, f16_exact);
-  else
-    r = packed_forward(p, x, t);
-  return {r[0].view(tokens.sizes()), r[1].view(tokens.sizes())};
+  const auto r = at::GradMode::is_enabled() && hidden.requires_grad()
+                     ? PackedHeadLogprobs::apply(hidden, wdev, t, tokens.sizes().vec(), N, K, fmt, fwht,
+                                                 f16_exact, bf16_exact)
+                     : packed_forward(p, as_rows(hidden), t, tokens.sizes());
+  return {r[0], r[1]};
 }
 
 }  // namespace

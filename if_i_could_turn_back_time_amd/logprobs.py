@@ -48,19 +48,22 @@ def head_logprobs(hidden: torch.Tensor, head, tokens: torch.Tensor) -> HeadLogpr
     entropy's, nor gives the weight any, whatever ``hidden`` holds there.
 
     The gradients' products take each logit's gradient in 16 bits, as a backward pass through 16-bit
-    logits does (with a packed head in fp32)."""
+    logits does, but for the given token's, whose rounding is made up for.  (A rotated packed head, and
+    one whose scales leave 16 bits, takes them in fp32.)"""
     if isinstance(head, (QuantLinear, PackedWeight)):
         if isinstance(head, QuantLinear):
             if head.bias is not None:
                 raise ValueError("head_logprobs takes a head without a bias; with one: "
                                  "token_logprobs(head(hidden), tokens)")
             n, k, fmt, f16_exact = head.out_features, head.in_features, head.fmt, head._f16_exact
+            bf16_exact = f16_exact if head._bf16_exact is None else head._bf16_exact
             if head.range_check and hidden.dim() and hidden.shape[-1] == k:
                 _kernel_input(hidden.detach().reshape(-1, k), k, fmt, head.fwht_block, True, f16_exact)
         else:
             n, k, fmt, f16_exact = head.N, head.K, head.fmt_name, head.f16_exact
+            bf16_exact = f16_exact  # a range within bf16's
         r = C.native().packed_head_logprobs(hidden, head.wdev, tokens, n, k, C.FMT_BY_NAME[fmt],
-                                            head.fwht_block, f16_exact)
+                                            head.fwht_block, f16_exact, bf16_exact)
     else:
         r = C.native().head_logprobs(hidden, head, tokens)
     return HeadLogprobs(*r)

@@ -628,7 +628,8 @@ size_t fb_head_logprobs_workspace_bytes(int64_t rows, int32_t K, int32_t vocab);
 
 /* The gradient: with G[r, v] as fb_token_logprobs_grad's (no alternatives), grad_x = G w and
  * grad_w = G^T x.  The logits are computed again, a piece of the vocabulary at a time; G enters the
- * products rounded to dtype (fp16: times a power of two of its row).  A row whose g are 0, or that has
+ * products rounded to dtype (fp16: times a power of two of its row), but for the given token's value,
+ * which keeps what its rounding loses.  A row whose g are 0, or that has
  * no token and no g_entropy, adds nothing to grad_w whatever its x holds.
  *   stats, entropy     as fb_head_logprobs wrote them
  *   g_*                fp32 [rows], or NULL (taken as 0)
@@ -641,6 +642,19 @@ int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_
                           void* ws, size_t ws_bytes, void* stream);
 size_t fb_head_logprobs_grad_workspace_bytes(int64_t rows, int32_t K, int32_t vocab,
                                              int32_t want_x, int32_t want_w);
+
+/* The same gradient of x under a packed head (s: N the vocabulary, B the rows; no rotation), whose
+ * logits fb_gemv or fb_gemm gave and whose stats and entropies fb_token_logprobs: the weight is decoded
+ * to 16 bits in the workspace first, and must be exact there (E2M1 scale bytes 104 .. 140 with F16 x, up
+ * to 252 with BF16).
+ *   x        [B, K] of s->x_dtype, contiguous, 16-byte aligned
+ *   stats    fp32 [B, 3] of fb_token_logprobs
+ *   grad_x   [B, K] of grad_x_dtype (F16, BF16 or F32), contiguous, 16-byte aligned */
+int fb_packed_head_grad(const void* wdev, const void* x, const fb_shape_t* s, const int64_t* token,
+                        const float* stats, const float* entropy, const float* g_logprob,
+                        const float* g_entropy, void* grad_x, int32_t grad_x_dtype, void* ws,
+                        size_t ws_bytes, void* stream);
+size_t fb_packed_head_grad_workspace_bytes(const fb_shape_t* s);
 
 #ifdef __cplusplus
 }
