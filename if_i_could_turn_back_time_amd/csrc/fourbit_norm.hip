@@ -26,37 +26,37 @@ __attribute__((visibility("hidden"))) int cu_count();
 namespace {
 
 // load and store of a vector that may be fp32 instead.
-template <int DT>
+template <int DT, bool EVEN>
 __device__ inline void load_vec(const void* p, int f32, int64_t from, int at, int n,
                                 float (&o)[Of<DT>::V]) {
   constexpr int V = Of<DT>::V;
-  if (DT == FB_DT_F32 || !f32) return load<DT>(p, from, at, n, o);
+  if (DT == FB_DT_F32 || !f32) return load<DT, EVEN>(p, from, at, n, o);
 #pragma unroll
   for (int h = 0; h < V; h += 4) {
     float v[4];
-    load<FB_DT_F32>(p, from, at + h, n - h, v);
+    load<FB_DT_F32, EVEN>(p, from, at + h, n - h, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[h + i] = v[i];
   }
 }
-template <int DT>
+template <int DT, bool EVEN>
 __device__ inline void store_vec(void* p, int f32, int64_t at, int n, const float (&o)[Of<DT>::V]) {
   constexpr int V = Of<DT>::V;
-  if (DT == FB_DT_F32 || !f32) return store<DT>(p, at, n, o);
+  if (DT == FB_DT_F32 || !f32) return store<DT, EVEN>(p, at, n, o);
 #pragma unroll
   for (int h = 0; h < V; h += 4) {
     const float v[4] = {o[h], o[h + 1], o[h + 2], o[h + 3]};
-    store<FB_DT_F32>(p, at + h, n - h, v);
+    store<FB_DT_F32, EVEN>(p, at + h, n - h, v);
   }
 }
 
 // V fp32 values to p[at] on, of d.
-template <int V>
+template <bool EVEN, int V>
 __device__ inline void store_part(float* p, int at, int d, const float (&v)[V]) {
 #pragma unroll
   for (int h = 0; h < V; h += 4) {
     const float o[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
-    store<FB_DT_F32>(p, at + h, d - at - h, o);
+    store<FB_DT_F32, EVEN>(p, at + h, d - at - h, o);
   }
 }
 
@@ -94,6 +94,8 @@ __device__ inline void group_sum(float (&v)[N], float (*red)[N]) {
   }
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 struct NormArgs {
   fb_norm_t n;
   int bf32, wf32, gf32;  // branch_weight, weight, gate are fp32 beside 16-bit rows
@@ -111,8 +113,8 @@ struct NormArgs {
 template <int T>
 constexpr int kBlock = T == 64 ? 256 : T;  // waves that share a row share no workgroup with another
 
-template <int DT, int T, int NV>
-__global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
+template <int DT, int T, int NV, bool EVEN>
+__global__ __launch_bounds__(kBlock<T>, 4) void norm_kernel(NormArgs a) {
   constexpr int V = Of<DT>::V, G = kBlock<T> / T;
   __shared__ float red[2][T / 64][1];
   int turn = 0;
@@ -121,8 +123,8 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * T + t) * V;
-    load_vec<DT>(a.n.weight, a.wf32, 0, at, d - at, w[j]);
-    if (a.n.branch_weight) load_vec<DT>(a.n.branch_weight, a.bf32, 0, at, d - at, wb[j]);
+    load_vec<DT, EVEN>(a.n.weight, a.wf32, 0, at, d - at, w[j]);
+    if (a.n.branch_weight) load_vec<DT, EVEN>(a.n.branch_weight, a.bf32, 0, at, d - at, wb[j]);
   }
   const float inv = 1.f / (float)d;
   for (int64_t r0 = (int64_t)blockIdx.x * G; r0 < a.n.rows; r0 += (int64_t)gridDim.x * G) {
@@ -133,14 +135,14 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      xr[j] = raw<DT>(a.n.x, r * a.n.x_stride, at, d - at);
-      if (a.n.branch) br[j] = raw<DT>(a.n.branch, r * a.n.branch_stride, at, d - at);
+      xr[j] = raw<DT, EVEN>(a.n.x, r * a.n.x_stride, at, d - at);
+      if (a.n.branch) br[j] = raw<DT, EVEN>(a.n.branch, r * a.n.branch_stride, at, d - at);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      unpack<DT>(settled<DT>(xr[j], at, d - at), x[j]);
-      if (a.n.branch) unpack<DT>(settled<DT>(br[j], at, d - at), b[j]);
+      unpack<DT>(settled<DT, EVEN>(xr[j], at, d - at), x[j]);
+      if (a.n.branch) unpack<DT>(settled<DT, EVEN>(br[j], at, d - at), b[j]);
     }
     if (a.n.branch) {
       if (a.n.branch_weight) {
@@ -161,11 +163,11 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
       for (int j = 0; j < NV; ++j) {
         const int at = (j * T + t) * V;
         float g[V];
-        if (a.n.gate) load_vec<DT>(a.n.gate, a.gf32, g0, at, d - at, g);
+        if (a.n.gate) load_vec<DT, EVEN>(a.n.gate, a.gf32, g0, at, d - at, g);
 #pragma unroll
         for (int i = 0; i < V; ++i)
           x[j][i] = __builtin_fmaf(a.n.gate ? a.n.scale * g[i] : a.n.scale, b[j][i], x[j][i]);
-        if (mine) store<DT>(a.h, r * d + at, d - at, x[j]);
+        if (mine) store<DT, EVEN>(a.h, r * d + at, d - at, x[j]);
       }
     }
     float s[1] = {0.f};
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
       float y[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) y[i] = x[j][i] * r2 * w[j][i];
-      store<DT>(a.y, r * d + at, d - at, y);
+      store<DT, EVEN>(a.y, r * d + at, d - at, y);
     }
     if (a.stats && t == 0) {
       a.stats[2 * r] = r1;
@@ -195,15 +197,15 @@ __global__ __launch_bounds__(kBlock<T>) void norm_kernel(NormArgs a) {
 struct Raw2 {
   u32x4 lo, hi;
 };
-template <int DT>
+template <int DT, bool EVEN>
 __device__ inline Raw2 raw_vec(const void* p, int f32, int64_t from, int at, int n) {
-  if (DT == FB_DT_F32 || !f32) return {raw<DT>(p, from, at, n), u32x4{0, 0, 0, 0}};
-  return {raw<FB_DT_F32>(p, from, at, n), raw<FB_DT_F32>(p, from, at + 4, n - 4)};
+  if (DT == FB_DT_F32 || !f32) return {raw<DT, EVEN>(p, from, at, n), u32x4{0, 0, 0, 0}};
+  return {raw<FB_DT_F32, EVEN>(p, from, at, n), raw<FB_DT_F32, EVEN>(p, from, at + 4, n - 4)};
 }
-template <int DT>
+template <int DT, bool EVEN>
 __device__ inline void unpack_vec(const Raw2& r, int f32, int at, int n, float (&o)[Of<DT>::V]) {
-  if (DT == FB_DT_F32 || !f32) return unpack<DT>(settled<DT>(r.lo, at, n), o);
-  const u32x4 lo = settled<FB_DT_F32>(r.lo, at, n), hi = settled<FB_DT_F32>(r.hi, at + 4, n - 4);
+  if (DT == FB_DT_F32 || !f32) return unpack<DT>(settled<DT, EVEN>(r.lo, at, n), o);
+  const u32x4 lo = settled<FB_DT_F32, EVEN>(r.lo, at, n), hi = settled<FB_DT_F32, EVEN>(r.hi, at + 4, n - 4);
 #pragma unroll
   for (int i = 0; i < Of<DT>::V; ++i) {
     const unsigned u = i < 4 ? lo[i & 3] : hi[i & 3];
@@ -216,24 +218,69 @@ __device__ inline void unpack_vec(const Raw2& r, int f32, int at, int n, float (
 // unit's is written; else the unit leaves its part, in place 0 where the gate's first row of it is the
 // unit's first, in place 1 otherwise (its last gate).  A row is asked for while the one before it is
 // worked on, and kept as it came: what is needed again after the sums is unpacked again.
-template <int DT, int T, int NV>
+//
+// KIND -1: any call.  From 0 on: rows of whole pieces with a branch, kPost and kGate as bits of it say
+// (the code of what is not there costs registers, and they are what bounds the rows in flight).
+constexpr int kAny = -1, kPost = 1, kGate = 2;
+template <int DT, int T, int NV, int KIND>
 __global__ __launch_bounds__(kBlock<T>) void norm_grad_kernel(NormArgs a) {
+  constexpr bool EVEN = KIND != kAny;
   constexpr int V = Of<DT>::V, G = kBlock<T> / T;
+  // Wide rows: no room to keep what the sums are made of, or the next row; and as many of the weights' and
+  // the gate's sums as LDS holds are there.
+  constexpr bool LEAN = T == 1024;
+  constexpr int kInLds = !LEAN ? 0 : NV * V <= 8 ? 3 : NV * V <= 16 ? 2 : 1;
+  __shared__ f32x4 lds_sums[kInLds ? kInLds : 1][kInLds ? NV * V / 4 : 1][kInLds ? T : 1];
   __shared__ float red[2][T / 64][3];
   const int t = threadIdx.x % T, group = threadIdx.x / T, d = a.n.width;
   const int unit = blockIdx.x * G + group;
   const int64_t first = (int64_t)unit * a.rows_per_unit;
   const int64_t end = min(first + a.rows_per_unit, a.n.rows);
-  const bool branch = a.n.branch, post = a.n.branch_weight, gate = a.n.gate;
+  const bool branch = KIND != kAny || a.n.branch;
+  const bool post = KIND != kAny ? KIND & kPost : a.n.branch_weight != nullptr;
+  const bool gate = KIND != kAny ? KIND & kGate : a.n.gate != nullptr;
   if (first >= end) return;  // the whole group
-  float sw[NV][V], swb[NV][V], sg[NV][V], w[NV][V], wb[NV][V];
+  float sums[3][NV][V], kept_w[NV][V], kept_wb[NV][V];
+  // Sums 0 (weight), 1 (branch weight), 2 (gate) of piece j: the value of one of its values ...
+  const auto sum_at = [&](int k, int j, int i) __attribute__((always_inline)) -> float {
+    return k < kInLds ? lds_sums[k < kInLds ? k : 0][(j * V + i) / 4][t][i & 3] : sums[k][j][i];
+  };
+  // ... grows by the products of two, or is cleared
+  const auto grow = [&](int k, int j, const float (&p)[V], const float (&q)[V])
+      __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < V; h += 4) {
+      f32x4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(p[h + i], q[h + i], sum_at(k, j, h + i));
+      if (k < kInLds)
+        lds_sums[k < kInLds ? k : 0][(j * V + h) / 4][t] = v;
+      else
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[k][j][h + i] = v[i];
+    }
+  };
+  const auto clear = [&](int k, int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < V; h += 4) {
+      if (k < kInLds) lds_sums[k < kInLds ? k : 0][(j * V + h) / 4][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[k][j][h + i] = 0.f;
+    }
+  };
+  const auto sums_of = [&](int k, int j, float (&o)[V]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = sum_at(k, j, i);
+  };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * T + t) * V;
-    load_vec<DT>(a.n.weight, a.wf32, 0, at, d - at, w[j]);
-    if (post) load_vec<DT>(a.n.branch_weight, a.bf32, 0, at, d - at, wb[j]);
+    if (!LEAN) {
+      load_vec<DT, EVEN>(a.n.weight, a.wf32, 0, at, d - at, kept_w[j]);
+      if (post) load_vec<DT, EVEN>(a.n.branch_weight, a.bf32, 0, at, d - at, kept_wb[j]);
+    }
 #pragma unroll
-    for (int i = 0; i < V; ++i) sw[j][i] = swb[j][i] = sg[j][i] = 0.f;
+    for (int k = 0; k < 3; ++k) clear(k, j);
   }
   const float inv = 1.f / (float)d;
   int64_t gi = gate ? first / a.n.gate_rows : 0;
@@ -248,104 +295,139 @@ __global__ __launch_bounds__(kBlock<T>) void norm_grad_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * T + t) * V;
-      x[j] = raw<DT>(a.n.x, r * a.n.x_stride, at, d - at);
-      if (branch) b[j] = raw<DT>(a.n.branch, r * a.n.branch_stride, at, d - at);
-      if (gate) g[j] = raw_vec<DT>(a.n.gate, a.gf32, of * d, at, d - at);
+      x[j] = raw<DT, EVEN>(a.n.x, r * a.n.x_stride, at, d - at);
+      if (branch) b[j] = raw<DT, EVEN>(a.n.branch, r * a.n.branch_stride, at, d - at);
+      if (gate) g[j] = raw_vec<DT, EVEN>(a.n.gate, a.gf32, of * d, at, d - at);
       gy[j] = gh[j] = u32x4{0, 0, 0, 0};
-      if (a.dy) gy[j] = raw<DT>(a.dy, r * d, at, d - at);
-      if (a.dh) gh[j] = raw<DT>(a.dh, r * d, at, d - at);
+      if (a.dy) gy[j] = raw<DT, EVEN>(a.dy, r * d, at, d - at);
+      if (a.dh) gh[j] = raw<DT, EVEN>(a.dh, r * d, at, d - at);
     }
+  };
+  // Piece j: n, u = dh + r2 dn, the branch (n_b after a norm), f = scale gate, q, dn, dy, the weights.
+  struct Piece {
+    float n[V], u[V], nb[V], f[V], q[V], dn[V], dy[V], wb[V];
+  };
+  const auto piece = [&](int j) __attribute__((always_inline)) {
+    Piece p;
+    const int at = (j * T + t) * V;
+    float w[V];
+    unpack<DT>(settled<DT, EVEN>(x[j], at, d - at), p.n);
+    unpack<DT>(settled<DT, EVEN>(gy[j], at, d - at), p.dy);
+    unpack<DT>(settled<DT, EVEN>(gh[j], at, d - at), p.u);
+    if (branch) {
+      unpack<DT>(settled<DT, EVEN>(b[j], at, d - at), p.nb);
+      if (gate) unpack_vec<DT, EVEN>(g[j], a.gf32, at, d - at, p.f);
+    }
+    if (LEAN) {
+      load_vec<DT, EVEN>(a.n.weight, a.wf32, 0, at, d - at, w);
+      if (post) load_vec<DT, EVEN>(a.n.branch_weight, a.bf32, 0, at, d - at, p.wb);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (!LEAN) {
+        w[i] = kept_w[j][i];
+        if (post) p.wb[i] = kept_wb[j][i];
+      }
+      p.q[i] = 0.f;
+      if (branch) {
+        if (post) p.nb[i] *= r1;
+        p.f[i] = gate ? a.n.scale * p.f[i] : a.n.scale;
+        p.q[i] = post ? p.f[i] * p.wb[i] * p.nb[i] : p.f[i] * p.nb[i];
+      }
+      p.n[i] = (p.n[i] + p.q[i]) * r2;
+      p.dn[i] = p.dy[i] * w[i];
+      p.u[i] = __builtin_fmaf(r2, p.dn[i], p.u[i]);
+    }
+    return p;
   };
   fetch(first, gi);
   for (int64_t r = first; r < end; ++r) {
-    float n[NV][V], u[NV][V], nb[NV][V], f[NV][V];  // u: dh + r2 dn, f: scale gate
     float s[3] = {0.f, 0.f, 0.f};
-    const float ra = r1, rb = r2;
+    Piece kept[LEAN ? 1 : NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = (j * T + t) * V;
-      float xx[V], dy[V];
-      unpack<DT>(settled<DT>(x[j], at, d - at), xx);
-      unpack<DT>(settled<DT>(gy[j], at, d - at), dy);
-      unpack<DT>(settled<DT>(gh[j], at, d - at), u[j]);
-      if (branch) {
-        unpack<DT>(settled<DT>(b[j], at, d - at), nb[j]);
-        if (gate) unpack_vec<DT>(g[j], a.gf32, at, d - at, f[j]);
-      }
+      const Piece p = piece(j);
+      if (!LEAN) kept[j] = p;
+      grow(0, j, p.dy, p.n);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float q = 0.f;
-        if (branch) {
-          if (post) nb[j][i] *= ra;
-          f[j][i] = gate ? a.n.scale * f[j][i] : a.n.scale;
-          q = post ? f[j][i] * wb[j][i] * nb[j][i] : f[j][i] * nb[j][i];
-        }
-        n[j][i] = (xx[i] + q) * rb;
-        const float dn = dy[i] * w[j][i];
-        u[j][i] = __builtin_fmaf(rb, dn, u[j][i]);
-        sw[j][i] = __builtin_fmaf(dy[i], n[j][i], sw[j][i]);
-        s[0] = __builtin_fmaf(dn, n[j][i], s[0]);
-        s[1] = __builtin_fmaf(u[j][i], q, s[1]);
-        s[2] = __builtin_fmaf(n[j][i], q, s[2]);
+        s[0] = __builtin_fmaf(p.dn[i], p.n[i], s[0]);
+        s[1] = __builtin_fmaf(p.u[i], p.q[i], s[1]);
+        s[2] = __builtin_fmaf(p.n[i], p.q[i], s[2]);
       }
+      if (LEAN) __builtin_amdgcn_sched_barrier(0);
     }
     const int64_t of = gi;
+    const float ra = r1, rb = r2;
     const bool flush = gate && (--left == 0 || r + 1 == end);
     if (gate && left == 0) {
       ++gi;
       left = a.n.gate_rows;
     }
-    if (r + 1 < end) fetch(r + 1, gi);
+    if (!LEAN && r + 1 < end) fetch(r + 1, gi);
     group_sum<T>(s, red[turn ^= 1]);
     const float m1 = s[0] * inv * rb;           // dx = u - m1 n
     const float m2 = (s[1] - m1 * s[2]) * inv;  // mean of wb g t n_b
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (LEAN)  // or the compiler keeps what it worked out before
+        asm volatile("" : "+v"(x[j]), "+v"(b[j]), "+v"(gy[j]), "+v"(gh[j]), "+v"(g[j].lo), "+v"(g[j].hi));
+      Piece p = LEAN ? piece(j) : kept[LEAN ? 0 : j];
       const int at = (j * T + t) * V;
 #pragma unroll
-      for (int i = 0; i < V; ++i) u[j][i] = __builtin_fmaf(-m1, n[j][i], u[j][i]);
-      if (a.dx) store<DT>(a.dx, r * d + at, d - at, u[j]);
+      for (int i = 0; i < V; ++i) p.u[i] = __builtin_fmaf(-m1, p.n[i], p.u[i]);
+      if (a.dx) store<DT, EVEN>(a.dx, r * d + at, d - at, p.u);
       if (branch) {
+        if (gate) {
+          float tt[V], b2[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            tt[i] = a.n.scale * p.u[i];
+            b2[i] = post ? p.wb[i] * p.nb[i] : p.nb[i];
+          }
+          grow(2, j, tt, b2);
+        }
         float o[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (gate)
-            sg[j][i] = __builtin_fmaf(a.n.scale * u[j][i], post ? wb[j][i] * nb[j][i] : nb[j][i], sg[j][i]);
-          const float tf = u[j][i] * f[j][i];  // g t
-          o[i] = tf;
-          if (post) {
-            swb[j][i] = __builtin_fmaf(tf, nb[j][i], swb[j][i]);
-            o[i] = ra * __builtin_fmaf(-m2, nb[j][i], tf * wb[j][i]);
-          }
+        for (int i = 0; i < V; ++i) o[i] = p.u[i] * p.f[i];  // g t
+        if (post) {
+          grow(1, j, o, p.nb);
+#pragma unroll
+          for (int i = 0; i < V; ++i) o[i] = ra * __builtin_fmaf(-m2, p.nb[i], o[i] * p.wb[i]);
         }
-        if (a.db) store<DT>(a.db, r * d + at, d - at, o);
+        if (a.db) store<DT, EVEN>(a.db, r * d + at, d - at, o);
       }
+      if (LEAN) __builtin_amdgcn_sched_barrier(0);
     }
+    if (LEAN && r + 1 < end) fetch(r + 1, gi);
     if (flush) {
       const int64_t g0 = of * a.n.gate_rows, g1 = min(g0 + a.n.gate_rows, a.n.rows);
       const bool whole = g0 >= first && g1 <= end;
-      if (a.dgate) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int at = (j * T + t) * V;
-          if (whole) {
-            store_vec<DT>(a.dgate, a.gf32, of * d + at, d - at, sg[j]);
-          } else {
-            store_part(a.pg + ((int64_t)unit * 2 + (g0 > first)) * d, at, d, sg[j]);
-          }
-        }
+      for (int j = 0; j < NV; ++j) {
+        const int at = (j * T + t) * V;
+        float o[V];
+        sums_of(2, j, o);
+        clear(2, j);
+        if (a.dgate && whole)
+          store_vec<DT, EVEN>(a.dgate, a.gf32, of * d + at, d - at, o);
+        else if (a.dgate)
+          store_part<EVEN>(a.pg + ((int64_t)unit * 2 + (g0 > first)) * d, at, d, o);
       }
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) sg[j][i] = 0.f;
     }
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * T + t) * V;
-    if (a.dw) store_part(a.pw + (int64_t)unit * d, at, d, sw[j]);
-    if (a.dwb) store_part(a.pwb + (int64_t)unit * d, at, d, swb[j]);
+    float o[V];
+    if (a.dw) {
+      sums_of(0, j, o);
+      store_part<EVEN>(a.pw + (int64_t)unit * d, at, d, o);
+    }
+    if (a.dwb) {
+      sums_of(1, j, o);
+      store_part<EVEN>(a.pwb + (int64_t)unit * d, at, d, o);
+    }
   }
 }
 
@@ -459,9 +541,8 @@ Split split_of(int width) {
 }
 // The gradient keeps three sums for each value: half as many of them a thread.
 Split grad_split_of(int width) {
-  for (int t = 64; t <= 512; t *= 2)
+  for (int t = 64; t <= 1024; t *= 2)
     if (width <= t * 8) return {t, 8};
-  if (width <= 8192) return {512, 16};
   return {1024, width <= 16384 ? 16 : 32};
 }
 
@@ -497,8 +578,11 @@ int run_norm(const NormArgs& a, hipStream_t hs) {
     constexpr int T = decltype(c)::kThreads, NV = decltype(c)::kVecs, G = kBlock<T> / T;
     const int64_t groups = (a.n.rows + G - 1) / G;
     const int64_t most = (int64_t)fb_gpu::cu_count() * (2048 / kBlock<T>);
-    hipLaunchKernelGGL((norm_kernel<DT, T, NV>), dim3((unsigned)std::min(groups, most)),
-                       dim3(kBlock<T>), 0, hs, a);
+    const dim3 grid((unsigned)std::min(groups, most)), block(kBlock<T>);
+    if (a.n.width % 8 == 0)
+      hipLaunchKernelGGL((norm_kernel<DT, T, NV, true>), grid, block, 0, hs, a);
+    else
+      hipLaunchKernelGGL((norm_kernel<DT, T, NV, false>), grid, block, 0, hs, a);
     return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
   };
   const Split s = split_of(a.n.width);
@@ -517,15 +601,24 @@ template <int DT>
 int run_norm_grad(const NormArgs& a, hipStream_t hs) {
   const auto go = [&](auto c) {
     constexpr int T = decltype(c)::kThreads, NV = decltype(c)::kVecs, G = kBlock<T> / T;
-    hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV>), dim3((unsigned)((a.units + G - 1) / G)),
-                       dim3(kBlock<T>), 0, hs, a);
+    const dim3 grid((unsigned)((a.units + G - 1) / G)), block(kBlock<T>);
+    const int kind = !a.n.branch || a.n.width % 8 ? kAny
+                                                  : (a.n.branch_weight ? kPost : 0) + (a.n.gate ? kGate : 0);
+    if constexpr (NV * Of<DT>::V <= 16) {
+      if (kind == 0) hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV, 0>), grid, block, 0, hs, a);
+      if (kind == 1) hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV, 1>), grid, block, 0, hs, a);
+      if (kind == 2) hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV, 2>), grid, block, 0, hs, a);
+      if (kind == 3) hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV, 3>), grid, block, 0, hs, a);
+    }
+    if (NV * Of<DT>::V > 16 || kind == kAny)
+      hipLaunchKernelGGL((norm_grad_kernel<DT, T, NV, kAny>), grid, block, 0, hs, a);
     return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
   };
   const Split s = grad_split_of(a.n.width);
   int st;
   if (s.values == 32) st = go(Config<1024, 32, DT>{});
-  else if (s.threads == 1024) st = go(Config<1024, 16, DT>{});
-  else if (s.values == 16) st = go(Config<512, 16, DT>{});
+  else if (s.values == 16) st = go(Config<1024, 16, DT>{});
+  else if (s.threads == 1024) st = go(Config<1024, 8, DT>{});
   else if (s.threads == 512) st = go(Config<512, 8, DT>{});
   else if (s.threads == 256) st = go(Config<256, 8, DT>{});
   else if (s.threads == 128) st = go(Config<128, 8, DT>{});

@@ -33,13 +33,16 @@ struct Of<FB_DT_BF16> {
 // and has `n` more there.  The last piece of a row of an odd width is read where it ends with the row,
 // and `settled` moves its values to the front (value by value it took three times as long as all the
 // others); 0 beyond the row.  Apart, so that a caller can ask for many pieces before it needs one.
-template <int DT>
+// EVEN: rows are whole pieces; the rest of the code, and half the registers, go then.
+template <int DT, bool EVEN = false>
 __device__ inline u32x4 raw(const void* p, int64_t from, int at, int n) {
   using T = typename Of<DT>::T;
   constexpr int V = Of<DT>::V;
   const T* s = static_cast<const T*>(p) + from + at;
   u32x4 w{0, 0, 0, 0};
-  if (n > 0 && (at || n >= V)) {
+  if constexpr (EVEN) {
+    if (n > 0) w = *reinterpret_cast<const u32x4_any*>(s);
+  } else if (n > 0 && (at || n >= V)) {
     w = *reinterpret_cast<const u32x4_any*>(s + min(n - V, 0));
   } else if (n > 0) {  // a row shorter than a piece
 #pragma unroll
@@ -53,10 +56,10 @@ __device__ inline u32x4 raw(const void* p, int64_t from, int at, int n) {
   }
   return w;
 }
-template <int DT>
+template <int DT, bool EVEN = false>
 __device__ inline u32x4 settled(const u32x4& w, int at, int n) {
   constexpr int V = Of<DT>::V;
-  if (n >= V || n <= 0 || !at) return w;
+  if (EVEN || n >= V || n <= 0 || !at) return w;
   const unsigned bits = (V - n) * (128 / V);
   unsigned long long lo = w[0] | (unsigned long long)w[1] << 32;
   unsigned long long hi = w[2] | (unsigned long long)w[3] << 32;
@@ -85,23 +88,23 @@ __device__ inline void unpack(const u32x4& w, float (&o)[Of<DT>::V]) {
     }
   }
 }
-template <int DT>
+template <int DT, bool EVEN = false>
 __device__ inline void load(const void* p, int64_t from, int at, int n, float (&o)[Of<DT>::V]) {
-  unpack<DT>(settled<DT>(raw<DT>(p, from, at, n), at, n), o);
+  unpack<DT>(settled<DT, EVEN>(raw<DT, EVEN>(p, from, at, n), at, n), o);
 }
-template <int DT>
+template <int DT, bool EVEN = false>
 __device__ inline void store(void* p, int64_t at, int n, const float (&v)[Of<DT>::V]) {
   using T = typename Of<DT>::T;
   constexpr int V = Of<DT>::V;
   T* d = static_cast<T*>(p) + at;
-  if (n >= V) {
+  if (EVEN ? n > 0 : n >= V) {
     T o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = (T)v[i];
     u32x4 w;
     __builtin_memcpy(&w, o, 16);
     *reinterpret_cast<u32x4_any*>(d) = w;
-  } else {
+  } else if constexpr (!EVEN) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) d[i] = (T)v[i];
