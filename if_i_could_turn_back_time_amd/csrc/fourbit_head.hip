@@ -729,7 +729,7 @@ __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, i
 // host side
 // ---------------------------------------------------------------------------------
 constexpr int64_t kMostG = 1ll << 30;       // bytes of G at once
-constexpr int64_t kMostRows = 1 << 24;
+constexpr int64_t kMostRows = 1 << 23;      // 256 threads each stay below a launch's 2^32
 constexpr int64_t kStatRows = 1 << 14;      // rows of logits whose parts are held at once
 
 // Tiles to choose from, with what a workgroup of each takes in us: a chunk of the contraction with all
@@ -860,6 +860,8 @@ bool bad_align(std::initializer_list<const void*> ps, unsigned mask) {
   return false;
 }
 
+constexpr int64_t kMostSums = 1ll << 33;    // rows x K of grad_x
+
 int head_check(int32_t dtype, int64_t rows, int32_t K, int32_t vocab, int64_t ldx, int64_t ldw) {
   if (dtype != FB_DT_F16 && dtype != FB_DT_BF16) return FB_ERR_DTYPE;
   const int64_t k8 = ((int64_t)K + 7) / 8 * 8;
@@ -972,7 +974,6 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
   }
   if (grad_x) {
     const int64_t n = ((int64_t)rows * K + 1023) / 1024;
-    if (n > (1 << 23)) return FB_ERR_SHAPE;
     hipLaunchKernelGGL(head_sum<DT>, dim3((unsigned)n), dim3(256), 0, hs, acc, p.parts, (int)rows, K,
                        undo, lost, in.token, vocab, reinterpret_cast<const uint16_t*>(in.p), in.ldp,
                        grad_x, grad_x_dtype);
@@ -1030,6 +1031,7 @@ int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_
                           void* ws, size_t ws_bytes, void* stream) {
   const int st = head_check(dtype, rows, K, vocab, x_stride, w_stride);
   if (st != FB_OK) return st;
+  if (grad_x && rows * K > kMostSums) return FB_ERR_SHAPE;
   if (rows == 0 || (!grad_x && !grad_w)) return FB_OK;
   if (!x || !w || !token || !stats || (g_entropy && !entropy) || !ws) return FB_ERR_NULL;
   if (bad_align({x, w}, 15) || bad_align({token}, 7) || bad_align({grad_x, grad_w}, 7) ||
@@ -1076,6 +1078,7 @@ int fb_packed_head_grad(const void* wdev, const void* x, const fb_shape_t* s, co
     return FB_ERR_DTYPE;
   st = head_check(s->x_dtype, s->B, s->K, s->N, s->K, s->K);
   if (st != FB_OK) return st;
+  if ((int64_t)s->B * s->K > kMostSums) return FB_ERR_SHAPE;
   if (bad_align({wdev, x, grad_x}, 15) || bad_align({token}, 7) ||
       bad_align({stats, entropy, g_logprob, g_entropy}, 3) || bad_align({ws}, 255))
     return FB_ERR_ALIGN;

@@ -10,6 +10,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -575,6 +576,25 @@ void first_derivative(const char* what) {
   if (at::GradMode::is_enabled()) throw std::runtime_error(what);
 }
 
+// Autograd hands a gradient to an input's node on the stream that the node was made on.  Of a graph that
+// was recorded on another stream and is still alive, that leads out of a capture, which torch ends the
+// process for: refused while it can be.
+void capturable(std::initializer_list<std::optional<at::Tensor>> inputs) {
+  for (const auto& t : inputs) {
+    if (!t || !t->defined() || !t->requires_grad()) continue;
+    const c10::hip::HIPStream now = c10::hip::getCurrentHIPStream(t->device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(now.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone)
+      return;
+    const std::shared_ptr<torch::autograd::Node> node =
+        t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto made = node ? node->stream() : std::nullopt;
+    if (made && *made != now.unwrap())
+      throw std::runtime_error("an autograd graph of this input recorded outside this capture is still "
+                               "alive: drop its results before capturing a backward pass");
+  }
+}
+
 // x as [rows, width], the values of a row side by side and rows a whole stride apart: a view where
 // that can be, else a copy.
 at::Tensor as_rows(const at::Tensor& x) {
@@ -646,6 +666,7 @@ at::Tensor token_embedding(const at::Tensor& tokens, const at::Tensor& weight, d
   const at::Tensor t = flat_tokens(tokens);
   auto sizes = tokens.sizes().vec();
   sizes.push_back(weight.size(1));
+  if (at::GradMode::is_enabled()) capturable({weight});
   return at::GradMode::is_enabled() && weight.requires_grad()
              ? TokenEmbedding::apply(weight, t, sizes, scale)
              : embedding_forward(weight, t, sizes, scale);
@@ -814,6 +835,7 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::
     gate_rows = std::max<int64_t>(1, rows ? M / rows : 1);
   }
   const auto grad = [](const std::optional<at::Tensor>& t) { return t && t->requires_grad(); };
+  if (at::GradMode::is_enabled()) capturable({x, branch, gate, weight, branch_weight});
   std::vector<at::Tensor> r;
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || grad(branch) ||
                                      grad(gate) || grad(branch_weight)))
@@ -1066,7 +1088,7 @@ at::Tensor head_tokens(const at::Tensor& x, const at::Tensor& tokens, int64_t K,
   want(x.dim() >= 1 && x.size(-1) == K, "hidden must be [..., width] with the head's width");
   want(tokens.sizes() == x.sizes().slice(0, x.dim() - 1),
        "tokens must have hidden's shape without the last dimension");
-  want(tokens.numel() <= (1 << 24), "too many tokens");
+  want(tokens.numel() <= (1 << 23), "too many tokens");
   return flat_tokens(tokens);
 }
 
@@ -1081,6 +1103,7 @@ std::tuple<at::Tensor, at::Tensor> head_logprobs(const at::Tensor& hidden, const
   want((hidden.scalar_type() == at::kHalf || hidden.scalar_type() == at::kBFloat16) &&
            hidden.scalar_type() == weight.scalar_type(),
        "hidden and the head's weight must both be float16 or both bfloat16");
+  if (at::GradMode::is_enabled()) capturable({hidden, weight});
   const auto r = at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad())
                      ? HeadLogprobs::apply(hidden, weight, t, tokens.sizes().vec())
                      : head_forward(as_rows(hidden), as_rows(weight), t, tokens.sizes());
@@ -1098,6 +1121,7 @@ std::tuple<at::Tensor, at::Tensor> packed_head_logprobs(const at::Tensor& hidden
   const fb_shape_t s = packed_shape(p, 1, FB_DT_F16, FB_DT_F32);
   want(fb_device_bytes(&s) && (size_t)wdev.numel() >= fb_device_bytes(&s) && s.K <= kMaxGemmK,
        "the packed head is not of its format's size");
+  if (at::GradMode::is_enabled()) capturable({hidden});
   const auto r = at::GradMode::is_enabled() && hidden.requires_grad()
                      ? PackedHeadLogprobs::apply(hidden, wdev, t, tokens.sizes().vec(), N, K, fmt, fwht,
                                                  f16_exact, bf16_exact)

@@ -620,7 +620,7 @@ size_t fb_residual_norm_grad_workspace_bytes(const fb_norm_t* n);
  *   stats  fp32 [rows, 2]: (a, b) with log p = logit - a - ln 2 b, what the gradient needs; NULL: not
  *          wanted
  *   ws     256-byte aligned, fb_head_logprobs_workspace_bytes (its contents are not kept)
- * Products are exact and summed in fp32.  K up to 2^20, vocab up to 2^24, rows up to 2^24. */
+ * Products are exact and summed in fp32.  K up to 2^20, vocab up to 2^24, rows up to 2^23. */
 int fb_head_logprobs(const void* x, int64_t x_stride, const void* w, int64_t w_stride, int32_t dtype,
                      int64_t rows, int32_t K, int32_t vocab, const int64_t* token, float* logprob,
                      float* entropy, float* stats, void* ws, size_t ws_bytes, void* stream);
@@ -634,7 +634,8 @@ size_t fb_head_logprobs_workspace_bytes(int64_t rows, int32_t K, int32_t vocab);
  *   stats, entropy     as fb_head_logprobs wrote them
  *   g_*                fp32 [rows], or NULL (taken as 0)
  *   grad_x, grad_w     [rows, K], [vocab, K] of dtype, contiguous, 8-byte aligned; NULL: not wanted
- *   ws                 256-byte aligned, fb_head_logprobs_grad_workspace_bytes with which are wanted */
+ *   ws                 256-byte aligned, fb_head_logprobs_grad_workspace_bytes with which are wanted
+ * rows x K up to 2^33 where grad_x is wanted. */
 int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
                           int32_t dtype, int64_t rows, int32_t K, int32_t vocab,
                           const int64_t* token, const float* stats, const float* entropy,

@@ -159,3 +159,19 @@ def test_refusals():
         torch.autograd.grad(token_embedding(t, w).square().sum(), w, create_graph=True)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda w: token_embedding(t, w), (w,))
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    """An eager graph of the leaf that is still alive would lead the backward pass out of the capture."""
+    w = torch.randn(9, 4, device="cuda", requires_grad=True)
+    t = torch.tensor([1, 2], device="cuda")
+    alive = token_embedding(t, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph, stream=side):
+            token_embedding(t, w)
+    torch.cuda.synchronize()
+    gw, = torch.autograd.grad(alive.sum(), w)
+    assert float(gw.sum()) == 8

@@ -239,6 +239,20 @@ def test_captured_and_on_another_stream():
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
+def test_capture_beside_an_eager_graph_is_refused():
+    x, w, t, gl, _ = some(20, 50, 24, torch.bfloat16)
+    w.requires_grad_(True)
+    alive = head_logprobs(x, w, t).logprob
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph, stream=side):
+            head_logprobs(x, w, t)
+    torch.cuda.synchronize()
+    assert torch.isfinite(torch.autograd.grad(alive, w, gl)[0]).all()
+
+
 # ------------------------------------------------------------------ packed heads
 def packed_case(fmt, V, K, block=0):
     g = torch.Generator().manual_seed(V)

@@ -282,3 +282,20 @@ def test_refusals():
         torch.autograd.grad(residual_norm(y, w).normed.square().sum(), y, create_graph=True)
     with pytest.raises(RuntimeError, match="traced"):
         torch.jit.trace(lambda x: tuple(residual_norm(x, w, x)), (x,))
+
+
+def test_capture_beside_an_eager_graph_is_refused():
+    x = torch.randn(3, 16, device="cuda", requires_grad=True)
+    w = torch.ones(16, device="cuda")
+    b = torch.randn(3, 16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for made in (lambda: (x, residual_norm(x, w, b).normed), lambda: (2 * x, None)):
+        given, alive = made()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(graph, stream=side):
+                residual_norm(given, w, b)
+        torch.cuda.synchronize()
+        del given, alive
+    assert residual_norm(x, w, b).normed.requires_grad

@@ -95,7 +95,7 @@ def test_head():
 
     for f in (rc, grad):
         assert f(dt=2) == DTYPE and f(dt=-1) == DTYPE
-        assert f(rows=-1) == SHAPE and f(rows=(1 << 24) + 1) == SHAPE and f(K=0) == SHAPE
+        assert f(rows=-1) == SHAPE and f(rows=(1 << 23) + 1) == SHAPE and f(K=0) == SHAPE
         assert f(V=0) == SHAPE and f(V=(1 << 24) + 1) == SHAPE and f(xs=56) == SHAPE
         assert f(K=65, xs=72) == SHAPE and f(wst=1 << 21) == SHAPE
         assert f(xs=68) == ALIGN and f(x=P + 8) == ALIGN and f(w=P + 2) == ALIGN and f(t=P + 4) == ALIGN
@@ -104,11 +104,32 @@ def test_head():
         assert f(nb=0) == WORKSPACE and f(rows=0, x=None) == 0
     assert rc(lp=None) == NULL and rc(ent=None) == NULL
     assert grad(st=None) == NULL and grad(ent=None) == NULL and grad(gw=P + 4) == ALIGN
+    assert grad(rows=1 << 23, K=2048, xs=2048, wst=2048) == SHAPE
     need = L.fb_head_logprobs_workspace_bytes(5, 64, 10)
     assert need > 0 and rc(nb=need - 1) == WORKSPACE
     need = L.fb_head_logprobs_grad_workspace_bytes(5, 64, 10, 1, 1)
     assert need > 0 and grad(nb=need - 1) == WORKSPACE
     assert L.fb_head_logprobs_workspace_bytes(0, 64, 10) == 0
+
+
+def test_packed_head():
+    L = C.lib()
+
+    def rc(wdev=P, x=P, t=P, st=P, ent=P, ge=P, gx=P, gdt=2, ws=P, nb=BIG, **kw):
+        s = C.FbShape(**{**dict(N=32, K=128, B=5, group=32, fmt=1, fwht_block=0, x_dtype=1, y_dtype=2),
+                         **kw})
+        return L.fb_packed_head_grad(wdev, x, ctypes.byref(s), t, st, ent, P, ge, gx, gdt, ws, nb, None)
+
+    assert rc(wdev=None) == NULL and rc(x=None) == NULL and rc(t=None) == NULL and rc(st=None) == NULL
+    assert rc(ent=None) == NULL and rc(gx=None) == NULL and rc(ws=None) == NULL
+    assert rc(K=100) == SHAPE and rc(group=64) == -3 and rc(fmt=7) == -4
+    assert rc(fwht_block=128, x_dtype=0) == -6 and rc(fmt=0, group=128, x_dtype=1) == DTYPE
+    assert rc(gdt=3) == DTYPE and rc(x_dtype=2) == DTYPE
+    assert rc(wdev=P + 8) == ALIGN and rc(gx=P + 8) == ALIGN and rc(ws=P + 16) == ALIGN
+    s = C.FbShape(N=32, K=128, B=5, group=32, fmt=1, fwht_block=0, x_dtype=1, y_dtype=2)
+    need = L.fb_packed_head_grad_workspace_bytes(ctypes.byref(s))
+    assert need > 0 and rc(nb=need - 1) == WORKSPACE
+    assert L.fb_packed_head_grad_workspace_bytes(None) == 0
 
 
 def test_tensors_on_the_cpu_are_refused():
