@@ -1,5 +1,6 @@
 """A small decoder of packed linear layers that answers, from its prompts to the scores of what it
-said: the cache, the attention over it, its eviction and the log probabilities used together.
+said: the embedding, the norms between blocks, the cache, the attention over it, its eviction and the
+log probabilities used together.
 
     python examples/answer.py [--sequences 4] [--prompt 300] [--new 64] [--keep 128]
 
@@ -16,7 +17,8 @@ from torch import nn
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."))
 from if_i_could_turn_back_time_amd import (KVCache, cache_append, cache_attention,  # noqa: E402
-                                           cache_evict, quantize_module, token_logprobs)
+                                           cache_evict, head_logprobs, quantize_module,
+                                           residual_norm, token_embedding, token_logprobs)
 
 
 class Norm(nn.Module):
@@ -24,10 +26,9 @@ class Norm(nn.Module):
         super().__init__()
         self.weight = nn.Parameter(torch.ones(width))
 
-    def forward(self, x):
-        x32 = x.float()
-        x32 = x32 * torch.rsqrt(x32.square().mean(-1, keepdim=True) + 1e-6)
-        return (x32 * self.weight).to(x.dtype)
+    def forward(self, x, branch=None):
+        """The stream x with a block's output added, and its norm, the next block's input."""
+        return residual_norm(x, self.weight, branch)
 
 
 def rotated(x, pos):
@@ -50,16 +51,18 @@ class Block(nn.Module):
         self.up = nn.Linear(width, 4 * width, bias=False)
         self.down = nn.Linear(2 * width, width, bias=False)
 
-    def forward(self, x, pos, cache, seqs, weights):
-        """``seqs``: the sequences' table, what they held before, with these tokens, and the
-        further arguments of the calls."""
+    def forward(self, x, branch, pos, cache, seqs, weights):
+        """The stream x and what the block before this one adds to it; the same of this block.
+        ``seqs``: the sequences' table, what they held before, with these tokens, and the further
+        arguments of the calls."""
         table, before, after, cu, more = seqs
-        q, k, v = self.qkv(self.norm(x)).unflatten(-1, (-1, self.D)).split(self.split, 1)
+        x, y = self.norm(x, branch)
+        q, k, v = self.qkv(y).unflatten(-1, (-1, self.D)).split(self.split, 1)
         cache_append(cache, rotated(k, pos), v, table, before, cu, max_new=more["max_new"])
         y = cache_attention(rotated(q, pos), cache, table, after, cu, weights=weights, **more)
-        x = x + self.out(y.flatten(1))
-        a, b = self.up(self.norm2(x)).chunk(2, -1)
-        return x + self.down(nn.functional.silu(a) * b)
+        x, y = self.norm2(x, self.out(y.flatten(1)))
+        a, b = self.up(y).chunk(2, -1)
+        return x, self.down(nn.functional.silu(a) * b)
 
 
 class Decoder(nn.Module):
@@ -73,13 +76,13 @@ class Decoder(nn.Module):
         self.cached, self.head_dim = cached, head_dim
 
     def hidden(self, tokens, pos, caches, seqs, weights):
-        x = self.embed(tokens)
+        x, branch = token_embedding(tokens, self.embed.weight), None
         for block, cache, w in zip(self.blocks, caches, weights):
-            x = block(x, pos, cache, seqs, w)
-        return x
+            x, branch = block(x, branch, pos, cache, seqs, w)
+        return x + branch
 
     def logits(self, hidden):
-        return self.head(self.norm(hidden))
+        return self.head(self.norm(hidden).normed)
 
 
 class Answers:
@@ -192,7 +195,7 @@ def tune(model: Decoder, texts: list[torch.Tensor], steps: int, rate: float = 0.
     gains = torch.optim.SGD([model.norm.weight], lr=rate)
     losses = []
     for _ in range(steps):
-        r = token_logprobs(model.logits(hidden), following)
+        r = head_logprobs(model.norm(hidden).normed, model.head, following)
         loss = -r.logprob.sum() / (following >= 0).sum()
         gains.zero_grad()
         loss.backward()

@@ -589,7 +589,7 @@ void capturable(std::initializer_list<std::optional<at::Tensor>> inputs) {
     const std::shared_ptr<torch::autograd::Node> node =
         t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto made = node ? node->stream() : std::nullopt;
-    if (made && *made != now.unwrap())
+    if (made && made->id() != now.id())  // (autograd's streams are of another device type by name)
       throw std::runtime_error("an autograd graph of this input recorded outside this capture is still "
                                "alive: drop its results before capturing a backward pass");
   }
