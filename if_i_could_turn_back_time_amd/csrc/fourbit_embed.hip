@@ -294,12 +294,11 @@ __device__ inline void add_rows(const SumArgs& a, unsigned place, int l0, int n,
 
 // Shares of kShare sorted places that are one token's, a wave (and its columns) each.
 template <int DT>
-__global__ __launch_bounds__(256) void token_shares(SumArgs a) {
+__device__ inline void token_shares(const SumArgs& a, int64_t group, int64_t groups) {
   constexpr int V = Of<DT>::V;
   const int lane = threadIdx.x & 63, at = (blockIdx.x * kVecs * 64 + lane) * V;
   const int64_t shares = a.rows / kShare;
-  for (int64_t c = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); c < shares;
-       c += (int64_t)gridDim.y * 4) {
+  for (int64_t c = group * 4 + (threadIdx.x >> 6); c < shares; c += groups * 4) {
     const int64_t i = c * kShare + min(lane, kShare - 1);
     const unsigned k = a.key[i], place = a.place[i];
     const unsigned k0 = __builtin_amdgcn_readfirstlane(k);
@@ -330,12 +329,11 @@ __device__ inline void store_run(const SumArgs& a, unsigned k, int at, float (&s
 // each.
 constexpr int kLong = 32;
 template <int DT>
-__global__ __launch_bounds__(256) void token_runs(SumArgs a) {
+__device__ inline void token_runs(const SumArgs& a, int64_t group, int64_t groups) {
   constexpr int V = Of<DT>::V;
   const int lane = threadIdx.x & 63, at = (blockIdx.x * kVecs * 64 + lane) * V;
   const unsigned none = 0xFFFFFFFFu;
-  for (int64_t i = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); i < a.rows;
-       i += (int64_t)gridDim.y * 4) {
+  for (int64_t i = group * 4 + (threadIdx.x >> 6); i < a.rows; i += groups * 4) {
     const unsigned before = i ? a.key[i - 1] : none;
     const unsigned key = i + lane < a.rows ? a.key[i + lane] : none;
     const unsigned place = i + lane < a.rows ? a.place[i + lane] : 0;
@@ -347,6 +345,15 @@ __global__ __launch_bounds__(256) void token_runs(SumArgs a) {
     add_rows<DT, 8>(a, place, 0, __builtin_ctzll(other), at, s);
     store_run<DT>(a, k, at, s);
   }
+}
+
+// Both in one launch: the first `shares` workgroups of a column sum shares.
+template <int DT>
+__global__ __launch_bounds__(256) void token_sums(SumArgs a, int shares) {
+  if ((int)blockIdx.y < shares)
+    token_shares<DT>(a, blockIdx.y, shares);
+  else
+    token_runs<DT>(a, blockIdx.y - shares, gridDim.y - shares);
 }
 
 // The longer runs, 16 waves each: every wave adds a row before the first whole share, each 16th of the
@@ -440,14 +447,15 @@ dim3 grid_of(int K, int32_t dtype, int64_t rows) {
 template <int DT>
 int run_sums(const SumArgs& a, hipStream_t hs) {
   constexpr int kColumns = 64 * kVecs * Of<DT>::V;
-  const auto grid = [&](int64_t n) {
-    return dim3((a.K + kColumns - 1) / kColumns, (unsigned)std::min<int64_t>((n + 3) / 4, 65535));
+  const unsigned x = (a.K + kColumns - 1) / kColumns;
+  const auto groups = [](int64_t n, int64_t each) {
+    return (int)std::min<int64_t>((n + each - 1) / each, 32767);
   };
-  hipLaunchKernelGGL(token_runs<DT>, grid(a.rows), dim3(256), 0, hs, a);
-  if (a.rows >= kLong) {
-    hipLaunchKernelGGL(token_shares<DT>, grid(a.rows / kShare), dim3(256), 0, hs, a);
-    hipLaunchKernelGGL(token_long_runs<DT>, grid((a.rows + kLong - 1) / kLong * 4), dim3(1024), 0, hs, a);
-  }
+  const bool any_long = a.rows >= kLong;
+  const int shares = any_long ? groups(a.rows / kShare, 4) : 0, runs = groups(a.rows, 4);
+  hipLaunchKernelGGL(token_sums<DT>, dim3(x, shares + runs), dim3(256), 0, hs, a, shares);
+  if (any_long)
+    hipLaunchKernelGGL(token_long_runs<DT>, dim3(x, groups(a.rows, kLong)), dim3(1024), 0, hs, a);
   return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
 }
 
