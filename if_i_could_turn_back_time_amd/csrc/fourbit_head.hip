@@ -15,8 +15,9 @@
 // G in 16 bits costs each of its values half a step; products and all sums are fp32.  One value of a row
 // stands out, the given token's, and its half step alone would be as large as the result's own rounding:
 // what it lost is kept in fp32 and goes into both results, times its row of W (head_sum) or of x (grad_w's
-// tiles end with the rows whose token they hold, which a sort by token finds).  In fp16 each row of G has a power of two of
-// its own that brings it near the type's largest values, and grad_w's x one that takes it off again.
+// tiles end with the rows whose token they hold, which a sort by token finds).  In fp16 each row of G has
+// a power of two of its own that brings it near the type's largest values, and grad_w's x one that takes
+// it off again.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -429,55 +430,55 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
     const auto rows = [&](auto with_entropy) {
       constexpr bool ENT = decltype(with_entropy)::value;
 #pragma unroll
-    for (int j = 0; j < RQ; ++j) {
-      const int r = min(ql + j * 16, a.nq - 1);
-      const bool mine = ql + j * 16 < a.nq;
-      const int64_t token = a.token[r];
-      const bool any = token >= 0 && token < a.vocab;
-      const float g = any && a.g_logprob ? a.g_logprob[r] : 0.f;
-      const float ge = ENT ? a.g_entropy[r] : 0.f;
-      float m, l2z;  // log2 p = (l - m) log2(e) - l2z
-      if (a.three) {
-        // (l - a) log2(e) - R - b, relative to a logit near the largest instead
-        const float off = a.stats[3 * r + 1] * kLn2;
-        m = a.stats[3 * r] + off;
-        l2z = a.stats[3 * r + 2] + __builtin_fmaf(-off, kLog2e, a.stats[3 * r + 1]);
-      } else {
-        m = a.stats[2 * r];
-        l2z = a.stats[2 * r + 1];
-      }
-      const float up = a.scale[r];
-      const float all = -up * (g + (ENT ? ge * a.entropy[r] : 0.f));
-      const float slope = -up * ge * kLn2;
-      const auto value = [&](float l) {
-        const float y = __builtin_fmaf(l - m, kLog2e, -l2z), p = __builtin_amdgcn_exp2f(y);
-        return p * (ENT ? __builtin_fmaf(slope, fmaxf(y, kLow), all) : all);
-      };
-      // a row without a gradient is 0 whatever its logits are
-      const unsigned keep = up == 0.f ? 0u : ~0u;
-#pragma unroll
-      for (int i = 0; i < RP; ++i) {
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[e] = value(acc[i][j][e]);
-          if (!whole && pl + i * 16 + e >= a.np) o[e] = 0.f;
+      for (int j = 0; j < RQ; ++j) {
+        const int r = min(ql + j * 16, a.nq - 1);
+        const bool mine = ql + j * 16 < a.nq;
+        const int64_t token = a.token[r];
+        const bool any = token >= 0 && token < a.vocab;
+        const float g = any && a.g_logprob ? a.g_logprob[r] : 0.f;
+        const float ge = ENT ? a.g_entropy[r] : 0.f;
+        float m, l2z;  // log2 p = (l - m) log2(e) - l2z
+        if (a.three) {
+          // (l - a) log2(e) - R - b, relative to a logit near the largest instead
+          const float off = a.stats[3 * r + 1] * kLn2;
+          m = a.stats[3 * r] + off;
+          l2z = a.stats[3 * r + 2] + __builtin_fmaf(-off, kLog2e, a.stats[3 * r + 1]);
+        } else {
+          m = a.stats[2 * r];
+          l2z = a.stats[2 * r + 1];
         }
-        put(i, j, pack2<DT>(o[0], o[1]) & keep, pack2<DT>(o[2], o[3]) & keep);
-      }
-      const int64_t t = token - a.v0 - pl;  // the given token, from this lane's first one on
-      if (any && keep && t >= 0 && t < RP * 16 && (t & 15) < 4) {
+        const float up = a.scale[r];
+        const float all = -up * (g + (ENT ? ge * a.entropy[r] : 0.f));
+        const float slope = -up * ge * kLn2;
+        const auto value = [&](float l) {
+          const float y = __builtin_fmaf(l - m, kLog2e, -l2z), p = __builtin_amdgcn_exp2f(y);
+          return p * (ENT ? __builtin_fmaf(slope, fmaxf(y, kLow), all) : all);
+        };
+        // a row without a gradient is 0 whatever its logits are
+        const unsigned keep = up == 0.f ? 0u : ~0u;
 #pragma unroll
-        for (int i = 0; i < RP; ++i)
+        for (int i = 0; i < RP; ++i) {
+          float o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (t == i * 16 + e) {
-              const float v = __builtin_fmaf(up, g, value(acc[i][j][e]));
-              put_one(i, j, e, (uint16_t)pack2<DT>(v, 0.f));
-              if (mine) a.lost[r] = v - rounded<DT>(v);
-            }
+          for (int e = 0; e < 4; ++e) {
+            o[e] = value(acc[i][j][e]);
+            if (!whole && pl + i * 16 + e >= a.np) o[e] = 0.f;
+          }
+          put(i, j, pack2<DT>(o[0], o[1]) & keep, pack2<DT>(o[2], o[3]) & keep);
+        }
+        const int64_t t = token - a.v0 - pl;  // the given token, from this lane's first one on
+        if (any && keep && t >= 0 && t < RP * 16 && (t & 15) < 4) {
+#pragma unroll
+          for (int i = 0; i < RP; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (t == i * 16 + e) {
+                const float v = __builtin_fmaf(up, g, value(acc[i][j][e]));
+                put_one(i, j, e, (uint16_t)pack2<DT>(v, 0.f));
+                if (mine) a.lost[r] = v - rounded<DT>(v);
+              }
+        }
       }
-    }
     };
     if (a.g_entropy)
       rows(std::true_type{});

@@ -96,6 +96,21 @@ def test_shapes_types_and_strides():
     check(t, 50, 24, torch.bfloat16, g=gr[:1, :1, :1, :24].expand(3, 5, 7, 24))
 
 
+def test_offsets_beyond_32_bits():
+    V, K = 1_100_000, 2048
+    w = torch.zeros(V, K, device="cuda", dtype=torch.bfloat16)
+    t = torch.tensor([V - 1, 5, V - 2, V - 1, 1048577, 524289], device="cuda")
+    w[t] = torch.randn(6, K, device="cuda").bfloat16()
+    w.requires_grad_(True)
+    out = token_embedding(t, w)
+    assert torch.equal(out, w.detach()[t])
+    g = torch.randint(-8, 9, (6, K), device="cuda").bfloat16()
+    gw, = torch.autograd.grad(out, w, g)
+    assert torch.equal(gw[t], torch.stack([g[0] + g[3], g[1], g[2], g[0] + g[3], g[4], g[5]]))
+    gw[t] = 0
+    assert not gw.view(torch.int16).any()
+
+
 def test_no_tokens():
     w = torch.randn(9, 4, device="cuda", requires_grad=True)
     out = token_embedding(torch.empty(2, 0, dtype=torch.int64, device="cuda"), w)

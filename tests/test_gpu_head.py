@@ -103,6 +103,57 @@ def test_large(M, V, K):
     check(M, V, K, torch.bfloat16)
 
 
+def test_pieces():
+    """More rows than are reduced, and more of G than is held, at once; a sort over memory."""
+    check(20000, 30000, 64, torch.bfloat16)
+
+
+def test_offsets_beyond_32_bits():
+    """A weight of more than 4 GiB, all of it 0 but its last rows."""
+    V, K, M, last = 1_100_000, 2048, 20, 300
+    w = torch.zeros(V, K, device="cuda", dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(3)
+    w[-last:] = (torch.randint(-2, 3, (last, K), generator=g) / 32).bfloat16().cuda()
+    x = (torch.randint(-4, 5, (M, K), generator=g) / 4).bfloat16().cuda()
+    t = torch.randint(V - last, V, (M,), generator=g).cuda()
+    t[::4] = torch.randint(V - last, (5,), generator=g).cuda()
+    gl, ge = torch.randn(2, M, generator=g).cuda()
+    w.requires_grad_(True), x.requires_grad_(True)
+    r = head_logprobs(x, w, t)
+    gx, gw = torch.autograd.grad((r.logprob, r.entropy), (x, w), (gl, ge))
+    xd, wd = x.detach().double(), w.detach()[-last:].double()
+    l = xd @ wd.T
+    top = l.amax(-1, keepdim=True).clamp(min=0)
+    z = (l - top).exp().sum(-1, keepdim=True) + (V - last) * (-top).exp()
+    lse = top + z.log()
+    p, p0 = (l - lse).exp(), (-lse).exp()
+    ent = (-(p * (l - lse)).sum(-1, keepdim=True) + (V - last) * p0 * lse)
+    own = t >= V - last
+    at = (t - (V - last)).clamp(min=0)[:, None]
+    lp = torch.where(own, l.gather(1, at)[:, 0], 0.0) - lse[:, 0]
+    assert_close((r.logprob.detach(), r.entropy.detach()), (lp, ent[:, 0]))
+    gl, ge = gl.double()[:, None], ge.double()[:, None]
+    G = -p * (gl + ge * (l - lse + ent))
+    G.scatter_add_(1, at, torch.where(own[:, None], gl, 0.0))
+    G0 = -p0 * (gl - ge * (lse - ent))
+    half = 2.0 ** -8
+    size = (G.abs() + 1e-3 * (gl.abs() + 24 * ge.abs())).T @ xd.abs()
+    assert ((gw[-last:].double() - G.T @ xd).abs() <= half * (2 * size + (G.T @ xd).abs())).all()
+    rest = (G0.T @ xd)[0]
+    there = torch.zeros(V - last, dtype=torch.bool, device="cuda")
+    there[t[~own]] = True
+    size = (G0.abs().T @ xd.abs())[0]
+    for rows in (slice(0, 3), slice(524286, 524290), slice(1048574, 1048578), slice(V - last - 3, V - last)):
+        err = (gw[rows].double() - rest).abs()
+        assert ((err <= half * 2 * size + 1e-30) | there[rows][:, None]).all()
+    # a token in the part of zeros: its row has the given token's value too
+    for i in torch.nonzero(~own)[:, 0].tolist():
+        want = rest + gl[i] * xd[i]
+        assert ((gw[t[i]].double() - want).abs() <= half * 2 * (size + gl[i].abs() * xd[i].abs())).all()
+    want = G @ wd
+    assert ((gx.double() - want).abs() <= half * 2.1 * (G.abs() @ wd.abs()) + 1e-6).all()
+
+
 def test_only_some_gradients():
     for need in ((True, False), (False, True)):
         x, w, t, gl, ge = some(40, 90, 24, torch.bfloat16)

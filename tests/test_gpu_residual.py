@@ -184,6 +184,25 @@ def test_strides_and_alignment():
     check((3, 100), torch.float32, given={"weight": long[1::2], "branch_weight": long[101:]})
 
 
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes of rows: the last ones are what they are by themselves."""
+    rows, d, n = 1_100_000, 2048, 40
+    def wide():
+        t = torch.zeros(rows, d, device="cuda", dtype=torch.bfloat16)
+        t[-n:] = torch.randn(n, d, device="cuda").bfloat16()
+        return t
+    x, b, gate, gh, gy = (wide() for _ in range(5))
+    w, wb = torch.randn(2, d, device="cuda")
+    got = []
+    for cut in (slice(None), slice(-n, None)):
+        v = [t[cut].requires_grad_(True) for t in (x, b, gate)]
+        r = residual_norm(v[0], w, v[1], gate=v[2], branch_weight=wb)
+        grads = torch.autograd.grad((r.stream, r.normed), v, (gh[cut], gy[cut]))
+        got.append([t[-n:].detach().clone() for t in (r.stream, r.normed, *grads)])
+        del r, grads, v
+    assert all(torch.equal(a, c) for a, c in zip(*got))
+
+
 def test_no_rows():
     x = torch.empty(0, 3, 16, device="cuda", requires_grad=True)
     w = torch.ones(16, device="cuda", requires_grad=True)
