@@ -196,12 +196,18 @@ struct Sums {
   }
 };
 
-// A tile of TP x TQ of p q^T, WP x WQ waves.
-template <int DT, bool PT, bool QT, int TP, int TQ, int WP, int WQ, int MODE>
+// A tile of TP x TQ of p q^T, WP x WQ waves, D chunks staged at a time.  With D > 1 (few rows: the
+// weight's bytes are the work) the tiles begin at chunks of their own and go round: all at the same
+// columns of rows of a power of two of bytes, the requests meet in few of the memory's channels (16 x
+// 32000 x 4096: 61 us, 49 so with D = 2).
+template <int DT, bool PT, bool QT, int TP, int TQ, int WP, int WQ, int D, int MODE>
 __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) {
   constexpr int WAVES = WP * WQ;
   constexpr int RP = TP / WP / 16, RQ = TQ / WQ / 16;
-  __shared__ __align__(1024) uint8_t p0[TP * 128], p1[TP * 128], q0[TQ * 128], q1[TQ * 128];
+  constexpr bool kTurned = D > 1;
+  static_assert(!kTurned || (!PT && !QT && MODE != kProduct), "no parts, and rows of the contraction");
+  __shared__ __align__(1024) uint8_t p0[TP * 128 * D], p1[TP * 128 * D], q0[TQ * 128 * D],
+      q1[TQ * 128 * D];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wp = wave % WP, wq = wave / WP;
@@ -220,15 +226,24 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
   const int tp = in / gq, tq = group * 4 + in % gq;
   const int tp0 = tp * TP, tq0 = tq * TQ;
   const int c0 = part * a.chunks;
-  const int n = min(a.chunks, (a.k + kChunk - 1) / kChunk - c0);
+  const int n = (min(a.chunks, (a.k + kChunk - 1) / kChunk - c0) + D - 1) / D;  // stages
+  // the same for a token in every call: its logits are the same sums in both passes
+  const int turn = kTurned ? (a.v0 + tp0) / 256 % n : 0;
 
   Side<PT, TP, WAVES> sp;
   Side<QT, TQ, WAVES> sq;
   sp.init(wave, lane, a.ldp);
   sq.init(wave, lane, a.ldq);
   const auto request = [&](int c, uint8_t* pb, uint8_t* qb) {
-    sp.stage(a.p, a.ldp, a.np, a.k, tp0, c0 + c, wave, pb);
-    sq.stage(a.q, a.ldq, a.nq, a.k, tq0, c0 + c, wave, qb);
+    if (kTurned) {
+      c += turn;
+      if (c >= n) c -= n;
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      sp.stage(a.p, a.ldp, a.np, a.k, tp0, c0 + c * D + d, wave, pb + d * (TP * 128));
+      sq.stage(a.q, a.ldq, a.nq, a.k, tq0, c0 + c * D + d, wave, qb + d * (TQ * 128));
+    }
   };
   f32x4 acc[RP][RQ];
 #pragma unroll
@@ -257,8 +272,10 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
     }
   };
   const auto step = [&](int c, uint8_t* pb, uint8_t* qb, const uint8_t* pn, const uint8_t* qn) {
-    half(pb, qb, 1, 0);
-    // the next chunk is there, and no wave reads this one any more
+#pragma unroll
+    for (int h = 1; h < 2 * D; ++h)
+      half(pb + (h >> 1) * (TP * 128), qb + (h >> 1) * (TQ * 128), h & 1, (h & 1) ^ 1);
+    // the next stage is there, and no wave reads this one any more
     arrive();
     if (c + 2 < n) request(c + 2, pb, qb);
     half(pn, qn, 0, 1);
@@ -324,7 +341,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) 
   // row: straight from the accumulators (32 bytes of 16 rows each) they took 92 of 486 us of grad_w of
   // 2048 x 32000 x 4096.  The 16-byte units of a row are permuted by its number.
   constexpr int kUnits = RP * 2, kWaveBytes = RP * RQ * 512, kPer = TP * 128 / kWaveBytes;
-  static_assert(kPer >= 1 && (kPer >= WAVES || (TP == TQ && kPer * 4 >= WAVES)), "all waves' parts fit");
+  static_assert(kPer >= 1 && (kPer * 2 >= WAVES || (TP == TQ && kPer * 4 >= WAVES)), "all waves' parts fit");
   uint8_t* const mine_lds = (wave / kPer == 0   ? p0
                              : wave / kPer == 1 ? p1
                              : wave / kPer == 2 ? q0
@@ -733,9 +750,10 @@ constexpr int64_t kMostG = 1ll << 30;       // bytes of G at once
 constexpr int64_t kMostRows = 1 << 23;      // 256 threads each stay below a launch's 2^32
 constexpr int64_t kStatRows = 1 << 14;      // rows of logits whose parts are held at once
 
-// Tiles to choose from, with what a workgroup of each takes in us: a chunk of the contraction with all
-// of a CU's workgroups running and with one, where the contraction lies along rows and where (TR) not, and
-// the rest.  Fitted to timings of the four products of 2048 x 32000 x 4096, 1024 x 32000 x 4096, 4096 x
+// Tiles to choose from: two for any product, two for few rows of grad_x, three for few rows of logits.
+// With what a workgroup takes in us, of those that are chosen by it: a chunk of the contraction with all of
+// a CU's workgroups running and with one, where the contraction lies along rows and where (TR) not, and the
+// rest.  Fitted to timings of the four products of 2048 x 32000 x 4096, 1024 x 32000 x 4096, 4096 x
 // 131072 x 4096 and 777 x 50001 x 1000.
 struct Shape {
   int tp, tq, slots;  // workgroups of a CU
@@ -744,7 +762,10 @@ struct Shape {
 constexpr Shape kShapes[] = {{256, 256, 1, 1.55, 1.55, 1.5, 1.5, 9},
                              {128, 128, 2, 0.95, 0.75, 1.13, 0.85, 7},
                              {128, 64, 2, 0.8, 0.6, 0.9, 0.7, 6},
-                             {128, 16, 4, 0.8, 0.4, 0.8, 0.4, 5}};
+                             {128, 16, 4, 0.8, 0.4, 0.8, 0.4, 5},
+                             {64, 64, 2, 0, 0, 0, 0, 0},
+                             {128, 16, 2, 0, 0, 0, 0, 0},
+                             {64, 16, 4, 0, 0, 0, 0, 0}};
 
 double product_us(int shape, bool tr, int64_t np, int64_t nq, int64_t k, int parts, int cus) {
   const Shape& s = kShapes[shape];
@@ -755,10 +776,16 @@ double product_us(int shape, bool tr, int64_t np, int64_t nq, int64_t k, int par
          (left ? chunks * (left <= cus ? alone : full) + s.rest : 0.0);
 }
 
-int pick_shape(bool tr, int64_t np, int64_t nq, int64_t k, int cus) {
-  if (nq <= 16) return 3;
-  if (nq <= 64) return 2;
+int pick_wide(bool tr, int64_t np, int64_t nq, int64_t k, int cus) {
   return nq <= 128 || product_us(1, tr, np, nq, k, 1, cus) < product_us(0, tr, np, nq, k, 1, cus);
+}
+
+// Of logits.  Tiles of 64 tokens up to one of 128 a CU: 16 x 32000 x 4096 44.4 us, by 128 tokens 48.8;
+// 16 x 131072 x 4096 182 and 171.
+int pick_shape(int64_t np, int64_t nq, int64_t k, int cus) {
+  if (nq <= 16) return (np + 127) / 128 <= cus ? 6 : 5;
+  if (nq <= 64) return 4;
+  return pick_wide(false, np, nq, k, cus);
 }
 
 template <int DT, bool PT, bool QT, int MODE>
@@ -773,11 +800,16 @@ int launch_product(ProductArgs a, int shape, int parts, hipStream_t hs) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), 0, hs, a);
     return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
   };
-  if (shape == 0) return go(product_kernel<DT, PT, QT, 256, 256, 2, 4, MODE>, 512);
-  if (shape == 1) return go(product_kernel<DT, PT, QT, 128, 128, 2, 2, MODE>, 256);
-  if constexpr (!QT) {
-    if (shape == 2) return go(product_kernel<DT, PT, QT, 128, 64, 4, 1, MODE>, 256);
-    return go(product_kernel<DT, PT, QT, 128, 16, 4, 1, MODE>, 256);
+  if (shape == 0) return go(product_kernel<DT, PT, QT, 256, 256, 2, 4, 1, MODE>, 512);
+  if (shape == 1) return go(product_kernel<DT, PT, QT, 128, 128, 2, 2, 1, MODE>, 256);
+  if constexpr (MODE == kProduct && !QT) {
+    if (shape == 2) return go(product_kernel<DT, PT, QT, 128, 64, 4, 1, 1, MODE>, 256);
+    if (shape == 3) return go(product_kernel<DT, PT, QT, 128, 16, 4, 1, 1, MODE>, 256);
+  }
+  if constexpr (MODE != kProduct) {
+    if (shape == 4) return go(product_kernel<DT, PT, QT, 64, 64, 2, 2, 2, MODE>, 256);
+    if (shape == 5) return go(product_kernel<DT, PT, QT, 128, 16, 4, 1, 2, MODE>, 256);
+    if (shape == 6) return go(product_kernel<DT, PT, QT, 64, 16, 2, 1, 2, MODE>, 128);
   }
   return FB_ERR_SHAPE;
 }
@@ -792,7 +824,7 @@ struct StatPlan {
 StatPlan stat_plan(int64_t rows, int K, int vocab, int cus) {
   StatPlan p{};
   p.rows = std::min(rows, kStatRows);
-  p.shape = pick_shape(false, vocab, p.rows, K, cus);
+  p.shape = pick_shape(vocab, p.rows, K, cus);
   const Shape s = kShapes[p.shape];
   p.parts = (vocab + s.tp - 1) / s.tp;
   p.part_bytes = up256((size_t)p.parts * p.rows * 4);
@@ -811,8 +843,8 @@ GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
   const int64_t v256 = ((int64_t)vocab + 255) / 256 * 256;
   p.piece = std::min(v256, std::max<int64_t>(256, kMostG / (rows * 2) / 256 * 256));
   const int64_t most = std::min<int64_t>(p.piece, vocab);
-  p.gshape = pick_shape(false, most, rows, K, cus);
-  p.wshape = product_us(1, true, K, most, rows, 1, cus) < product_us(0, true, K, most, rows, 1, cus);
+  p.gshape = pick_shape(most, rows, K, cus);
+  p.wshape = pick_wide(true, K, most, rows, cus);
   p.parts = 1;
   if (gx) {
     const int64_t chunks = (most + kChunk - 1) / kChunk;
