@@ -201,7 +201,7 @@ struct Sums {
 // columns of rows of a power of two of bytes, the requests meet in few of the memory's channels (16 x
 // 32000 x 4096: 61 us, 49 so with D = 2).
 template <int DT, bool PT, bool QT, int TP, int TQ, int WP, int WQ, int D, int MODE>
-__global__ __launch_bounds__(WP* WQ * 64, 2) void product_kernel(ProductArgs a) {
+__global__ __launch_bounds__(WP* WQ * 64, D * TP * TQ == 32768 ? 1 : 2) void product_kernel(ProductArgs a) {
   constexpr int WAVES = WP * WQ;
   constexpr int RP = TP / WP / 16, RQ = TQ / WQ / 16;
   constexpr bool kTurned = D > 1;
@@ -750,7 +750,7 @@ constexpr int64_t kMostG = 1ll << 30;       // bytes of G at once
 constexpr int64_t kMostRows = 1 << 23;      // 256 threads each stay below a launch's 2^32
 constexpr int64_t kStatRows = 1 << 14;      // rows of logits whose parts are held at once
 
-// Tiles to choose from: two for any product, two for few rows of grad_x, three for few rows of logits.
+// Tiles to choose from: two for any product, two for few rows of grad_x, four for few rows of logits.
 // With what a workgroup takes in us, of those that are chosen by it: a chunk of the contraction with all of
 // a CU's workgroups running and with one, where the contraction lies along rows and where (TR) not, and the
 // rest.  Fitted to timings of the four products of 2048 x 32000 x 4096, 1024 x 32000 x 4096, 4096 x
@@ -765,7 +765,8 @@ constexpr Shape kShapes[] = {{256, 256, 1, 1.55, 1.55, 1.5, 1.5, 9},
                              {128, 16, 4, 0.8, 0.4, 0.8, 0.4, 5},
                              {64, 64, 2, 0, 0, 0, 0, 0},
                              {128, 16, 2, 0, 0, 0, 0, 0},
-                             {64, 16, 4, 0, 0, 0, 0, 0}};
+                             {64, 16, 4, 0, 0, 0, 0, 0},
+                             {128, 128, 1, 0, 0, 0, 0, 0}};
 
 double product_us(int shape, bool tr, int64_t np, int64_t nq, int64_t k, int parts, int cus) {
   const Shape& s = kShapes[shape];
@@ -781,10 +782,13 @@ int pick_wide(bool tr, int64_t np, int64_t nq, int64_t k, int cus) {
 }
 
 // Of logits.  Tiles of 64 tokens up to one of 128 a CU: 16 x 32000 x 4096 44.4 us, by 128 tokens 48.8;
-// 16 x 131072 x 4096 182 and 171.
+// 16 x 131072 x 4096 182 and 171.  Two chunks of 128 x 128 at a time, one tile a CU, where there are no
+// more: 128 x 32000 x 4096 58 us, one chunk 71; 128 x 131072 x 4096 231 and 186.
 int pick_shape(int64_t np, int64_t nq, int64_t k, int cus) {
-  if (nq <= 16) return (np + 127) / 128 <= cus ? 6 : 5;
+  const bool few = (np + 127) / 128 <= cus;
+  if (nq <= 16) return few ? 6 : 5;
   if (nq <= 64) return 4;
+  if (nq <= 128 && few) return 7;
   return pick_wide(false, np, nq, k, cus);
 }
 
@@ -807,6 +811,7 @@ int launch_product(ProductArgs a, int shape, int parts, hipStream_t hs) {
     if (shape == 3) return go(product_kernel<DT, PT, QT, 128, 16, 4, 1, 1, MODE>, 256);
   }
   if constexpr (MODE != kProduct) {
+    if (shape == 7) return go(product_kernel<DT, PT, QT, 128, 128, 2, 2, 2, MODE>, 256);
     if (shape == 4) return go(product_kernel<DT, PT, QT, 64, 64, 2, 2, 2, MODE>, 256);
     if (shape == 5) return go(product_kernel<DT, PT, QT, 128, 16, 4, 1, 2, MODE>, 256);
     if (shape == 6) return go(product_kernel<DT, PT, QT, 64, 16, 2, 1, 2, MODE>, 128);

@@ -103,6 +103,13 @@ def test_large(M, V, K):
     check(M, V, K, torch.bfloat16)
 
 
+@pytest.mark.parametrize("M", [1, 16, 40, 64, 100])
+@pytest.mark.parametrize("V, K", [(3000, 64), (3000, 200), (3000, 328), (1800, 1096), (34000, 200)])
+def test_few_rows(M, V, K):
+    """Tiles that begin at different columns, of which the last may be less than a stage."""
+    check(M, V, K, torch.float16 if K == 328 else torch.bfloat16)
+
+
 def test_pieces():
     """More rows than are reduced, and more of G than is held, at once; a sort over memory."""
     check(20000, 30000, 64, torch.bfloat16)
