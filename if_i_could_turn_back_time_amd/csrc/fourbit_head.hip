@@ -234,6 +234,15 @@ __global__ __launch_bounds__(WP* WQ * 64, D * TP * TQ == 32768 ? 1 : 2) void pro
   Side<QT, TQ, WAVES> sq;
   sp.init(wave, lane, a.ldp);
   sq.init(wave, lane, a.ldq);
+  // grad_w: the rows whose given tokens are of this tile, sorted places s0 to s1.  What is needed of
+  // the first 64 of them after the products is asked for before them.
+  constexpr bool kLost = MODE == kProduct && QT;
+  constexpr int kParts = WAVES * 64 / kChunk;  // threads of a row
+  __shared__ int place_lds[kLost ? kChunk : 1];
+  const int s0 = kLost ? a.start[min((a.v0 + tq0) / 128, a.starts)] : 0;
+  const int s1 = kLost ? a.start[min((a.v0 + tq0 + TQ) / 128, a.starts)] : 0;
+  int key = 0, place = 0;
+  float lost = 0.f;
   const auto request = [&](int c, uint8_t* pb, uint8_t* qb) {
     if (kTurned) {
       c += turn;
@@ -282,7 +291,16 @@ __global__ __launch_bounds__(WP* WQ * 64, D * TP * TQ == 32768 ? 1 : 2) void pro
   };
   if (n > 0) {
     request(0, p0, q0);
+    if (kLost && s1 > s0) {
+      const int i = min(s0 + (int)threadIdx.x / kParts, s1 - 1);
+      key = a.key[i];
+      place = a.place[i];
+    }
     arrive();
+    if (kLost && s1 > s0) {
+      lost = a.lost[place];
+      place_lds[threadIdx.x / kParts] = place;
+    }
     if (n > 1) request(1, p1, q1);
 #pragma unroll
     for (int i = 0; i < RP + RQ; ++i) read(p0, q0, 0, 0, i);
@@ -292,33 +310,42 @@ __global__ __launch_bounds__(WP* WQ * 64, D * TP * TQ == 32768 ? 1 : 2) void pro
     }
   }
 
-  if constexpr (MODE == kProduct && QT) {
-    // What the rows' given tokens lost, of the tokens in this tile: 64 rows at a time as one more chunk,
-    // with one value of q in each.
-    const int s0 = a.start[min((a.v0 + tq0) / 128, a.starts)];
-    const int s1 = a.start[min((a.v0 + tq0 + TQ) / 128, a.starts)];
+  if constexpr (kLost) {
+    // What they lost, as chunks of 64 rows more, with one value of q in each.
     for (int at = s0; at < s1; at += kChunk) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < TQ * 8; i += WAVES * 64)
-        reinterpret_cast<u32x4*>(q0)[i] = u32x4{0, 0, 0, 0};
+      const int k = threadIdx.x / kParts;
+      if (at != s0) {
+        const int i = min(at + k, s1 - 1);
+        key = a.key[i];
+        place = a.place[i];
+        lost = a.lost[place];
+      }
+      __syncthreads();  // no wave reads a tile, or places, any more
+      if (at != s0) {
+        place_lds[k] = place;
+        __syncthreads();
+      }
 #pragma unroll
       for (int j = 0; j < sp.kRequests; ++j) {
         constexpr int PER = TP / 8;
-        const int i = wave * sp.kRequests + j, k = i * (64 / PER) + lane / PER;
-        const int w = ((lane % PER) >> 1) ^ row_mask(k);
+        const int i = wave * sp.kRequests + j, r = i * (64 / PER) + lane / PER;
+        const int w = ((lane % PER) >> 1) ^ row_mask(r);
         const int64_t col = tp0 + w * 16 + (lane & 1) * 8;
-        const int64_t row = a.place[min(at + k, s1 - 1)];
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(a.p + (row * a.ldp +
+            (const __attribute__((address_space(1))) void*)(a.p + (place_lds[r] * a.ldp +
                                                                    (col < a.ldp ? col : 0)) * 2),
             (__attribute__((address_space(3))) void*)(p0 + i * 1024), 16, 0, 0);
       }
-      __syncthreads();
-      const int k = threadIdx.x;
-      if (k < kChunk && at + k < s1) {
-        const int v = (int)a.key[at + k] - a.v0 - tq0;
-        reinterpret_cast<uint16_t*>(q0)[k * TQ + ((v >> 4) ^ row_mask(k)) * 16 + (v & 15)] =
-            (uint16_t)pack2<DT>(a.lost[a.place[at + k]], 0.f);
+      const int v = key - a.v0 - tq0;
+      const unsigned value = at + k < s1 ? pack2<DT>(lost, 0.f) << (16 * (v & 1)) : 0u;
+#pragma unroll
+      for (int e = 0; e < TQ / 8 / kParts; ++e) {
+        const int u = threadIdx.x % kParts * (TQ / 8 / kParts) + e;  // 8 values
+        const bool here = (u >> 1) == ((v >> 4) ^ row_mask(k)) && (u & 1) == ((v >> 3) & 1);
+        u32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = here && ((v >> 1) & 3) == j ? value : 0u;
+        *reinterpret_cast<u32x4*>(q0 + k * (TQ * 2) + u * 16) = o;
       }
       arrive();
 #pragma unroll
