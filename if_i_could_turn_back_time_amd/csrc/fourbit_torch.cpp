@@ -962,7 +962,8 @@ at::Tensor packed_rows(const Packed& p, const at::Tensor& x) {
   const int64_t kp = (p.K + 127) / 128 * 128;
   const at::Tensor c = x.contiguous();
   if (kdt == xdt && kp == p.K && !(reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u)) return c;
-  at::Tensor out = at::empty({x.size(0), kp}, x.options().dtype(kdt == FB_DT_F16 ? at::kHalf : at::kBFloat16));
+  at::Tensor out =
+      at::empty({x.size(0), kp}, x.options().dtype(kdt == FB_DT_F16 ? at::kHalf : at::kBFloat16));
   check(fb_cast_rows(c.data_ptr(), xdt, (int32_t)x.size(0), (int32_t)p.K, out.data_ptr(), kdt, (int32_t)kp,
                      stream_of(x)));
   return out;
@@ -1042,7 +1043,8 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
     const int xdt = dtype_code(x.scalar_type());
     const at::Tensor xk = M ? packed_rows(p, x) : at::Tensor();
     // the weight in 16 bits, as x, where it is exact there and not rotated; else in fp32 terms
-    const bool exact = p.fmt != FB_FMT_E2M1 || !M || (xk.scalar_type() == at::kHalf ? p.f16_exact : p.bf16_exact);
+    const bool exact = p.fmt != FB_FMT_E2M1 || !M ||
+                       (xk.scalar_type() == at::kHalf ? p.f16_exact : p.bf16_exact);
     if (M && !p.fwht && exact) {
       fb_shape_t sh = packed_shape(p, M, dtype_code(xk.scalar_type()), FB_DT_F32);
       const size_t need = fb_packed_head_grad_workspace_bytes(&sh);
@@ -1068,8 +1070,9 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
             f32_of(ent) + r, g[0].defined() ? f32_of(g[0]) + r : nullptr,
             g[1].defined() ? f32_of(g[1]) + r : nullptr, nullptr, gl.data_ptr(), stream_of(x)));
         sh.B = (int32_t)n;
-        check(fb_grad_x(p.wdev.data_ptr(), gl.data_ptr(), static_cast<char*>(gx.data_ptr()) + r * kp * gx.element_size(),
-                        &sh, xdt, p.f16_exact, ws.data_ptr(), need, stream_of(x)));
+        check(fb_grad_x(p.wdev.data_ptr(), gl.data_ptr(),
+                        static_cast<char*>(gx.data_ptr()) + r * kp * gx.element_size(), &sh, xdt,
+                        p.f16_exact, ws.data_ptr(), need, stream_of(x)));
       }
     }
     if (kp != p.K) gx = gx.narrow(1, 0, p.K).contiguous();
