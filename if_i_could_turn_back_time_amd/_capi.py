@@ -48,7 +48,7 @@ EXPORTED = (
     "fb_cache_evict", "fb_token_logprobs", "fb_token_logprobs_grad",
     "fb_embed", "fb_embed_grad", "fb_embed_grad_workspace_bytes",
     "fb_residual_norm", "fb_residual_norm_grad", "fb_residual_norm_grad_workspace_bytes",
-    "fb_head_logprobs", "fb_head_logprobs_workspace_bytes", "fb_head_logprobs_grad",
+    "fb_pad_rows", "fb_head_logprobs", "fb_head_logprobs_workspace_bytes", "fb_head_logprobs_grad",
     "fb_head_logprobs_grad_workspace_bytes", "fb_packed_head_grad",
     "fb_packed_head_grad_workspace_bytes",
 )
@@ -164,6 +164,7 @@ def lib() -> ctypes.CDLL:
         "fb_residual_norm_grad_workspace_bytes": (sz, [np_]),
         "fb_head_logprobs": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i32, i32, vp, vp, vp, vp,
                                             vp, sz, vp]),
+        "fb_pad_rows": (ctypes.c_int, [vp, i64, i64, i32, vp, i64, vp]),
         "fb_head_logprobs_workspace_bytes": (sz, [i64, i32, i32]),
         "fb_head_logprobs_grad": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i32, i32, vp, vp, vp,
                                                  vp, vp, vp, vp, vp, sz, vp]),

@@ -625,10 +625,15 @@ __global__ __launch_bounds__(1024) void head_join(const float* __restrict__ pm,
 __global__ __launch_bounds__(256) void head_starts(const unsigned* __restrict__ key, int rows,
                                                    int vocab, int tiles, unsigned* __restrict__ start) {
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i > rows) return;
-  const auto tile = [&](int at) { return key[at] >= (unsigned)vocab ? tiles : (int)(key[at] / 128); };
-  const int from = i ? tile(i - 1) + 1 : 0, to = i < rows ? tile(i) : tiles;
-  for (int t = from; t <= to; ++t) start[t] = i;
+  if (i > tiles) return;
+  const unsigned from = min((unsigned)vocab, 128u * i);
+  int lo = 0, hi = rows;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (key[mid] < from) lo = mid + 1;
+    else hi = mid;
+  }
+  start[i] = lo;
 }
 
 // A packed weight in 16 bits, [N, K], a block of 16 rows by 512 columns a wave: lane L has row L % 16 of
@@ -759,6 +764,7 @@ __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, i
   if ((K & 3) == 0) {
     const int64_t r = i / K, t = token[r];
     f32x4 s = *reinterpret_cast<const f32x4*>(acc + i);
+#pragma unroll 8
     for (int p = 1; p < parts; ++p) s += *reinterpret_cast<const f32x4*>(acc + p * n + i);
     const float l = lost[r];
     if (l != 0.f && t >= 0 && t < vocab) {
@@ -772,10 +778,33 @@ __global__ __launch_bounds__(256) void head_sum(const float* __restrict__ acc, i
     for (int64_t at = i; at < n && at < i + 4; ++at) {
       const int64_t r = at / K, t = token[r];
       float s = acc[at];
+#pragma unroll 8
       for (int p = 1; p < parts; ++p) s += acc[p * n + at];
       if (lost[r] != 0.f && t >= 0 && t < vocab) s += lost[r] * value(w[t * ldw + (at - r * K)]);
       store_y(out, at, s * undo[r], odt);
     }
+  }
+}
+
+// Rows of 16-bit values, zeros behind them: `rows_of` rows of `units` 8 values a workgroup.  102177 x 3002:
+// 248 us, 4.9 TB/s.
+__global__ __launch_bounds__(256) void head_pad(const uint16_t* __restrict__ src, int64_t stride,
+                                                int64_t rows, int K, uint16_t* __restrict__ dst,
+                                                int64_t ld, unsigned units, unsigned rows_of) {
+  const int64_t r0 = (int64_t)blockIdx.x * rows_of;
+  for (unsigned i = threadIdx.x; i < units * rows_of; i += 256) {
+    const unsigned y = i / units, u = i - y * units;
+    if (r0 + y >= rows) break;
+    const uint16_t* const from = src + (r0 + y) * stride + u * 8;
+    u32x4 v{0, 0, 0, 0};
+    if ((int)(u * 8 + 8) <= K) {
+      v = *reinterpret_cast<const u32x4_any*>(from);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if ((int)(u * 8) + e < K) v[e / 2] |= (unsigned)from[e] << (16 * (e & 1));
+    }
+    *reinterpret_cast<u32x4*>(dst + (r0 + y) * ld + u * 8) = v;
   }
 }
 
@@ -992,7 +1021,7 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
   if (grad_w) {
     const int st = fb_gpu::sort_tokens(in.token, rows, vocab, key, place, nullptr, 0, ws + p.at_sort, hs);
     if (st != FB_OK) return st;
-    hipLaunchKernelGGL(head_starts, dim3((unsigned)(rows / 256 + 1)), dim3(256), 0, hs, key, (int)rows,
+    hipLaunchKernelGGL(head_starts, dim3((unsigned)(starts / 256 + 1)), dim3(256), 0, hs, key, (int)rows,
                        vocab, starts, start);
     if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   }
@@ -1129,6 +1158,20 @@ int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_
                                    hs)
              : run_grad<FB_DT_BF16>(a, p, rows, K, vocab, grad_x, dtype, grad_w, static_cast<uint8_t*>(ws),
                                     hs);
+}
+
+int fb_pad_rows(const void* src, int64_t src_stride, int64_t rows, int32_t K, void* dst,
+                int64_t dst_stride, void* stream) {
+  if (!src || !dst) return FB_ERR_NULL;
+  if (rows < 1 || rows > (1 << 24) || K < 1 || K > (1 << 20) || src_stride < 0 ||
+      src_stride > (1ll << 40) || dst_stride < K || dst_stride > (1 << 20) || dst_stride % 8)
+    return FB_ERR_SHAPE;
+  if (bad_align({src}, 1) || bad_align({dst}, 15)) return FB_ERR_ALIGN;
+  const unsigned units = (unsigned)(K + 7) / 8, rows_of = std::max(1u, 1024 / units);
+  hipLaunchKernelGGL(head_pad, dim3((unsigned)((rows + rows_of - 1) / rows_of)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), static_cast<const uint16_t*>(src), src_stride,
+                     rows, K, static_cast<uint16_t*>(dst), dst_stride, units, rows_of);
+  return hipGetLastError() == hipSuccess ? FB_OK : FB_ERR_HIP;
 }
 
 size_t fb_packed_head_grad_workspace_bytes(const fb_shape_t* s) {

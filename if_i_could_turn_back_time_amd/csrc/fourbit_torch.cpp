@@ -852,23 +852,23 @@ at::Tensor head_side(const at::Tensor& t) {
   if (K % 8 == 0 && row_stride(t) % 8 == 0 && row_stride(t) >= K && row_stride(t) <= (1 << 20) &&
       !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u))
     return t;
-  const int64_t ld = (K + 127) / 128 * 128;
-  const at::Tensor c = t.contiguous();
-  at::Tensor out = at::empty({t.size(0), ld}, c.options());
-  const int dt = dtype_code(t.scalar_type());
-  check(fb_cast_rows(c.data_ptr(), dt, (int32_t)t.size(0), (int32_t)K, out.data_ptr(), dt, (int32_t)ld,
-                     stream_of(t)));
+  const int64_t ld = (K + 7) / 8 * 8;
+  at::Tensor out =
+      at::empty({t.size(0), ld}, t.options().memory_format(at::MemoryFormat::Contiguous));
+  check(fb_pad_rows(t.data_ptr(), row_stride(t), t.size(0), (int32_t)K, out.data_ptr(), ld,
+                    stream_of(t)));
   return out;
 }
 
-// logprob, entropy (of the tokens' shape), stats for rows x.
+// logprob, entropy (of the tokens' shape), stats for rows x; and x and w as the products take them (the
+// gradient's take them again: a copy, where one was made, is kept for it).
 std::vector<at::Tensor> head_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& token,
                                      at::IntArrayRef sizes) {
   c10::DeviceGuard guard(x.device());
   const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
   const auto f = x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
   at::Tensor lp = at::empty(sizes, f), ent = at::empty(sizes, f), st = at::empty({M, 2}, f);
-  if (M == 0) return {lp, ent, st};
+  if (M == 0) return {lp, ent, st, x, w};
   const at::Tensor xs = head_side(x), ws_ = head_side(w);
   const size_t need = fb_head_logprobs_workspace_bytes(M, (int32_t)K, (int32_t)V);
   const at::Tensor ws = scratch(need, x);
@@ -877,7 +877,7 @@ std::vector<at::Tensor> head_forward(const at::Tensor& x, const at::Tensor& w, c
                          static_cast<const int64_t*>(token.data_ptr()),
                          static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()),
                          static_cast<float*>(st.data_ptr()), ws.data_ptr(), need, stream_of(x)));
-  return {lp, ent, st};
+  return {lp, ent, st, xs, ws_};
 }
 
 const float* f32_of(const at::Tensor& t) {
@@ -891,7 +891,7 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
                                                 const std::vector<int64_t>& sizes) {
     const at::Tensor x = as_rows(hidden), w = as_rows(weight);
     const auto r = head_forward(x, w, token, sizes);
-    ctx->save_for_backward({x, w, token, r[1], r[2]});
+    ctx->save_for_backward({x, w, token, r[1], r[2], r[3], r[4]});
     ctx->saved_data["sizes"] = hidden.sizes().vec();
     ctx->set_materialize_grads(false);
     return {r[0], r[1]};
@@ -901,6 +901,7 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
     first_derivative("head_logprobs has no second derivative");
     const auto s = ctx->get_saved_variables();
     const at::Tensor &x = s[0], &w = s[1], &token = s[2], &ent = s[3], &st = s[4];
+    const at::Tensor &xs = s[5], &ws_ = s[6];
     c10::DeviceGuard guard(x.device());
     at::Tensor g[2];
     for (int i = 0; i < 2; ++i)
@@ -915,7 +916,6 @@ struct HeadLogprobs : torch::autograd::Function<HeadLogprobs> {
       if (M == 0) gw.zero_();
     }
     if (M) {
-      const at::Tensor xs = head_side(x), ws_ = head_side(w);
       const size_t need = fb_head_logprobs_grad_workspace_bytes(M, (int32_t)K, (int32_t)V,
                                                                 gx.defined(), gw.defined());
       const at::Tensor ws = scratch(need, x);

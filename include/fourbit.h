@@ -626,6 +626,12 @@ int fb_head_logprobs(const void* x, int64_t x_stride, const void* w, int64_t w_s
                      float* entropy, float* stats, void* ws, size_t ws_bytes, void* stream);
 size_t fb_head_logprobs_workspace_bytes(int64_t rows, int32_t K, int32_t vocab);
 
+/* Rows of 16-bit values as fb_head_logprobs takes them, from rows of any width, stride (elements) and
+ * 2-byte alignment: K values of each and zeros up to the next multiple of 8.  dst: 16-byte aligned, a
+ * stride that is a multiple of 8.  K up to 2^20, rows up to 2^24. */
+int fb_pad_rows(const void* src, int64_t src_stride, int64_t rows, int32_t K, void* dst,
+                int64_t dst_stride, void* stream);
+
 /* The gradient: with G[r, v] as fb_token_logprobs_grad's (no alternatives), grad_x = G w and
  * grad_w = G^T x.  The logits are computed again, a piece of the vocabulary at a time; G enters the
  * products rounded to dtype (fp16: times a power of two of its row), but for the given token's value,

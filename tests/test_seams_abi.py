@@ -112,6 +112,19 @@ def test_head():
     assert L.fb_head_logprobs_workspace_bytes(0, 64, 10) == 0
 
 
+def test_pad_rows():
+    L = C.lib()
+
+    def rc(src=P + 2, stride=7, rows=5, K=7, dst=P, ld=8):
+        return L.fb_pad_rows(src, stride, rows, K, dst, ld, None)
+
+    assert rc(src=None) == NULL and rc(dst=None) == NULL
+    assert rc(rows=0) == SHAPE and rc(rows=(1 << 24) + 1) == SHAPE and rc(K=0) == SHAPE
+    assert rc(K=9) == SHAPE and rc(ld=12) == SHAPE and rc(stride=-1) == SHAPE
+    assert rc(K=(1 << 20) + 1, ld=(1 << 20) + 8) == SHAPE
+    assert rc(src=P + 1) == ALIGN and rc(dst=P + 8) == ALIGN
+
+
 def test_packed_head():
     L = C.lib()
 
