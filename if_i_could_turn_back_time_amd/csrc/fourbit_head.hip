@@ -199,10 +199,10 @@ struct Sums {
 };
 
 // A tile of TP x TQ of p q^T, WP x WQ waves, D chunks staged at a time.  Operands go from memory straight
-// to LDS, a chunk ahead, and from there to registers half a chunk ahead of the products.  256 x 256 is the
-// least tile whose requests the memory side keeps up with: 4096 x 131072 x 4096 takes 3.3 ms (1.32
-// PFLOP/s, matrix instructions two thirds of the cycles) as kStats, 3.5 as kGradient, 3.1 for grad_x and
-// 3.5 for grad_w; without its requests the loop runs at 1.7 to 2.2 PFLOP/s.  With D > 1 (few rows: the
+// to LDS, a chunk ahead, and from there to registers half a chunk ahead of the products.  What bounds
+// the large tiles is requests: 4096 x 131072 x 4096 takes 3.3 ms (1.32 PFLOP/s, matrix instructions two
+// thirds of the cycles) as kStats, 3.5 as kGradient, 3.1 for grad_x and 3.5 for grad_w, where 128 x 128
+// takes 4.0 to 4.4; without its requests the loop runs at 1.7 to 2.2 PFLOP/s.  With D > 1 (few rows: the
 // weight's bytes are the work) the tiles begin at chunks of their own and go round: all at the same
 // columns of rows of a power of two of bytes, the requests meet in few of the memory's channels (16 x
 // 32000 x 4096: 61 us, 49 so with D = 2).
