@@ -1074,6 +1074,12 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
                         static_cast<char*>(gx.data_ptr()) + r * kp * gx.element_size(), &sh, xdt,
                         p.f16_exact, ws.data_ptr(), need, stream_of(x)));
       }
+      // rows that nothing comes in for, whose logits may be NaN
+      at::Tensor some = at::zeros({M}, token.options().dtype(at::kBool));
+      if (g[0].defined())
+        some.logical_or_(token.ge(0).logical_and_(token.lt(p.N)).logical_and_(g[0].view({M})));
+      if (g[1].defined()) some.logical_or_(g[1].view({M}));
+      gx.masked_fill_(some.logical_not_().unsqueeze(1), 0);
     }
     if (kp != p.K) gx = gx.narrow(1, 0, p.K).contiguous();
     return {gx.view(ctx->saved_data["sizes"].toIntVector()), at::Tensor(), at::Tensor(), at::Tensor(),
