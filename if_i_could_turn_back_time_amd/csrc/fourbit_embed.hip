@@ -533,7 +533,7 @@ int fb_gpu::sort_tokens(const int64_t* token, int64_t rows, int32_t vocab, unsig
   hipLaunchKernelGGL(embed_keys, dim3(cus), dim3(256), 0, hs, token, rows, vocab, item[0], zeros,
                      units, tail, (int)(bytes & 15));
   int from = 0;
-  for (int shift = 0; shift < bits; shift += 8, from ^= 1) {
+  for (int shift = 0; rows && shift < bits; shift += 8, from ^= 1) {
     const bool last = shift + 8 >= bits;
     hipLaunchKernelGGL(embed_count, dim3(p.tiles), dim3(256), 0, hs, item[from], rows, shift, count,
                        p.tiles);

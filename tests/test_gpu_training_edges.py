@@ -51,3 +51,15 @@ def test_padding_under_packed_heads(fmt, block, scale, dt, M):
     ge[7] = 1
     got, = torch.autograd.grad(head_logprobs(x, head, t).entropy, x, ge)
     assert got[7].any() and not got[9].any()
+
+
+# ------------------------------------------------------------------ nothing to do
+@pytest.mark.parametrize("V", [9, 262143, 262144, 300000])
+def test_embedding_of_no_tokens(V):
+    """An empty batch's gradient is 0, on both sides of the limits of the small sort."""
+    for dt in (torch.bfloat16, torch.float32):
+        w = torch.randn(V, 5, device="cuda").to(dt).requires_grad_(True)
+        out = token_embedding(torch.empty(0, 3, dtype=torch.int64, device="cuda"), w)
+        assert out.shape == (0, 3, 5)
+        gw, = torch.autograd.grad(out, w, torch.empty_like(out))
+        assert gw.shape == w.shape and gw.dtype == dt and not gw.any()
