@@ -1167,7 +1167,9 @@ int fb_pad_rows(const void* src, int64_t src_stride, int64_t rows, int32_t K, vo
       src_stride > (1ll << 40) || dst_stride < K || dst_stride > (1 << 20) || dst_stride % 8)
     return FB_ERR_SHAPE;
   if (bad_align({src}, 1) || bad_align({dst}, 15)) return FB_ERR_ALIGN;
-  const unsigned units = (unsigned)(K + 7) / 8, rows_of = std::max(1u, 1024 / units);
+  // a launch has fewer than 2^32 threads: at most 2^22 workgroups
+  const unsigned units = (unsigned)(K + 7) / 8;
+  const unsigned rows_of = std::max({1u, 1024 / units, (unsigned)((rows + (1 << 22) - 1) >> 22)});
   hipLaunchKernelGGL(head_pad, dim3((unsigned)((rows + rows_of - 1) / rows_of)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), static_cast<const uint16_t*>(src), src_stride,
                      rows, K, static_cast<uint16_t*>(dst), dst_stride, units, rows_of);

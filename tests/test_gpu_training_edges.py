@@ -63,3 +63,23 @@ def test_embedding_of_no_tokens(V):
         assert out.shape == (0, 3, 5)
         gw, = torch.autograd.grad(out, w, torch.empty_like(out))
         assert gw.shape == w.shape and gw.dtype == dt and not gw.any()
+
+
+# ------------------------------------------------------------------ launches of 2^32 threads
+def test_padding_most_rows():
+    """As many rows as fb_pad_rows takes, of a width that has a workgroup for each."""
+    rows, K, ld = 1 << 24, 4097, 4104
+    torch.cuda.empty_cache()
+    src = torch.randint(1, 30000, (K,), dtype=torch.int16, device="cuda")
+    dst = torch.empty(rows, ld, dtype=torch.int16, device="cuda")
+    dst[::4099] = -1
+    dst[-1] = -1
+    rc = C.lib().fb_pad_rows(src.data_ptr(), 0, rows, K, dst.data_ptr(), ld,
+                             torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0
+    want = torch.cat([src, torch.zeros(ld - K, dtype=torch.int16, device="cuda")])
+    for r in range(0, rows, 1 << 18):
+        assert bool((dst[r:r + (1 << 18)] == want).all()), r
+    del dst
+    torch.cuda.empty_cache()
