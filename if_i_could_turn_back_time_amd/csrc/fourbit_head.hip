@@ -17,7 +17,9 @@
 // what it lost is kept in fp32 and goes into both results, times its row of W (head_sum) or of x (grad_w's
 // tiles end with the rows whose token they hold, which a sort by token finds).  In fp16 each row of G has
 // a power of two of its own that brings it near the type's largest values, and grad_w's x one that takes
-// it off again.
+// it off again, times a common one that brings the largest of them near the type's largest values too: a
+// row's x keeps its bits as far as 2^-30 of the largest row's g x, which is the distance between the least
+// and the largest values that the result may have in fp16.
 // The logits are worked out twice rather than kept: 2 of the 8 M V K operations, for M V values that are
 // never in memory beyond a piece.
 #include <hip/hip_runtime.h>
@@ -670,40 +672,69 @@ __global__ __launch_bounds__(256) void head_decode(const uint8_t* __restrict__ w
       *reinterpret_cast<u32x4*>(out + (n0 + i) * K + col) = rows[wave][i][lane ^ i];
 }
 
-// What bounds |G| in row r: 0 where no gradient comes in.
+// What bounds |G| in row r: 0 where no gradient comes in.  The entropy's part is p |log p + H|: at most
+// 1 / e + log 2^24 = 17.1 times its gradient, for p <= 1 and at most 2^24 tokens.
 __device__ inline float row_bound(int64_t r, const int64_t* token, int vocab, const float* g,
                                   const float* ge) {
   const int64_t t = token[r];
   float b = g && t >= 0 && t < vocab ? __builtin_fabsf(g[r]) : 0.f;
-  if (ge) b += 24.f * __builtin_fabsf(ge[r]);  // 1 + log of the largest vocabulary
+  if (ge) b += 24.f * __builtin_fabsf(ge[r]);
   return b;
 }
-// The least exponent with bound <= 2^e.
+// The least exponent with bound < 2^e, from -100 to 127.
 __device__ inline int bound_exp(float b) {
   const int e = (int)(__builtin_bit_cast(unsigned, b) >> 23) - 126;
   return e < -100 ? -100 : e > 127 ? 127 : e;
 }
 constexpr int kF16Exp = 14;
 
-// fp16: *top = the largest row's exponent.
-__global__ __launch_bounds__(1024) void head_top(const int64_t* __restrict__ token, int vocab,
-                                                 const float* __restrict__ g,
-                                                 const float* __restrict__ ge, int rows,
+// fp16: reach[r] = the exponent of what bounds the row's g x; -1000 without a gradient.  777 x 1000: 5 us.
+__global__ __launch_bounds__(256) void head_reach(const uint8_t* __restrict__ x, int64_t ldx, int K8,
+                                                  const int64_t* __restrict__ token, int vocab,
+                                                  const float* __restrict__ g,
+                                                  const float* __restrict__ ge,
+                                                  float* __restrict__ reach) {
+  __shared__ unsigned red[4];
+  const int64_t r = blockIdx.x;
+  const u32x4* const src = reinterpret_cast<const u32x4*>(x + r * ldx * 2);
+  unsigned most = 0;  // of the values' bits, without their signs
+  for (int i = threadIdx.x; i < K8; i += 256) {
+    const u32x4 v = src[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = max(most, max(v[j] & 0x7FFFu, v[j] >> 16 & 0x7FFFu));
+  }
+  for (int s = 32; s; s >>= 1) most = max(most, __shfl_xor(most, s));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x) return;
+  most = min(max(max(red[0], red[1]), max(red[2], red[3])), 0x7BFFu);  // infinities: as the largest number
+  const float b = row_bound(r, token, vocab, g, ge);
+  reach[r] = b == 0.f ? -1000.f
+                      : (float)(bound_exp(b) +
+                                bound_exp((float)__builtin_bit_cast(_Float16, (unsigned short)most)));
+}
+
+// top[1] = the largest reach, top[0] = what grad_w's sums are multiplied by.
+__global__ __launch_bounds__(1024) void head_top(const float* __restrict__ reach, int rows,
                                                  float* __restrict__ top) {
-  __shared__ int red[1024];
-  int e = -100;
-  for (int r = threadIdx.x; r < rows; r += 1024) e = max(e, bound_exp(row_bound(r, token, vocab, g, ge)));
+  __shared__ float red[1024];
+  float e = -200.f;
+  for (int r = threadIdx.x; r < rows; r += 1024) e = fmaxf(e, reach[r]);
   red[threadIdx.x] = e;
   __syncthreads();
   for (int s = 512; s; s >>= 1) {
-    if ((int)threadIdx.x < s) red[threadIdx.x] = max(red[threadIdx.x], red[threadIdx.x + s]);
+    if ((int)threadIdx.x < s) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + s]);
     __syncthreads();
   }
-  if (threadIdx.x == 0) top[0] = __builtin_ldexpf(1.f, red[0] - kF16Exp);
+  if (threadIdx.x == 0) {
+    top[0] = __builtin_ldexpf(1.f, (int)red[0] - kF16Exp - 16);
+    top[1] = red[0];
+  }
 }
 
-// A row's power of two and x as grad_w takes it: times what brings the row's G back to the scale of
-// the largest row's, 0 where the row has no gradient (whatever x holds there).
+// A row's power of two and x as grad_w takes it: times what makes G x of all rows 2^(30 - top[1]) times
+// what they are, so that the largest x is just below 2^16; 0 where the row has no gradient (whatever x
+// holds there).
 template <int DT>
 __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, int64_t ldx, int K8,
                                                  const int64_t* __restrict__ token, int vocab,
@@ -714,12 +745,13 @@ __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, 
                                                  float* __restrict__ lost, uint8_t* __restrict__ xs) {
   const int64_t r = blockIdx.x;
   const float b = row_bound(r, token, vocab, g, ge);
-  float up = b == 0.f ? 0.f : 1.f, down = up;
+  float up = b == 0.f ? 0.f : 1.f, down = up, f = up;
   if constexpr (DT == FB_DT_F16) {
     if (b != 0.f) {
-      const int e = kF16Exp - bound_exp(b);
-      up = __builtin_ldexpf(1.f, e);
-      down = __builtin_ldexpf(1.f, -e);
+      const int e = bound_exp(b);
+      up = __builtin_ldexpf(1.f, kF16Exp - e);
+      down = __builtin_ldexpf(1.f, e - kF16Exp);
+      if (xs) f = __builtin_ldexpf(1.f, 16 + e - (int)top[1]);
     }
   }
   if (threadIdx.x == 0) {
@@ -728,18 +760,15 @@ __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, 
     lost[r] = 0.f;
   }
   if (!xs) return;
-  const float f = DT == FB_DT_F16 && b != 0.f ? down / top[0] : up;
   const u32x4* const src = reinterpret_cast<const u32x4*>(x + r * ldx * 2);
   u32x4* const dst = reinterpret_cast<u32x4*>(xs + r * K8 * 16);
   for (int i = threadIdx.x; i < K8; i += 256) {
     u32x4 v = b == 0.f ? u32x4{0, 0, 0, 0} : src[i];
     if constexpr (DT == FB_DT_F16) {
-      if (f != 1.f) {
-        half8_t h = __builtin_bit_cast(half8_t, v);
+      half8_t h = __builtin_bit_cast(half8_t, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = (_Float16)((float)h[e] * f);
-        v = __builtin_bit_cast(u32x4, h);
-      }
+      for (int e = 0; e < 8; ++e) h[e] = (_Float16)((float)h[e] * f);
+      v = __builtin_bit_cast(u32x4, h);
     }
     dst[i] = v;
   }
@@ -943,7 +972,7 @@ GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
   p.at_scale = take(rows * 4);
   p.at_undo = take(rows * 4);
   p.at_lost = take(rows * 4);
-  p.at_top = take(4);
+  p.at_top = take(8);
   p.at_x = take(gw ? (size_t)rows * ((K + 7) / 8) * 16 : 0);
   p.at_g = take((size_t)rows * p.piece * 2);
   p.at_acc = take(gx ? (size_t)p.parts * rows * K * 4 : 0);
@@ -1007,9 +1036,12 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
   uint8_t* const xs = ws + p.at_x;
   float* const acc = reinterpret_cast<float*>(ws + p.at_acc);
   const int K8 = (K + 7) / 8;
-  if (DT == FB_DT_F16)
-    hipLaunchKernelGGL(head_top, dim3(1), dim3(1024), 0, hs, in.token, vocab, in.g_logprob,
-                       in.g_entropy, (int)rows, top);
+  if (DT == FB_DT_F16 && grad_w) {
+    float* const reach = scale;  // head_rows' afterwards
+    hipLaunchKernelGGL(head_reach, dim3((unsigned)rows), dim3(256), 0, hs, in.q, in.ldq, K8, in.token,
+                       vocab, in.g_logprob, in.g_entropy, reach);
+    hipLaunchKernelGGL(head_top, dim3(1), dim3(1024), 0, hs, reach, (int)rows, top);
+  }
   hipLaunchKernelGGL(head_rows<DT>, dim3((unsigned)rows), dim3(256), 0, hs, in.q, in.ldq, K8,
                      in.token, vocab, in.g_logprob, in.g_entropy, top, scale, undo, lost,
                      grad_w ? xs : nullptr);

@@ -635,7 +635,9 @@ int fb_pad_rows(const void* src, int64_t src_stride, int64_t rows, int32_t K, vo
 /* The gradient: with G[r, v] as fb_token_logprobs_grad's (no alternatives), grad_x = G w and
  * grad_w = G^T x.  The logits are computed again, a piece of the vocabulary at a time; G enters the
  * products rounded to dtype (fp16: times a power of two of its row), but for the given token's value,
- * which keeps what its rounding loses.  A row whose g are 0, or that has
+ * which keeps what its rounding loses.  In fp16 grad_w takes x times a power of two for each row, in
+ * fp16: a row whose bound of |G| times its largest |x| is 2^-30 of the largest row's, or more, keeps x's
+ * bits but where the result's would be below fp16's normal numbers.  A row whose g are 0, or that has
  * no token and no g_entropy, adds nothing to grad_w whatever its x holds.
  *   stats, entropy     as fb_head_logprobs wrote them
  *   g_*                fp32 [rows], or NULL (taken as 0)

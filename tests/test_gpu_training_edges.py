@@ -83,3 +83,68 @@ def test_padding_most_rows():
         assert bool((dst[r:r + (1 << 18)] == want).all()), r
     del dst
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ gradients far apart
+@pytest.mark.parametrize("entropy", [False, True])
+@pytest.mark.parametrize("most", [32.0, 1024.0])
+@pytest.mark.parametrize("less", [12, 16, 20])
+def test_weight_gradient_of_small_gradients(less, most, entropy):
+    """fp16: rows whose gradients are 2^-12 to 2^-20 of the largest give their tokens' rows of the weight
+    what they give alone.  Two kinds of rows, with the tokens of one vocabulary's half each: the other
+    half's have probabilities of exp(-128), which are 0 in fp32."""
+    V, K, M = 64, 40, 48
+    g = torch.Generator().manual_seed(less)
+    x = torch.randn(M, K, generator=g).half()
+    w = torch.zeros(V, K).half()
+    x[:, 0], w[:, 0] = 8, 8
+    x[1::2, 0], w[V // 2:, 0] = -8, -8
+    t = torch.randint(V // 2, (M,), generator=g)
+    t[1::2] += V // 2
+    gl = (0.5 + torch.rand(M, generator=g)) * most
+    ge = (0.5 + torch.rand(M, generator=g)) * most / 32 if entropy else torch.zeros(M)
+    gl[1::2] *= 2.0 ** -less
+    ge[1::2] *= 2.0 ** -less
+    x, w, t, gl, ge = (v.cuda() for v in (x, w, t, gl, ge))
+    x.requires_grad_(True), w.requires_grad_(True)
+    r = head_logprobs(x, w, t)
+    _, gw = torch.autograd.grad((r.logprob, r.entropy) if entropy else r.logprob, (x, w),
+                                (gl, ge) if entropy else gl)
+    _, _, _, want, G = exact(x.detach(), w.detach(), t, gl, ge)
+    half, info = 2.0 ** -11, torch.finfo(torch.float16)
+    # Each G: p is 1/32 in both (logits that are equal, exactly), off by a few steps of fp32 where the
+    # entropy comes in, then half a step of fp16; its products with x in sums of M; the result's rounding,
+    # of half its least step where it is small.
+    own = 64 * U * (G.abs() + (gl.abs() + 16 * ge.abs()).double()[:, None] / 32)
+    own[::2, V // 2:] = 0
+    own[1::2, :V // 2] = 0
+    off = (half * G.abs() + own + M * U * G.abs()).T @ x.detach().double().abs()
+    allowed = off * (1 + half) + half * want.abs() + info.smallest_normal * info.eps / 2
+    err = (gw.double() - want).abs()
+    assert (err <= allowed).all(), float((err / allowed).max())
+    # and in sum: roundings are as likely up as down, so their sums are far below that bound
+    for part in (slice(0, V // 2), slice(V // 2, V)):
+        e, n = err[part][:, 1:].norm(), want[part][:, 1:].norm()
+        floor = info.smallest_normal * info.eps / 2 * (V // 2 * K) ** 0.5
+        assert e <= 2 * half * n + floor, float(e / n)
+
+
+def test_weight_gradient_of_rows_of_all_sizes():
+    """fp16: hidden states from 2^-12 to 2^12 under gradients that take it back: every row counts alike."""
+    V, K, M = 128, 24, 64
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(M, K, generator=g)
+    size = torch.randint(-12, 13, (M, 1), generator=g)
+    x = torch.ldexp(x, size).half()
+    w = torch.zeros(V, K).half()
+    t = torch.randperm(V, generator=g)[:M]
+    gl = torch.ldexp(1 + torch.rand(M, generator=g), -size[:, 0])
+    x, w, t, gl = (v.cuda() for v in (x, w, t, gl))
+    w.requires_grad_(True)
+    gw, = torch.autograd.grad(head_logprobs(x, w, t).logprob, w, gl)
+    *_, want, G = exact(x, w.detach(), t, gl, 0 * gl)
+    half = 2.0 ** -11
+    off = ((half + (64 + M) * U) * G.abs()).T @ x.double().abs()
+    info = torch.finfo(torch.float16)
+    allowed = off * (1 + half) + half * want.abs() + info.smallest_normal * info.eps / 2
+    assert ((gw.double() - want).abs() <= allowed).all()
