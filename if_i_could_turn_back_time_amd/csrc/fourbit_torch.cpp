@@ -1057,19 +1057,18 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
       const int64_t step = packed_piece(p, M);
       const auto f = x.options().dtype(at::kFloat);
       const at::Tensor y = at::empty({step, p.N}, f), gl = at::empty({step, p.N}, f);
-      fb_shape_t sh = packed_shape(p, step, FB_DT_F16, FB_DT_F32);
-      const size_t need = fb_grad_x_workspace_bytes(&sh, p.f16_exact);
-      want(need, "a packed head of this many rows has no gradient");
-      const at::Tensor ws = scratch(need, x);
       for (int64_t r = 0; r < M; r += step) {
         const int64_t n = std::min(step, M - r);
+        fb_shape_t sh = packed_shape(p, n, FB_DT_F16, FB_DT_F32);
+        const size_t need = fb_grad_x_workspace_bytes(&sh, p.f16_exact);  // fewer rows may need more
+        want(need, "a packed head of this many rows has no gradient");
+        const at::Tensor ws = scratch(need, x);
         packed_logits(p, xk, r, n, y);
         check(fb_token_logprobs_grad(
             y.data_ptr(), FB_DT_F32, p.N, n, (int32_t)p.N,
             static_cast<const int64_t*>(token.data_ptr()) + r, 0, nullptr, f32_of(st) + 3 * r,
             f32_of(ent) + r, g[0].defined() ? f32_of(g[0]) + r : nullptr,
             g[1].defined() ? f32_of(g[1]) + r : nullptr, nullptr, gl.data_ptr(), stream_of(x)));
-        sh.B = (int32_t)n;
         check(fb_grad_x(p.wdev.data_ptr(), gl.data_ptr(),
                         static_cast<char*>(gx.data_ptr()) + r * kp * gx.element_size(), &sh, xdt,
                         p.f16_exact, ws.data_ptr(), need, stream_of(x)));

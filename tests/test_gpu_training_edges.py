@@ -148,3 +148,56 @@ def test_weight_gradient_of_rows_of_all_sizes():
     info = torch.finfo(torch.float16)
     allowed = off * (1 + half) + half * want.abs() + info.smallest_normal * info.eps / 2
     assert ((gw.double() - want).abs() <= allowed).all()
+
+
+# ------------------------------------------------------------------ pieces
+def _check_packed(head, w, x, t, gl, ge, terms=1, size=None):
+    """Results and gradient of hidden states whose logits are exact in fp32.  size: of w's terms."""
+    size = w.abs() if size is None else size
+    r = head_logprobs(x, head, t)
+    got, = torch.autograd.grad((r.logprob, r.entropy), x, (gl, ge))
+    lp, ent, gx, _, G = exact(x.detach(), w, t, gl, ge)
+    assert_close((r.logprob.detach(), r.entropy.detach()), (lp, ent))
+    p = torch.softmax(x.detach().double() @ w.T, -1)
+    dt = x.dtype
+    half = torch.finfo(dt).eps / 2
+    n = int((p > 2.0 ** -149).sum(-1).max())  # terms of a sum that are not 0 in fp32
+    own = 1024 * U * (gl.abs() + 16 * ge.abs()).double()[:, None] * (G.abs() + p)
+    off = (half * G.abs() + own + terms * n * U * G.abs()) @ size
+    small = 2.0 ** -38 * (gl.abs() + 24 * ge.abs()).double()[:, None] * size.sum(0)
+    assert got.dtype == dt and got.shape == x.shape
+    err = (got.double() - gx).abs()
+    assert (err <= off * (1 + half) + half * gx.abs() + small).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_packed_head_in_pieces_of_rows(dt):
+    """More rows than have their logits at once (2,672 of 50,000), of a width that is padded to 256."""
+    M, V, K = 2800, 50000, 200
+    torch.manual_seed(9)
+    head = QuantLinear(nn.Linear(K, V, bias=False), fmt="e2m1").cuda()
+    w = head.dequantized_weight().cuda().double()
+    g = torch.Generator().manual_seed(2)
+    x = (torch.randint(-4, 5, (M, K), generator=g) / 4).to(dt).cuda().requires_grad_(True)
+    t = torch.randint(-1, V, (M,), generator=g).cuda()
+    gl, ge = torch.randn(2, M, generator=g).cuda()
+    _check_packed(head, w, x, t, gl, ge, terms=3)
+
+
+def test_rotated_head_in_pieces_of_rows():
+    """A last piece of rows may take more workspace than a whole one (5,441 rows of 1,000 x 256, 8,192)."""
+    V, K, M = 1000, 256, 8192 + 5441
+    head = _head("gf4", 128, V=V, K=K)
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randint(-4, 5, (M, K), generator=g) / 4).half().cuda()
+    t = torch.randint(V, (M,), generator=g).cuda()
+    gl = torch.randn(M, generator=g).cuda()
+
+    def grads(rows):
+        a = x[rows].clone().requires_grad_(True)
+        return torch.autograd.grad(head_logprobs(a, head, t[rows]).logprob, a, gl[rows])[0]
+
+    got = grads(slice(None))
+    for rows in (slice(0, 8192), slice(8192, None)):  # the pieces by themselves: the same calls
+        assert torch.equal(got[rows], grads(rows))
+    assert got.abs().amax(-1).min() > 0
