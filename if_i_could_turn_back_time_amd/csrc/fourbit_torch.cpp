@@ -31,6 +31,7 @@ constexpr int64_t kMaxRotatedValues = 1 << 29;  // of x, rotated at once: a copy
 // Rows of grad_y at once: bounds fb_grad_x's 16-bit terms of them, and each pass's decode of W
 // is under 1% of its products.
 constexpr int64_t kGradRows = 8192;
+constexpr int64_t kGradVocab = 1 << 18;  // fb_grad_x's limit of a weight's rows
 
 void check(int code) {
   if (code != FB_OK) throw std::runtime_error(fb_strerror(code));
@@ -1011,6 +1012,29 @@ std::vector<at::Tensor> packed_forward(const Packed& p, const at::Tensor& x, con
   return {lp, ent, st};
 }
 
+// gl W for n rows of fp32 gl [>= n, N] into gx [n, kp], in fp32 terms, as many tokens as fb_grad_x takes
+// at once.
+void packed_grad_rows(const Packed& p, const at::Tensor& gl, int64_t n, const at::Tensor& gx) {
+  at::Tensor sum;
+  for (int64_t v = 0; v < p.N; v += kGradVocab) {
+    Packed part = p;
+    part.N = std::min(kGradVocab, p.N - v);
+    const fb_shape_t s = packed_shape(part, n, FB_DT_F16, FB_DT_F32);
+    part.N = v;  // of what lies before it, whole tiles of 16 rows
+    const fb_shape_t before = packed_shape(part, 1, FB_DT_F16, FB_DT_F32);
+    const bool all = s.N == p.N;
+    const at::Tensor g = all ? gl : gl.narrow(0, 0, n).narrow(1, v, s.N).contiguous();
+    const at::Tensor out = all ? gx : at::empty(gx.sizes(), gx.options().dtype(at::kFloat));
+    const size_t need = fb_grad_x_workspace_bytes(&s, p.f16_exact);  // fewer rows may need more
+    const at::Tensor ws = scratch(need, gx);
+    check(fb_grad_x(static_cast<const char*>(p.wdev.data_ptr()) + (v ? fb_device_bytes(&before) : 0),
+                    g.data_ptr(), out.data_ptr(), &s, dtype_code(out.scalar_type()), p.f16_exact,
+                    ws.data_ptr(), need, stream_of(gx)));
+    if (!all) sum = sum.defined() ? sum.add_(out) : out;
+  }
+  if (sum.defined()) gx.copy_(sum);
+}
+
 struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx,
                                                 const at::Tensor& hidden, const at::Tensor& wdev,
@@ -1059,19 +1083,13 @@ struct PackedHeadLogprobs : torch::autograd::Function<PackedHeadLogprobs> {
       const at::Tensor y = at::empty({step, p.N}, f), gl = at::empty({step, p.N}, f);
       for (int64_t r = 0; r < M; r += step) {
         const int64_t n = std::min(step, M - r);
-        fb_shape_t sh = packed_shape(p, n, FB_DT_F16, FB_DT_F32);
-        const size_t need = fb_grad_x_workspace_bytes(&sh, p.f16_exact);  // fewer rows may need more
-        want(need, "a packed head of this many rows has no gradient");
-        const at::Tensor ws = scratch(need, x);
         packed_logits(p, xk, r, n, y);
         check(fb_token_logprobs_grad(
             y.data_ptr(), FB_DT_F32, p.N, n, (int32_t)p.N,
             static_cast<const int64_t*>(token.data_ptr()) + r, 0, nullptr, f32_of(st) + 3 * r,
             f32_of(ent) + r, g[0].defined() ? f32_of(g[0]) + r : nullptr,
             g[1].defined() ? f32_of(g[1]) + r : nullptr, nullptr, gl.data_ptr(), stream_of(x)));
-        check(fb_grad_x(p.wdev.data_ptr(), gl.data_ptr(),
-                        static_cast<char*>(gx.data_ptr()) + r * kp * gx.element_size(), &sh, xdt,
-                        p.f16_exact, ws.data_ptr(), need, stream_of(x)));
+        packed_grad_rows(p, gl, n, gx.narrow(0, r, n));
       }
       // rows that nothing comes in for, whose logits may be NaN
       at::Tensor some = at::zeros({M}, token.options().dtype(at::kBool));

@@ -201,3 +201,33 @@ def test_rotated_head_in_pieces_of_rows():
     for rows in (slice(0, 8192), slice(8192, None)):  # the pieces by themselves: the same calls
         assert torch.equal(got[rows], grads(rows))
     assert got.abs().amax(-1).min() > 0
+
+
+# ------------------------------------------------------------------ large vocabularies
+@pytest.mark.parametrize("block, dt", [(4, torch.float16), (0, torch.bfloat16)])
+def test_packed_head_of_a_large_vocabulary(block, dt):
+    """More tokens than fb_grad_x takes, in pieces of rows too.  Few of the tokens can come up, some on
+    both sides of the first piece's end: the others' logits are 128 below, their probabilities 0."""
+    V, K, M = (1 << 18) + 56, 128, 600
+    g = torch.Generator().manual_seed(3)
+    w = torch.randn(V, K, generator=g) / 8
+    some_tokens = torch.cat([torch.arange(20), torch.arange((1 << 18) - 10, (1 << 18) + 10),
+                             torch.arange(V - 20, V)])
+    w[:, :4] = 0
+    w[:, 0] = -8
+    w[some_tokens, 0] = 8
+    head = PackedWeight.quantize(w, "e2m1", fwht_block=block, device="cuda")
+    w = head.dequant_device(torch.float32).double()
+    size = w.abs()
+    if block:  # a rotation of 4 halves: exact
+        h = torch.tensor([[1, 1, 1, 1], [1, -1, 1, -1], [1, 1, -1, -1], [1, -1, -1, 1]]).double() / 2
+        rot = torch.block_diag(*[h] * (K // 4)).cuda()
+        w, size = w @ rot, 2 * size @ rot.abs()  # and its sums are rounded
+    assert torch.equal(w[some_tokens.cuda(), 0], torch.full((60,), 8.0, device="cuda").double())
+    x = torch.randint(-4, 5, (M, K), generator=g) / 4
+    x[:, :4] = 0
+    x[:, 0] = 8
+    x = x.to(dt).cuda().requires_grad_(True)
+    t = some_tokens[torch.randint(len(some_tokens), (M,), generator=g)].cuda()
+    gl, ge = torch.randn(2, M, generator=g).cuda()
+    _check_packed(head, w, x, t, gl, ge, terms=3, size=size)
