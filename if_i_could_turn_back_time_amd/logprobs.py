@@ -48,8 +48,8 @@ def head_logprobs(hidden: torch.Tensor, head, tokens: torch.Tensor) -> HeadLogpr
     entropy's, nor gives the weight any, whatever ``hidden`` holds there.
 
     The gradients' products take each logit's gradient in 16 bits, as a backward pass through 16-bit
-    logits does, but for the given token's, whose rounding is made up for.  (A rotated packed head, and
-    one whose scales leave 16 bits, takes them in fp32.)"""
+    logits does, but for the given token's, whose rounding is made up for.  (A packed head takes them in
+    fp32 under fp32 ``hidden``, and where it is rotated or its scales leave 16 bits.)"""
     if isinstance(head, (QuantLinear, PackedWeight)):
         if isinstance(head, QuantLinear):
             if head.bias is not None:

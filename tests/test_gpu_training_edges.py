@@ -150,6 +150,42 @@ def test_weight_gradient_of_rows_of_all_sizes():
     assert ((gw.double() - want).abs() <= allowed).all()
 
 
+# ------------------------------------------------------------------ fp32 hidden states
+@pytest.mark.parametrize("M", [5, 40])
+@pytest.mark.parametrize("fmt", ["e2m1", "gf4"])
+@pytest.mark.parametrize("entropy", [False, True])
+def test_packed_head_keeps_fp32(fmt, M, entropy):
+    """The gradient of fp32 hidden states is in fp32 terms throughout."""
+    V, K = 64, 256
+    head = _head(fmt, 0, V=V, K=K)
+    w = head.dequant_device(torch.float32).double()
+    g = torch.Generator().manual_seed(M)
+    x = (torch.randint(-4, 5, (M, K), generator=g) / 4).cuda().requires_grad_(True)
+    t = torch.randint(V, (M,), generator=g).cuda()
+    gl, ge = torch.randn(2, M, generator=g).cuda()
+    if not entropy:
+        ge = 0 * ge
+    r = head_logprobs(x, head, t)
+    got, = torch.autograd.grad((r.logprob, r.entropy) if entropy else r.logprob, x,
+                               (gl, ge) if entropy else gl)
+    xd = x.detach().double()
+    _, ent, gx, _, G = exact(xd, w, t, gl, ge)
+    logp = torch.log_softmax(xd @ w.T, -1)
+    p = logp.exp()
+    gl, ge = gl.abs().double()[:, None], ge.abs().double()[:, None]
+    # logits: K sums of terms (exact for E2M1, whose steps are few); the exponent of 2 below 16, three
+    # roundings of it and those of the sum: 2^-18, and as much of p; the entropy 2^-15
+    logit = K * U * (xd.abs() @ w.abs().T) if fmt == "gf4" else torch.zeros_like(p)
+    dp = 2.0 ** -18 + 2 * logit.amax(-1, keepdim=True)
+    dh = 2.0 ** -15 + 16 * logit.amax(-1, keepdim=True)
+    own = p * (dp * (gl + ge * (logp.abs() + ent[:, None] + 1)) + dh * ge) + 4 * U * G.abs()
+    # the products' terms are exact in three 16-bit parts, 3 V of which are summed
+    allowed = own @ w.abs() + 4 * V * U * (G.abs() @ w.abs()) + 2 * U * gx.abs()
+    assert got.dtype == torch.float32
+    err = (got.double() - gx).abs()
+    assert (err <= allowed).all(), float((err / allowed).max())
+
+
 # ------------------------------------------------------------------ pieces
 def _check_packed(head, w, x, t, gl, ge, terms=1, size=None):
     """Results and gradient of hidden states whose logits are exact in fp32.  size: of w's terms."""
@@ -204,7 +240,7 @@ def test_rotated_head_in_pieces_of_rows():
 
 
 # ------------------------------------------------------------------ large vocabularies
-@pytest.mark.parametrize("block, dt", [(4, torch.float16), (0, torch.bfloat16)])
+@pytest.mark.parametrize("block, dt", [(4, torch.float16), (0, torch.bfloat16), (0, torch.float32)])
 def test_packed_head_of_a_large_vocabulary(block, dt):
     """More tokens than fb_grad_x takes, in pieces of rows too.  Few of the tokens can come up, some on
     both sides of the first piece's end: the others' logits are 128 below, their probabilities 0."""
