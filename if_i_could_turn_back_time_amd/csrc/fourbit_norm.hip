@@ -76,6 +76,11 @@ __device__ inline float wave_sum(float v) {
   v += moved<0x143, 0xC>(v);
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
+// The instruction takes numbers below 2^-126 for 0: they are brought above first.
+__device__ inline float rsqrt_of(float v) {
+  const bool low = v < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(low ? v * 0x1p60f : v) * (low ? 0x1p30f : 1.f);
+}
 // N sums over a group of T threads.  Calls take turns with two `red`: one barrier a call is enough then.
 template <int T, int N>
 __device__ inline void group_sum(float (&v)[N], float (*red)[N]) {
@@ -154,7 +159,7 @@ __global__ __launch_bounds__(kBlock<T>, 4) void norm_kernel(NormArgs a) {
 #pragma unroll
           for (int i = 0; i < V; ++i) s[0] = __builtin_fmaf(b[j][i], b[j][i], s[0]);
         group_sum<T>(s, red[turn ^= 1]);
-        r1 = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], inv, a.n.eps));
+        r1 = rsqrt_of(__builtin_fmaf(s[0], inv, a.n.eps));
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(kBlock<T>, 4) void norm_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) s[0] = __builtin_fmaf(x[j][i], x[j][i], s[0]);
     group_sum<T>(s, red[turn ^= 1]);
-    const float r2 = __builtin_amdgcn_rsqf(__builtin_fmaf(s[0], inv, a.n.eps));
+    const float r2 = rsqrt_of(__builtin_fmaf(s[0], inv, a.n.eps));
     if (!mine) continue;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {

@@ -267,3 +267,27 @@ def test_packed_head_of_a_large_vocabulary(block, dt):
     t = some_tokens[torch.randint(len(some_tokens), (M,), generator=g)].cuda()
     gl, ge = torch.randn(2, M, generator=g).cuda()
     _check_packed(head, w, x, t, gl, ge, terms=3, size=size)
+
+
+# ------------------------------------------------------------------ the least values
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("e", [-60, -63, -64, -70, -74])
+def test_norms_of_the_least_values(e, dt):
+    """Rows whose squares are below fp32's normal numbers are normalised as others are, without an eps."""
+    M, d = 7, 256
+    g = torch.Generator().manual_seed(-e)
+    sign = 1 - 2 * torch.randint(2, (3, M, d), generator=g)
+    x, b, gy = (torch.ldexp(s.double(), torch.tensor(n)).to(dt).cuda()
+                for s, n in zip(sign, (e, e, 0)))
+    w = torch.ones(d, device="cuda", dtype=dt)
+    x.requires_grad_(True)
+    r = residual_norm(x, w, eps=0.0)
+    # every square is 2^(2 e), which fp32 has: 1 in size
+    assert ((r.normed.double() - sign[0].cuda()).abs() <= 2.0 ** -20).all()
+    gx, = torch.autograd.grad(r.normed, x, gy)
+    n = sign[0].cuda().double()
+    want = (gy.double() - n * (gy.double() * n).mean(-1, keepdim=True)) * 2.0 ** -e
+    # a few roundings in fp32, and the type's
+    assert ((gx.double() - want).abs() <= (torch.finfo(dt).eps + 2.0 ** -18) * 2.0 ** -e).all()
+    r = residual_norm(torch.zeros_like(x), w, b, branch_weight=w, eps=0.0)
+    assert ((r.stream.double() - sign[1].cuda()).abs() <= 2.0 ** -20).all()
