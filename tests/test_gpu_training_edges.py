@@ -291,3 +291,107 @@ def test_norms_of_the_least_values(e, dt):
     assert ((gx.double() - want).abs() <= (torch.finfo(dt).eps + 2.0 ** -18) * 2.0 ** -e).all()
     r = residual_norm(torch.zeros_like(x), w, b, branch_weight=w, eps=0.0)
     assert ((r.stream.double() - sign[1].cuda()).abs() <= 2.0 ** -20).all()
+
+
+# ------------------------------------------------------------------ a step whose loss is the entropy
+def test_step_of_the_entropy_against_torch():
+    tokens, following = _batch(4)
+    got = []
+    for plain in (False, True):
+        net = Net(plain)
+        params = _trained(net)
+        _, ent = net(tokens, following)
+        got.append(torch.autograd.grad(ent.sum() / 100, params))
+    for i, (a, b) in enumerate(zip(*got)):
+        a, b = a.double(), b.double()
+        # a dozen roundings to bf16 on the way in both, each of 2^-9 of a vector's length at most on average
+        assert b.norm() > 0 and (a - b).norm() <= 24 * 2.0 ** -9 * b.norm(), i
+
+
+# ------------------------------------------------------------------ the entropy's gradient alone
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M, V, K", [(200, 8000, 256), (33, 3000, 120)])
+def test_gradient_of_the_entropy_alone(M, V, K, dt):
+    """Its large values lie at other tokens than the given one, whose rounding alone is made up for: what
+    the logits' gradient loses in 16 bits is there in the results, and no more."""
+    x, w, t, _, ge = some(M, V, K, dt, padded=False)
+    x.requires_grad_(True), w.requires_grad_(True)
+    got = torch.autograd.grad(head_logprobs(x, w, t).entropy, (x, w), ge)
+    _, _, gx, gw, G = exact(x.detach(), w.detach(), t, 0 * ge, ge)
+    up = torch.ldexp(torch.ones_like(G[:, :1]), 14 - G.abs().amax(-1, keepdim=True).log2().ceil().int())
+    lost = (G * up).to(dt).double() / up - G
+    for a, b, e in zip(got, (gx, gw), (lost @ w.detach().double(), lost.T @ x.detach().double())):
+        # two sets of roundings, and a quarter for those that fall to the other side
+        assert (a.double() - b).norm() <= 1.25 * ((b.to(dt).double() - b).norm() + e.norm())
+
+
+# ------------------------------------------------------------------ captured, and in part
+@pytest.mark.parametrize("fmt, block, dt", [("e2m1", 0, torch.bfloat16), ("e2m1", 0, torch.float32),
+                                            ("gf4", 128, torch.float16)])
+@pytest.mark.parametrize("M", [12, 90])
+def test_captured_packed_heads(fmt, block, dt, M):
+    """Every way to a packed head's gradient, replayed with new data, padding among it."""
+    head = _head(fmt, block)
+    g = torch.Generator().manual_seed(M)
+
+    def batch():
+        t = torch.randint(-2, 300, (M,), generator=g)
+        return ((torch.randint(-4, 5, (M, 256), generator=g) / 4).to(dt).cuda(), t.cuda(),
+                *torch.randn(2, M, generator=g).cuda())
+
+    x, t, gl, ge = batch()
+    x.requires_grad_(True)
+
+    def step():
+        r = head_logprobs(x, head, t)
+        return (r.logprob.detach(), r.entropy.detach(),
+                *torch.autograd.grad((r.logprob, r.entropy), x, (gl, ge)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        fresh = batch()
+        with torch.no_grad():
+            for a, b in zip((x, t, gl, ge), fresh):
+                a.copy_(b)
+            ge[:3] = 0
+            if i == 2:
+                x[t < 0] = float("nan")
+                ge[t < 0] = 0
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+        assert torch.equal(got[1].nan_to_num(-1), want[1].nan_to_num(-1))
+        assert torch.isfinite(got[2]).all() and (i != 2 or bool((got[2][t < 0] == 0).all()))
+
+
+def test_one_gradient_in_fp16():
+    """The hidden states' gradient is the same bits with the weight's and without it, and the other way."""
+    x, w, t, gl, ge = some(60, 90, 24, torch.float16)
+    gl[::3] *= 2.0 ** -18
+    full = [v.clone().requires_grad_(True) for v in (x, w)]
+    r = head_logprobs(*full, t)
+    want = torch.autograd.grad((r.logprob, r.entropy), full, (gl, 0.1 * ge))
+    for i in range(2):
+        one = [x.clone(), w.clone()]
+        one[i].requires_grad_(True)
+        r = head_logprobs(*one, t)
+        got, = torch.autograd.grad((r.logprob, r.entropy), one[i], (gl, 0.1 * ge))
+        assert torch.equal(got, want[i])
+
+
+def test_fp16_without_any_gradient():
+    """Incoming gradients of 0, and of the largest numbers, in fp16."""
+    x, w, t, gl, _ = some(20, 30, 16, torch.float16, padded=False)
+    x.requires_grad_(True), w.requires_grad_(True)
+    for g in torch.autograd.grad(head_logprobs(x, w, t).logprob, (x, w), 0 * gl):
+        assert (g == 0).all()
+    gx, gw = torch.autograd.grad(head_logprobs(x, w, t).logprob, (x, w), 2.0 ** 100 * (1 + gl.abs()))
+    assert not gx.isnan().any() and not gw.isnan().any() and gx.isinf().any() and gw.isinf().any()
