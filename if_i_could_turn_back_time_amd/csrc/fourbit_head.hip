@@ -687,6 +687,7 @@ __device__ inline int bound_exp(float b) {
   return e < -100 ? -100 : e > 127 ? 127 : e;
 }
 constexpr int kF16Exp = 14;
+constexpr float kLeastReach = -200.f;  // of all rows
 
 // fp16: reach[r] = the exponent of what bounds the row's g x; -1000 without a gradient.  777 x 1000: 5 us.
 __global__ __launch_bounds__(256) void head_reach(const uint8_t* __restrict__ x, int64_t ldx, int K8,
@@ -714,11 +715,13 @@ __global__ __launch_bounds__(256) void head_reach(const uint8_t* __restrict__ x,
                                 bound_exp((float)__builtin_bit_cast(_Float16, (unsigned short)most)));
 }
 
-// top[1] = the largest reach, top[0] = what grad_w's sums are multiplied by.
+// top[1] = the largest reach, top[0] = what grad_w's sums are multiplied by.  Up to kTopRows rows
+// head_rows does that by itself: a launch, 5 us of 90 of a small call with its gradients.
+constexpr int kTopRows = 1024;
 __global__ __launch_bounds__(1024) void head_top(const float* __restrict__ reach, int rows,
                                                  float* __restrict__ top) {
   __shared__ float red[1024];
-  float e = -200.f;
+  float e = kLeastReach;
   for (int r = threadIdx.x; r < rows; r += 1024) e = fmaxf(e, reach[r]);
   red[threadIdx.x] = e;
   __syncthreads();
@@ -732,26 +735,39 @@ __global__ __launch_bounds__(1024) void head_top(const float* __restrict__ reach
   }
 }
 
-// A row's power of two and x as grad_w takes it: times what makes G x of all rows 2^(30 - top[1]) times
-// what they are, so that the largest x is just below 2^16; 0 where the row has no gradient (whatever x
-// holds there).
+// A row's power of two and x as grad_w takes it: times what makes G x of all rows 2^(30 - the largest
+// reach) times what they are, so that the largest x is just below 2^16; 0 where the row has no gradient
+// (whatever x holds there).
 template <int DT>
 __global__ __launch_bounds__(256) void head_rows(const uint8_t* __restrict__ x, int64_t ldx, int K8,
                                                  const int64_t* __restrict__ token, int vocab,
                                                  const float* __restrict__ g,
                                                  const float* __restrict__ ge,
-                                                 const float* __restrict__ top,
-                                                 float* __restrict__ scale, float* __restrict__ undo,
-                                                 float* __restrict__ lost, uint8_t* __restrict__ xs) {
+                                                 const float* __restrict__ reach, int rows,
+                                                 float* __restrict__ top, float* __restrict__ scale,
+                                                 float* __restrict__ undo, float* __restrict__ lost,
+                                                 uint8_t* __restrict__ xs) {
   const int64_t r = blockIdx.x;
   const float b = row_bound(r, token, vocab, g, ge);
   float up = b == 0.f ? 0.f : 1.f, down = up, f = up;
   if constexpr (DT == FB_DT_F16) {
+    float most = kLeastReach;
+    if (xs && rows <= kTopRows) {
+      __shared__ float red[4];
+      for (int i = threadIdx.x; i < rows; i += 256) most = fmaxf(most, reach[i]);
+      for (int s = 32; s; s >>= 1) most = fmaxf(most, __shfl_xor(most, s));
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+      __syncthreads();
+      most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+      if (r == 0 && threadIdx.x == 0) top[0] = __builtin_ldexpf(1.f, (int)most - kF16Exp - 16);
+    } else if (xs) {
+      most = top[1];
+    }
     if (b != 0.f) {
       const int e = bound_exp(b);
       up = __builtin_ldexpf(1.f, kF16Exp - e);
       down = __builtin_ldexpf(1.f, e - kF16Exp);
-      if (xs) f = __builtin_ldexpf(1.f, 16 + e - (int)top[1]);
+      f = __builtin_ldexpf(1.f, 16 + e - (int)most);
     }
   }
   if (threadIdx.x == 0) {
@@ -934,7 +950,7 @@ StatPlan stat_plan(int64_t rows, int K, int vocab, int cus) {
 struct GradPlan {
   int64_t piece;  // tokens of the vocabulary at once
   int gshape, xshape, wshape, parts;
-  size_t at_scale, at_undo, at_lost, at_top, at_x, at_g, at_acc;
+  size_t at_scale, at_undo, at_lost, at_top, at_reach, at_x, at_g, at_acc;
   size_t at_key, at_place, at_start, at_sort, bytes;
 };
 GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
@@ -973,6 +989,7 @@ GradPlan grad_plan(int64_t rows, int K, int vocab, bool gx, bool gw, int cus) {
   p.at_undo = take(rows * 4);
   p.at_lost = take(rows * 4);
   p.at_top = take(8);
+  p.at_reach = take(gw ? rows * 4 : 0);
   p.at_x = take(gw ? (size_t)rows * ((K + 7) / 8) * 16 : 0);
   p.at_g = take((size_t)rows * p.piece * 2);
   p.at_acc = take(gx ? (size_t)p.parts * rows * K * 4 : 0);
@@ -1033,18 +1050,19 @@ int run_grad(const ProductArgs& in, const GradPlan& p, int64_t rows, int32_t K, 
   float* const undo = reinterpret_cast<float*>(ws + p.at_undo);
   float* const lost = reinterpret_cast<float*>(ws + p.at_lost);
   float* const top = reinterpret_cast<float*>(ws + p.at_top);
+  float* const reach = reinterpret_cast<float*>(ws + p.at_reach);
   uint8_t* const xs = ws + p.at_x;
   float* const acc = reinterpret_cast<float*>(ws + p.at_acc);
   const int K8 = (K + 7) / 8;
   if (DT == FB_DT_F16 && grad_w) {
-    float* const reach = scale;  // head_rows' afterwards
     hipLaunchKernelGGL(head_reach, dim3((unsigned)rows), dim3(256), 0, hs, in.q, in.ldq, K8, in.token,
                        vocab, in.g_logprob, in.g_entropy, reach);
-    hipLaunchKernelGGL(head_top, dim3(1), dim3(1024), 0, hs, reach, (int)rows, top);
+    if (rows > kTopRows)
+      hipLaunchKernelGGL(head_top, dim3(1), dim3(1024), 0, hs, reach, (int)rows, top);
   }
   hipLaunchKernelGGL(head_rows<DT>, dim3((unsigned)rows), dim3(256), 0, hs, in.q, in.ldq, K8,
-                     in.token, vocab, in.g_logprob, in.g_entropy, top, scale, undo, lost,
-                     grad_w ? xs : nullptr);
+                     in.token, vocab, in.g_logprob, in.g_entropy, reach, (int)rows, top, scale, undo,
+                     lost, grad_w ? xs : nullptr);
   if (hipGetLastError() != hipSuccess) return FB_ERR_HIP;
   unsigned* const key = reinterpret_cast<unsigned*>(ws + p.at_key);
   unsigned* const place = reinterpret_cast<unsigned*>(ws + p.at_place);

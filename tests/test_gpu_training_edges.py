@@ -150,6 +150,31 @@ def test_weight_gradient_of_rows_of_all_sizes():
     assert ((gw.double() - want).abs() <= allowed).all()
 
 
+@pytest.mark.parametrize("M", [1023, 1024, 1025, 3000])
+def test_weight_gradient_scales_of_many_rows(M):
+    """fp16: one row's gradient far above the others', wherever it is."""
+    V, K = 96, 40
+    for at in (0, 300, M - 1):
+        g = torch.Generator().manual_seed(M + at)
+        x, w = torch.randn(M, K, generator=g).half(), torch.zeros(V, K).half()
+        t = torch.randint(V - 1, (M,), generator=g)
+        x[:, 0], w[:, 0] = 0, 0
+        x[at, 0], w[V - 1, 0], t[at] = 64, 8, V - 1  # the row's own token alone: exp(-512) for others
+        gl = torch.randn(M, generator=g)
+        gl[at] = 2.0 ** 18
+        x, w, t, gl = (v.cuda() for v in (x, w, t, gl))
+        w.requires_grad_(True)
+        gw, = torch.autograd.grad(head_logprobs(x, w, t).logprob, w, gl)
+        *_, want, G = exact(x, w.detach(), t, gl, 0 * gl)
+        # as in test_weight_gradient_of_small_gradients; p is 1/96 of the other rows, to fp32
+        half, info = 2.0 ** -11, torch.finfo(torch.float16)
+        G[at] = 0  # 1 - p, which is 0 in fp32 too
+        off = ((half + (64 + M) * U) * G.abs() + 64 * U / V * gl.abs()[:, None] * (gl.abs()[:, None] < 100)
+               ).T @ x.double().abs()
+        allowed = off * (1 + half) + half * want.abs() + info.smallest_normal * info.eps / 2
+        assert ((gw.double() - want).abs() <= allowed).all()
+
+
 # ------------------------------------------------------------------ fp32 hidden states
 @pytest.mark.parametrize("M", [5, 40])
 @pytest.mark.parametrize("fmt", ["e2m1", "gf4"])
