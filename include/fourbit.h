@@ -568,7 +568,7 @@ int fb_embed(const void* w, int64_t w_stride, int32_t dtype, int32_t vocab, int3
              const int64_t* token, int64_t rows, float scale, void* out, void* stream);
 
 /* Its gradient: grad[v] = scale * the sum of the rows of g whose token is v, all of [vocab, K], in
- * fp32 and in an order that the tokens alone decide, rounded once.
+ * fp32 and in an order that the tokens alone decide, rounded once; 0 throughout where there are no rows.
  *   g     [rows, K] of dtype, rows g_stride elements apart
  *   grad  [vocab, K] of dtype, contiguous, 16-byte aligned
  *   ws    256-byte aligned, fb_embed_grad_workspace_bytes (its contents are not kept) */
@@ -603,7 +603,7 @@ int fb_residual_norm(const fb_norm_t* n, void* h, void* y, float* stats, void* s
 /* Its gradient from g_h and g_y (contiguous [rows, width] of dtype, or NULL: 0).  Any of the results
  * may be NULL: grad_x and grad_branch [rows, width] of dtype, grad_weight, grad_branch_weight and
  * grad_gate of the shapes and types of what they belong to.  Sums over rows are in fp32 and in an order
- * that the sizes alone decide.
+ * that the sizes alone decide.  Of no rows nothing is written, the sums over rows neither.
  *   ws  256-byte aligned, fb_residual_norm_grad_workspace_bytes (its contents are not kept) */
 int fb_residual_norm_grad(const fb_norm_t* n, const float* stats, const void* g_h, const void* g_y,
                           void* grad_x, void* grad_branch, void* grad_weight,
@@ -635,7 +635,8 @@ int fb_pad_rows(const void* src, int64_t src_stride, int64_t rows, int32_t K, vo
 /* The gradient: with G[r, v] as fb_token_logprobs_grad's (no alternatives), grad_x = G w and
  * grad_w = G^T x.  The logits are computed again, a piece of the vocabulary at a time; G enters the
  * products rounded to dtype (fp16: times a power of two of its row), but for the given token's value,
- * which keeps what its rounding loses.  In fp16 grad_w takes x times a power of two for each row, in
+ * which keeps what its rounding loses: the results' error is between that of their own rounding and 1.4
+ * times as much (entropies' gradients).  In fp16 grad_w takes x times a power of two for each row, in
  * fp16: a row whose bound of |G| times its largest |x| is 2^-30 of the largest row's, or more, keeps x's
  * bits but where the result's would be below fp16's normal numbers.  A row whose g are 0, or that has
  * no token and no g_entropy, adds nothing to grad_w whatever its x holds.
@@ -643,7 +644,7 @@ int fb_pad_rows(const void* src, int64_t src_stride, int64_t rows, int32_t K, vo
  *   g_*                fp32 [rows], or NULL (taken as 0)
  *   grad_x, grad_w     [rows, K], [vocab, K] of dtype, contiguous, 8-byte aligned; NULL: not wanted
  *   ws                 256-byte aligned, fb_head_logprobs_grad_workspace_bytes with which are wanted
- * rows x K up to 2^33 where grad_x is wanted. */
+ * rows x K up to 2^33 where grad_x is wanted.  Of no rows nothing is written, grad_w neither. */
 int fb_head_logprobs_grad(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
                           int32_t dtype, int64_t rows, int32_t K, int32_t vocab,
                           const int64_t* token, const float* stats, const float* entropy,
